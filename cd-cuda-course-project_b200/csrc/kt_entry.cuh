@@ -51,6 +51,16 @@
 #define KT_WITH_FA 0
 #endif
 #include "naive.cuh"
+// The training and serving operators are not tuner families: only the default
+// library builds them.
+#if !KT_SELECTIVE
+#define KT_WITH_LM 1
+#include "layernorm_train.cuh"
+#include "logprob.cuh"
+#include "w4.cuh"
+#else
+#define KT_WITH_LM 0
+#endif
 
 #define KT_STR2(x) #x
 #define KT_STR(x) KT_STR2(x)
@@ -202,6 +212,87 @@ int kt_naive_attention_bf16(const uint16_t* Q, const uint16_t* K, const uint16_t
                             int64_t H, int64_t S, int64_t D, float scale, int causal, kt_stream_t stream) {
   kt::clear_error();
   return kt::naive::attention(Q, K, V, O, B, H, S, D, scale, causal, stream);
+}
+
+size_t kt_layernorm_bwd_workspace_bytes(int64_t rows, int64_t cols) {
+#if KT_WITH_LM
+  return kt::ln_train::workspace_bytes(rows, cols);
+#else
+  (void)rows;
+  (void)cols;
+  return 0;
+#endif
+}
+
+int kt_layernorm_train_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd,
+                           int8_t* q8, uint8_t* q8_exp, int64_t rows, int64_t cols, float eps, int dtype,
+                           int wdtype, kt_stream_t stream) {
+  kt::clear_error();
+#if KT_WITH_LM
+  return kt::ln_train::forward({x, gamma, beta, y, mean, rstd, q8, q8_exp, rows, cols, eps, wdtype}, dtype, stream);
+#else
+  return kt::unsupported("layernorm training");
+#endif
+}
+
+int kt_layernorm_train_bwd(const void* dy, const void* x, const int8_t* q8, const uint8_t* q8_exp, const void* gamma,
+                           const float* mean, const float* rstd, void* dx, void* dgamma, void* dbeta, int64_t rows,
+                           int64_t cols, int dtype, int wdtype, void* workspace, size_t ws_bytes,
+                           kt_stream_t stream) {
+  kt::clear_error();
+#if KT_WITH_LM
+  return kt::ln_train::backward({dy, x, q8, q8_exp, gamma, mean, rstd, dx, nullptr, rows, cols, wdtype}, dtype, dgamma,
+                                dbeta, workspace, ws_bytes, stream);
+#else
+  return kt::unsupported("layernorm training");
+#endif
+}
+
+int kt_token_logprobs(const void* logits, int64_t ld, const int64_t* targets, int64_t rows, int64_t vocab, float scale,
+                      int64_t ignore_index, int top_k, float* logprob, float* entropy, float* lse,
+                      float* top_logprob, int64_t* top_index, int dtype, kt_stream_t stream) {
+  kt::clear_error();
+#if KT_WITH_LM
+  return kt::logprob::forward({logits, ld, targets, rows, vocab, ignore_index, scale, top_k, logprob, entropy, lse,
+                               top_logprob, top_index}, dtype, stream);
+#else
+  return kt::unsupported("token log probabilities");
+#endif
+}
+
+int kt_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* targets, const float* lse,
+                          const float* entropy, const float* grad_logprob, const float* grad_entropy, int64_t rows,
+                          int64_t vocab, float scale, int64_t ignore_index, void* dlogits, int64_t ld_dlogits,
+                          int dtype, kt_stream_t stream) {
+  kt::clear_error();
+#if KT_WITH_LM
+  return kt::logprob::backward({logits, ld, targets, lse, entropy, grad_logprob, grad_entropy, rows, vocab,
+                                ignore_index, scale, dlogits, ld_dlogits, 0}, dtype, stream);
+#else
+  return kt::unsupported("token log probabilities");
+#endif
+}
+
+int kt_w4_quantize(const void* w, int64_t N, int64_t K, int group, int dtype, uint8_t* packed, void* scales,
+                   int scale_dtype, kt_stream_t stream) {
+  kt::clear_error();
+#if KT_WITH_LM
+  return kt::w4::quantize(w, N, K, group, dtype, packed, scales, scale_dtype, stream);
+#else
+  return kt::unsupported("4-bit weights");
+#endif
+}
+
+int kt_w4_linear(const void* x, int64_t ldx, const uint8_t* packed, const void* scales, const uint8_t* zeros,
+                 const void* bias, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int group, int dtype,
+                 int scale_dtype, kt_stream_t stream) {
+  kt::clear_error();
+#if KT_WITH_LM
+  return kt::w4::linear({x, ldx, packed, scales, zeros, bias, y, ldy, M, N, K, scale_dtype, 0, 0}, group, dtype,
+                        stream);
+#else
+  return kt::unsupported("4-bit weights");
+#endif
 }
 
 int kt_run(int op, const kt_args* a, kt_stream_t s) {

@@ -1,0 +1,641 @@
+// layernorm_train.cuh — LayerNorm with its backward pass (fp32, bf16, fp16),
+// optionally keeping the input for the backward pass in 8 bits.
+//
+// Forward, per row of C columns:
+//   mu = mean(x)   r = 1/sqrt(mean((x-mu)^2) + eps)   y = gamma (x-mu) r + beta
+// and mu, r (fp32) are saved. Backward, with xh = (x-mu) r and w = dy gamma:
+//   dx = r (w - mean(w) - xh mean(w xh))
+//   dgamma = sum over rows of dy xh      dbeta = sum over rows of dy
+// All sums and statistics are fp32; y, dx, dgamma, dbeta are rounded once.
+//
+// 8-bit checkpoint (forward writes it, backward reads it in x's place): blocks
+// of 32 columns share a power of two, E = exponent field of the block's largest
+// magnitude as fp32, at least 7; q = x 2^(133-E) rounded to nearest even and
+// limited to +-127, standing for q 2^(E-133). With a power of two both steps
+// are exact but for the one rounding, so the numbers do not depend on who
+// computes them. A block that holds an infinity or a NaN has E = 255 and stands
+// for NaN. mu and r come from the unrounded x.
+//
+// Bound by memory: forward reads x and writes y, backward reads dy and x (or 8
+// bits of it) and writes dx. TPR threads hold one row in registers as 16-byte
+// pieces. The rows of a CTA are grid.x apart, which makes them equally aligned,
+// so a thread always holds the same columns: gamma and beta stay in its
+// registers, and dgamma and dbeta are summed there over all rows of the CTA and
+// written once, as one partial row per CTA. A second kernel adds the partial
+// rows in their order, so results do not change from run to run.
+#pragma once
+#include <type_traits>
+
+#include "elem.cuh"
+
+namespace kt {
+namespace ln_train {
+
+struct FwdArgs {
+  const void* x;
+  const void* gamma;  // may be null: 1
+  const void* beta;   // may be null: 0
+  void* y;
+  float* mean;
+  float* rstd;
+  int8_t* q8;        // with 8-bit checkpoints
+  uint8_t* q8_exp;   // rows x ceil(cols / 32)
+  int64_t rows;
+  int64_t cols;
+  float eps;
+  int wdtype;
+};
+
+struct BwdArgs {
+  const void* dy;
+  const void* x;  // null with 8-bit checkpoints
+  const int8_t* q8;
+  const uint8_t* q8_exp;
+  const void* gamma;
+  const float* mean;
+  const float* rstd;
+  void* dx;
+  float* partial;  // [parts][2][cols]: dgamma, dbeta
+  int64_t rows;
+  int64_t cols;
+  int wdtype;
+};
+
+// ---------------------------------------------------------------- 8-bit blocks
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+// Exponent code of a block from the largest bit pattern of its magnitudes
+// (infinities and NaNs have the largest patterns).
+__device__ __forceinline__ uint32_t block_code(uint32_t bits) {
+  const uint32_t e = bits >> 23;
+  return e < 7u ? 7u : e;
+}
+__device__ __forceinline__ float code_up(uint32_t code) {
+  return code == 255u ? 0.f : __uint_as_float((260u - code) << 23);
+}
+__device__ __forceinline__ float code_down(uint32_t code) {
+  return code == 255u ? __uint_as_float(0x7FC00000u) : __uint_as_float((code - 6u) << 23);
+}
+__device__ __forceinline__ int quant8(float v, float up) {
+  // a non-finite value meets up = 0 only; its NaN becomes 0
+  return min(127, max(-127, __float2int_rn(v * up)));
+}
+
+// ---------------------------------------------------------------- row pieces
+// Columns [e0, e0+V) of a row as raw 16 bytes; columns outside [0, cols) are 0.
+// `row + e0` lies on a 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ uint4 load_piece(const T* row, int e0, int cols) {
+  constexpr int V = elem::kVec<T>;
+  if (e0 >= 0 && e0 + V <= cols) return elem::ld_once16(row + e0);
+  float f[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) f[j] = (e0 + j >= 0 && e0 + j < cols) ? elem::to_f(row[e0 + j]) : 0.f;
+  return elem::pack_vec<T>(f);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_piece(T* row, int e0, int cols, const float (&f)[elem::kVec<T>]) {
+  constexpr int V = elem::kVec<T>;
+  if (e0 >= 0 && e0 + V <= cols) {
+    *reinterpret_cast<uint4*>(row + e0) = elem::pack_vec<T>(f);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if (e0 + j >= 0 && e0 + j < cols) row[e0 + j] = elem::from_f<T>(f[j]);
+}
+
+// Sum over the TPR threads of a row; every thread gets it. `scratch` holds
+// TPR/32 values; two calls in a row need different scratch.
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* scratch) {
+  v = warp_sum(v);
+  if constexpr (TPR > 32) {
+    constexpr int NW = TPR / 32;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = warp_sum(lane < NW ? scratch[lane] : 0.f);
+  }
+  return v;
+}
+
+template <int TPR>
+__device__ __forceinline__ float2 row_sum2(float a, float b, float2* scratch) {
+  a = warp_sum(a);
+  b = warp_sum(b);
+  if constexpr (TPR > 32) {
+    constexpr int NW = TPR / 32;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) scratch[threadIdx.x >> 5] = make_float2(a, b);
+    __syncthreads();
+    const float2 s = lane < NW ? scratch[lane] : make_float2(0.f, 0.f);
+    a = warp_sum(s.x);
+    b = warp_sum(s.y);
+  }
+  return make_float2(a, b);
+}
+
+// ---------------------------------------------------------------- forward
+template <typename T, int TPR, int VPT, bool CKPT>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR)
+fwd_rows(const FwdArgs p) {
+  constexpr int V = elem::kVec<T>;
+  constexpr int RB = TPR == 32 ? 8 : 1;  // rows of a CTA at a time
+  __shared__ float red[2][32];
+  const int t = threadIdx.x % TPR;
+  const int cols = (int)p.cols;
+  const float fcols = (float)cols;
+  const int64_t first = (int64_t)blockIdx.x * RB + threadIdx.x / TPR;
+  const int64_t stride = (int64_t)gridDim.x * RB;
+  const int shift = elem::misalign<T>(static_cast<const T*>(p.x) + first * cols);
+  float g[VPT][V], b[VPT][V];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int e = (t + i * TPR) * V - shift + j;
+      const bool in = e >= 0 && e < cols;
+      g[i][j] = in && p.gamma ? elem::ld_weight(p.gamma, p.wdtype, e) : 1.f;
+      b[i][j] = in && p.beta ? elem::ld_weight(p.beta, p.wdtype, e) : 0.f;
+    }
+  uint4 next[VPT];
+  auto fetch = [&](int64_t row) {
+    const T* xr = static_cast<const T*>(p.x) + row * cols;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int e0 = (t + i * TPR) * V - shift;
+      next[i] = e0 < cols ? load_piece<T>(xr, e0, cols) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  if (first < p.rows) fetch(first);
+  for (int64_t row = first; row < p.rows; row += stride) {
+    float v[VPT][V];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      elem::unpack_vec<T>(next[i], v[i]);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s += v[i][j];
+    }
+    if (row + stride < p.rows) fetch(row + stride);
+    const float mean = row_sum<TPR>(s, red[0]) / fcols;
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int e = (t + i * TPR) * V - shift + j;
+        const float d = v[i][j] - mean;
+        if (e >= 0 && e < cols) q = fmaf(d, d, q);
+      }
+    const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red[1]) / fcols + p.eps);
+    if (t == 0) {
+      p.mean[row] = mean;
+      p.rstd[row] = rstd;
+    }
+    T* yr = static_cast<T*>(p.y) + row * cols;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t + i * TPR;
+      const int e0 = c * V - shift;
+      if constexpr (CKPT) {
+        constexpr int LPB = 32 / V;  // lanes that share a block of 32 columns
+        uint32_t top = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) top = max(top, abs_bits(v[i][j]));
+#pragma unroll
+        for (int o = 1; o < LPB; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const uint32_t code = block_code(top);
+        if (e0 < cols) {
+          const float up = code_up(code);
+          uint32_t w[V / 4];
+#pragma unroll
+          for (int k = 0; k < V / 4; ++k) {
+            w[k] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[k] |= ((uint32_t)quant8(v[i][4 * k + j], up) & 255u) << (8 * j);
+          }
+          int8_t* qr = p.q8 + row * cols + e0;
+          if constexpr (V == 8) *reinterpret_cast<uint2*>(qr) = make_uint2(w[0], w[1]);
+          else *reinterpret_cast<uint32_t*>(qr) = w[0];
+          if (c % LPB == 0) p.q8_exp[row * ((cols + 31) / 32) + c / LPB] = (uint8_t)code;
+        }
+      }
+      if (e0 < cols) {
+        float o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = fmaf((v[i][j] - mean) * rstd, g[i][j], b[i][j]);
+        store_piece<T>(yr, e0, cols, o);
+      }
+    }
+  }
+}
+
+// Any width and alignment: a CTA per row, the row read once per step (from L2
+// after the first). Lanes hold consecutive columns, so a warp's 32 columns are
+// one block of the checkpoint.
+template <typename T, bool CKPT>
+__global__ void __launch_bounds__(256) fwd_any(const FwdArgs p) {
+  __shared__ float red[2][32];
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const T* xr = static_cast<const T*>(p.x) + row * p.cols;
+    T* yr = static_cast<T*>(p.y) + row * p.cols;
+    float s = 0.f;
+    for (int64_t e = threadIdx.x; e < p.cols; e += 256) s += elem::to_f(xr[e]);
+    const float mean = row_sum<256>(s, red[0]) / (float)p.cols;
+    float q = 0.f;
+    for (int64_t e = threadIdx.x; e < p.cols; e += 256) {
+      const float d = elem::to_f(xr[e]) - mean;
+      q = fmaf(d, d, q);
+    }
+    const float rstd = 1.f / sqrtf(row_sum<256>(q, red[1]) / (float)p.cols + p.eps);
+    if (threadIdx.x == 0) {
+      p.mean[row] = mean;
+      p.rstd[row] = rstd;
+    }
+    for (int64_t e0 = threadIdx.x & ~31; e0 < p.cols; e0 += 256) {
+      const int64_t e = e0 + (threadIdx.x & 31);
+      const float v = e < p.cols ? elem::to_f(xr[e]) : 0.f;
+      if constexpr (CKPT) {
+        const uint32_t code = block_code(__reduce_max_sync(0xffffffffu, abs_bits(v)));
+        if (e < p.cols) p.q8[row * p.cols + e] = (int8_t)quant8(v, code_up(code));
+        if ((threadIdx.x & 31) == 0) p.q8_exp[row * ((p.cols + 31) / 32) + e0 / 32] = (uint8_t)code;
+      }
+      if (e < p.cols) {
+        const float g = p.gamma ? elem::ld_weight(p.gamma, p.wdtype, e) : 1.f;
+        const float b = p.beta ? elem::ld_weight(p.beta, p.wdtype, e) : 0.f;
+        yr[e] = elem::from_f<T>(fmaf((v - mean) * rstd, g, b));
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- backward
+template <typename T, int TPR, int VPT, bool CKPT>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR)
+bwd_rows(const BwdArgs p) {
+  constexpr int V = elem::kVec<T>;
+  constexpr int RB = TPR == 32 ? 8 : 1;
+  extern __shared__ float part[];  // RB > 1: 2 x cols sums of the CTA
+  __shared__ float2 red[2][32];
+  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  const int cols = (int)p.cols;
+  const float fcols = (float)cols;
+  const int64_t first = (int64_t)blockIdx.x * RB + sub;
+  const int64_t stride = (int64_t)gridDim.x * RB;
+  const int shift = elem::misalign<T>(static_cast<const T*>(p.dy) + first * cols);
+  float g[VPT][V], dg[VPT][V], db[VPT][V];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int e = (t + i * TPR) * V - shift + j;
+      g[i][j] = e >= 0 && e < cols && p.gamma ? elem::ld_weight(p.gamma, p.wdtype, e) : 1.f;
+      dg[i][j] = db[i][j] = 0.f;
+    }
+  uint4 ny[VPT], nx[VPT];  // of nx, 8-bit checkpoints use .x and .y, and .z for the block's code
+  float nmean = 0.f, nrstd = 0.f;
+  auto fetch = [&](int64_t row) {
+    const T* dyr = static_cast<const T*>(p.dy) + row * cols;
+    nmean = p.mean[row];
+    nrstd = p.rstd[row];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = t + i * TPR;
+      const int e0 = c * V - shift;
+      ny[i] = nx[i] = make_uint4(0, 0, 0, 0);
+      if (e0 < cols) {
+        ny[i] = load_piece<T>(dyr, e0, cols);
+        if constexpr (CKPT) {
+          const int8_t* qr = p.q8 + row * cols + e0;
+          if constexpr (V == 8) {
+            const uint2 w = *reinterpret_cast<const uint2*>(qr);
+            nx[i].x = w.x;
+            nx[i].y = w.y;
+          } else {
+            nx[i].x = *reinterpret_cast<const uint32_t*>(qr);
+          }
+          nx[i].z = p.q8_exp[row * ((cols + 31) / 32) + c / (32 / V)];
+        } else {
+          nx[i] = load_piece<T>(static_cast<const T*>(p.x) + row * cols, e0, cols);
+        }
+      }
+    }
+  };
+  if (first < p.rows) fetch(first);
+  int turn = 0;
+  for (int64_t row = first; row < p.rows; row += stride, turn ^= 1) {
+    float xh[VPT][V], w[VPT][V];
+    float s1 = 0.f, s2 = 0.f;
+    const float mean = nmean, rstd = nrstd;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int e0 = (t + i * TPR) * V - shift;
+      if constexpr (CKPT) {
+        const float down = code_down(e0 < cols ? nx[i].z : 7u);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const uint32_t word = j < 4 ? nx[i].x : nx[i].y;
+          xh[i][j] = (float)(int8_t)(word >> (8 * (j & 3))) * down;
+        }
+      } else {
+        elem::unpack_vec<T>(nx[i], xh[i]);
+      }
+      float d[V];
+      elem::unpack_vec<T>(ny[i], d);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const bool in = e0 + j >= 0 && e0 + j < cols;
+        xh[i][j] = in ? (xh[i][j] - mean) * rstd : 0.f;
+        dg[i][j] = fmaf(d[j], xh[i][j], dg[i][j]);
+        db[i][j] += d[j];
+        w[i][j] = d[j] * g[i][j];
+        s1 = fmaf(w[i][j], xh[i][j], s1);
+        s2 += w[i][j];
+      }
+    }
+    if (row + stride < p.rows) fetch(row + stride);
+    const float2 s = row_sum2<TPR>(s1, s2, red[turn]);
+    const float c1 = s.x / fcols, c2 = s.y / fcols;
+    T* dxr = static_cast<T*>(p.dx) + row * cols;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int e0 = (t + i * TPR) * V - shift;
+      if (e0 < cols) {
+        float o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = rstd * (w[i][j] - c2 - xh[i][j] * c1);
+        store_piece<T>(dxr, e0, cols, o);
+      }
+    }
+  }
+  if (p.partial == nullptr) return;
+  float* out = p.partial + (int64_t)blockIdx.x * 2 * cols;
+  if constexpr (RB == 1) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int e = (t + i * TPR) * V - shift + j;
+        if (e >= 0 && e < cols) {
+          out[e] = dg[i][j];
+          out[cols + e] = db[i][j];
+        }
+      }
+  } else {
+    for (int w = 0; w < RB; ++w) {  // in the order of the warps
+      if (sub == w) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const int e = (t + i * TPR) * V - shift + j;
+            if (e >= 0 && e < cols) {
+              part[e] = w ? part[e] + dg[i][j] : dg[i][j];
+              part[cols + e] = w ? part[cols + e] + db[i][j] : db[i][j];
+            }
+          }
+      }
+      __syncthreads();
+    }
+    for (int e = threadIdx.x; e < 2 * cols; e += 256) out[e] = part[e];
+  }
+}
+
+// Any width and alignment: dx by a CTA per row, and the partial sums by columns.
+template <typename T, bool CKPT>
+__device__ __forceinline__ float x_hat(const BwdArgs& p, int64_t row, int64_t e, float mean, float rstd) {
+  float v;
+  if constexpr (CKPT)
+    v = (float)p.q8[row * p.cols + e] * code_down(p.q8_exp[row * ((p.cols + 31) / 32) + e / 32]);
+  else
+    v = elem::to_f(static_cast<const T*>(p.x)[row * p.cols + e]);
+  return (v - mean) * rstd;
+}
+
+template <typename T, bool CKPT>
+__global__ void __launch_bounds__(256) bwd_any_dx(const BwdArgs p) {
+  __shared__ float2 red[2][32];
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    const T* dyr = static_cast<const T*>(p.dy) + row * p.cols;
+    T* dxr = static_cast<T*>(p.dx) + row * p.cols;
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    float s1 = 0.f, s2 = 0.f;
+    for (int64_t e = threadIdx.x; e < p.cols; e += 256) {
+      const float w = elem::to_f(dyr[e]) * (p.gamma ? elem::ld_weight(p.gamma, p.wdtype, e) : 1.f);
+      s1 = fmaf(w, x_hat<T, CKPT>(p, row, e, mean, rstd), s1);
+      s2 += w;
+    }
+    const float2 s = row_sum2<256>(s1, s2, red[turn]);
+    const float c1 = s.x / (float)p.cols, c2 = s.y / (float)p.cols;
+    for (int64_t e = threadIdx.x; e < p.cols; e += 256) {
+      const float w = elem::to_f(dyr[e]) * (p.gamma ? elem::ld_weight(p.gamma, p.wdtype, e) : 1.f);
+      dxr[e] = elem::from_f<T>(rstd * (w - c2 - x_hat<T, CKPT>(p, row, e, mean, rstd) * c1));
+    }
+  }
+}
+
+template <typename T, bool CKPT>
+__global__ void __launch_bounds__(256) bwd_any_cols(const BwdArgs p) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= p.cols) return;
+  const int64_t lo = p.rows * blockIdx.y / gridDim.y, hi = p.rows * (blockIdx.y + 1) / gridDim.y;
+  float dg = 0.f, db = 0.f;
+  for (int64_t row = lo; row < hi; ++row) {
+    const float d = elem::to_f(static_cast<const T*>(p.dy)[row * p.cols + e]);
+    dg = fmaf(d, x_hat<T, CKPT>(p, row, e, p.mean[row], p.rstd[row]), dg);
+    db += d;
+  }
+  float* out = p.partial + (int64_t)blockIdx.y * 2 * p.cols;
+  out[e] = dg;
+  out[p.cols + e] = db;
+}
+
+// dgamma, dbeta: the partial rows added in their order. 32 columns x 8 slices of
+// the partial rows per CTA, the slices joined in shared memory.
+__global__ void __launch_bounds__(256)
+bwd_join(const float* __restrict__ partial, int parts, int64_t cols, void* dgamma, void* dbeta, int wdtype) {
+  __shared__ float slice[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t e = (int64_t)blockIdx.x * 32 + lane;  // over 2 x cols: dgamma, then dbeta
+  float s = 0.f;
+  if (e < 2 * cols)
+    for (int r = parts * w / 8; r < parts * (w + 1) / 8; ++r) s += partial[(int64_t)r * 2 * cols + e];
+  slice[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && e < 2 * cols) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += slice[k][lane];
+    if (e < cols) {
+      if (dgamma) elem::st_weight(dgamma, wdtype, e, s);
+    } else if (dbeta) {
+      elem::st_weight(dbeta, wdtype, e - cols, s);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host
+constexpr int64_t kMaxParts = 1184;  // 8 CTAs on each of 148 SMs
+
+// Partial rows that one call may use.
+inline int64_t max_parts(int64_t rows) { return rows < kMaxParts ? rows : kMaxParts; }
+
+inline size_t workspace_bytes(int64_t rows, int64_t cols) {
+  if (rows <= 0 || cols <= 0) return 0;
+  return (size_t)max_parts(rows) * 2 * (size_t)cols * sizeof(float);
+}
+
+// CTAs for `rows`: what the device holds at once, at most one per `rb` rows and
+// kMaxParts; a multiple of 8 where a CTA has several rows, so that rows `grid`
+// apart start at equal offsets within 16 bytes.
+template <class K>
+inline int row_grid(K kern, int block, int rb, size_t smem, int64_t rows, int* grid) {
+  int per_sm = 0;
+  const int rc = resident_ctas((const void*)kern, block, smem, &per_sm, "layernorm_train: launch shape");
+  if (rc != KT_OK) return rc;
+  if (per_sm < 1) return fail(KT_ERR_UNSUPPORTED, "layernorm_train: no CTA fits");
+  const int64_t need = (rows + rb - 1) / rb;
+  int64_t g = (int64_t)sm_count() * per_sm;
+  if (g > kMaxParts) g = kMaxParts;
+  g = g / 8 * 8;
+  *grid = (int)(need <= g ? need : (g > 0 ? g : 8));
+  return KT_OK;
+}
+
+// Calls f with the smallest (threads per row, pieces per thread) that holds a
+// row of `pieces` 16-byte pieces; false when none does.
+template <class F>
+inline bool with_shape(int64_t pieces, F f) {
+  if (pieces <= 32) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{}), true;
+  if (pieces <= 128) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{}), true;
+  if (pieces <= 512) return f(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{}), true;
+  if (pieces <= 1024) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{}), true;
+  if (pieces <= 2048) return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{}), true;
+  return false;
+}
+
+inline int check_common(const char* what, int64_t rows, int64_t cols, int dtype, int wdtype) {
+  if (rows < 0 || cols < 0)
+    return fail(KT_ERR_ARG, "%s: negative shape rows=%lld cols=%lld", what, (long long)rows, (long long)cols);
+  if (elem::size_of(dtype) == 0) return fail(KT_ERR_ARG, "%s: unknown dtype %d", what, dtype);
+  if (wdtype != KT_F32 && wdtype != dtype)
+    return fail(KT_ERR_ARG, "%s: weights are fp32 or of the input's type", what);
+  if (cols > INT32_MAX / 2) return fail(KT_ERR_UNSUPPORTED, "%s: cols > 2^30", what);
+  return KT_OK;
+}
+
+template <typename T, bool CKPT>
+inline int fwd_typed(const FwdArgs& a, cudaStream_t st) {
+  constexpr int V = elem::kVec<T>;
+  const int shift = elem::misalign<T>(a.x);
+  bool fast = elem::misalign<T>(a.y) == shift;
+  if (CKPT) fast = fast && shift == 0 && a.cols % V == 0 && elem::aligned_to(a.q8, V);
+  const int64_t pieces = (a.cols + V - 1) / V + (a.cols % V || shift ? 1 : 0);
+  int rc = KT_OK;
+  if (fast && with_shape(pieces, [&](auto tpr, auto vpt) {
+        constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
+        constexpr int RB = TPR == 32 ? 8 : 1, BLOCK = TPR == 32 ? 256 : TPR;
+        auto kern = fwd_rows<T, TPR, VPT, CKPT>;
+        int grid = 0;
+        rc = row_grid(kern, BLOCK, RB, 0, a.rows, &grid);
+        if (rc != KT_OK) return;
+        kern<<<grid, BLOCK, 0, st>>>(a);
+        rc = check_launch("layernorm_train fwd_rows");
+      }))
+    return rc;
+  const int64_t g = a.rows < 4 * sm_count() ? a.rows : 4 * sm_count();
+  fwd_any<T, CKPT><<<(int)g, 256, 0, st>>>(a);
+  return check_launch("layernorm_train fwd_any");
+}
+
+inline int forward(const FwdArgs& a, int dtype, cudaStream_t st) {
+  int rc = check_common("layernorm_train", a.rows, a.cols, dtype, a.wdtype);
+  if (rc != KT_OK) return rc;
+  if (!(a.eps >= 0.f)) return fail(KT_ERR_ARG, "layernorm_train: eps must be >= 0");
+  if ((a.q8 == nullptr) != (a.q8_exp == nullptr))
+    return fail(KT_ERR_ARG, "layernorm_train: q8 and q8_exp are given together");
+  if (a.rows == 0 || a.cols == 0) return KT_OK;
+  if (!a.x || !a.y || !a.mean || !a.rstd) return fail(KT_ERR_ARG, "layernorm_train: null pointer");
+  const int sz = elem::size_of(dtype), wsz = elem::size_of(a.wdtype);
+  if (!elem::aligned_to(a.x, sz) || !elem::aligned_to(a.y, sz) || !elem::aligned_to(a.gamma, wsz) ||
+      !elem::aligned_to(a.beta, wsz) || !elem::aligned_to(a.mean, 4) || !elem::aligned_to(a.rstd, 4))
+    return fail(KT_ERR_ARG, "layernorm_train: a pointer is not aligned to its elements");
+  if (dtype == KT_F32) return a.q8 ? fwd_typed<float, true>(a, st) : fwd_typed<float, false>(a, st);
+  if (dtype == KT_BF16) return a.q8 ? fwd_typed<__nv_bfloat16, true>(a, st) : fwd_typed<__nv_bfloat16, false>(a, st);
+  return a.q8 ? fwd_typed<__half, true>(a, st) : fwd_typed<__half, false>(a, st);
+}
+
+template <typename T, bool CKPT>
+inline int bwd_typed(const BwdArgs& a, void* dgamma, void* dbeta, cudaStream_t st) {
+  constexpr int V = elem::kVec<T>;
+  const int shift = elem::misalign<T>(a.dy);
+  bool fast = elem::misalign<T>(a.dx) == shift;
+  if (CKPT) fast = fast && shift == 0 && a.cols % V == 0 && elem::aligned_to(a.q8, V);
+  else fast = fast && elem::misalign<T>(a.x) == shift;
+  const int64_t pieces = (a.cols + V - 1) / V + (a.cols % V || shift ? 1 : 0);
+  int rc = KT_OK, parts = 0;
+  if (!(fast && with_shape(pieces, [&](auto tpr, auto vpt) {
+          constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
+          constexpr int RB = TPR == 32 ? 8 : 1, BLOCK = TPR == 32 ? 256 : TPR;
+          auto kern = bwd_rows<T, TPR, VPT, CKPT>;
+          const size_t smem = RB > 1 ? 2 * (size_t)a.cols * sizeof(float) : 0;
+          rc = row_grid(kern, BLOCK, RB, smem, a.rows, &parts);
+          if (rc != KT_OK) return;
+          kern<<<parts, BLOCK, smem, st>>>(a);
+          rc = check_launch("layernorm_train bwd_rows");
+        }))) {
+    const int64_t g = a.rows < 4 * sm_count() ? a.rows : 4 * sm_count();
+    bwd_any_dx<T, CKPT><<<(int)g, 256, 0, st>>>(a);
+    rc = check_launch("layernorm_train bwd_any_dx");
+    if (rc == KT_OK && a.partial) {
+      parts = (int)(a.rows < 64 ? a.rows : 64);
+      bwd_any_cols<T, CKPT><<<dim3((unsigned)((a.cols + 255) / 256), (unsigned)parts), 256, 0, st>>>(a);
+      rc = check_launch("layernorm_train bwd_any_cols");
+    }
+  }
+  if (rc != KT_OK || a.partial == nullptr) return rc;
+  bwd_join<<<(unsigned)((2 * a.cols + 31) / 32), 256, 0, st>>>(a.partial, parts, a.cols, dgamma, dbeta, a.wdtype);
+  return check_launch("layernorm_train bwd_join");
+}
+
+inline int backward(BwdArgs a, int dtype, void* dgamma, void* dbeta, void* workspace, size_t ws_bytes,
+                    cudaStream_t st) {
+  int rc = check_common("layernorm_train bwd", a.rows, a.cols, dtype, a.wdtype);
+  if (rc != KT_OK) return rc;
+  if ((a.q8 == nullptr) != (a.q8_exp == nullptr))
+    return fail(KT_ERR_ARG, "layernorm_train bwd: q8 and q8_exp are given together");
+  if (a.cols == 0) return KT_OK;
+  const int sz = elem::size_of(dtype), wsz = elem::size_of(a.wdtype);
+  if (!elem::aligned_to(dgamma, wsz) || !elem::aligned_to(dbeta, wsz))
+    return fail(KT_ERR_ARG, "layernorm_train bwd: a pointer is not aligned to its elements");
+  if (a.rows == 0) {  // empty sums
+    if (dgamma) rc = cuda_status(cudaMemsetAsync(dgamma, 0, (size_t)a.cols * wsz, st), "layernorm_train bwd: dgamma");
+    if (rc == KT_OK && dbeta)
+      rc = cuda_status(cudaMemsetAsync(dbeta, 0, (size_t)a.cols * wsz, st), "layernorm_train bwd: dbeta");
+    return rc;
+  }
+  if (!a.dy || !a.dx || !a.mean || !a.rstd) return fail(KT_ERR_ARG, "layernorm_train bwd: null pointer");
+  if ((a.x == nullptr) == (a.q8 == nullptr))
+    return fail(KT_ERR_ARG, "layernorm_train bwd: give x or its 8-bit checkpoint, not both");
+  if (!elem::aligned_to(a.dy, sz) || !elem::aligned_to(a.x, sz) || !elem::aligned_to(a.dx, sz) ||
+      !elem::aligned_to(a.gamma, wsz) || !elem::aligned_to(a.mean, 4) || !elem::aligned_to(a.rstd, 4))
+    return fail(KT_ERR_ARG, "layernorm_train bwd: a pointer is not aligned to its elements");
+  a.partial = nullptr;
+  if (dgamma || dbeta) {
+    if (workspace == nullptr || ws_bytes < workspace_bytes(a.rows, a.cols) || !aligned16(workspace))
+      return fail(KT_ERR_ARG, "layernorm_train bwd: workspace too small or not 16-byte aligned (%zu < %zu bytes)",
+                  ws_bytes, workspace_bytes(a.rows, a.cols));
+    a.partial = static_cast<float*>(workspace);
+  }
+  if (dtype == KT_F32) return a.q8 ? bwd_typed<float, true>(a, dgamma, dbeta, st)
+                                   : bwd_typed<float, false>(a, dgamma, dbeta, st);
+  if (dtype == KT_BF16) return a.q8 ? bwd_typed<__nv_bfloat16, true>(a, dgamma, dbeta, st)
+                                    : bwd_typed<__nv_bfloat16, false>(a, dgamma, dbeta, st);
+  return a.q8 ? bwd_typed<__half, true>(a, dgamma, dbeta, st) : bwd_typed<__half, false>(a, dgamma, dbeta, st);
+}
+
+}  // namespace ln_train
+}  // namespace kt

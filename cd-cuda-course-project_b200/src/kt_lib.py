@@ -38,6 +38,10 @@ STATUS_NAMES = {
 KT_GEMM_FFMA = 0
 KT_GEMM_TF32 = 1
 
+KT_F32 = 0
+KT_BF16 = 1
+KT_F16 = 2
+
 KT_XRANK_MAX = 8
 KT_XRANK_EXCHANGE_BYTES = 256
 
@@ -60,6 +64,8 @@ EXPORTED_SYMBOLS = (
     "kt_softmax_f32", "kt_layernorm_f32", "kt_reduce_workspace_bytes", "kt_reduce_sum_f32",
     "kt_reduce_sum_f32_xrank",
     "kt_gemm_f32", "kt_fa_fwd_bf16",
+    "kt_layernorm_train_fwd", "kt_layernorm_bwd_workspace_bytes", "kt_layernorm_train_bwd",
+    "kt_token_logprobs", "kt_token_logprobs_bwd", "kt_w4_quantize", "kt_w4_linear",
     "kt_naive_softmax_f32", "kt_naive_layernorm_f32", "kt_naive_reduce_sum_f32",
     "kt_naive_gemm_f32", "kt_naive_attention_bf16",
     "kt_run", "kt_time", "kt_device_error",
@@ -116,6 +122,13 @@ _SIGNATURES = {
                                        ctypes.c_uint64, _vp]),
     "kt_gemm_f32": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp]),
     "kt_fa_fwd_bf16": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _f32, _int, _vp]),
+    "kt_layernorm_train_fwd": (_int, [_vp] * 8 + [_i64, _i64, _f32, _int, _int, _vp]),
+    "kt_layernorm_bwd_workspace_bytes": (_size, [_i64, _i64]),
+    "kt_layernorm_train_bwd": (_int, [_vp] * 10 + [_i64, _i64, _int, _int, _vp, _size, _vp]),
+    "kt_token_logprobs": (_int, [_vp, _i64, _vp, _i64, _i64, _f32, _i64, _int, _vp, _vp, _vp, _vp, _vp, _int, _vp]),
+    "kt_token_logprobs_bwd": (_int, [_vp, _i64] + [_vp] * 5 + [_i64, _i64, _f32, _i64, _vp, _i64, _int, _vp]),
+    "kt_w4_quantize": (_int, [_vp, _i64, _i64, _int, _int, _vp, _vp, _int, _vp]),
+    "kt_w4_linear": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _int, _vp]),
     "kt_naive_softmax_f32": (_int, [_vp, _vp, _i64, _i64, _vp]),
     "kt_naive_layernorm_f32": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _f32, _vp]),
     "kt_naive_reduce_sum_f32": (_int, [_vp, _i64, _vp, _vp, _vp, _size, _vp]),
@@ -201,6 +214,50 @@ class KtLibrary:
                     scale: float, causal: bool, stream: Optional[int] = None) -> None:
         self._check(self._lib.kt_fa_fwd_bf16(Q, K, V, O, B, H, S, D, scale, int(bool(causal)), stream),
                     "kt_fa_fwd_bf16")
+
+    def layernorm_train_fwd(self, x: int, gamma: Optional[int], beta: Optional[int], y: int, mean: int, rstd: int,
+                            q8: Optional[int], q8_exp: Optional[int], rows: int, cols: int, eps: float, dtype: int,
+                            wdtype: int, stream: Optional[int] = None) -> None:
+        self._check(self._lib.kt_layernorm_train_fwd(x, gamma, beta, y, mean, rstd, q8, q8_exp, rows, cols, eps,
+                                                     dtype, wdtype, stream), "kt_layernorm_train_fwd")
+
+    def layernorm_bwd_workspace_bytes(self, rows: int, cols: int) -> int:
+        return int(self._lib.kt_layernorm_bwd_workspace_bytes(rows, cols))
+
+    def layernorm_train_bwd(self, dy: int, x: Optional[int], q8: Optional[int], q8_exp: Optional[int],
+                            gamma: Optional[int], mean: int, rstd: int, dx: int, dgamma: Optional[int],
+                            dbeta: Optional[int], rows: int, cols: int, dtype: int, wdtype: int,
+                            workspace: Optional[int], ws_bytes: int, stream: Optional[int] = None) -> None:
+        self._check(self._lib.kt_layernorm_train_bwd(dy, x, q8, q8_exp, gamma, mean, rstd, dx, dgamma, dbeta, rows,
+                                                     cols, dtype, wdtype, workspace, ws_bytes, stream),
+                    "kt_layernorm_train_bwd")
+
+    def token_logprobs(self, logits: int, ld: int, targets: Optional[int], rows: int, vocab: int, scale: float,
+                       ignore_index: int, top_k: int, logprob: Optional[int], entropy: Optional[int], lse: int,
+                       top_logprob: Optional[int], top_index: Optional[int], dtype: int,
+                       stream: Optional[int] = None) -> None:
+        self._check(self._lib.kt_token_logprobs(logits, ld, targets, rows, vocab, scale, ignore_index, top_k, logprob,
+                                                entropy, lse, top_logprob, top_index, dtype, stream),
+                    "kt_token_logprobs")
+
+    def token_logprobs_bwd(self, logits: int, ld: int, targets: Optional[int], lse: int, entropy: Optional[int],
+                           grad_logprob: Optional[int], grad_entropy: Optional[int], rows: int, vocab: int,
+                           scale: float, ignore_index: int, dlogits: int, ld_dlogits: int, dtype: int,
+                           stream: Optional[int] = None) -> None:
+        self._check(self._lib.kt_token_logprobs_bwd(logits, ld, targets, lse, entropy, grad_logprob, grad_entropy,
+                                                    rows, vocab, scale, ignore_index, dlogits, ld_dlogits, dtype,
+                                                    stream), "kt_token_logprobs_bwd")
+
+    def w4_quantize(self, w: int, N: int, K: int, group: int, dtype: int, packed: int, scales: int, scale_dtype: int,
+                    stream: Optional[int] = None) -> None:
+        self._check(self._lib.kt_w4_quantize(w, N, K, group, dtype, packed, scales, scale_dtype, stream),
+                    "kt_w4_quantize")
+
+    def w4_linear(self, x: int, ldx: int, packed: int, scales: int, zeros: Optional[int], bias: Optional[int], y: int,
+                  ldy: int, M: int, N: int, K: int, group: int, dtype: int, scale_dtype: int,
+                  stream: Optional[int] = None) -> None:
+        self._check(self._lib.kt_w4_linear(x, ldx, packed, scales, zeros, bias, y, ldy, M, N, K, group, dtype,
+                                           scale_dtype, stream), "kt_w4_linear")
 
     def run(self, op: int | str, args: KtArgs, stream: Optional[int] = None) -> None:
         op_id = OP_IDS[op] if isinstance(op, str) else int(op)

@@ -3,14 +3,15 @@ kt_ops.py — torch-facing wrappers over the C ABI.
 
 torch provides device memory and streams only; every computation goes
 through the loaded kernel library. Each wrapper checks device, dtype and
-contiguity, allocates the output, and launches on torch's current stream.
+contiguity, allocates the output, and launches on torch's current stream (the
+training and serving operators: of their tensors' device).
 There is no CPU or torch fallback: a missing library raises.
 """
 
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -111,3 +112,285 @@ def fa_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: Optional[fl
     sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
     lib.fa_fwd_bf16(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), B, H, S, D, sc, causal, _stream())
     return o
+
+
+# ---------------------------------------------------------------------------
+# Training and serving operators (fp32, bf16, fp16)
+# ---------------------------------------------------------------------------
+
+_DTYPES = {torch.float32: kt_lib.KT_F32, torch.bfloat16: kt_lib.KT_BF16, torch.float16: kt_lib.KT_F16}
+
+
+def _dtype(t: torch.Tensor, name: str) -> int:
+    try:
+        return _DTYPES[t.dtype]
+    except KeyError:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}") from None
+
+
+def _on_device(t: torch.Tensor, like: torch.Tensor, name: str) -> None:
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, not on {like.device}")
+
+
+def _rows(t: torch.Tensor, name: str) -> None:
+    """A 2-D CUDA tensor whose rows are dense; the rows may be any distance apart."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be 2-D")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: the elements of a row must be contiguous")
+
+
+def _ld(t: torch.Tensor) -> int:
+    """Distance of a 2-D tensor's rows in elements."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _launch(t: torch.Tensor, fn, *args) -> None:
+    """fn(*args, stream) on t's device and that device's current stream."""
+    d = t.get_device()
+    if d == torch.cuda.current_device():
+        fn(*args, torch.cuda.current_stream(d).cuda_stream)
+    else:
+        with torch.cuda.device(d):
+            fn(*args, torch.cuda.current_stream(d).cuda_stream)
+
+
+def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return t.data_ptr() if t is not None else None
+
+
+class LayerNormSaved(NamedTuple):
+    """What layernorm_train keeps for layernorm_bwd: the input x, or its 8-bit
+    checkpoint (q8, q8_exp; include/kt_abi.h has the format), gamma, the rows'
+    statistics, and beta's type (None without beta)."""
+    x: Optional[torch.Tensor]
+    q8: Optional[torch.Tensor]
+    q8_exp: Optional[torch.Tensor]
+    gamma: Optional[torch.Tensor]
+    mean: torch.Tensor
+    rstd: torch.Tensor
+    beta_dtype: Optional[torch.dtype]
+
+
+def layernorm_train(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Optional[torch.Tensor] = None,
+                    eps: float = 1e-5, ckpt8: bool = False,
+                    lib: Optional[kt_lib.KtLibrary] = None) -> tuple[torch.Tensor, LayerNormSaved]:
+    """LayerNorm over the last dim of a 2-D fp32, bf16 or fp16 tensor, and what its backward pass needs.
+
+    gamma and beta (None: 1 and 0) are fp32 or of x's type. With ckpt8 the
+    backward pass gets x in 8 bits (blocks of 32 columns sharing a power of
+    two), so that x itself need not be kept.
+    """
+    dt = _dtype(x, "x")
+    _check(x, "x", x.dtype)
+    if x.dim() != 2:
+        raise ValueError("x must be 2-D (rows, cols)")
+    rows, cols = x.shape
+    wdt = kt_lib.KT_F32
+    for t, n in ((gamma, "gamma"), (beta, "beta")):
+        if t is not None:
+            wdt = _dtype(t, n)
+            _check(t, n, torch.float32 if wdt == kt_lib.KT_F32 else x.dtype)
+            _on_device(t, x, n)
+            if t.numel() != cols:
+                raise ValueError(f"layernorm_train: {n} must have {cols} elements")
+    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
+        raise ValueError("layernorm_train: gamma and beta must be of one type")
+    lib = lib or kt_lib.load()
+    y = torch.empty_like(x)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+    mean, rstd = stats[0], stats[1]
+    q8 = torch.empty((rows, cols), dtype=torch.int8, device=x.device) if ckpt8 else None
+    q8_exp = torch.empty((rows, (cols + 31) // 32), dtype=torch.uint8, device=x.device) if ckpt8 else None
+    _launch(x, lib.layernorm_train_fwd, x.data_ptr(), _ptr(gamma), _ptr(beta), y.data_ptr(), mean.data_ptr(),
+            rstd.data_ptr(), _ptr(q8), _ptr(q8_exp), rows, cols, float(eps), dt, wdt)
+    return y, LayerNormSaved(None if ckpt8 else x, q8, q8_exp, gamma, mean, rstd,
+                             beta.dtype if beta is not None else None)
+
+
+def layernorm_bwd(dy: torch.Tensor, saved: LayerNormSaved, weight_grads: bool = True,
+                  lib: Optional[kt_lib.KtLibrary] = None
+                  ) -> tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """(dx, dgamma, dbeta) of layernorm_train from dy. dgamma and dbeta are of
+    gamma's type and None where gamma or beta was None, or weight_grads is False."""
+    kept = saved.q8 if saved.x is None else saved.x
+    dt = _dtype(dy, "dy")
+    _check(dy, "dy", dy.dtype if saved.x is None else saved.x.dtype)
+    _on_device(dy, kept, "dy")
+    if dy.shape != kept.shape:
+        raise ValueError(f"layernorm_bwd: dy is {tuple(dy.shape)}, the input was {tuple(kept.shape)}")
+    rows, cols = dy.shape
+    gamma = saved.gamma
+    wt = gamma.dtype if gamma is not None else saved.beta_dtype or torch.float32
+    if wt not in (torch.float32, dy.dtype):
+        raise ValueError(f"dy must be {wt}, got {dy.dtype}")
+    wdt = _DTYPES[wt]
+    lib = lib or kt_lib.load()
+    dx = torch.empty_like(dy)
+    dgamma = dbeta = ws = None
+    ws_bytes = 0
+    if weight_grads and (gamma is not None or saved.beta_dtype is not None):
+        dgamma = torch.empty(cols, dtype=wt, device=dy.device) if gamma is not None else None
+        dbeta = torch.empty(cols, dtype=wt, device=dy.device) if saved.beta_dtype is not None else None
+        ws_bytes = lib.layernorm_bwd_workspace_bytes(rows, cols)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device)
+    _launch(dy, lib.layernorm_train_bwd, dy.data_ptr(), _ptr(saved.x), _ptr(saved.q8), _ptr(saved.q8_exp),
+            _ptr(gamma), saved.mean.data_ptr(), saved.rstd.data_ptr(), dx.data_ptr(), _ptr(dgamma), _ptr(dbeta),
+            rows, cols, dt, wdt, _ptr(ws), ws_bytes)
+    return dx, dgamma, dbeta
+
+
+class TokenLogprobs(NamedTuple):
+    """Per row of logits: the target's log probability (None without targets),
+    the entropy (nats), log sum exp, and the top k log probabilities with their columns (int64)."""
+    logprob: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    lse: torch.Tensor
+    top_logprob: torch.Tensor
+    top_index: torch.Tensor
+
+
+def _check_targets(targets: torch.Tensor, logits: torch.Tensor) -> None:
+    _check(targets, "targets", torch.int64)
+    _on_device(targets, logits, "targets")
+    if targets.dim() != 1 or targets.shape[0] != logits.shape[0]:
+        raise ValueError(f"targets must be ({logits.shape[0]},), got {tuple(targets.shape)}")
+
+
+def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top_k: int = 0, scale: float = 1.0,
+                   ignore_index: int = -100, lib: Optional[kt_lib.KtLibrary] = None) -> TokenLogprobs:
+    """Log probabilities of `targets` under softmax(scale * logits), with the
+    entropy and the top_k (up to 32) most likely columns of each row.
+
+    logits: (rows, vocab) fp32, bf16 or fp16, rows any distance apart; targets:
+    (rows,) int64. Rows whose target is ignore_index get log probability 0;
+    other targets that are no column get NaN and set the library's device error.
+    """
+    dt = _dtype(logits, "logits")
+    _rows(logits, "logits")
+    rows, vocab = logits.shape
+    if targets is not None:
+        _check_targets(targets, logits)
+    if not 0 <= top_k <= 32 or (rows and top_k > vocab):
+        raise ValueError(f"top_k must be between 0 and min(32, vocab), got {top_k}")
+    lib = lib or kt_lib.load()
+    dev = logits.device
+    stats = torch.empty((3, rows), dtype=torch.float32, device=dev)
+    logprob, entropy, lse = stats.unbind(0)
+    top_logprob = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    top_index = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
+    _launch(logits, lib.token_logprobs, logits.data_ptr(), _ld(logits), _ptr(targets), rows, vocab, float(scale),
+            ignore_index, top_k, logprob.data_ptr(), entropy.data_ptr(), lse.data_ptr(), top_logprob.data_ptr(),
+            top_index.data_ptr(), dt)
+    return TokenLogprobs(logprob if targets is not None else None, entropy, lse, top_logprob, top_index)
+
+
+def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], result: TokenLogprobs,
+                       grad_logprob: Optional[torch.Tensor] = None, grad_entropy: Optional[torch.Tensor] = None,
+                       scale: float = 1.0, ignore_index: int = -100, out: Optional[torch.Tensor] = None,
+                       lib: Optional[kt_lib.KtLibrary] = None) -> torch.Tensor:
+    """Gradient of the logits from those of the log probabilities and the
+    entropies (fp32, (rows,); None: 0); result, scale and ignore_index are those
+    of token_logprobs. `out` may be the logits themselves."""
+    dt = _dtype(logits, "logits")
+    _rows(logits, "logits")
+    rows, vocab = logits.shape
+    for t, n in ((grad_logprob, "grad_logprob"), (grad_entropy, "grad_entropy"), (result.lse, "result.lse"),
+                 (result.entropy, "result.entropy")):
+        if t is not None:
+            _check(t, n, torch.float32)
+            _on_device(t, logits, n)
+            if t.dim() != 1 or t.shape[0] != rows:
+                raise ValueError(f"{n} must be ({rows},), got {tuple(t.shape)}")
+    if targets is not None:
+        _check_targets(targets, logits)
+    elif grad_logprob is not None:
+        raise ValueError("grad_logprob needs targets")
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+    else:
+        _rows(out, "out")
+        _on_device(out, logits, "out")
+        if out.shape != logits.shape or out.dtype != logits.dtype:
+            raise ValueError(f"out must be {tuple(logits.shape)} {logits.dtype}")
+        if rows > 1 and out.stride(0) < vocab:
+            raise ValueError("out: rows overlap")
+    lib = lib or kt_lib.load()
+    _launch(logits, lib.token_logprobs_bwd, logits.data_ptr(), _ld(logits), _ptr(targets), result.lse.data_ptr(),
+            result.entropy.data_ptr(), _ptr(grad_logprob), _ptr(grad_entropy), rows, vocab, float(scale),
+            ignore_index, out.data_ptr(), _ld(out), dt)
+    return out
+
+
+class W4Weight(NamedTuple):
+    """An (N, K) matrix of 4-bit weights: packed (N, K/2) uint8, the even column
+    in the low half of a byte; scales (N, K/group); zeros (N, K/group) uint8
+    with values of 0..15, or None for 8. A weight is scale * (q - zero)."""
+    packed: torch.Tensor
+    scales: torch.Tensor
+    zeros: Optional[torch.Tensor] = None
+    group: int = 128
+
+
+def w4_quantize(weight: torch.Tensor, group: int = 128, scale_dtype: Optional[torch.dtype] = None,
+                lib: Optional[kt_lib.KtLibrary] = None) -> W4Weight:
+    """An (N, K) fp32, bf16 or fp16 matrix as symmetric 4-bit weights with one
+    scale (of scale_dtype, default the matrix's type) per `group` (32, 64 or 128) columns."""
+    dt = _dtype(weight, "weight")
+    _check(weight, "weight", weight.dtype)
+    if weight.dim() != 2:
+        raise ValueError("weight must be 2-D (N, K)")
+    N, K = weight.shape
+    if group not in (32, 64, 128) or K % group:
+        raise ValueError(f"group must be 32, 64 or 128 and divide K={K}, got {group}")
+    lib = lib or kt_lib.load()
+    packed = torch.empty((N, K // 2), dtype=torch.uint8, device=weight.device)
+    scales = torch.empty((N, K // group), dtype=scale_dtype or weight.dtype, device=weight.device)
+    _launch(weight, lib.w4_quantize, weight.data_ptr(), N, K, group, dt, packed.data_ptr(), scales.data_ptr(),
+            _dtype(scales, "scales"))
+    return W4Weight(packed, scales, None, group)
+
+
+def w4_linear(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None, lib: Optional[kt_lib.KtLibrary] = None) -> torch.Tensor:
+    """y = x w^T + bias for a few tokens x (M, K), fp32, bf16 or fp16, with 4-bit weights."""
+    packed, scales, zeros, group = weight
+    dt = _dtype(x, "x")
+    _rows(x, "x")
+    M, K = x.shape
+    _check(packed, "packed", torch.uint8)
+    _check(scales, "scales", scales.dtype)
+    if packed.dim() != 2 or packed.shape[1] * 2 != K:
+        raise ValueError(f"w4_linear: packed must be (N, {K // 2}), got {tuple(packed.shape)}")
+    N = packed.shape[0]
+    if group not in (32, 64, 128) or K % group:
+        raise ValueError(f"group must be 32, 64 or 128 and divide K={K}, got {group}")
+    per = (N, K // group)
+    if scales.shape != per:
+        raise ValueError(f"w4_linear: scales must be {per}, got {tuple(scales.shape)}")
+    _on_device(packed, x, "packed")
+    _on_device(scales, x, "scales")
+    if zeros is not None:
+        _check(zeros, "zeros", torch.uint8)
+        _on_device(zeros, x, "zeros")
+        if zeros.shape != per:
+            raise ValueError(f"w4_linear: zeros must be {per}, got {tuple(zeros.shape)}")
+    if bias is not None:
+        _check(bias, "bias", x.dtype)
+        _on_device(bias, x, "bias")
+        if bias.numel() != N:
+            raise ValueError(f"w4_linear: bias must have {N} elements")
+    if out is None:
+        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    else:
+        _check(out, "out", x.dtype)
+        _on_device(out, x, "out")
+        if out.shape != (M, N):
+            raise ValueError(f"out must be {(M, N)}, got {tuple(out.shape)}")
+    lib = lib or kt_lib.load()
+    _launch(x, lib.w4_linear, x.data_ptr(), _ld(x), packed.data_ptr(), scales.data_ptr(), _ptr(zeros), _ptr(bias),
+            out.data_ptr(), N, M, N, K, group, dt, _dtype(scales, "scales"))
+    return out

@@ -71,6 +71,13 @@ enum {
   KT_OP_NAIVE_ATTENTION = 105
 };
 
+/* Element types of the operators that take several (`dtype`). */
+enum {
+  KT_F32 = 0,
+  KT_BF16 = 1,
+  KT_F16 = 2
+};
+
 /* Generic argument block for kt_run / kt_time. Field meaning per op:
  *   SOFTMAX    in0=x           out0=y         d0=rows d1=cols
  *   LAYERNORM  in0=x in1=gamma in2=beta out0=y d0=rows d1=cols f0=eps
@@ -186,6 +193,76 @@ KT_API int kt_gemm_f32(const float* A, const float* B, float* C, int64_t M, int6
 KT_API int kt_fa_fwd_bf16(const uint16_t* Q, const uint16_t* K, const uint16_t* V, uint16_t* O,
                    int64_t B, int64_t H, int64_t S, int64_t D, float scale, int causal,
                    kt_stream_t stream);
+
+/* The operators below take fp32, bf16 or fp16 tensors (`dtype`); sums and
+ * statistics are fp32 and each output is rounded once. They belong to the
+ * default library; tuning variants return KT_ERR_UNSUPPORTED. None has a
+ * counterpart in the reference, whose kernels run forward in fp32 only. */
+
+/* LayerNorm over the last dim for training: y = gamma*(x-mean)*rstd + beta with
+ * rstd = 1/sqrt(var+eps), biased variance, and mean, rstd (fp32, `rows` each)
+ * saved for the backward pass. gamma and beta (may be NULL: 1 and 0) are of
+ * `wdtype`, fp32 or the input's type.
+ * With q8 and q8_exp (both or neither), an 8-bit checkpoint of x is written
+ * too: q8 is rows x cols, q8_exp rows x ceil(cols/32). Each block of 32 columns
+ * has E = the exponent field of its largest magnitude as fp32, at least 7 (255:
+ * the block holds an infinity or NaN and stands for NaN), and
+ * q = x * 2^(133-E) rounded to nearest even, limited to +-127, standing for
+ * q * 2^(E-133). */
+KT_API int kt_layernorm_train_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean,
+                                  float* rstd, int8_t* q8, uint8_t* q8_exp, int64_t rows, int64_t cols, float eps,
+                                  int dtype, int wdtype, kt_stream_t stream);
+
+/* Bytes of device scratch kt_layernorm_train_bwd needs for dgamma and dbeta. */
+KT_API size_t kt_layernorm_bwd_workspace_bytes(int64_t rows, int64_t cols);
+
+/* Its backward pass: dx, and dgamma, dbeta (of `wdtype`, either may be NULL)
+ * summed over the rows in a fixed order. Takes x or its 8-bit checkpoint (then
+ * x is NULL). `workspace` (kt_layernorm_bwd_workspace_bytes, 16-byte aligned,
+ * any content) is caller-owned scratch, not needed without dgamma and dbeta;
+ * calls that may overlap need one each. */
+KT_API int kt_layernorm_train_bwd(const void* dy, const void* x, const int8_t* q8, const uint8_t* q8_exp,
+                                  const void* gamma, const float* mean, const float* rstd, void* dx, void* dgamma,
+                                  void* dbeta, int64_t rows, int64_t cols, int dtype, int wdtype, void* workspace,
+                                  size_t ws_bytes, kt_stream_t stream);
+
+/* Per row of logits (`vocab` columns, rows `ld` elements apart), with
+ * z = scale*logits, scale > 0: lse = log(sum(exp(z))); logprob = z[target]-lse
+ * (0 where target == ignore_index; NaN where it is no column, and
+ * kt_device_error reports 2); entropy in nats; the top_k (0..32, <= vocab)
+ * largest log probabilities in order with their columns, rows x top_k, equal
+ * ones by lower column, NaN first. A row of only -inf has lse and log
+ * probabilities of -inf and entropy 0. targets (with logprob) and entropy may
+ * be NULL. */
+KT_API int kt_token_logprobs(const void* logits, int64_t ld, const int64_t* targets, int64_t rows, int64_t vocab,
+                             float scale, int64_t ignore_index, int top_k, float* logprob, float* entropy, float* lse,
+                             float* top_logprob, int64_t* top_index, int dtype, kt_stream_t stream);
+
+/* Gradient of the logits from those of logprob and entropy (either may be
+ * NULL: 0); lse and entropy are kt_token_logprobs'. Rows whose two gradients
+ * are 0, and rows of only -inf, get 0. dlogits (rows `ld_dlogits` apart) may be
+ * the logits themselves. */
+KT_API int kt_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* targets, const float* lse,
+                                 const float* entropy, const float* grad_logprob, const float* grad_entropy,
+                                 int64_t rows, int64_t vocab, float scale, int64_t ignore_index, void* dlogits,
+                                 int64_t ld_dlogits, int dtype, kt_stream_t stream);
+
+/* 4-bit weights: w (N x K) in groups of `group` (32, 64 or 128, a divisor of K)
+ * columns as q in 0..15, two to a byte (`packed`, N x K/2, the even column in
+ * the low half), and scales (N x K/group, of scale_dtype: any of the three),
+ * standing for s*(q-8). Quantises symmetrically: s = max|w|/7 of the group,
+ * q = 8 + w/s to nearest even; a group that is not finite gets the scale NaN. */
+KT_API int kt_w4_quantize(const void* w, int64_t N, int64_t K, int group, int dtype, uint8_t* packed, void* scales,
+                          int scale_dtype, kt_stream_t stream);
+
+/* y = x * w^T + bias for M tokens (x: M x K, y: M x N, rows ldx and ldy elements
+ * apart) with 4-bit weights standing for s*(q-z); zeros (N x K/group, values of
+ * 0..15) may be NULL: 8; bias (N, of `dtype`) may be NULL. Made for few tokens:
+ * the weights are read once for every 16. A group's sum of x*(q-z) is fp32 and
+ * scaled afterwards, so it must not overflow. `packed` is 16-byte aligned. */
+KT_API int kt_w4_linear(const void* x, int64_t ldx, const uint8_t* packed, const void* scales, const uint8_t* zeros,
+                        const void* bias, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int group, int dtype,
+                        int scale_dtype, kt_stream_t stream);
 
 /* Naive GPU baselines (one thread per row / per output element) used as the
  * Welch-t reference point, restating the algorithms of
