@@ -82,16 +82,54 @@ __device__ __forceinline__ int quant8(float v, float up) {
 }
 
 // ---------------------------------------------------------------- row pieces
-// Columns [e0, e0+V) of a row as raw 16 bytes; columns outside [0, cols) are 0.
-// `row + e0` lies on a 16-byte boundary.
+// A value that the compiler takes for a new one: what is computed from it is
+// not kept in registers across the rows. (Only a row's first and last piece need
+// those computations, and holding them for all pieces costs more registers than
+// the data.)
+__device__ __forceinline__ int opaque(int v) {
+  asm volatile("" : "+r"(v));
+  return v;
+}
+
+// `raw` with the columns outside [0, cols) as 0.
 template <typename T>
-__device__ __forceinline__ uint4 load_piece(const T* row, int e0, int cols) {
-  constexpr int V = elem::kVec<T>;
-  if (e0 >= 0 && e0 + V <= cols) return elem::ld_once16(row + e0);
-  float f[V];
+__device__ __forceinline__ uint4 masked(const uint4& raw, int e0, int cols) {
+  uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-  for (int j = 0; j < V; ++j) f[j] = (e0 + j >= 0 && e0 + j < cols) ? elem::to_f(row[e0 + j]) : 0.f;
-  return elem::pack_vec<T>(f);
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (sizeof(T) == 4) {
+      if (e0 + k < 0 || e0 + k >= cols) w[k] = 0;
+    } else {
+      if (e0 + 2 * k < 0 || e0 + 2 * k >= cols) w[k] &= 0xFFFF0000u;
+      if (e0 + 2 * k + 1 < 0 || e0 + 2 * k + 1 >= cols) w[k] &= 0x0000FFFFu;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Columns [e0, e0+V) of row `row` as raw 16 bytes; columns outside [0, cols) are
+// 0. They lie on a 16-byte boundary. A piece that a row's end cuts also holds
+// its neighbour's columns; only at the tensor's two ends may those not be there.
+template <typename T>
+__device__ __forceinline__ uint4 load_piece(const T* x, int64_t row, int64_t rows, int e0, int cols) {
+  constexpr int V = elem::kVec<T>;
+  const int64_t at = row * cols + e0;
+  if (e0 >= 0 && e0 + V <= cols) return elem::ld_once16(x + at);
+  const int e = opaque(e0);
+  if (e >= cols) return make_uint4(0, 0, 0, 0);
+  if (at >= 0 && at + V <= rows * cols) return masked<T>(elem::ld_once16(x + at), e, cols);
+  uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+  for (int j = 0; j < V; ++j) {
+    if (e + j < 0 || e + j >= cols) continue;
+    uint64_t bits;
+    if constexpr (sizeof(T) == 4) bits = reinterpret_cast<const uint32_t*>(x)[at + j];
+    else bits = reinterpret_cast<const uint16_t*>(x)[at + j];
+    bits <<= (j % (V / 2)) * 8 * (int)sizeof(T);
+    if (j < V / 2) lo |= bits;
+    else hi |= bits;
+  }
+  return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
 }
 
 template <typename T>
@@ -101,22 +139,37 @@ __device__ __forceinline__ void store_piece(T* row, int e0, int cols, const floa
     *reinterpret_cast<uint4*>(row + e0) = elem::pack_vec<T>(f);
     return;
   }
+  const int e = opaque(e0);
 #pragma unroll
   for (int j = 0; j < V; ++j)
-    if (e0 + j >= 0 && e0 + j < cols) row[e0 + j] = elem::from_f<T>(f[j]);
+    if (e + j >= 0 && e + j < cols) row[e + j] = elem::from_f<T>(f[j]);
 }
 
-// Sum over the TPR threads of a row; every thread gets it. `scratch` holds
-// TPR/32 values; two calls in a row need different scratch.
+// Rows of a CTA at a time, and its threads: rows of up to 64 threads share a CTA.
+template <int TPR>
+constexpr int kRows = TPR < 128 ? 128 / TPR : 1;
+template <int TPR>
+constexpr int kThreads = TPR * kRows<TPR>;
+
+constexpr int kFwdThreads = 768, kBwdThreads = 512;
+// Waits for the TPR threads of this row.
+template <int TPR>
+__device__ __forceinline__ void row_sync() {
+  if constexpr (kRows<TPR> == 1) __syncthreads();
+  else asm volatile("bar.sync %0, %1;" ::"r"(1 + (int)threadIdx.x / TPR), "n"(TPR) : "memory");
+}
+
+// Sum over the TPR threads of a row; every thread gets it. `scratch` holds a
+// value per warp of the CTA; two calls in a row need different scratch.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* scratch) {
   v = warp_sum(v);
   if constexpr (TPR > 32) {
     constexpr int NW = TPR / 32;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, row0 = threadIdx.x / TPR * NW;
     if (lane == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = warp_sum(lane < NW ? scratch[lane] : 0.f);
+    row_sync<TPR>();
+    v = warp_sum(lane < NW ? scratch[row0 + lane] : 0.f);
   }
   return v;
 }
@@ -127,55 +180,71 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float2* scratch) {
   b = warp_sum(b);
   if constexpr (TPR > 32) {
     constexpr int NW = TPR / 32;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, row0 = threadIdx.x / TPR * NW;
     if (lane == 0) scratch[threadIdx.x >> 5] = make_float2(a, b);
-    __syncthreads();
-    const float2 s = lane < NW ? scratch[lane] : make_float2(0.f, 0.f);
+    row_sync<TPR>();
+    const float2 s = lane < NW ? scratch[row0 + lane] : make_float2(0.f, 0.f);
     a = warp_sum(s.x);
     b = warp_sum(s.y);
   }
   return make_float2(a, b);
 }
 
+// Weights of columns [e0, e0 + V); `other` where there are none.
+template <typename T>
+__device__ __forceinline__ void load_weights(const void* w, int wdtype, int e0, int cols, float other,
+                                             float (&f)[elem::kVec<T>]) {
+  constexpr int V = elem::kVec<T>;
+  const char* at = static_cast<const char*>(w) + (int64_t)e0 * (wdtype == KT_F32 ? 4 : 2);
+  if (w != nullptr && e0 >= 0 && e0 + V <= cols && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
+    if (wdtype == KT_F32) {
+#pragma unroll
+      for (int k = 0; k < V / 4; ++k) {
+        const float4 v = reinterpret_cast<const float4*>(at)[k];
+        f[4 * k] = v.x; f[4 * k + 1] = v.y; f[4 * k + 2] = v.z; f[4 * k + 3] = v.w;
+      }
+    } else if constexpr (sizeof(T) == 2) {
+      elem::unpack_vec<T>(*reinterpret_cast<const uint4*>(at), f);
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    f[j] = w != nullptr && e0 + j >= 0 && e0 + j < cols ? elem::ld_weight(w, wdtype, e0 + j) : other;
+}
+
 // ---------------------------------------------------------------- forward
 template <typename T, int TPR, int VPT, bool CKPT>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR)
+__global__ void __launch_bounds__(kThreads<TPR>, kFwdThreads / kThreads<TPR>)
 fwd_rows(const FwdArgs p) {
   constexpr int V = elem::kVec<T>;
-  constexpr int RB = TPR == 32 ? 8 : 1;  // rows of a CTA at a time
   __shared__ float red[2][32];
   const int t = threadIdx.x % TPR;
   const int cols = (int)p.cols;
   const float fcols = (float)cols;
-  const int64_t first = (int64_t)blockIdx.x * RB + threadIdx.x / TPR;
-  const int64_t stride = (int64_t)gridDim.x * RB;
+  const int64_t first = (int64_t)blockIdx.x * kRows<TPR> + threadIdx.x / TPR;
+  const int64_t stride = (int64_t)gridDim.x * kRows<TPR>;
   const int shift = elem::misalign<T>(static_cast<const T*>(p.x) + first * cols);
-  float g[VPT][V], b[VPT][V];
-#pragma unroll
-  for (int i = 0; i < VPT; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int e = (t + i * TPR) * V - shift + j;
-      const bool in = e >= 0 && e < cols;
-      g[i][j] = in && p.gamma ? elem::ld_weight(p.gamma, p.wdtype, e) : 1.f;
-      b[i][j] = in && p.beta ? elem::ld_weight(p.beta, p.wdtype, e) : 0.f;
-    }
-  uint4 next[VPT];
+  const int e_first = t * V - shift;  // this thread's pieces start at e_first + i TPR V
+  uint4 raw[VPT];
   auto fetch = [&](int64_t row) {
-    const T* xr = static_cast<const T*>(p.x) + row * cols;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int e0 = (t + i * TPR) * V - shift;
-      next[i] = e0 < cols ? load_piece<T>(xr, e0, cols) : make_uint4(0, 0, 0, 0);
-    }
+    for (int i = 0; i < VPT; ++i)
+      raw[i] = load_piece<T>(static_cast<const T*>(p.x), row, p.rows, e_first + i * TPR * V, cols);
   };
   if (first < p.rows) fetch(first);
+  float g[VPT][V], b[VPT][V];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    load_weights<T>(p.gamma, p.wdtype, e_first + i * TPR * V, cols, 1.f, g[i]);
+    load_weights<T>(p.beta, p.wdtype, e_first + i * TPR * V, cols, 0.f, b[i]);
+  }
   for (int64_t row = first; row < p.rows; row += stride) {
     float v[VPT][V];
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      elem::unpack_vec<T>(next[i], v[i]);
+      elem::unpack_vec<T>(raw[i], v[i]);
 #pragma unroll
       for (int j = 0; j < V; ++j) s += v[i][j];
     }
@@ -183,13 +252,18 @@ fwd_rows(const FwdArgs p) {
     const float mean = row_sum<TPR>(s, red[0]) / fcols;
     float q = 0.f;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
+    for (int i = 0; i < VPT; ++i) {
+      const int e0 = e_first + i * TPR * V;
+      if (e0 >= 0 && e0 + V <= cols) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int e = (t + i * TPR) * V - shift + j;
-        const float d = v[i][j] - mean;
-        if (e >= 0 && e < cols) q = fmaf(d, d, q);
+        for (int j = 0; j < V; ++j) q = fmaf(v[i][j] - mean, v[i][j] - mean, q);
+      } else {  // a piece that the row's end cuts, or none of it in the row
+        const int e = opaque(e0);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (e + j >= 0 && e + j < cols) q = fmaf(v[i][j] - mean, v[i][j] - mean, q);
       }
+    }
     const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red[1]) / fcols + p.eps);
     if (t == 0) {
       p.mean[row] = mean;
@@ -198,8 +272,7 @@ fwd_rows(const FwdArgs p) {
     T* yr = static_cast<T*>(p.y) + row * cols;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = t + i * TPR;
-      const int e0 = c * V - shift;
+      const int e0 = e_first + i * TPR * V;
       if constexpr (CKPT) {
         constexpr int LPB = 32 / V;  // lanes that share a block of 32 columns
         uint32_t top = 0;
@@ -220,7 +293,7 @@ fwd_rows(const FwdArgs p) {
           int8_t* qr = p.q8 + row * cols + e0;
           if constexpr (V == 8) *reinterpret_cast<uint2*>(qr) = make_uint2(w[0], w[1]);
           else *reinterpret_cast<uint32_t*>(qr) = w[0];
-          if (c % LPB == 0) p.q8_exp[row * ((cols + 31) / 32) + c / LPB] = (uint8_t)code;
+          if (t % LPB == 0) p.q8_exp[row * ((cols + 31) / 32) + e0 / 32] = (uint8_t)code;
         }
       }
       if (e0 < cols) {
@@ -273,11 +346,31 @@ __global__ void __launch_bounds__(256) fwd_any(const FwdArgs p) {
 }
 
 // ---------------------------------------------------------------- backward
+// A piece of xh from x, or from its 8-bit checkpoint (.x, .y: eight values, .z:
+// the block's code).
+template <typename T, bool CKPT>
+__device__ __forceinline__ void x_hats(const uint4& raw, float mean, float rstd, float (&xh)[elem::kVec<T>]) {
+  constexpr int V = elem::kVec<T>;
+  if constexpr (CKPT) {
+    const float down = code_down(raw.z);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const uint32_t word = j < 4 ? raw.x : raw.y;
+      xh[j] = (fmaf((float)(int8_t)(word >> (8 * (j & 3))), down, -mean)) * rstd;  // the product is exact
+    }
+  } else {
+    elem::unpack_vec<T>(raw, xh);
+#pragma unroll
+    for (int j = 0; j < V; ++j) xh[j] = (xh[j] - mean) * rstd;
+  }
+}
+
+// Columns outside the row have dy = 0, so they add nothing to any sum.
 template <typename T, int TPR, int VPT, bool CKPT>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR)
+__global__ void __launch_bounds__(kThreads<TPR>, kBwdThreads / kThreads<TPR>)
 bwd_rows(const BwdArgs p) {
   constexpr int V = elem::kVec<T>;
-  constexpr int RB = TPR == 32 ? 8 : 1;
+  constexpr int RB = kRows<TPR>;
   extern __shared__ float part[];  // RB > 1: 2 x cols sums of the CTA
   __shared__ float2 red[2][32];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
@@ -286,29 +379,19 @@ bwd_rows(const BwdArgs p) {
   const int64_t first = (int64_t)blockIdx.x * RB + sub;
   const int64_t stride = (int64_t)gridDim.x * RB;
   const int shift = elem::misalign<T>(static_cast<const T*>(p.dy) + first * cols);
-  float g[VPT][V], dg[VPT][V], db[VPT][V];
-#pragma unroll
-  for (int i = 0; i < VPT; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int e = (t + i * TPR) * V - shift + j;
-      g[i][j] = e >= 0 && e < cols && p.gamma ? elem::ld_weight(p.gamma, p.wdtype, e) : 1.f;
-      dg[i][j] = db[i][j] = 0.f;
-    }
-  uint4 ny[VPT], nx[VPT];  // of nx, 8-bit checkpoints use .x and .y, and .z for the block's code
+  const int e_first = t * V - shift;
+  uint4 ny[VPT], nx[VPT];
   float nmean = 0.f, nrstd = 0.f;
   auto fetch = [&](int64_t row) {
-    const T* dyr = static_cast<const T*>(p.dy) + row * cols;
     nmean = p.mean[row];
     nrstd = p.rstd[row];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int c = t + i * TPR;
-      const int e0 = c * V - shift;
-      ny[i] = nx[i] = make_uint4(0, 0, 0, 0);
-      if (e0 < cols) {
-        ny[i] = load_piece<T>(dyr, e0, cols);
-        if constexpr (CKPT) {
+      const int e0 = e_first + i * TPR * V;
+      ny[i] = load_piece<T>(static_cast<const T*>(p.dy), row, p.rows, e0, cols);
+      if constexpr (CKPT) {
+        nx[i] = make_uint4(0, 0, 7, 0);
+        if (e0 < cols) {
           const int8_t* qr = p.q8 + row * cols + e0;
           if constexpr (V == 8) {
             const uint2 w = *reinterpret_cast<const uint2*>(qr);
@@ -317,57 +400,59 @@ bwd_rows(const BwdArgs p) {
           } else {
             nx[i].x = *reinterpret_cast<const uint32_t*>(qr);
           }
-          nx[i].z = p.q8_exp[row * ((cols + 31) / 32) + c / (32 / V)];
-        } else {
-          nx[i] = load_piece<T>(static_cast<const T*>(p.x) + row * cols, e0, cols);
+          nx[i].z = p.q8_exp[row * ((cols + 31) / 32) + e0 / 32];
         }
+      } else {
+        nx[i] = load_piece<T>(static_cast<const T*>(p.x), row, p.rows, e0, cols);
       }
     }
   };
   if (first < p.rows) fetch(first);
+  float g[VPT][V], dg[VPT][V], db[VPT][V];
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    load_weights<T>(p.gamma, p.wdtype, e_first + i * TPR * V, cols, 1.f, g[i]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) dg[i][j] = db[i][j] = 0.f;
+  }
   int turn = 0;
   for (int64_t row = first; row < p.rows; row += stride, turn ^= 1) {
-    float xh[VPT][V], w[VPT][V];
+    uint4 ry[VPT], rx[VPT];
     float s1 = 0.f, s2 = 0.f;
     const float mean = nmean, rstd = nrstd;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int e0 = (t + i * TPR) * V - shift;
-      if constexpr (CKPT) {
-        const float down = code_down(e0 < cols ? nx[i].z : 7u);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const uint32_t word = j < 4 ? nx[i].x : nx[i].y;
-          xh[i][j] = (float)(int8_t)(word >> (8 * (j & 3))) * down;
-        }
-      } else {
-        elem::unpack_vec<T>(nx[i], xh[i]);
-      }
-      float d[V];
-      elem::unpack_vec<T>(ny[i], d);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const bool in = e0 + j >= 0 && e0 + j < cols;
-        xh[i][j] = in ? (xh[i][j] - mean) * rstd : 0.f;
-        dg[i][j] = fmaf(d[j], xh[i][j], dg[i][j]);
-        db[i][j] += d[j];
-        w[i][j] = d[j] * g[i][j];
-        s1 = fmaf(w[i][j], xh[i][j], s1);
-        s2 += w[i][j];
-      }
+      ry[i] = ny[i];
+      rx[i] = nx[i];
     }
     if (row + stride < p.rows) fetch(row + stride);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float d[V], xh[V];
+      elem::unpack_vec<T>(ry[i], d);
+      x_hats<T, CKPT>(rx[i], mean, rstd, xh);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        dg[i][j] = fmaf(d[j], xh[j], dg[i][j]);
+        db[i][j] += d[j];
+        const float w = d[j] * g[i][j];
+        s1 = fmaf(w, xh[j], s1);
+        s2 += w;
+      }
+    }
     const float2 s = row_sum2<TPR>(s1, s2, red[turn]);
     const float c1 = s.x / fcols, c2 = s.y / fcols;
     T* dxr = static_cast<T*>(p.dx) + row * cols;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      const int e0 = (t + i * TPR) * V - shift;
+      const int e0 = e_first + i * TPR * V;
       if (e0 < cols) {
-        float o[V];
+        float d[V], xh[V];  // once more from the 16 bytes: holding them would cost twice the registers
+        elem::unpack_vec<T>(ry[i], d);
+        x_hats<T, CKPT>(rx[i], mean, rstd, xh);
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = rstd * (w[i][j] - c2 - xh[i][j] * c1);
-        store_piece<T>(dxr, e0, cols, o);
+        for (int j = 0; j < V; ++j) d[j] = rstd * (fmaf(d[j], g[i][j], -c2) - xh[j] * c1);
+        store_piece<T>(dxr, e0, cols, d);
       }
     }
   }
@@ -375,32 +460,32 @@ bwd_rows(const BwdArgs p) {
   float* out = p.partial + (int64_t)blockIdx.x * 2 * cols;
   if constexpr (RB == 1) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
+    for (int i = 0; i < VPT; ++i) {
+      const int e0 = e_first + i * TPR * V;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int e = (t + i * TPR) * V - shift + j;
-        if (e >= 0 && e < cols) {
-          out[e] = dg[i][j];
-          out[cols + e] = db[i][j];
+      for (int j = 0; j < V; ++j)
+        if (e0 + j >= 0 && e0 + j < cols) {
+          out[e0 + j] = dg[i][j];
+          out[cols + e0 + j] = db[i][j];
         }
-      }
+    }
   } else {
-    for (int w = 0; w < RB; ++w) {  // in the order of the warps
+    for (int w = 0; w < RB; ++w) {  // in the order of the rows
       if (sub == w) {
 #pragma unroll
-        for (int i = 0; i < VPT; ++i)
+        for (int i = 0; i < VPT; ++i) {
+          const int e0 = e_first + i * TPR * V;
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const int e = (t + i * TPR) * V - shift + j;
-            if (e >= 0 && e < cols) {
-              part[e] = w ? part[e] + dg[i][j] : dg[i][j];
-              part[cols + e] = w ? part[cols + e] + db[i][j] : db[i][j];
+          for (int j = 0; j < V; ++j)
+            if (e0 + j >= 0 && e0 + j < cols) {
+              part[e0 + j] = w ? part[e0 + j] + dg[i][j] : dg[i][j];
+              part[cols + e0 + j] = w ? part[cols + e0 + j] + db[i][j] : db[i][j];
             }
-          }
+        }
       }
       __syncthreads();
     }
-    for (int e = threadIdx.x; e < 2 * cols; e += 256) out[e] = part[e];
+    for (int e = threadIdx.x; e < 2 * cols; e += kThreads<TPR>) out[e] = part[e];
   }
 }
 
@@ -489,8 +574,8 @@ inline size_t workspace_bytes(int64_t rows, int64_t cols) {
 }
 
 // CTAs for `rows`: what the device holds at once, at most one per `rb` rows and
-// kMaxParts; a multiple of 8 where a CTA has several rows, so that rows `grid`
-// apart start at equal offsets within 16 bytes.
+// kMaxParts; a multiple of 8 where a CTA has several turns, so that its rows
+// start at equal offsets within 16 bytes.
 template <class K>
 inline int row_grid(K kern, int block, int rb, size_t smem, int64_t rows, int* grid) {
   int per_sm = 0;
@@ -505,15 +590,20 @@ inline int row_grid(K kern, int block, int rb, size_t smem, int64_t rows, int* g
   return KT_OK;
 }
 
-// Calls f with the smallest (threads per row, pieces per thread) that holds a
-// row of `pieces` 16-byte pieces; false when none does.
-template <class F>
+// Calls f with the threads per row and pieces per thread for a row of `pieces`
+// 16-byte pieces: 16 columns per thread, which leaves two to three CTAs of
+// 256 threads per SM their registers. False when a row is too wide.
+template <typename T, class F>
 inline bool with_shape(int64_t pieces, F f) {
-  if (pieces <= 32) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{}), true;
-  if (pieces <= 128) return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 4>{}), true;
-  if (pieces <= 512) return f(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{}), true;
-  if (pieces <= 1024) return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{}), true;
-  if (pieces <= 2048) return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{}), true;
+  constexpr int VPT = 16 / elem::kVec<T>;
+  using One = std::integral_constant<int, 1>;
+  using All = std::integral_constant<int, VPT>;
+  if (pieces <= 32) return f(std::integral_constant<int, 32>{}, One{}), true;
+  if (pieces <= 32 * VPT) return f(std::integral_constant<int, 32>{}, All{}), true;
+  if (pieces <= 64 * VPT) return f(std::integral_constant<int, 64>{}, All{}), true;
+  if (pieces <= 128 * VPT) return f(std::integral_constant<int, 128>{}, All{}), true;
+  if (pieces <= 256 * VPT) return f(std::integral_constant<int, 256>{}, All{}), true;
+  if (pieces <= 512 * VPT) return f(std::integral_constant<int, 512>{}, All{}), true;
   return false;
 }
 
@@ -535,9 +625,9 @@ inline int fwd_typed(const FwdArgs& a, cudaStream_t st) {
   if (CKPT) fast = fast && shift == 0 && a.cols % V == 0 && elem::aligned_to(a.q8, V);
   const int64_t pieces = (a.cols + V - 1) / V + (a.cols % V || shift ? 1 : 0);
   int rc = KT_OK;
-  if (fast && with_shape(pieces, [&](auto tpr, auto vpt) {
+  if (fast && with_shape<T>(pieces, [&](auto tpr, auto vpt) {
         constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
-        constexpr int RB = TPR == 32 ? 8 : 1, BLOCK = TPR == 32 ? 256 : TPR;
+        constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
         auto kern = fwd_rows<T, TPR, VPT, CKPT>;
         int grid = 0;
         rc = row_grid(kern, BLOCK, RB, 0, a.rows, &grid);
@@ -577,9 +667,9 @@ inline int bwd_typed(const BwdArgs& a, void* dgamma, void* dbeta, cudaStream_t s
   else fast = fast && elem::misalign<T>(a.x) == shift;
   const int64_t pieces = (a.cols + V - 1) / V + (a.cols % V || shift ? 1 : 0);
   int rc = KT_OK, parts = 0;
-  if (!(fast && with_shape(pieces, [&](auto tpr, auto vpt) {
+  if (!(fast && with_shape<T>(pieces, [&](auto tpr, auto vpt) {
           constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
-          constexpr int RB = TPR == 32 ? 8 : 1, BLOCK = TPR == 32 ? 256 : TPR;
+          constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
           auto kern = bwd_rows<T, TPR, VPT, CKPT>;
           const size_t smem = RB > 1 ? 2 * (size_t)a.cols * sizeof(float) : 0;
           rc = row_grid(kern, BLOCK, RB, smem, a.rows, &parts);

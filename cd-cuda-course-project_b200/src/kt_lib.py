@@ -279,6 +279,7 @@ class KtLibrary:
 
 
 _CACHE: dict[str, KtLibrary] = {}
+_DEFAULT: dict[Optional[str], KtLibrary] = {}  # by KT_LIBRARY: what load() without a path returned
 _LOCK = threading.Lock()
 
 
@@ -289,7 +290,14 @@ def default_library_path() -> Path:
 
 def load(path: Optional[os.PathLike | str] = None) -> KtLibrary:
     """Load (once per path) and return a kernel library; raises if it is missing."""
-    p = Path(path) if path is not None else default_library_path()
+    if path is None:
+        # resolving the path costs 18 us, several times a small kernel
+        env = os.environ.get("KT_LIBRARY")
+        lib = _DEFAULT.get(env)
+        if lib is None:
+            lib = _DEFAULT[env] = load(default_library_path())
+        return lib
+    p = Path(path)
     key = str(p.resolve()) if p.exists() else str(p)
     with _LOCK:
         lib = _CACHE.get(key)
