@@ -13,16 +13,17 @@
 // so are its products with x; the scale multiplies each group's fp32 sum. fp32
 // tokens are split exactly into three bf16 parts.
 //
-// A warp takes 16 rows and segments of 128 columns: each lane loads 16 bytes
-// (32 weights) of two rows, which are four words of each row, for eight
-// m16n8k16 steps. The columns a step covers can be any 16 as long as x has the
-// same order, so no weight is moved between lanes for groups of 128. For
-// smaller groups the four lanes of a row transpose their 4x4 words first, so
-// that each word index belongs to one group. x is staged in shared memory in
-// the order in which the steps read it.
+// A warp takes 32 rows and segments of 128 columns, 2 KB of weights, which it
+// copies with cp.async into a ring of its own, kStages deep: no warp waits for
+// another, and the loads in flight do not depend on registers. A step of
+// m16n8k16 may take any 16 columns if x has the same order, so a lane reads the
+// words of one group (the 16-byte chunks of a row are swizzled: no bank is read
+// twice) and uses each as it is. x is staged once per CTA in shared memory, in
+// the order of the steps; each 16 bytes of it serve two tiles of 16 rows.
 //
-// A CTA covers 16 rows x row-warps; its other warps, and the CTAs of a cluster,
-// split the columns, and their sums are added in a fixed order through
+// A CTA stays and takes blocks of 32 x row_warps rows in turn; its other warps,
+// and the CTAs of a cluster, split the columns (a cluster also holds an x that
+// one CTA cannot), and their sums are added in a fixed order through
 // (distributed) shared memory.
 #pragma once
 #include <cooperative_groups.h>
@@ -35,9 +36,12 @@ namespace w4 {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSeg = 128;          // columns of a warp step
+constexpr int kRows = 32;          // rows of a warp step
+constexpr int kStages = 3;         // of a warp's ring
+constexpr int kItem = kRows * kSeg / 2;  // bytes of a step
 constexpr int kMaxTokens = 16;     // of one CTA; more tokens take more CTAs
 constexpr int kMaxCluster = 8;
-constexpr int kStageBytes = 96 * 1024;  // at most, for x
+constexpr int64_t kMaxK = 131072;  // whose share of one fp32 token a cluster's CTA can hold
 
 struct Args {
   const void* x;
@@ -50,8 +54,9 @@ struct Args {
   int64_t ldy;
   int64_t M, N, K;
   int scale_dtype;
+  int tokens;      // of a CTA
   int row_warps;   // warps of a CTA along N
-  int chunk;       // columns staged at a time, a multiple of kSeg
+  int64_t blocks;  // of 32 x row_warps rows
 };
 
 // fp32 is multiplied as bf16 parts
@@ -106,19 +111,8 @@ __device__ __forceinline__ uint32_t weights(uint32_t word, int i, uint32_t zero)
   }
 }
 
-// 4x4 words among the four lanes of a row: lane t's word j becomes lane j's word t.
-__device__ __forceinline__ void transpose4(uint32_t (&w)[4], int t) {
-  // halves of 2x2 blocks, then single words
-  const bool hi = t & 2, odd = t & 1;
-  uint32_t a = hi ? w[0] : w[2], b = hi ? w[1] : w[3];
-  a = __shfl_xor_sync(0xffffffffu, a, 2);
-  b = __shfl_xor_sync(0xffffffffu, b, 2);
-  if (hi) { w[0] = a; w[1] = b; } else { w[2] = a; w[3] = b; }
-  a = odd ? w[0] : w[1];
-  b = odd ? w[2] : w[3];
-  a = __shfl_xor_sync(0xffffffffu, a, 1);
-  b = __shfl_xor_sync(0xffffffffu, b, 1);
-  if (odd) { w[0] = a; w[2] = b; } else { w[1] = a; w[3] = b; }
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 
 // Eight columns of a token, in the order in which the steps read them.
@@ -128,57 +122,86 @@ __device__ __forceinline__ uint4 order8(const float (&f)[8]) {
                     elem::pack2<H>(f[3], f[7]));
 }
 
+// Shared memory of a CTA: x [parts][tokens][share of K + 32 columns], the warps'
+// rings, the sums [column warps][8 NT tokens][rows].
+__host__ __device__ constexpr size_t x_row_bytes(int64_t segs) {
+  return (size_t)segs * kSeg * 2 + 64;  // 64: the eight lanes of a read cover all banks
+}
+constexpr size_t kRingBytes = (size_t)kWarps * kStages * kItem;
+constexpr size_t sums_bytes(int nt) { return (size_t)kWarps * kRows * 8 * nt * sizeof(float); }
+
 // GROUP: columns per scale. NT: blocks of 8 tokens of a CTA.
 template <typename T, int GROUP, int NT>
-__global__ void __launch_bounds__(kThreads) w4_kernel(const Args p) {
+__global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p) {
   namespace cg = cooperative_groups;
   using H = typename Mma<T>::type;
   constexpr int P = Mma<T>::parts;
   constexpr int GPS = kSeg / GROUP;  // groups of a segment
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];
   const cg::cluster_group cluster = cg::this_cluster();
   const int split = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int rw = warp % p.row_warps, kw = warp / p.row_warps, k_warps = kWarps / p.row_warps;
-  const int64_t block_row = (int64_t)blockIdx.x / split * (16 * p.row_warps);
-  const int64_t m0 = (int64_t)blockIdx.y * (8 * NT);
-  const int tokens = (int)(p.M - m0 < 8 * NT ? p.M - m0 : 8 * NT);
-  const int64_t segs = (p.K + kSeg - 1) / kSeg;
-  const int64_t seg_lo = segs * part / split, seg_hi = segs * (part + 1) / split;
+  const int k_warps = kWarps / p.row_warps, rw = warp / k_warps, kw = warp % k_warps;
+  const int rows = kRows * p.row_warps;
+  const int64_t m0 = (int64_t)blockIdx.y * p.tokens;
+  const int tokens = (int)(p.M - m0 < p.tokens ? p.M - m0 : p.tokens);
+  const int64_t segs = (p.K + kSeg - 1) / kSeg, most = (segs + split - 1) / split;
+  const int64_t seg_lo = min(part * most, segs), seg_hi = min(seg_lo + most, segs);
   const int64_t groups = p.K / GROUP;
+  const int64_t step = gridDim.x / split;  // blocks between two of this cluster
 
-  // rows past the last are computed as the last and not stored
-  const int64_t r0 = min(block_row + rw * 16 + g, p.N - 1), r1 = min(block_row + rw * 16 + g + 8, p.N - 1);
-  const uint8_t* w0 = p.packed + r0 * (p.K / 2);
-  const uint8_t* w1 = p.packed + r1 * (p.K / 2);
+  const int row_bytes = (int)x_row_bytes(most);
+  const int part_bytes = row_bytes * p.tokens;
+  uint8_t* ring = smem + (size_t)part_bytes * P + (size_t)warp * kStages * kItem;
+  float* sums = reinterpret_cast<float*>(smem + (size_t)part_bytes * P + kRingBytes);
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  const int swizzle = (g >> 1) & 3;
 
-  const int row_bytes = p.chunk * 2 + 64;  // of a token: 8 lanes of a read cover all banks
-  const int part_bytes = row_bytes * tokens;
-  float acc[NT][4];
+  // this warp's steps: its segments of a block, block after block
+  int64_t f_block = blockIdx.x / split, f_seg = seg_lo + kw;
+  int f_slot = 0;
+  auto fetch = [&]() {
+    while (f_block < p.blocks && f_seg >= seg_hi) {  // (once, unless this warp has no segment)
+      f_block += step;
+      f_seg = seg_lo + kw;
+      if (f_seg >= seg_hi) f_block = p.blocks;
+    }
+    if (f_block < p.blocks) {
+      const int64_t k0 = f_seg * kSeg + t * 32;
+      const int bytes = k0 < p.K ? 16 : 0;  // 0: zeros are written
+      const int64_t at = bytes ? k0 / 2 : 0;
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+      for (int i = 0; i < 4; ++i) {
+        // rows past the last are computed as the last and not stored
+        const int64_t r = min(f_block * rows + rw * kRows + g + 8 * i, p.N - 1);
+        copy16(ring_at + f_slot * kItem + (g + 8 * i) * 64 + ((t ^ swizzle) * 16), p.packed + r * (p.K / 2) + at,
+               bytes);
+      }
+      f_seg += k_warps;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    f_slot = f_slot + 1 == kStages ? 0 : f_slot + 1;
+  };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+  for (int i = 0; i < kStages - 1; ++i) fetch();
 
-  const int chunk_segs = p.chunk / kSeg;
-  for (int64_t c_lo = seg_lo; c_lo < seg_hi; c_lo += chunk_segs) {
-    const int64_t c_hi = min(c_lo + chunk_segs, seg_hi);
-    // x: eight columns at a time
-    const int units = (int)(c_hi - c_lo) * (kSeg / 8);
-    if (c_lo != seg_lo) __syncthreads();
+  // x: eight columns at a time
+  {
+    const int units = (int)(seg_hi - seg_lo) * (kSeg / 8);
+    const bool vec = sizeof(T) == 2 && elem::misalign<T>(p.x) == 0 && p.ldx % 8 == 0;
     for (int i = threadIdx.x; i < units * tokens; i += kThreads) {
       const int m = i / units, u = i - m * units;
-      const int64_t k0 = c_lo * kSeg + u * 8;
+      const int64_t k0 = seg_lo * kSeg + u * 8;
       float f[8];
       const T* xr = static_cast<const T*>(p.x) + (m0 + m) * p.ldx + k0;
+      if (sizeof(T) == 2 && vec && k0 < p.K) {  // K is a multiple of 32
+        if constexpr (sizeof(T) == 2) elem::unpack_vec<T>(*reinterpret_cast<const uint4*>(xr), f);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = k0 + j < p.K ? elem::to_f(xr[j]) : 0.f;
-      // of a segment's 16 units, lane t reads unit 4j + t at word j (transposed
-      // words), or unit 4t + j (words as loaded); both at place 4j + t
-      const int in_seg = u & 15;
-      const int place = (u & ~15) | (GROUP < kSeg ? in_seg : ((in_seg & 3) << 2) | (in_seg >> 2));
-      uint8_t* to = smem + m * row_bytes + place * 16;
+        for (int j = 0; j < 8; ++j) f[j] = k0 < p.K ? elem::to_f(xr[j]) : 0.f;
+      }
+      uint8_t* to = smem + m * row_bytes + u * 16;
       if constexpr (P == 1) {
         *reinterpret_cast<uint4*>(to) = order8<H>(f);
       } else {
@@ -194,48 +217,64 @@ __global__ void __launch_bounds__(kThreads) w4_kernel(const Args p) {
         }
       }
     }
-    __syncthreads();
+  }
+  __syncthreads();
 
-    for (int64_t s = c_lo + kw; s < c_hi; s += k_warps) {
-      const int64_t k0 = s * kSeg;
-      uint32_t a0[4] = {0, 0, 0, 0}, a1[4] = {0, 0, 0, 0};
-      if (k0 + t * 32 < p.K) {
-        const uint4 v0 = elem::ld_once16(w0 + k0 / 2 + t * 16), v1 = elem::ld_once16(w1 + k0 / 2 + t * 16);
-        a0[0] = v0.x; a0[1] = v0.y; a0[2] = v0.z; a0[3] = v0.w;
-        a1[0] = v1.x; a1[1] = v1.y; a1[2] = v1.z; a1[3] = v1.w;
-      }
-      if constexpr (GROUP < kSeg) {
-        transpose4(a0, t);
-        transpose4(a1, t);
-      }
-      float s0[GPS], s1[GPS];
-      uint32_t z0[GPS], z1[GPS];
+  int slot = 0;
+  for (int64_t block = blockIdx.x / split; block < p.blocks; block += step) {
+    float acc[2][NT][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.f;
+    int64_t grp_row[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) grp_row[i] = min(block * rows + rw * kRows + g + 8 * i, p.N - 1) * groups;
+
+    for (int64_t s = seg_lo + kw; s < seg_hi; s += k_warps) {
+      float sc[4][GPS];
+      uint32_t zr[4][GPS];
 #pragma unroll
       for (int q = 0; q < GPS; ++q) {
         const int64_t grp = min(s * GPS + q, groups - 1);  // past the last: x is 0
-        s0[q] = elem::ld_weight(p.scales, p.scale_dtype, r0 * groups + grp);
-        s1[q] = elem::ld_weight(p.scales, p.scale_dtype, r1 * groups + grp);
-        z0[q] = zero_pair<H>(p.zeros ? p.zeros[r0 * groups + grp] : 8);
-        z1[q] = zero_pair<H>(p.zeros ? p.zeros[r1 * groups + grp] : 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          sc[i][q] = elem::ld_weight(p.scales, p.scale_dtype, grp_row[i] + grp);
+          zr[i][q] = zero_pair<H>(p.zeros ? p.zeros[grp_row[i] + grp] : 8);
+        }
       }
-      const uint8_t* xs = smem + (s - c_lo) * (kSeg * 2) + t * 16;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      __syncwarp();  // the copies of all lanes have landed, and the slot before was read by all
+      fetch();
+      const uint8_t* xs = smem + (s - seg_lo) * (kSeg * 2) + t * 16;
+      const uint8_t* ws = ring + slot * kItem + g * 64 + t * 4;
+      slot = slot + 1 == kStages ? 0 : slot + 1;
 #pragma unroll
       for (int q = 0; q < GPS; ++q) {
-        float sum[NT][4];
+        float sum[2][NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sum[n][i] = 0.f;
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[r][n][i] = 0.f;
 #pragma unroll
         for (int jj = 0; jj < 4 / GPS; ++jj) {
           const int j = q * (4 / GPS) + jj;
-          uint32_t a[2][4];
+          uint32_t a[2][2][4];  // [tile][step]
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            a[h][0] = weights<H>(a0[j], 2 * h, z0[q]);
-            a[h][1] = weights<H>(a1[j], 2 * h, z1[q]);
-            a[h][2] = weights<H>(a0[j], 2 * h + 1, z0[q]);
-            a[h][3] = weights<H>(a1[j], 2 * h + 1, z1[q]);
+          for (int r = 0; r < 2; ++r) {
+            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(ws + r * 1024 + ((j ^ swizzle) * 16));
+            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(ws + r * 1024 + 512 + ((j ^ swizzle) * 16));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              a[r][h][0] = weights<H>(w0, 2 * h, zr[2 * r][q]);
+              a[r][h][1] = weights<H>(w1, 2 * h, zr[2 * r + 1][q]);
+              a[r][h][2] = weights<H>(w0, 2 * h + 1, zr[2 * r][q]);
+              a[r][h][3] = weights<H>(w1, 2 * h + 1, zr[2 * r + 1][q]);
+            }
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
@@ -243,54 +282,64 @@ __global__ void __launch_bounds__(kThreads) w4_kernel(const Args p) {
 #pragma unroll
             for (int o = 0; o < P; ++o) {
               const uint4 b = *reinterpret_cast<const uint4*>(xs + o * part_bytes + m * row_bytes + j * 64);
-              mma<H>(sum[n], a[0], b.x, b.y);
-              mma<H>(sum[n], a[1], b.z, b.w);
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                mma<H>(sum[r][n], a[r][0], b.x, b.y);
+                mma<H>(sum[r][n], a[r][1], b.z, b.w);
+              }
             }
           }
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          acc[n][0] = fmaf(s0[q], sum[n][0], acc[n][0]);
-          acc[n][1] = fmaf(s0[q], sum[n][1], acc[n][1]);
-          acc[n][2] = fmaf(s1[q], sum[n][2], acc[n][2]);
-          acc[n][3] = fmaf(s1[q], sum[n][3], acc[n][3]);
-        }
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              acc[r][n][i] = fmaf(sc[2 * r + (i >> 1)][q], sum[r][n][i], acc[r][n][i]);
       }
     }
-  }
 
-  // sums of the column-warps, then of the cluster, each in its order
-  constexpr int C = 8 * NT;
-  const int rows = 16 * p.row_warps;
-  float* sums = reinterpret_cast<float*>(smem);  // [k_warps][C][rows]
-  __syncthreads();
+    // sums of the column warps, then of the cluster, each in its order
+    constexpr int C = 8 * NT;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    float* to = sums + ((size_t)kw * C + n * 8 + 2 * t) * rows + rw * 16 + g;
-    to[0] = acc[n][0];
-    to[rows] = acc[n][1];
-    to[8] = acc[n][2];
-    to[rows + 8] = acc[n][3];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * tokens; i += kThreads) {
-    float v = sums[i];
-    for (int w = 1; w < k_warps; ++w) v += sums[w * C * rows + i];
-    sums[i] = v;
-  }
-  if (split > 1) cluster.sync();
-  else __syncthreads();
-  for (int i = threadIdx.x + part * kThreads; i < rows * tokens; i += split * kThreads) {
-    const int m = i / rows, r = i - m * rows;
-    float v = 0.f;
-    for (int q = 0; q < split; ++q) v += split > 1 ? cluster.map_shared_rank(sums, q)[i] : sums[i];
-    const int64_t n = block_row + r;
-    if (n < p.N) {
-      if (p.bias) v += elem::to_f(static_cast<const T*>(p.bias)[n]);
-      static_cast<T*>(p.y)[(m0 + m) * p.ldy + n] = elem::from_f<T>(v);
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float* to = sums + (size_t)(kw * C + n * 8 + 2 * t) * rows + rw * kRows + r * 16 + g;
+        to[0] = acc[r][n][0];
+        to[rows] = acc[r][n][1];
+        to[8] = acc[r][n][2];
+        to[rows + 8] = acc[r][n][3];
+      }
+    __syncthreads();
+    auto store = [&](int i, float v) {
+      const int m = i / rows;
+      const int64_t n = block * rows + (i - m * rows);
+      if (n < p.N) {
+        if (p.bias) v += elem::to_f(static_cast<const T*>(p.bias)[n]);
+        static_cast<T*>(p.y)[(m0 + m) * p.ldy + n] = elem::from_f<T>(v);
+      }
+    };
+    for (int i = threadIdx.x; i < rows * tokens; i += kThreads) {
+      float v = sums[i];
+      for (int w = 1; w < k_warps; ++w) v += sums[w * C * rows + i];
+      if (split > 1) sums[i] = v;
+      else store(i, v);
+    }
+    if (split > 1) {
+      cluster.sync();
+      for (int i = threadIdx.x + part * kThreads; i < rows * tokens; i += split * kThreads) {
+        float v = 0.f;
+        for (int q = 0; q < split; ++q) v += cluster.map_shared_rank(sums, q)[i];
+        store(i, v);
+      }
+      cluster.sync();  // the other CTAs read this one's sums
+    } else {
+      __syncthreads();
     }
   }
-  if (split > 1) cluster.sync();  // the other CTAs read this one's sums
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // Symmetric quantisation: s = max|w| / 7 of a group, rounded to the scales'
@@ -330,28 +379,42 @@ quantize_kernel(const T* __restrict__ w, int64_t total, int group, uint8_t* __re
 template <typename T, int GROUP, int NT>
 inline int launch_shape(Args a, cudaStream_t st) {
   auto kern = w4_kernel<T, GROUP, NT>;
-  const int64_t m_tiles = (a.M + 8 * NT - 1) / (8 * NT);
   const int64_t segs = (a.K + kSeg - 1) / kSeg;
-  a.row_warps = 4;
-  const int64_t blocks = (a.N + 16 * a.row_warps - 1) / (16 * a.row_warps);
-  // split the columns while the device is not full and each warp keeps two segments
+  const int sms = sm_count();
+  auto bytes_for = [&](int split) {
+    return (size_t)Mma<T>::parts * a.tokens * x_row_bytes((segs + split - 1) / split) + kRingBytes + sums_bytes(NT);
+  };
+  // as little of a cluster as lets two CTAs share an SM, or else fits at all
+  constexpr size_t kTwo = 113 * 1024, kOne = 226 * 1024;
   int split = 1;
-  while (split < kMaxCluster && blocks * m_tiles * split < 2 * sm_count() &&
-         segs >= 2 * split * 2 * (kWarps / a.row_warps))
-    split *= 2;
-  const int tokens = (int)(a.M < 8 * NT ? a.M : 8 * NT);
-  const int64_t own = (segs + split - 1) / split;
-  const int64_t fit = (kStageBytes / (Mma<T>::parts * tokens) - 64) / (2 * kSeg);
-  a.chunk = (int)((own < fit ? own : fit) * kSeg);
-  const size_t stage = (size_t)Mma<T>::parts * tokens * (a.chunk * 2 + 64);
-  const size_t sums = (size_t)(kWarps / a.row_warps) * 8 * NT * 16 * a.row_warps * sizeof(float);
-  const size_t bytes = stage > sums ? stage : sums;
-  int rc = ensure_smem((const void*)kern, bytes, "w4_linear: shared memory");
+  while (split < kMaxCluster && bytes_for(split) > kTwo) split *= 2;
+  while (split > 1 && bytes_for(split) > kTwo && bytes_for(split / 2) <= kOne) split /= 2;
+  if (bytes_for(split) > kOne) return fail(KT_ERR_UNSUPPORTED, "w4_linear: K=%lld is too large", (long long)a.K);
+  // more of it while the device is not full and every warp keeps two segments
+  auto blocks_for = [&](int row_warps) { return (a.N + kRows * row_warps - 1) / (kRows * row_warps); };
+  const int64_t m_tiles = (a.M + a.tokens - 1) / a.tokens;
+  while (split < kMaxCluster && blocks_for(1) * split * m_tiles < sms && segs >= 2 * split * 2 * kWarps) split *= 2;
+  const size_t bytes = bytes_for(split);
+  const int64_t slots = (int64_t)sms * (bytes <= kTwo ? 2 : 1) / split;
+  // rows of a block: many, unless fewer share the blocks out better
+  a.row_warps = 1;
+  double best = 0;
+  for (int r = kWarps; r >= 1; r /= 2) {
+    const int64_t blocks = blocks_for(r) * m_tiles, turns = (blocks + slots - 1) / slots;
+    const double used = (double)blocks / (double)(turns * slots);
+    if (used > best + 0.05) {
+      best = used;
+      a.row_warps = r;
+    }
+  }
+  a.blocks = blocks_for(a.row_warps);
+  const int64_t per_tile = slots / m_tiles > 0 ? slots / m_tiles : 1;
+  const int64_t clusters = a.blocks < per_tile ? a.blocks : per_tile;
+  if (m_tiles > 65535) return fail(KT_ERR_UNSUPPORTED, "w4_linear: M=%lld is too large", (long long)a.M);
+  const int rc = ensure_smem((const void*)kern, bytes, "w4_linear: shared memory");
   if (rc != KT_OK) return rc;
-  if (blocks * split > INT32_MAX || m_tiles > 65535)
-    return fail(KT_ERR_UNSUPPORTED, "w4_linear: N=%lld or M=%lld too large", (long long)a.N, (long long)a.M);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(blocks * split), (unsigned)m_tiles);
+  cfg.gridDim = dim3((unsigned)(clusters * split), (unsigned)m_tiles);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
@@ -365,8 +428,13 @@ inline int launch_shape(Args a, cudaStream_t st) {
 }
 
 template <typename T>
-inline int launch_typed(const Args& a, int group, cudaStream_t st) {
-  const bool one = a.M <= 8;
+inline int launch_typed(Args a, int group, cudaStream_t st) {
+  // tokens of a CTA: fewer where a cluster cannot hold the share of more
+  a.tokens = (int)(a.M < kMaxTokens ? a.M : kMaxTokens);
+  const int64_t segs = (a.K + kSeg - 1) / kSeg;
+  while (a.tokens > 1 && Mma<T>::parts * a.tokens * x_row_bytes((segs + kMaxCluster - 1) / kMaxCluster) > 160 * 1024)
+    a.tokens /= 2;
+  const bool one = a.tokens <= 8;
   if (group == 32) return one ? launch_shape<T, 32, 1>(a, st) : launch_shape<T, 32, 2>(a, st);
   if (group == 64) return one ? launch_shape<T, 64, 1>(a, st) : launch_shape<T, 64, 2>(a, st);
   return one ? launch_shape<T, 128, 1>(a, st) : launch_shape<T, 128, 2>(a, st);
@@ -379,7 +447,7 @@ inline int check_matrix(const char* what, int64_t N, int64_t K, int group, int d
   if (group != 32 && group != 64 && group != 128)
     return fail(KT_ERR_UNSUPPORTED, "%s: groups of 32, 64 or 128 columns, not %d", what, group);
   if (K % group) return fail(KT_ERR_ARG, "%s: K=%lld is not a multiple of the group %d", what, (long long)K, group);
-  if (K > (int64_t)1 << 30) return fail(KT_ERR_UNSUPPORTED, "%s: K > 2^30", what);
+  if (K > kMaxK) return fail(KT_ERR_UNSUPPORTED, "%s: K > %lld", what, (long long)kMaxK);
   return KT_OK;
 }
 
