@@ -8,10 +8,17 @@
 // fp32 multiply-adds per token would exceed from the second token on. So the
 // sums run on the tensor cores (mma.sync m16n8k16: 16 weight rows by 8 tokens,
 // fp32 accumulation; a tcgen05 tile of 128 rows would need the weights
-// unpacked through shared memory): q - z is exact in 16 bits (or-ing q into
-// the mantissa of 128 (bf16) or 1024 (fp16), then one packed subtraction), and
-// so are its products with x; the scale multiplies each group's fp32 sum. fp32
-// tokens are split exactly into three bf16 parts.
+// unpacked through shared memory): q - z is exact in 16 bits, and so are its
+// products with x; the scale multiplies each group's fp32 sum. fp32 tokens are
+// split exactly into three bf16 parts.
+//
+// Unpacking takes most of the instructions, so it costs 9 for 8 weights: one
+// mask for each pair of nibbles (bits 0-3 and 4-7 of both halves of a word, then
+// the same of the word shifted by 8) and one packed multiply-add. In fp16 the
+// nibble is or-ed into the mantissa of 1024, which makes it 1024 + q or
+// 1024 + 16 q; a bf16 of nothing but a nibble in its low 8 bits is q 2^-133 or
+// q 2^-129 (its subnormals and first binade are one linear range), which a power
+// of two brings to (q - z) / 64; the 64 comes back when the sums are done.
 //
 // A warp takes 32 rows and segments of 128 columns, 2 KB of weights, which it
 // copies with cp.async into a ring of its own, kStages deep: no warp waits for
@@ -53,10 +60,10 @@ struct Args {
   void* y;
   int64_t ldy;
   int64_t M, N, K;
-  int scale_dtype;
   int tokens;      // of a CTA
   int row_warps;   // warps of a CTA along N
   int64_t blocks;  // of 32 x row_warps rows
+  bool whole_groups;  // a segment's scales (and zeros) can be loaded at once
 };
 
 // fp32 is multiplied as bf16 parts
@@ -71,45 +78,61 @@ struct Mma<float> {
   static constexpr int parts = 3;
 };
 
+// d = a b (+ d)
 template <typename H>
-__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool add) {
+  const float c0 = add ? d[0] : 0.f, c1 = add ? d[1] : 0.f, c2 = add ? d[2] : 0.f, c3 = add ? d[3] : 0.f;
+  if constexpr (std::is_same<H, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
-// (base + zero) twice, where base + q has q in its low mantissa bits.
+// What a group's zero and scale become for the unpacking below.
 template <typename H>
-__device__ __forceinline__ uint32_t zero_pair(int zero);
+struct Unpack;
 template <>
-__device__ __forceinline__ uint32_t zero_pair<__nv_bfloat16>(int zero) { return 0x43004300u + 0x00010001u * zero; }
-template <>
-__device__ __forceinline__ uint32_t zero_pair<__half>(int zero) { return 0x64006400u + 0x00010001u * zero; }
-
-// Pair i of a word: columns i and i + 4 of its eight, minus the zero.
-template <typename H>
-__device__ __forceinline__ uint32_t weights(uint32_t word, int i, uint32_t zero) {
-  constexpr uint32_t base = std::is_same<H, __half>::value ? 0x64006400u : 0x43004300u;
-  const uint32_t q = ((word >> (4 * i)) & 0x000F000Fu) | base;
-  if constexpr (std::is_same<H, __half>::value) {
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&q), *reinterpret_cast<const __half2*>(&zero));
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __nv_bfloat162 v =
-        __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&q), *reinterpret_cast<const __nv_bfloat162*>(&zero));
+struct Unpack<__half> {
+  static constexpr float scale = 1.f;
+  uint32_t low, high;  // pairs of 1024 + z, and of -(64 + z)
+  __device__ __forceinline__ explicit Unpack(uint32_t zero)
+      : low(0x64006400u + 0x00010001u * zero), high(0xD400D400u + 0x00100010u * zero) {}
+  // nibbles at bits 0-3 and 16-19 / at bits 4-7 and 20-23 of a word, minus z
+  __device__ __forceinline__ uint32_t at0(uint32_t w) const {
+    const uint32_t q = (w & 0x000F000Fu) | 0x64006400u;
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&q), *reinterpret_cast<const __half2*>(&low));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
-}
+  __device__ __forceinline__ uint32_t at4(uint32_t w) const {
+    const uint32_t q = (w & 0x00F000F0u) | 0x64006400u, s = 0x2C002C00u;  // 1/16
+    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&q), *reinterpret_cast<const __half2*>(&s),
+                              *reinterpret_cast<const __half2*>(&high));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+};
+template <>
+struct Unpack<__nv_bfloat16> {
+  static constexpr float scale = 64.f;
+  uint32_t minus;  // pair of -z / 64
+  __device__ __forceinline__ explicit Unpack(uint32_t zero) {
+    const __nv_bfloat162 v = __float2bfloat162_rn((float)zero * -0.015625f);
+    minus = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  __device__ __forceinline__ static uint32_t fma(uint32_t q, uint32_t power, uint32_t minus) {
+    const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&q),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&power),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&minus));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  __device__ __forceinline__ uint32_t at0(uint32_t w) const { return fma(w & 0x000F000Fu, 0x7F007F00u, minus); }
+  __device__ __forceinline__ uint32_t at4(uint32_t w) const { return fma(w & 0x00F000F0u, 0x7D007D00u, minus); }
+};
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
@@ -130,8 +153,25 @@ __host__ __device__ constexpr size_t x_row_bytes(int64_t segs) {
 constexpr size_t kRingBytes = (size_t)kWarps * kStages * kItem;
 constexpr size_t sums_bytes(int nt) { return (size_t)kWarps * kRows * 8 * nt * sizeof(float); }
 
-// GROUP: columns per scale. NT: blocks of 8 tokens of a CTA.
-template <typename T, int GROUP, int NT>
+// The scales and zeros of a lane's four rows for a segment, as loaded.
+template <typename S, int GPS>
+struct GroupWords {
+  static constexpr int W = (GPS * (int)sizeof(S) + 3) / 4;
+  uint32_t s[4][W];
+  uint32_t z[4];  // a byte per group
+  __device__ __forceinline__ float scale(int row, int q) const {
+    if constexpr (sizeof(S) == 4) {
+      return __uint_as_float(s[row][q]);
+    } else {
+      const float2 v = elem::unpack2<S>(s[row][q / 2]);
+      return q & 1 ? v.y : v.x;
+    }
+  }
+  __device__ __forceinline__ uint32_t zero(int row, int q) const { return (z[row] >> (8 * q)) & 255u; }
+};
+
+// GROUP: columns per scale. NT: blocks of 8 tokens of a CTA. S: type of the scales.
+template <typename T, typename S, int GROUP, int NT>
 __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p) {
   namespace cg = cooperative_groups;
   using H = typename Mma<T>::type;
@@ -161,24 +201,30 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p) {
   // this warp's steps: its segments of a block, block after block
   int64_t f_block = blockIdx.x / split, f_seg = seg_lo + kw;
   int f_slot = 0;
-  auto fetch = [&]() {
-    while (f_block < p.blocks && f_seg >= seg_hi) {  // (once, unless this warp has no segment)
-      f_block += step;
-      f_seg = seg_lo + kw;
-      if (f_seg >= seg_hi) f_block = p.blocks;
-    }
-    if (f_block < p.blocks) {
-      const int64_t k0 = f_seg * kSeg + t * 32;
-      const int bytes = k0 < p.K ? 16 : 0;  // 0: zeros are written
-      const int64_t at = bytes ? k0 / 2 : 0;
+  const uint8_t* f_rows;  // the first of this lane's rows of the block, at its columns
+  int f_more[4];          // bytes from there to each of the four
+  auto set_rows = [&]() {
+    // rows past the last are computed as the last and not stored
+    const int64_t r0 = f_block * rows + rw * kRows + g;
+    f_rows = p.packed + min(r0, p.N - 1) * (p.K / 2) + t * 16;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // rows past the last are computed as the last and not stored
-        const int64_t r = min(f_block * rows + rw * kRows + g + 8 * i, p.N - 1);
-        copy16(ring_at + f_slot * kItem + (g + 8 * i) * 64 + ((t ^ swizzle) * 16), p.packed + r * (p.K / 2) + at,
-               bytes);
-      }
+    for (int i = 0; i < 4; ++i) f_more[i] = (int)((min(r0 + 8 * i, p.N - 1) - min(r0, p.N - 1)) * (p.K / 2));
+  };
+  set_rows();
+  if (f_seg >= seg_hi) f_block = p.blocks;  // no segment for this warp
+  auto fetch = [&]() {
+    if (f_block < p.blocks) {
+      const bool in = f_seg * kSeg + t * 32 < p.K;
+      const uint8_t* at = in ? f_rows + f_seg * (kSeg / 2) : p.packed;  // size 0: zeros are written
+      const uint32_t to = ring_at + f_slot * kItem + g * 64 + ((t ^ swizzle) * 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) copy16(to + i * 512, at + (in ? f_more[i] : 0), in ? 16 : 0);
       f_seg += k_warps;
+      if (f_seg >= seg_hi) {
+        f_seg = seg_lo + kw;
+        f_block += step;
+        if (f_block < p.blocks) set_rows();
+      }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     f_slot = f_slot + 1 == kStages ? 0 : f_slot + 1;
@@ -229,51 +275,82 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p) {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.f;
-    int64_t grp_row[4];
+    const int64_t row0 = block * rows + rw * kRows + g;
+    const S* scales = static_cast<const S*>(p.scales) + min(row0, p.N - 1) * groups;
+    const uint8_t* zeros = p.zeros + (p.zeros ? min(row0, p.N - 1) * groups : 0);
+    int more[4];  // groups from the first of the four rows to each
 #pragma unroll
-    for (int i = 0; i < 4; ++i) grp_row[i] = min(block * rows + rw * kRows + g + 8 * i, p.N - 1) * groups;
+    for (int i = 0; i < 4; ++i) more[i] = (int)((min(row0 + 8 * i, p.N - 1) - min(row0, p.N - 1)) * groups);
+    GroupWords<S, GPS> words;
+    auto load_groups = [&](int64_t seg) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const S* at = scales + more[i] + seg * GPS;
+        if (GPS == 1 || p.whole_groups) {  // a segment's groups in one load
+          if constexpr (words.W == 4) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
+            words.s[i][0] = v.x; words.s[i][1] = v.y; words.s[i][2] = v.z; words.s[i][3] = v.w;
+          } else if constexpr (words.W == 2) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
+            words.s[i][0] = v.x; words.s[i][1] = v.y;
+          } else if constexpr (GPS * sizeof(S) == 4) {
+            words.s[i][0] = __ldg(reinterpret_cast<const uint32_t*>(at));
+          } else {
+            words.s[i][0] = __ldg(reinterpret_cast<const uint16_t*>(at));
+          }
+          if (p.zeros) {
+            const uint8_t* z = zeros + more[i] + seg * GPS;
+            if constexpr (GPS == 4) words.z[i] = __ldg(reinterpret_cast<const uint32_t*>(z));
+            else if constexpr (GPS == 2) words.z[i] = __ldg(reinterpret_cast<const uint16_t*>(z));
+            else words.z[i] = __ldg(z);
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < words.W; ++q) words.s[i][q] = 0;
+          words.z[i] = 0;
+#pragma unroll
+          for (int q = 0; q < GPS; ++q) {
+            const int64_t in = min(seg * GPS + q, groups - 1) - seg * GPS;  // past the last: x is 0
+            if constexpr (sizeof(S) == 4) words.s[i][q] = __ldg(reinterpret_cast<const uint32_t*>(at) + in);
+            else words.s[i][q / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(at) + in) << (16 * (q & 1));
+            if (p.zeros) words.z[i] |= (uint32_t)__ldg(zeros + more[i] + seg * GPS + in) << (8 * q);
+          }
+        }
+        if (!p.zeros) words.z[i] = 0x08080808u;
+      }
+    };
+    if (seg_lo + kw < seg_hi) load_groups(seg_lo + kw);
 
     for (int64_t s = seg_lo + kw; s < seg_hi; s += k_warps) {
-      float sc[4][GPS];
-      uint32_t zr[4][GPS];
-#pragma unroll
-      for (int q = 0; q < GPS; ++q) {
-        const int64_t grp = min(s * GPS + q, groups - 1);  // past the last: x is 0
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          sc[i][q] = elem::ld_weight(p.scales, p.scale_dtype, grp_row[i] + grp);
-          zr[i][q] = zero_pair<H>(p.zeros ? p.zeros[grp_row[i] + grp] : 8);
-        }
-      }
       asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
       __syncwarp();  // the copies of all lanes have landed, and the slot before was read by all
       fetch();
+      const GroupWords<S, GPS> cur = words;
+      if (s + k_warps < seg_hi) load_groups(s + k_warps);
       const uint8_t* xs = smem + (s - seg_lo) * (kSeg * 2) + t * 16;
       const uint8_t* ws = ring + slot * kItem + g * 64 + t * 4;
       slot = slot + 1 == kStages ? 0 : slot + 1;
 #pragma unroll
       for (int q = 0; q < GPS; ++q) {
         float sum[2][NT][4];
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum[r][n][i] = 0.f;
+        const Unpack<H> u0(cur.zero(0, q)), u1(cur.zero(1, q)), u2(cur.zero(2, q)), u3(cur.zero(3, q));
 #pragma unroll
         for (int jj = 0; jj < 4 / GPS; ++jj) {
           const int j = q * (4 / GPS) + jj;
           uint32_t a[2][2][4];  // [tile][step]
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(ws + r * 1024 + ((j ^ swizzle) * 16));
-            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(ws + r * 1024 + 512 + ((j ^ swizzle) * 16));
+            uint32_t w0 = *reinterpret_cast<const uint32_t*>(ws + r * 1024 + ((j ^ swizzle) * 16));
+            uint32_t w1 = *reinterpret_cast<const uint32_t*>(ws + r * 1024 + 512 + ((j ^ swizzle) * 16));
+            const Unpack<H>&v0 = r ? u2 : u0, &v1 = r ? u3 : u1;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              a[r][h][0] = weights<H>(w0, 2 * h, zr[2 * r][q]);
-              a[r][h][1] = weights<H>(w1, 2 * h, zr[2 * r + 1][q]);
-              a[r][h][2] = weights<H>(w0, 2 * h + 1, zr[2 * r][q]);
-              a[r][h][3] = weights<H>(w1, 2 * h + 1, zr[2 * r + 1][q]);
+              a[r][h][0] = v0.at0(w0);
+              a[r][h][1] = v1.at0(w1);
+              a[r][h][2] = v0.at4(w0);
+              a[r][h][3] = v1.at4(w1);
+              w0 >>= 8;
+              w1 >>= 8;
             }
           }
 #pragma unroll
@@ -284,8 +361,8 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p) {
               const uint4 b = *reinterpret_cast<const uint4*>(xs + o * part_bytes + m * row_bytes + j * 64);
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                mma<H>(sum[r][n], a[r][0], b.x, b.y);
-                mma<H>(sum[r][n], a[r][1], b.z, b.w);
+                mma<H>(sum[r][n], a[r][0], b.x, b.y, jj > 0 || o > 0);
+                mma<H>(sum[r][n], a[r][1], b.z, b.w, true);
               }
             }
           }
@@ -296,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p) {
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              acc[r][n][i] = fmaf(sc[2 * r + (i >> 1)][q], sum[r][n][i], acc[r][n][i]);
+              acc[r][n][i] = fmaf(cur.scale(2 * r + (i >> 1), q), sum[r][n][i], acc[r][n][i]);
       }
     }
 
@@ -307,10 +384,10 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float* to = sums + (size_t)(kw * C + n * 8 + 2 * t) * rows + rw * kRows + r * 16 + g;
-        to[0] = acc[r][n][0];
-        to[rows] = acc[r][n][1];
-        to[8] = acc[r][n][2];
-        to[rows + 8] = acc[r][n][3];
+        to[0] = acc[r][n][0] * Unpack<H>::scale;
+        to[rows] = acc[r][n][1] * Unpack<H>::scale;
+        to[8] = acc[r][n][2] * Unpack<H>::scale;
+        to[rows + 8] = acc[r][n][3] * Unpack<H>::scale;
       }
     __syncthreads();
     auto store = [&](int i, float v) {
@@ -376,9 +453,12 @@ quantize_kernel(const T* __restrict__ w, int64_t total, int group, uint8_t* __re
 }
 
 // ---------------------------------------------------------------- host
-template <typename T, int GROUP, int NT>
+template <typename T, typename S, int GROUP, int NT>
 inline int launch_shape(Args a, cudaStream_t st) {
-  auto kern = w4_kernel<T, GROUP, NT>;
+  auto kern = w4_kernel<T, S, GROUP, NT>;
+  constexpr int GPS = kSeg / GROUP;
+  a.whole_groups = a.K % kSeg == 0 && elem::aligned_to(a.scales, GPS * (int)sizeof(S)) &&
+                   elem::aligned_to(a.zeros, GPS);
   const int64_t segs = (a.K + kSeg - 1) / kSeg;
   const int sms = sm_count();
   auto bytes_for = [&](int split) {
@@ -427,7 +507,7 @@ inline int launch_shape(Args a, cudaStream_t st) {
   return cuda_status(cudaLaunchKernelEx(&cfg, kern, a), "w4_linear launch");
 }
 
-template <typename T>
+template <typename T, typename S>
 inline int launch_typed(Args a, int group, cudaStream_t st) {
   // tokens of a CTA: fewer where a cluster cannot hold the share of more
   a.tokens = (int)(a.M < kMaxTokens ? a.M : kMaxTokens);
@@ -435,9 +515,9 @@ inline int launch_typed(Args a, int group, cudaStream_t st) {
   while (a.tokens > 1 && Mma<T>::parts * a.tokens * x_row_bytes((segs + kMaxCluster - 1) / kMaxCluster) > 160 * 1024)
     a.tokens /= 2;
   const bool one = a.tokens <= 8;
-  if (group == 32) return one ? launch_shape<T, 32, 1>(a, st) : launch_shape<T, 32, 2>(a, st);
-  if (group == 64) return one ? launch_shape<T, 64, 1>(a, st) : launch_shape<T, 64, 2>(a, st);
-  return one ? launch_shape<T, 128, 1>(a, st) : launch_shape<T, 128, 2>(a, st);
+  if (group == 32) return one ? launch_shape<T, S, 32, 1>(a, st) : launch_shape<T, S, 32, 2>(a, st);
+  if (group == 64) return one ? launch_shape<T, S, 64, 1>(a, st) : launch_shape<T, S, 64, 2>(a, st);
+  return one ? launch_shape<T, S, 128, 1>(a, st) : launch_shape<T, S, 128, 2>(a, st);
 }
 
 inline int check_matrix(const char* what, int64_t N, int64_t K, int group, int dtype, int scale_dtype) {
@@ -451,9 +531,11 @@ inline int check_matrix(const char* what, int64_t N, int64_t K, int group, int d
   return KT_OK;
 }
 
-inline int linear(const Args& a, int group, int dtype, cudaStream_t st) {
-  const int rc = check_matrix("w4_linear", a.N, a.K, group, dtype, a.scale_dtype);
+inline int linear(const Args& a, int group, int dtype, int scale_dtype, cudaStream_t st) {
+  const int rc = check_matrix("w4_linear", a.N, a.K, group, dtype, scale_dtype);
   if (rc != KT_OK) return rc;
+  if (scale_dtype != KT_F32 && scale_dtype != dtype)
+    return fail(KT_ERR_ARG, "w4_linear: scales are fp32 or of the tokens' type");
   if (a.M < 0) return fail(KT_ERR_ARG, "w4_linear: negative M=%lld", (long long)a.M);
   if (a.M == 0 || a.N == 0) return KT_OK;
   if (a.K == 0) return fail(KT_ERR_ARG, "w4_linear: K must be positive");
@@ -462,11 +544,13 @@ inline int linear(const Args& a, int group, int dtype, cudaStream_t st) {
   const int sz = elem::size_of(dtype);
   if (!aligned16(a.packed)) return fail(KT_ERR_ARG, "w4_linear: packed weights must be 16-byte aligned");
   if (!elem::aligned_to(a.x, sz) || !elem::aligned_to(a.y, sz) || !elem::aligned_to(a.bias, sz) ||
-      !elem::aligned_to(a.scales, elem::size_of(a.scale_dtype)))
+      !elem::aligned_to(a.scales, elem::size_of(scale_dtype)))
     return fail(KT_ERR_ARG, "w4_linear: a pointer is not aligned to its elements");
-  if (dtype == KT_F32) return launch_typed<float>(a, group, st);
-  if (dtype == KT_BF16) return launch_typed<__nv_bfloat16>(a, group, st);
-  return launch_typed<__half>(a, group, st);
+  const bool f32 = scale_dtype == KT_F32;
+  if (dtype == KT_F32) return launch_typed<float, float>(a, group, st);
+  if (dtype == KT_BF16) return f32 ? launch_typed<__nv_bfloat16, float>(a, group, st)
+                                   : launch_typed<__nv_bfloat16, __nv_bfloat16>(a, group, st);
+  return f32 ? launch_typed<__half, float>(a, group, st) : launch_typed<__half, __half>(a, group, st);
 }
 
 inline int quantize(const void* w, int64_t N, int64_t K, int group, int dtype, uint8_t* packed, void* scales,

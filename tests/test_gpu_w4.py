@@ -74,8 +74,8 @@ def test_columns_that_end_inside_a_segment(dev, lib, group, k, t):
 
 @pytest.mark.parametrize("t", TYPES)
 def test_scale_types_and_no_bias(dev, lib, t):
-    for st in TYPES:
-        x, w, bias = make(dev, 3, 100, 512, 64, t, st=st)
+    for st, group in ((torch.float32, 32), (torch.float32, 128), (t, 64)):
+        x, w, bias = make(dev, 3, 100, 512, group, t, st=st)
         check(x, w, bias, lib)
         check(x, w, None, lib)
 
@@ -169,6 +169,7 @@ def test_empty_and_refusals(dev, lib):
            lambda: kt_ops.w4_linear(x, w._replace(group=64), bias, lib=lib),
            lambda: kt_ops.w4_linear(x, w._replace(zeros=w.zeros[:-1]), bias, lib=lib),
            lambda: kt_ops.w4_linear(x, w._replace(scales=w.scales.double()), bias, lib=lib),
+           lambda: kt_ops.w4_linear(x, w._replace(scales=w.scales.bfloat16()), bias, lib=lib),
            lambda: kt_ops.w4_linear(x, w._replace(packed=w.packed.cpu()), bias, lib=lib),
            lambda: kt_ops.w4_linear(x, w, bias, out=torch.empty(2, 47, dtype=x.dtype, device=dev), lib=lib),
            lambda: kt_ops.w4_quantize(x, 96, lib=lib),
