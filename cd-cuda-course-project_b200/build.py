@@ -34,6 +34,7 @@ BASE_FLAGS = [
     "-lineinfo",
     "-std=c++17",
     "-Xptxas", "-v",
+    "--split-compile", "0",  # the kernels of one library are optimised on all cores
     "--shared",
     "-Xcompiler", "-fPIC",
     # hidden by default: only the KT_API entry points are exported, so the

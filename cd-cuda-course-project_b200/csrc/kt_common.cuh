@@ -80,10 +80,20 @@ struct FactsTable {
     size_t smem;
     int per_sm;
   };
+  struct Clusters {
+    const void* fn;
+    int dev;
+    int block;
+    size_t smem;
+    int size;
+    int count;
+  };
   std::mutex mu;
-  Smem smem[64];
+  Clusters clusters[256];
+  int n_clusters = 0;
+  Smem smem[256];
   int n_smem = 0;
-  Occ occ[64];
+  Occ occ[256];
   int n_occ = 0;
 };
 inline FactsTable& facts() {
@@ -101,7 +111,7 @@ inline int ensure_smem_locked(FactsTable& t, const void* fn, int dev, size_t byt
       return rc;
     }
   int rc = cuda_status(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what);
-  if (rc == KT_OK && t.n_smem < 64) t.smem[t.n_smem++] = FactsTable::Smem{fn, dev, bytes};
+  if (rc == KT_OK && t.n_smem < 256) t.smem[t.n_smem++] = FactsTable::Smem{fn, dev, bytes};
   return rc;
 }
 }  // namespace detail
@@ -135,8 +145,44 @@ inline int resident_ctas(const void* fn, int block, size_t smem, int* per_sm, co
   int n = 0;
   rc = cuda_status(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, block, smem), what);
   if (rc != KT_OK) return rc;
-  if (t.n_occ < 64) t.occ[t.n_occ++] = detail::FactsTable::Occ{fn, dev, block, smem, n};
+  if (t.n_occ < 256) t.occ[t.n_occ++] = detail::FactsTable::Occ{fn, dev, block, smem, n};
   *per_sm = n;
+  return KT_OK;
+}
+
+// ensure_smem, then the number of clusters of `size` CTAs (block, smem) that the
+// device holds at once. (Fewer than SMs x CTAs per SM / size where the SMs of a
+// partition are no multiple of the cluster.)
+inline int resident_clusters(const void* fn, int block, size_t smem, int size, int* count, const char* what) {
+  int dev = 0;
+  int rc = cuda_status(cudaGetDevice(&dev), what);
+  if (rc != KT_OK) return rc;
+  detail::FactsTable& t = detail::facts();
+  std::lock_guard<std::mutex> lock(t.mu);
+  rc = detail::ensure_smem_locked(t, fn, dev, smem, what);
+  if (rc != KT_OK) return rc;
+  for (int i = 0; i < t.n_clusters; ++i) {
+    const auto& e = t.clusters[i];
+    if (e.fn == fn && e.dev == dev && e.block == block && e.smem == smem && e.size == size) {
+      *count = e.count;
+      return KT_OK;
+    }
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)size);
+  cfg.blockDim = dim3((unsigned)block);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)size;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  rc = cuda_status(cudaOccupancyMaxActiveClusters(&n, fn, &cfg), what);
+  if (rc != KT_OK) return rc;
+  if (t.n_clusters < 256) t.clusters[t.n_clusters++] = detail::FactsTable::Clusters{fn, dev, block, smem, size, n};
+  *count = n;
   return KT_OK;
 }
 

@@ -285,11 +285,10 @@ int kt_w4_quantize(const void* w, int64_t N, int64_t K, int group, int dtype, ui
 
 int kt_w4_linear(const void* x, int64_t ldx, const uint8_t* packed, const void* scales, const uint8_t* zeros,
                  const void* bias, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int group, int dtype,
-                 int scale_dtype, kt_stream_t stream) {
+                 kt_stream_t stream) {
   kt::clear_error();
 #if KT_WITH_LM
-  return kt::w4::linear({x, ldx, packed, scales, zeros, bias, y, ldy, M, N, K, 0, 0, 0, false}, group, dtype,
-                        scale_dtype, stream);
+  return kt::w4::linear({x, ldx, packed, scales, zeros, bias, y, ldy, M, N, K, 0, 0, 0}, group, dtype, stream);
 #else
   return kt::unsupported("4-bit weights");
 #endif

@@ -14,28 +14,32 @@
 //
 // Unpacking takes most of the instructions, so it costs 9 for 8 weights: one
 // mask for each pair of nibbles (bits 0-3 and 4-7 of both halves of a word, then
-// the same of the word shifted by 8) and one packed multiply-add. In fp16 the
-// nibble is or-ed into the mantissa of 1024, which makes it 1024 + q or
-// 1024 + 16 q; a bf16 of nothing but a nibble in its low 8 bits is q 2^-133 or
-// q 2^-129 (its subnormals and first binade are one linear range), which a power
-// of two brings to (q - z) / 64; the 64 comes back when the sums are done.
+// the same of the word shifted by 8) and one packed multiply-add. A 16-bit float
+// of nothing but a nibble in its low 8 bits is q 2^-133 or q 2^-129 in bf16
+// (whose subnormals and first binade are one linear range), q 2^-24 or q 2^-20
+// in fp16; a power of two and -z make it (q - z) / 64 or / 512, exactly, and
+// that factor comes back when the sums are done.
 //
-// A warp takes 32 rows and segments of 128 columns, 2 KB of weights, which it
-// copies with cp.async into a ring of its own, kStages deep: no warp waits for
-// another, and the loads in flight do not depend on registers. A step of
-// m16n8k16 may take any 16 columns if x has the same order, so a lane reads the
-// words of one group (the 16-byte chunks of a row are swizzled: no bank is read
-// twice) and uses each as it is. x is staged once per CTA in shared memory, in
-// the order of the steps; each 16 bytes of it serve two tiles of 16 rows.
+// A warp takes 32 rows and segments of 128 columns, 2 KB of weights, which one
+// TMA load brings into a ring of its own, kStages deep: no warp waits for
+// another, and the loads in flight cost neither registers nor address
+// arithmetic. A step of m16n8k16 may take any 16 columns if x has the same
+// order, so a lane reads the words of one group (TMA's 64-byte swizzle: no bank
+// is read twice) and uses each as it is. x is staged once per CTA in shared
+// memory, in the order of the steps; each 16 bytes of it serve two tiles of 16
+// rows.
 //
 // A CTA stays and takes blocks of 32 x row_warps rows in turn; its other warps,
 // and the CTAs of a cluster, split the columns (a cluster also holds an x that
-// one CTA cannot), and their sums are added in a fixed order through
-// (distributed) shared memory.
+// one CTA cannot). Their sums are added in a fixed order through (distributed)
+// shared memory, one block late: a warp that has left its sums arrives at the
+// cluster's barrier and goes on with the next block, and waits there before it
+// adds the sums of the block before.
 #pragma once
 #include <cooperative_groups.h>
 
 #include "elem.cuh"
+#include "sm100.cuh"
 
 namespace kt {
 namespace w4 {
@@ -63,7 +67,6 @@ struct Args {
   int tokens;      // of a CTA
   int row_warps;   // warps of a CTA along N
   int64_t blocks;  // of 32 x row_warps rows
-  bool whole_groups;  // a segment's scales (and zeros) can be loaded at once
 };
 
 // fp32 is multiplied as bf16 parts
@@ -94,35 +97,17 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
-// What a group's zero and scale become for the unpacking below.
+// Pairs of weights of one type H: `power` brings a nibble at bits 0-3 (low) and
+// 4-7 (high) of both halves of a word, read as H, to q / scale.
 template <typename H>
-struct Unpack;
+struct Nibbles;
 template <>
-struct Unpack<__half> {
-  static constexpr float scale = 1.f;
-  uint32_t low, high;  // pairs of 1024 + z, and of -(64 + z)
-  __device__ __forceinline__ explicit Unpack(uint32_t zero)
-      : low(0x64006400u + 0x00010001u * zero), high(0xD400D400u + 0x00100010u * zero) {}
-  // nibbles at bits 0-3 and 16-19 / at bits 4-7 and 20-23 of a word, minus z
-  __device__ __forceinline__ uint32_t at0(uint32_t w) const {
-    const uint32_t q = (w & 0x000F000Fu) | 0x64006400u;
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&q), *reinterpret_cast<const __half2*>(&low));
+struct Nibbles<__nv_bfloat16> {
+  static constexpr float scale = 64.f;                               // 2^-133 2^127
+  static constexpr uint32_t low = 0x7F007F00u, high = 0x7D007D00u;  // 2^127, 2^123
+  __device__ __forceinline__ static uint32_t minus(uint32_t zero) {  // pair of -zero / scale
+    const __nv_bfloat162 v = __float2bfloat162_rn((float)zero * (-1.f / scale));
     return *reinterpret_cast<const uint32_t*>(&v);
-  }
-  __device__ __forceinline__ uint32_t at4(uint32_t w) const {
-    const uint32_t q = (w & 0x00F000F0u) | 0x64006400u, s = 0x2C002C00u;  // 1/16
-    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&q), *reinterpret_cast<const __half2*>(&s),
-                              *reinterpret_cast<const __half2*>(&high));
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-};
-template <>
-struct Unpack<__nv_bfloat16> {
-  static constexpr float scale = 64.f;
-  uint32_t minus;  // pair of -z / 64
-  __device__ __forceinline__ explicit Unpack(uint32_t zero) {
-    const __nv_bfloat162 v = __float2bfloat162_rn((float)zero * -0.015625f);
-    minus = *reinterpret_cast<const uint32_t*>(&v);
   }
   __device__ __forceinline__ static uint32_t fma(uint32_t q, uint32_t power, uint32_t minus) {
     const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&q),
@@ -130,13 +115,21 @@ struct Unpack<__nv_bfloat16> {
                                      *reinterpret_cast<const __nv_bfloat162*>(&minus));
     return *reinterpret_cast<const uint32_t*>(&v);
   }
-  __device__ __forceinline__ uint32_t at0(uint32_t w) const { return fma(w & 0x000F000Fu, 0x7F007F00u, minus); }
-  __device__ __forceinline__ uint32_t at4(uint32_t w) const { return fma(w & 0x00F000F0u, 0x7D007D00u, minus); }
 };
-
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
+template <>
+struct Nibbles<__half> {
+  static constexpr float scale = 512.f;                              // 2^-24 2^15
+  static constexpr uint32_t low = 0x78007800u, high = 0x68006800u;  // 2^15, 2^11
+  __device__ __forceinline__ static uint32_t minus(uint32_t zero) {
+    const __half2 v = __float2half2_rn((float)zero * (-1.f / scale));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  __device__ __forceinline__ static uint32_t fma(uint32_t q, uint32_t power, uint32_t minus) {
+    const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&q), *reinterpret_cast<const __half2*>(&power),
+                              *reinterpret_cast<const __half2*>(&minus));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+};
 
 // Eight columns of a token, in the order in which the steps read them.
 template <typename H>
@@ -145,20 +138,71 @@ __device__ __forceinline__ uint4 order8(const float (&f)[8]) {
                     elem::pack2<H>(f[3], f[7]));
 }
 
-// Shared memory of a CTA: x [parts][tokens][share of K + 32 columns], the warps'
-// rings, the sums [column warps][8 NT tokens][rows].
+// Shared memory of a CTA: the warps' rings and their barriers, the sums
+// [2 turns][column warps][8 NT tokens][rows], x [parts][tokens][share of K + 32
+// columns].
 __host__ __device__ constexpr size_t x_row_bytes(int64_t segs) {
   return (size_t)segs * kSeg * 2 + 64;  // 64: the eight lanes of a read cover all banks
 }
 constexpr size_t kRingBytes = (size_t)kWarps * kStages * kItem;
-constexpr size_t sums_bytes(int nt) { return (size_t)kWarps * kRows * 8 * nt * sizeof(float); }
+constexpr size_t kBarBytes = (size_t)kWarps * kStages * 8;
+__host__ __device__ constexpr size_t sums_bytes(int nt) { return 2 * (size_t)kWarps * kRows * 8 * nt * sizeof(float); }
+constexpr size_t kAlign = 1024;  // of the rings, for the swizzle
+
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
+  return v;
+}
+
+// How scales and zeros are read: a segment's in one load (kWhole: no zeros),
+// or one by one, where a row's do not start on a boundary of such loads.
+enum Groups { kWhole, kWholeZeros, kSingle };
 
 // The scales and zeros of a lane's four rows for a segment, as loaded.
-template <typename S, int GPS>
+template <typename S, int GPS, Groups MODE>
 struct GroupWords {
   static constexpr int W = (GPS * (int)sizeof(S) + 3) / 4;
   uint32_t s[4][W];
   uint32_t z[4];  // a byte per group
+
+  __device__ __forceinline__ void load(const S* scales, const uint8_t* zeros, const uint32_t (&more)[4], int first,
+                                       int groups) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = more[i] + (uint32_t)first;
+      if constexpr (MODE != kSingle) {
+        const S* from = scales + at;
+        if constexpr (W == 4) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(from));
+          s[i][0] = v.x; s[i][1] = v.y; s[i][2] = v.z; s[i][3] = v.w;
+        } else if constexpr (W == 2) {
+          const uint2 v = __ldg(reinterpret_cast<const uint2*>(from));
+          s[i][0] = v.x; s[i][1] = v.y;
+        } else if constexpr (GPS * sizeof(S) == 4) {
+          s[i][0] = __ldg(reinterpret_cast<const uint32_t*>(from));
+        } else {
+          s[i][0] = __ldg(reinterpret_cast<const uint16_t*>(from));
+        }
+        if constexpr (MODE == kWholeZeros) {
+          if constexpr (GPS == 4) z[i] = __ldg(reinterpret_cast<const uint32_t*>(zeros + at));
+          else if constexpr (GPS == 2) z[i] = __ldg(reinterpret_cast<const uint16_t*>(zeros + at));
+          else z[i] = __ldg(zeros + at);
+        }
+      } else {
+        z[i] = zeros ? 0 : 0x08080808u;
+#pragma unroll
+        for (int q = 0; q < W; ++q) s[i][q] = 0;
+#pragma unroll
+        for (int q = 0; q < GPS; ++q) {
+          if (first + q >= groups) continue;  // past the last: x is 0
+          if constexpr (sizeof(S) == 4) s[i][q] = __ldg(reinterpret_cast<const uint32_t*>(scales) + at + q);
+          else s[i][q / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(scales) + at + q) << (16 * (q & 1));
+          if (zeros) z[i] |= (uint32_t)__ldg(zeros + at + q) << (8 * q);
+        }
+      }
+    }
+  }
   __device__ __forceinline__ float scale(int row, int q) const {
     if constexpr (sizeof(S) == 4) {
       return __uint_as_float(s[row][q]);
@@ -167,78 +211,83 @@ struct GroupWords {
       return q & 1 ? v.y : v.x;
     }
   }
-  __device__ __forceinline__ uint32_t zero(int row, int q) const { return (z[row] >> (8 * q)) & 255u; }
+  __device__ __forceinline__ uint32_t zero(int row, int q) const {
+    if constexpr (MODE == kWhole) return 8;
+    else if constexpr (GPS == 1) return z[row] & 255u;
+    else return __byte_perm(z[row], 0, 0x4440 + q);
+  }
 };
 
-// GROUP: columns per scale. NT: blocks of 8 tokens of a CTA. S: type of the scales.
-template <typename T, typename S, int GROUP, int NT>
-__global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p) {
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// GROUP: columns per scale. NT: blocks of 8 tokens of a CTA.
+template <typename T, int GROUP, int NT, Groups MODE>
+__global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p, const __grid_constant__ CUtensorMap map) {
   namespace cg = cooperative_groups;
+  using namespace sm100;
   using H = typename Mma<T>::type;
   constexpr int P = Mma<T>::parts;
   constexpr int GPS = kSeg / GROUP;  // groups of a segment
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((kAlign - (smem_u32(smem_raw) & (kAlign - 1))) & (kAlign - 1));
   const cg::cluster_group cluster = cg::this_cluster();
   const int split = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
   const int g = lane >> 2, t = lane & 3;
   const int k_warps = kWarps / p.row_warps, rw = warp / k_warps, kw = warp % k_warps;
   const int rows = kRows * p.row_warps;
   const int64_t m0 = (int64_t)blockIdx.y * p.tokens;
   const int tokens = (int)(p.M - m0 < p.tokens ? p.M - m0 : p.tokens);
-  const int64_t segs = (p.K + kSeg - 1) / kSeg, most = (segs + split - 1) / split;
-  const int64_t seg_lo = min(part * most, segs), seg_hi = min(seg_lo + most, segs);
+  const int segs = (int)((p.K + kSeg - 1) / kSeg), most = (segs + split - 1) / split;
+  const int seg_lo = min(part * most, segs), seg_hi = min(seg_lo + most, segs);
   const int64_t groups = p.K / GROUP;
-  const int64_t step = gridDim.x / split;  // blocks between two of this cluster
+  const int step = (int)gridDim.x / split;  // blocks between two of this cluster
 
   const int row_bytes = (int)x_row_bytes(most);
   const int part_bytes = row_bytes * p.tokens;
-  uint8_t* ring = smem + (size_t)part_bytes * P + (size_t)warp * kStages * kItem;
-  float* sums = reinterpret_cast<float*>(smem + (size_t)part_bytes * P + kRingBytes);
-  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+  const uint32_t ring = smem_u32(smem) + warp * kStages * kItem;
+  const uint32_t bars = smem_u32(smem) + (uint32_t)kRingBytes + warp * kStages * 8;
+  float* sums = reinterpret_cast<float*>(smem + kRingBytes + kBarBytes);
+  uint8_t* xsm = smem + kRingBytes + kBarBytes + sums_bytes(NT);
   const int swizzle = (g >> 1) & 3;
 
   // this warp's steps: its segments of a block, block after block
-  int64_t f_block = blockIdx.x / split, f_seg = seg_lo + kw;
-  int f_slot = 0;
-  const uint8_t* f_rows;  // the first of this lane's rows of the block, at its columns
-  int f_more[4];          // bytes from there to each of the four
-  auto set_rows = [&]() {
-    // rows past the last are computed as the last and not stored
-    const int64_t r0 = f_block * rows + rw * kRows + g;
-    f_rows = p.packed + min(r0, p.N - 1) * (p.K / 2) + t * 16;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f_more[i] = (int)((min(r0 + 8 * i, p.N - 1) - min(r0, p.N - 1)) * (p.K / 2));
-  };
-  set_rows();
-  if (f_seg >= seg_hi) f_block = p.blocks;  // no segment for this warp
-  auto fetch = [&]() {
-    if (f_block < p.blocks) {
-      const bool in = f_seg * kSeg + t * 32 < p.K;
-      const uint8_t* at = in ? f_rows + f_seg * (kSeg / 2) : p.packed;  // size 0: zeros are written
-      const uint32_t to = ring_at + f_slot * kItem + g * 64 + ((t ^ swizzle) * 16);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) copy16(to + i * 512, at + (in ? f_more[i] : 0), in ? 16 : 0);
-      f_seg += k_warps;
-      if (f_seg >= seg_hi) {
-        f_seg = seg_lo + kw;
-        f_block += step;
-        if (f_block < p.blocks) set_rows();
-      }
+  int f_block = (int)(blockIdx.x / split), f_seg = seg_lo + kw, f_slot = 0;
+  if (f_seg >= seg_hi) f_block = (int)p.blocks;  // none
+  auto fetch = [&]() {  // rows and columns past the last are zeros
+    if (f_block >= p.blocks) return;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(bars + 8 * f_slot, kItem);
+      tma_load_2d(ring + f_slot * kItem, &map, f_seg * (kSeg / 2), f_block * rows + rw * kRows, bars + 8 * f_slot);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
     f_slot = f_slot + 1 == kStages ? 0 : f_slot + 1;
+    f_seg += k_warps;
+    if (f_seg >= seg_hi) {
+      f_seg = seg_lo + kw;
+      f_block += step;
+    }
   };
+  if (lane == 0) {
+    tma_prefetch_desc(&map);
+    for (int i = 0; i < kStages; ++i) mbar_init(bars + 8 * i, 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) fetch();
 
   // x: eight columns at a time
   {
-    const int units = (int)(seg_hi - seg_lo) * (kSeg / 8);
+    const int units = (seg_hi - seg_lo) * (kSeg / 8);
     const bool vec = sizeof(T) == 2 && elem::misalign<T>(p.x) == 0 && p.ldx % 8 == 0;
     for (int i = threadIdx.x; i < units * tokens; i += kThreads) {
       const int m = i / units, u = i - m * units;
-      const int64_t k0 = seg_lo * kSeg + u * 8;
+      const int64_t k0 = (int64_t)seg_lo * kSeg + u * 8;
       float f[8];
       const T* xr = static_cast<const T*>(p.x) + (m0 + m) * p.ldx + k0;
       if (sizeof(T) == 2 && vec && k0 < p.K) {  // K is a multiple of 32
@@ -247,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = k0 < p.K ? elem::to_f(xr[j]) : 0.f;
       }
-      uint8_t* to = smem + m * row_bytes + u * 16;
+      uint8_t* to = xsm + m * row_bytes + u * 16;
       if constexpr (P == 1) {
         *reinterpret_cast<uint4*>(to) = order8<H>(f);
       } else {
@@ -266,8 +315,37 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p) {
   }
   __syncthreads();
 
-  int slot = 0;
-  for (int64_t block = blockIdx.x / split; block < p.blocks; block += step) {
+  // adds the sums of `block`, which all CTAs of the cluster have left in turn `turn`
+  constexpr int C = 8 * NT;
+  constexpr int kTurn = kWarps * kRows * C;
+  auto finish = [&](int block, int turn) {
+    const float* from = sums + turn * kTurn;
+    for (int i = threadIdx.x + part * kThreads; i < rows * tokens; i += split * kThreads) {
+      const int m = i / rows;
+      const int64_t n = (int64_t)block * rows + (i - m * rows);
+      float v = 0.f;
+      for (int q = 0; q < split; ++q) {
+        const float* at = split > 1 ? cluster.map_shared_rank(from, q) : from;
+        for (int w = 0; w < k_warps; ++w) v += at[w * C * rows + i];
+      }
+      if (n < p.N) {
+        v *= Nibbles<H>::scale;
+        if (p.bias) v += elem::to_f(static_cast<const T*>(p.bias)[n]);
+        static_cast<T*>(p.y)[(m0 + m) * p.ldy + n] = elem::from_f<T>(v);
+      }
+    }
+  };
+
+  const uint8_t* x_rows[NT];  // this lane's token of each block of 8; those past the last are not stored
+#pragma unroll
+  for (int n = 0; n < NT; ++n) x_rows[n] = xsm + (n * 8 + g < tokens ? n * 8 + g : 0) * row_bytes + t * 16;
+  uint32_t word_at[4];  // of word j of this lane's first row in a slot
+#pragma unroll
+  for (int j = 0; j < 4; ++j) word_at[j] = ring + g * 64 + ((j ^ swizzle) * 16) + t * 4;
+  int slot = 0, turn = 0;
+  uint32_t parity = 0;
+  bool ok = true;
+  for (int block = (int)(blockIdx.x / split); block < p.blocks; block += step, turn ^= 1) {
     float acc[2][NT][4];
 #pragma unroll
     for (int r = 0; r < 2; ++r)
@@ -275,90 +353,66 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p) {
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.f;
-    const int64_t row0 = block * rows + rw * kRows + g;
-    const S* scales = static_cast<const S*>(p.scales) + min(row0, p.N - 1) * groups;
-    const uint8_t* zeros = p.zeros + (p.zeros ? min(row0, p.N - 1) * groups : 0);
-    int more[4];  // groups from the first of the four rows to each
+    const int64_t row0 = (int64_t)block * rows;
+    const T* scales = static_cast<const T*>(p.scales) + row0 * groups;
+    const uint8_t* zeros = p.zeros + (p.zeros ? row0 * groups : 0);
+    uint32_t more[4];  // groups from the block's first row to this lane's four
 #pragma unroll
-    for (int i = 0; i < 4; ++i) more[i] = (int)((min(row0 + 8 * i, p.N - 1) - min(row0, p.N - 1)) * groups);
-    GroupWords<S, GPS> words;
-    auto load_groups = [&](int64_t seg) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const S* at = scales + more[i] + seg * GPS;
-        if (GPS == 1 || p.whole_groups) {  // a segment's groups in one load
-          if constexpr (words.W == 4) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4*>(at));
-            words.s[i][0] = v.x; words.s[i][1] = v.y; words.s[i][2] = v.z; words.s[i][3] = v.w;
-          } else if constexpr (words.W == 2) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
-            words.s[i][0] = v.x; words.s[i][1] = v.y;
-          } else if constexpr (GPS * sizeof(S) == 4) {
-            words.s[i][0] = __ldg(reinterpret_cast<const uint32_t*>(at));
-          } else {
-            words.s[i][0] = __ldg(reinterpret_cast<const uint16_t*>(at));
-          }
-          if (p.zeros) {
-            const uint8_t* z = zeros + more[i] + seg * GPS;
-            if constexpr (GPS == 4) words.z[i] = __ldg(reinterpret_cast<const uint32_t*>(z));
-            else if constexpr (GPS == 2) words.z[i] = __ldg(reinterpret_cast<const uint16_t*>(z));
-            else words.z[i] = __ldg(z);
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < words.W; ++q) words.s[i][q] = 0;
-          words.z[i] = 0;
-#pragma unroll
-          for (int q = 0; q < GPS; ++q) {
-            const int64_t in = min(seg * GPS + q, groups - 1) - seg * GPS;  // past the last: x is 0
-            if constexpr (sizeof(S) == 4) words.s[i][q] = __ldg(reinterpret_cast<const uint32_t*>(at) + in);
-            else words.s[i][q / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(at) + in) << (16 * (q & 1));
-            if (p.zeros) words.z[i] |= (uint32_t)__ldg(zeros + more[i] + seg * GPS + in) << (8 * q);
-          }
-        }
-        if (!p.zeros) words.z[i] = 0x08080808u;
-      }
-    };
-    if (seg_lo + kw < seg_hi) load_groups(seg_lo + kw);
+    for (int i = 0; i < 4; ++i)
+      more[i] = (uint32_t)((min(row0 + rw * kRows + g + 8 * i, p.N - 1) - row0) * groups);
+    GroupWords<T, GPS, MODE> words;
+    if (seg_lo + kw < seg_hi) words.load(scales, zeros, more, (seg_lo + kw) * GPS, (int)groups);
 
-    for (int64_t s = seg_lo + kw; s < seg_hi; s += k_warps) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-      __syncwarp();  // the copies of all lanes have landed, and the slot before was read by all
+    for (int s = seg_lo + kw; s < seg_hi; s += k_warps) {
+      // (the vote also orders the lanes' reads of the slot before, which fetch() fills)
+      if (ok && !__all_sync(0xffffffffu, mbar_wait(bars + 8 * slot, parity))) {
+        // gave up: load nothing more, and wait (as long again) for what is in flight
+        ok = false;
+        f_block = (int)p.blocks;
+        raise_device_error(DEV_MBAR_TIMEOUT);
+        for (int i = 0; i < kStages - 1; ++i) {
+          const int at = (slot + i) % kStages;
+          (void)mbar_wait(bars + 8 * at, slot + i < kStages ? parity : parity ^ 1);
+        }
+      }
       fetch();
-      const GroupWords<S, GPS> cur = words;
-      if (s + k_warps < seg_hi) load_groups(s + k_warps);
-      const uint8_t* xs = smem + (s - seg_lo) * (kSeg * 2) + t * 16;
-      const uint8_t* ws = ring + slot * kItem + g * 64 + t * 4;
-      slot = slot + 1 == kStages ? 0 : slot + 1;
+      const GroupWords<T, GPS, MODE> cur = words;
+      if (s + k_warps < seg_hi) words.load(scales, zeros, more, (s + k_warps) * GPS, (int)groups);
+      const int x_at = (s - seg_lo) * (kSeg * 2);
+      const uint32_t slot_at = slot * kItem;
+      if (++slot == kStages) {
+        slot = 0;
+        parity ^= 1;
+      }
 #pragma unroll
       for (int q = 0; q < GPS; ++q) {
         float sum[2][NT][4];
-        const Unpack<H> u0(cur.zero(0, q)), u1(cur.zero(1, q)), u2(cur.zero(2, q)), u3(cur.zero(3, q));
+        uint32_t minus[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) minus[i] = Nibbles<H>::minus(cur.zero(i, q));
 #pragma unroll
         for (int jj = 0; jj < 4 / GPS; ++jj) {
           const int j = q * (4 / GPS) + jj;
           uint32_t a[2][2][4];  // [tile][step]
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            uint32_t w0 = *reinterpret_cast<const uint32_t*>(ws + r * 1024 + ((j ^ swizzle) * 16));
-            uint32_t w1 = *reinterpret_cast<const uint32_t*>(ws + r * 1024 + 512 + ((j ^ swizzle) * 16));
-            const Unpack<H>&v0 = r ? u2 : u0, &v1 = r ? u3 : u1;
+            uint32_t w0 = lds32(word_at[j] + slot_at + r * 1024), w1 = lds32(word_at[j] + slot_at + r * 1024 + 512);
+            const uint32_t z0 = minus[2 * r], z1 = minus[2 * r + 1];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              a[r][h][0] = v0.at0(w0);
-              a[r][h][1] = v1.at0(w1);
-              a[r][h][2] = v0.at4(w0);
-              a[r][h][3] = v1.at4(w1);
+              a[r][h][0] = Nibbles<H>::fma(w0 & 0x000F000Fu, Nibbles<H>::low, z0);
+              a[r][h][1] = Nibbles<H>::fma(w1 & 0x000F000Fu, Nibbles<H>::low, z1);
+              a[r][h][2] = Nibbles<H>::fma(w0 & 0x00F000F0u, Nibbles<H>::high, z0);
+              a[r][h][3] = Nibbles<H>::fma(w1 & 0x00F000F0u, Nibbles<H>::high, z1);
               w0 >>= 8;
               w1 >>= 8;
             }
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const int m = n * 8 + g < tokens ? n * 8 + g : 0;  // columns past the last are not stored
 #pragma unroll
             for (int o = 0; o < P; ++o) {
-              const uint4 b = *reinterpret_cast<const uint4*>(xs + o * part_bytes + m * row_bytes + j * 64);
+              const uint4 b = *reinterpret_cast<const uint4*>(x_rows[n] + o * part_bytes + x_at + j * 64);
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
                 mma<H>(sum[r][n], a[r][0], b.x, b.y, jj > 0 || o > 0);
@@ -377,46 +431,29 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p) {
       }
     }
 
-    // sums of the column warps, then of the cluster, each in its order
-    constexpr int C = 8 * NT;
+    if (block != (int)(blockIdx.x / split)) {
+      cluster_wait();
+      finish(block - step, turn ^ 1);
+    }
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float* to = sums + (size_t)(kw * C + n * 8 + 2 * t) * rows + rw * kRows + r * 16 + g;
-        to[0] = acc[r][n][0] * Unpack<H>::scale;
-        to[rows] = acc[r][n][1] * Unpack<H>::scale;
-        to[8] = acc[r][n][2] * Unpack<H>::scale;
-        to[rows + 8] = acc[r][n][3] * Unpack<H>::scale;
+        float* to = sums + turn * kTurn + (kw * C + n * 8 + 2 * t) * rows + rw * kRows + r * 16 + g;
+        to[0] = acc[r][n][0];
+        to[rows] = acc[r][n][1];
+        to[8] = acc[r][n][2];
+        to[rows + 8] = acc[r][n][3];
       }
-    __syncthreads();
-    auto store = [&](int i, float v) {
-      const int m = i / rows;
-      const int64_t n = block * rows + (i - m * rows);
-      if (n < p.N) {
-        if (p.bias) v += elem::to_f(static_cast<const T*>(p.bias)[n]);
-        static_cast<T*>(p.y)[(m0 + m) * p.ldy + n] = elem::from_f<T>(v);
-      }
-    };
-    for (int i = threadIdx.x; i < rows * tokens; i += kThreads) {
-      float v = sums[i];
-      for (int w = 1; w < k_warps; ++w) v += sums[w * C * rows + i];
-      if (split > 1) sums[i] = v;
-      else store(i, v);
-    }
-    if (split > 1) {
-      cluster.sync();
-      for (int i = threadIdx.x + part * kThreads; i < rows * tokens; i += split * kThreads) {
-        float v = 0.f;
-        for (int q = 0; q < split; ++q) v += cluster.map_shared_rank(sums, q)[i];
-        store(i, v);
-      }
-      cluster.sync();  // the other CTAs read this one's sums
-    } else {
-      __syncthreads();
+    cluster_arrive();
+    if (block + step >= p.blocks) {
+      cluster_wait();
+      finish(block, turn);
     }
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  // the other CTAs read this one's sums
+  cluster_arrive();
+  cluster_wait();
 }
 
 // Symmetric quantisation: s = max|w| / 7 of a group, rounded to the scales'
@@ -453,16 +490,14 @@ quantize_kernel(const T* __restrict__ w, int64_t total, int group, uint8_t* __re
 }
 
 // ---------------------------------------------------------------- host
-template <typename T, typename S, int GROUP, int NT>
+template <typename T, int GROUP, int NT, Groups MODE>
 inline int launch_shape(Args a, cudaStream_t st) {
-  auto kern = w4_kernel<T, S, GROUP, NT>;
-  constexpr int GPS = kSeg / GROUP;
-  a.whole_groups = a.K % kSeg == 0 && elem::aligned_to(a.scales, GPS * (int)sizeof(S)) &&
-                   elem::aligned_to(a.zeros, GPS);
+  auto kern = w4_kernel<T, GROUP, NT, MODE>;
   const int64_t segs = (a.K + kSeg - 1) / kSeg;
   const int sms = sm_count();
   auto bytes_for = [&](int split) {
-    return (size_t)Mma<T>::parts * a.tokens * x_row_bytes((segs + split - 1) / split) + kRingBytes + sums_bytes(NT);
+    return (size_t)Mma<T>::parts * a.tokens * x_row_bytes((segs + split - 1) / split) + kRingBytes + kBarBytes +
+           sums_bytes(NT) + kAlign;
   };
   // as little of a cluster as lets two CTAs share an SM, or else fits at all
   constexpr size_t kTwo = 113 * 1024, kOne = 226 * 1024;
@@ -475,7 +510,11 @@ inline int launch_shape(Args a, cudaStream_t st) {
   const int64_t m_tiles = (a.M + a.tokens - 1) / a.tokens;
   while (split < kMaxCluster && blocks_for(1) * split * m_tiles < sms && segs >= 2 * split * 2 * kWarps) split *= 2;
   const size_t bytes = bytes_for(split);
-  const int64_t slots = (int64_t)sms * (bytes <= kTwo ? 2 : 1) / split;
+  int resident = 0;
+  int rc = resident_clusters((const void*)kern, kThreads, bytes, split, &resident, "w4_linear: launch shape");
+  if (rc != KT_OK) return rc;
+  if (resident < 1) return fail(KT_ERR_UNSUPPORTED, "w4_linear: no cluster fits");
+  const int64_t slots = resident;
   // rows of a block: many, unless fewer share the blocks out better
   a.row_warps = 1;
   double best = 0;
@@ -491,7 +530,10 @@ inline int launch_shape(Args a, cudaStream_t st) {
   const int64_t per_tile = slots / m_tiles > 0 ? slots / m_tiles : 1;
   const int64_t clusters = a.blocks < per_tile ? a.blocks : per_tile;
   if (m_tiles > 65535) return fail(KT_ERR_UNSUPPORTED, "w4_linear: M=%lld is too large", (long long)a.M);
-  const int rc = ensure_smem((const void*)kern, bytes, "w4_linear: shared memory");
+  if (a.N > INT32_MAX - kRows * kWarps) return fail(KT_ERR_UNSUPPORTED, "w4_linear: N=%lld is too large", (long long)a.N);
+  CUtensorMap map;
+  rc = make_tmap_2d(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.packed, (uint64_t)a.N, (uint64_t)a.K / 2,
+                    (uint64_t)a.K / 2, kSeg / 2, kRows, CU_TENSOR_MAP_SWIZZLE_64B);
   if (rc != KT_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(clusters * split), (unsigned)m_tiles);
@@ -504,20 +546,29 @@ inline int launch_shape(Args a, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, kern, a), "w4_linear launch");
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, a, map), "w4_linear launch");
 }
 
-template <typename T, typename S>
+template <typename T, int GROUP, int NT>
+inline int launch_groups(const Args& a, cudaStream_t st) {
+  constexpr int GPS = kSeg / GROUP;
+  const bool whole = a.K % kSeg == 0 && elem::aligned_to(a.scales, GPS * (int)sizeof(T)) &&
+                     elem::aligned_to(a.zeros, GPS);
+  if (!whole) return launch_shape<T, GROUP, NT, kSingle>(a, st);
+  return a.zeros ? launch_shape<T, GROUP, NT, kWholeZeros>(a, st) : launch_shape<T, GROUP, NT, kWhole>(a, st);
+}
+
+template <typename T>
 inline int launch_typed(Args a, int group, cudaStream_t st) {
   // tokens of a CTA: fewer where a cluster cannot hold the share of more
   a.tokens = (int)(a.M < kMaxTokens ? a.M : kMaxTokens);
   const int64_t segs = (a.K + kSeg - 1) / kSeg;
-  while (a.tokens > 1 && Mma<T>::parts * a.tokens * x_row_bytes((segs + kMaxCluster - 1) / kMaxCluster) > 160 * 1024)
+  while (a.tokens > 1 && Mma<T>::parts * a.tokens * x_row_bytes((segs + kMaxCluster - 1) / kMaxCluster) > 130 * 1024)
     a.tokens /= 2;
   const bool one = a.tokens <= 8;
-  if (group == 32) return one ? launch_shape<T, S, 32, 1>(a, st) : launch_shape<T, S, 32, 2>(a, st);
-  if (group == 64) return one ? launch_shape<T, S, 64, 1>(a, st) : launch_shape<T, S, 64, 2>(a, st);
-  return one ? launch_shape<T, S, 128, 1>(a, st) : launch_shape<T, S, 128, 2>(a, st);
+  if (group == 32) return one ? launch_groups<T, 32, 1>(a, st) : launch_groups<T, 32, 2>(a, st);
+  if (group == 64) return one ? launch_groups<T, 64, 1>(a, st) : launch_groups<T, 64, 2>(a, st);
+  return one ? launch_groups<T, 128, 1>(a, st) : launch_groups<T, 128, 2>(a, st);
 }
 
 inline int check_matrix(const char* what, int64_t N, int64_t K, int group, int dtype, int scale_dtype) {
@@ -531,11 +582,9 @@ inline int check_matrix(const char* what, int64_t N, int64_t K, int group, int d
   return KT_OK;
 }
 
-inline int linear(const Args& a, int group, int dtype, int scale_dtype, cudaStream_t st) {
-  const int rc = check_matrix("w4_linear", a.N, a.K, group, dtype, scale_dtype);
+inline int linear(const Args& a, int group, int dtype, cudaStream_t st) {
+  const int rc = check_matrix("w4_linear", a.N, a.K, group, dtype, dtype);
   if (rc != KT_OK) return rc;
-  if (scale_dtype != KT_F32 && scale_dtype != dtype)
-    return fail(KT_ERR_ARG, "w4_linear: scales are fp32 or of the tokens' type");
   if (a.M < 0) return fail(KT_ERR_ARG, "w4_linear: negative M=%lld", (long long)a.M);
   if (a.M == 0 || a.N == 0) return KT_OK;
   if (a.K == 0) return fail(KT_ERR_ARG, "w4_linear: K must be positive");
@@ -544,13 +593,11 @@ inline int linear(const Args& a, int group, int dtype, int scale_dtype, cudaStre
   const int sz = elem::size_of(dtype);
   if (!aligned16(a.packed)) return fail(KT_ERR_ARG, "w4_linear: packed weights must be 16-byte aligned");
   if (!elem::aligned_to(a.x, sz) || !elem::aligned_to(a.y, sz) || !elem::aligned_to(a.bias, sz) ||
-      !elem::aligned_to(a.scales, elem::size_of(scale_dtype)))
+      !elem::aligned_to(a.scales, sz))
     return fail(KT_ERR_ARG, "w4_linear: a pointer is not aligned to its elements");
-  const bool f32 = scale_dtype == KT_F32;
-  if (dtype == KT_F32) return launch_typed<float, float>(a, group, st);
-  if (dtype == KT_BF16) return f32 ? launch_typed<__nv_bfloat16, float>(a, group, st)
-                                   : launch_typed<__nv_bfloat16, __nv_bfloat16>(a, group, st);
-  return f32 ? launch_typed<__half, float>(a, group, st) : launch_typed<__half, __half>(a, group, st);
+  if (dtype == KT_F32) return launch_typed<float>(a, group, st);
+  if (dtype == KT_BF16) return launch_typed<__nv_bfloat16>(a, group, st);
+  return launch_typed<__half>(a, group, st);
 }
 
 inline int quantize(const void* w, int64_t N, int64_t K, int group, int dtype, uint8_t* packed, void* scales,

@@ -128,7 +128,7 @@ _SIGNATURES = {
     "kt_token_logprobs": (_int, [_vp, _i64, _vp, _i64, _i64, _f32, _i64, _int, _vp, _vp, _vp, _vp, _vp, _int, _vp]),
     "kt_token_logprobs_bwd": (_int, [_vp, _i64] + [_vp] * 5 + [_i64, _i64, _f32, _i64, _vp, _i64, _int, _vp]),
     "kt_w4_quantize": (_int, [_vp, _i64, _i64, _int, _int, _vp, _vp, _int, _vp]),
-    "kt_w4_linear": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _int, _vp]),
+    "kt_w4_linear": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _vp]),
     "kt_naive_softmax_f32": (_int, [_vp, _vp, _i64, _i64, _vp]),
     "kt_naive_layernorm_f32": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _f32, _vp]),
     "kt_naive_reduce_sum_f32": (_int, [_vp, _i64, _vp, _vp, _vp, _size, _vp]),
@@ -254,10 +254,9 @@ class KtLibrary:
                     "kt_w4_quantize")
 
     def w4_linear(self, x: int, ldx: int, packed: int, scales: int, zeros: Optional[int], bias: Optional[int], y: int,
-                  ldy: int, M: int, N: int, K: int, group: int, dtype: int, scale_dtype: int,
-                  stream: Optional[int] = None) -> None:
+                  ldy: int, M: int, N: int, K: int, group: int, dtype: int, stream: Optional[int] = None) -> None:
         self._check(self._lib.kt_w4_linear(x, ldx, packed, scales, zeros, bias, y, ldy, M, N, K, group, dtype,
-                                           scale_dtype, stream), "kt_w4_linear")
+                                           stream), "kt_w4_linear")
 
     def run(self, op: int | str, args: KtArgs, stream: Optional[int] = None) -> None:
         op_id = OP_IDS[op] if isinstance(op, str) else int(op)

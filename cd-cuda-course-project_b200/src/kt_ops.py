@@ -327,7 +327,7 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], re
 
 class W4Weight(NamedTuple):
     """An (N, K) matrix of 4-bit weights: packed (N, K/2) uint8, the even column
-    in the low half of a byte; scales (N, K/group), fp32 or of the tokens' type;
+    in the low half of a byte; scales (N, K/group) of the tokens' type;
     zeros (N, K/group) uint8 with values of 0..15, or None for 8. A weight is
     scale * (q - zero)."""
     packed: torch.Tensor
@@ -363,7 +363,7 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
     _rows(x, "x")
     M, K = x.shape
     _check(packed, "packed", torch.uint8)
-    _check(scales, "scales", torch.float32 if scales.dtype == torch.float32 else x.dtype)
+    _check(scales, "scales", x.dtype)
     if packed.dim() != 2 or packed.shape[1] * 2 != K:
         raise ValueError(f"w4_linear: packed must be (N, {K // 2}), got {tuple(packed.shape)}")
     N = packed.shape[0]
@@ -393,5 +393,5 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
             raise ValueError(f"out must be {(M, N)}, got {tuple(out.shape)}")
     lib = lib or kt_lib.load()
     _launch(x, lib.w4_linear, x.data_ptr(), _ld(x), packed.data_ptr(), scales.data_ptr(), _ptr(zeros), _ptr(bias),
-            out.data_ptr(), N, M, N, K, group, dt, _dtype(scales, "scales"))
+            out.data_ptr(), N, M, N, K, group, dt)
     return out

@@ -256,14 +256,14 @@ KT_API int kt_w4_quantize(const void* w, int64_t N, int64_t K, int group, int dt
                           int scale_dtype, kt_stream_t stream);
 
 /* y = x * w^T + bias for M tokens (x: M x K, y: M x N, rows ldx and ldy elements
- * apart) with 4-bit weights standing for s*(q-z); scales of fp32 or of `dtype`;
+ * apart) with 4-bit weights standing for s*(q-z); scales of `dtype`;
  * zeros (N x K/group, values of 0..15) may be NULL: 8; bias (N, of `dtype`) may
  * be NULL; K up to 131072. Made for few tokens:
  * the weights are read once for every 16. A group's sum of x*(q-z) is fp32 and
  * scaled afterwards, so it must not overflow. `packed` is 16-byte aligned. */
 KT_API int kt_w4_linear(const void* x, int64_t ldx, const uint8_t* packed, const void* scales, const uint8_t* zeros,
                         const void* bias, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int group, int dtype,
-                        int scale_dtype, kt_stream_t stream);
+                        kt_stream_t stream);
 
 /* Naive GPU baselines (one thread per row / per output element) used as the
  * Welch-t reference point, restating the algorithms of

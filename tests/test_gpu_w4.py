@@ -31,10 +31,10 @@ def values(w):
     return (q * w.scales.double().unsqueeze(-1)).view(n, 2 * half)
 
 
-def make(dev, m, n, k, group, t, st=None, zeros=True, seed=0):
+def make(dev, m, n, k, group, t, zeros=True, seed=0):
     g = torch.Generator(device=dev).manual_seed(seed * 131 + m * 17 + n * 3 + k)
     packed = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device=dev, generator=g)
-    scales = (torch.rand(n, k // group, device=dev, generator=g) * 0.1 + 0.01).to(st or t)
+    scales = (torch.rand(n, k // group, device=dev, generator=g) * 0.1 + 0.01).to(t)
     z = torch.randint(0, 16, (n, k // group), dtype=torch.uint8, device=dev, generator=g) if zeros else None
     x = torch.randn(m, k, device=dev, generator=g).to(t)
     bias = torch.randn(n, device=dev, generator=g).to(t)
@@ -73,11 +73,16 @@ def test_columns_that_end_inside_a_segment(dev, lib, group, k, t):
 
 
 @pytest.mark.parametrize("t", TYPES)
-def test_scale_types_and_no_bias(dev, lib, t):
-    for st, group in ((torch.float32, 32), (torch.float32, 128), (t, 64)):
-        x, w, bias = make(dev, 3, 100, 512, group, t, st=st)
-        check(x, w, bias, lib)
-        check(x, w, None, lib)
+def test_no_bias_and_unaligned_scales(dev, lib, t):
+    for group in (32, 64, 128):
+        x, w, bias = make(dev, 3, 100, 512, group, t)
+        want = check(x, w, None, lib)
+        base = torch.empty(100 * 512 // group + 1, dtype=t, device=dev)
+        scales = base[1:].view(100, -1).copy_(w.scales)
+        zbase = torch.empty(100 * 512 // group + 1, dtype=torch.uint8, device=dev)
+        zeros = zbase[1:].view(100, -1).copy_(w.zeros)
+        assert torch.equal(kt_ops.w4_linear(x, w._replace(scales=scales), lib=lib), want)
+        assert torch.equal(kt_ops.w4_linear(x, w._replace(zeros=zeros), lib=lib), want)
 
 
 @pytest.mark.parametrize("t", TYPES)
