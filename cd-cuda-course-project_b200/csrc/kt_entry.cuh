@@ -288,7 +288,7 @@ int kt_w4_linear(const void* x, int64_t ldx, const uint8_t* packed, const void* 
                  kt_stream_t stream) {
   kt::clear_error();
 #if KT_WITH_LM
-  return kt::w4::linear({x, ldx, packed, scales, zeros, bias, y, ldy, M, N, K, 0, 0, 0}, group, dtype, stream);
+  return kt::w4::linear({x, ldx, packed, scales, zeros, bias, y, ldy, M, N, K, 0, 0, 0, 0}, group, dtype, stream);
 #else
   return kt::unsupported("4-bit weights");
 #endif

@@ -29,12 +29,13 @@
 // memory, in the order of the steps; each 16 bytes of it serve two tiles of 16
 // rows.
 //
-// A CTA stays and takes blocks of 32 x row_warps rows in turn; its other warps,
-// and the CTAs of a cluster, split the columns (a cluster also holds an x that
-// one CTA cannot). Their sums are added in a fixed order through (distributed)
-// shared memory, one block late: a warp that has left its sums arrives at the
-// cluster's barrier and goes on with the next block, and waits there before it
-// adds the sums of the block before.
+// One CTA of 16 warps per SM holds x. Its warps form groups of k_warps that split
+// the columns of 32 rows; groups take their rows in turn, each at its own pace,
+// and add their sums in a fixed order through shared memory. Where x does not
+// fit one CTA, or rows are few, a cluster splits the columns as well: its CTAs go
+// row by row together, and add their sums through distributed shared memory one
+// turn late (a warp that has left its sums arrives at the cluster's barrier, goes
+// on with the next rows, and waits there before it adds the sums before).
 #pragma once
 #include <cooperative_groups.h>
 
@@ -44,11 +45,11 @@
 namespace kt {
 namespace w4 {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSeg = 128;          // columns of a warp step
 constexpr int kRows = 32;          // rows of a warp step
-constexpr int kStages = 3;         // of a warp's ring
+constexpr int kMinStages = 2, kMaxStages = 4;  // of a warp's ring
 constexpr int kItem = kRows * kSeg / 2;  // bytes of a step
 constexpr int kMaxTokens = 16;     // of one CTA; more tokens take more CTAs
 constexpr int kMaxCluster = 8;
@@ -64,9 +65,10 @@ struct Args {
   void* y;
   int64_t ldy;
   int64_t M, N, K;
-  int tokens;      // of a CTA
-  int row_warps;   // warps of a CTA along N
-  int64_t blocks;  // of 32 x row_warps rows
+  int tokens;   // of a CTA
+  int k_warps;  // warps that split the columns of 32 rows
+  int units;    // of 32 rows
+  int stages;
 };
 
 // fp32 is multiplied as bf16 parts
@@ -106,8 +108,7 @@ struct Nibbles<__nv_bfloat16> {
   static constexpr float scale = 64.f;                               // 2^-133 2^127
   static constexpr uint32_t low = 0x7F007F00u, high = 0x7D007D00u;  // 2^127, 2^123
   __device__ __forceinline__ static uint32_t minus(uint32_t zero) {  // pair of -zero / scale
-    const __nv_bfloat162 v = __float2bfloat162_rn((float)zero * (-1.f / scale));
-    return *reinterpret_cast<const uint32_t*>(&v);
+    return fma(zero * 0x00010001u, low ^ 0x80008000u, 0x80008000u);  // (+ -0)
   }
   __device__ __forceinline__ static uint32_t fma(uint32_t q, uint32_t power, uint32_t minus) {
     const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&q),
@@ -121,8 +122,7 @@ struct Nibbles<__half> {
   static constexpr float scale = 512.f;                              // 2^-24 2^15
   static constexpr uint32_t low = 0x78007800u, high = 0x68006800u;  // 2^15, 2^11
   __device__ __forceinline__ static uint32_t minus(uint32_t zero) {
-    const __half2 v = __float2half2_rn((float)zero * (-1.f / scale));
-    return *reinterpret_cast<const uint32_t*>(&v);
+    return fma(zero * 0x00010001u, low ^ 0x80008000u, 0x80008000u);
   }
   __device__ __forceinline__ static uint32_t fma(uint32_t q, uint32_t power, uint32_t minus) {
     const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&q), *reinterpret_cast<const __half2*>(&power),
@@ -139,21 +139,14 @@ __device__ __forceinline__ uint4 order8(const float (&f)[8]) {
 }
 
 // Shared memory of a CTA: the warps' rings and their barriers, the sums
-// [2 turns][column warps][8 NT tokens][rows], x [parts][tokens][share of K + 32
+// [1 or 2 turns][warps][8 NT tokens][rows], x [parts][tokens][share of K + 32
 // columns].
 __host__ __device__ constexpr size_t x_row_bytes(int64_t segs) {
   return (size_t)segs * kSeg * 2 + 64;  // 64: the eight lanes of a read cover all banks
 }
-constexpr size_t kRingBytes = (size_t)kWarps * kStages * kItem;
-constexpr size_t kBarBytes = (size_t)kWarps * kStages * 8;
-__host__ __device__ constexpr size_t sums_bytes(int nt) { return 2 * (size_t)kWarps * kRows * 8 * nt * sizeof(float); }
+constexpr size_t kBarBytes = (size_t)kWarps * kMaxStages * 8;
+__host__ __device__ constexpr size_t sums_bytes(int nt) { return (size_t)kWarps * kRows * 8 * nt * sizeof(float); }
 constexpr size_t kAlign = 1024;  // of the rings, for the swizzle
-
-__device__ __forceinline__ uint32_t lds32(uint32_t at) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at));
-  return v;
-}
 
 // How scales and zeros are read: a segment's in one load (kWhole: no zeros),
 // or one by one, where a row's do not start on a boundary of such loads.
@@ -227,59 +220,62 @@ __device__ __forceinline__ void cluster_wait() {
 
 // GROUP: columns per scale. NT: blocks of 8 tokens of a CTA.
 template <typename T, int GROUP, int NT, Groups MODE>
-__global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p, const __grid_constant__ CUtensorMap map) {
+__global__ void __launch_bounds__(kThreads, 1) w4_kernel(const Args p, const __grid_constant__ CUtensorMap map) {
   namespace cg = cooperative_groups;
   using namespace sm100;
   using H = typename Mma<T>::type;
   constexpr int P = Mma<T>::parts;
   constexpr int GPS = kSeg / GROUP;  // groups of a segment
+  constexpr int C = 8 * NT;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((kAlign - (smem_u32(smem_raw) & (kAlign - 1))) & (kAlign - 1));
   const cg::cluster_group cluster = cg::this_cluster();
   const int split = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0);
   const int g = lane >> 2, t = lane & 3;
-  const int k_warps = kWarps / p.row_warps, rw = warp / k_warps, kw = warp % k_warps;
-  const int rows = kRows * p.row_warps;
+  const int k_warps = p.k_warps, rw = warp / k_warps, kw = warp % k_warps;
   const int64_t m0 = (int64_t)blockIdx.y * p.tokens;
   const int tokens = (int)(p.M - m0 < p.tokens ? p.M - m0 : p.tokens);
   const int segs = (int)((p.K + kSeg - 1) / kSeg), most = (segs + split - 1) / split;
   const int seg_lo = min(part * most, segs), seg_hi = min(seg_lo + most, segs);
   const int64_t groups = p.K / GROUP;
-  const int step = (int)gridDim.x / split;  // blocks between two of this cluster
+  // units of 32 rows: this group's first, and how many are between two of its turns
+  const int first = (int)(blockIdx.x / split) * (kWarps / k_warps) + rw;
+  const int step = (int)(gridDim.x / split) * (kWarps / k_warps);
 
+  const int stages = p.stages;
   const int row_bytes = (int)x_row_bytes(most);
   const int part_bytes = row_bytes * p.tokens;
-  const uint32_t ring = smem_u32(smem) + warp * kStages * kItem;
-  const uint32_t bars = smem_u32(smem) + (uint32_t)kRingBytes + warp * kStages * 8;
-  float* sums = reinterpret_cast<float*>(smem + kRingBytes + kBarBytes);
-  uint8_t* xsm = smem + kRingBytes + kBarBytes + sums_bytes(NT);
+  const uint32_t ring_bytes = (uint32_t)(kWarps * stages * kItem);
+  const uint8_t* ring = smem + warp * stages * kItem;
+  const uint32_t bars = smem_u32(smem) + ring_bytes + warp * kMaxStages * 8;
+  float* sums = reinterpret_cast<float*>(smem + ring_bytes + kBarBytes);
+  uint8_t* xsm = smem + ring_bytes + kBarBytes + sums_bytes(NT) * (split > 1 ? 2 : 1);
   const int swizzle = (g >> 1) & 3;
 
-  // this warp's steps: its segments of a block, block after block
-  int f_block = (int)(blockIdx.x / split), f_seg = seg_lo + kw, f_slot = 0;
-  if (f_seg >= seg_hi) f_block = (int)p.blocks;  // none
+  // this warp's steps: its segments of a unit, unit after unit
+  int f_unit = first, f_seg = seg_lo + kw, f_slot = 0;
+  if (f_seg >= seg_hi) f_unit = p.units;  // none
   auto fetch = [&]() {  // rows and columns past the last are zeros
-    if (f_block >= p.blocks) return;
+    if (f_unit >= p.units) return;
     if (lane == 0) {
       mbar_arrive_expect_tx(bars + 8 * f_slot, kItem);
-      tma_load_2d(ring + f_slot * kItem, &map, f_seg * (kSeg / 2), f_block * rows + rw * kRows, bars + 8 * f_slot);
+      tma_load_2d(smem_u32(ring) + f_slot * kItem, &map, f_seg * (kSeg / 2), f_unit * kRows, bars + 8 * f_slot);
     }
-    f_slot = f_slot + 1 == kStages ? 0 : f_slot + 1;
+    f_slot = f_slot + 1 == stages ? 0 : f_slot + 1;
     f_seg += k_warps;
     if (f_seg >= seg_hi) {
       f_seg = seg_lo + kw;
-      f_block += step;
+      f_unit += step;
     }
   };
   if (lane == 0) {
     tma_prefetch_desc(&map);
-    for (int i = 0; i < kStages; ++i) mbar_init(bars + 8 * i, 1);
+    for (int i = 0; i < stages; ++i) mbar_init(bars + 8 * i, 1);
     fence_mbar_init();
   }
   __syncwarp();
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) fetch();
+  for (int i = 0; i < stages - 1; ++i) fetch();
 
   // x: eight columns at a time
   {
@@ -315,18 +311,18 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p, const __g
   }
   __syncthreads();
 
-  // adds the sums of `block`, which all CTAs of the cluster have left in turn `turn`
-  constexpr int C = 8 * NT;
-  constexpr int kTurn = kWarps * kRows * C;
-  auto finish = [&](int block, int turn) {
-    const float* from = sums + turn * kTurn;
-    for (int i = threadIdx.x + part * kThreads; i < rows * tokens; i += split * kThreads) {
-      const int m = i / rows;
-      const int64_t n = (int64_t)block * rows + (i - m * rows);
+  // adds the sums of `unit`, which its warps (in all CTAs of the cluster) have
+  // left in turn `turn`, and stores the rows
+  auto finish = [&](int unit, int turn) {
+    const float* from = sums + (turn * kWarps + rw * k_warps) * (kRows * C);
+    const int threads = k_warps * 32;  // of this CTA that share the work
+    for (int i = (part * k_warps + kw) * 32 + lane; i < kRows * tokens; i += split * threads) {
+      const int m = i / kRows;
+      const int64_t n = (int64_t)unit * kRows + i % kRows;
       float v = 0.f;
       for (int q = 0; q < split; ++q) {
         const float* at = split > 1 ? cluster.map_shared_rank(from, q) : from;
-        for (int w = 0; w < k_warps; ++w) v += at[w * C * rows + i];
+        for (int w = 0; w < k_warps; ++w) v += at[w * (kRows * C) + i];
       }
       if (n < p.N) {
         v *= Nibbles<H>::scale;
@@ -335,17 +331,22 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p, const __g
       }
     }
   };
+  auto group_sync = [&]() {
+    if (k_warps == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + rw), "r"(k_warps * 32) : "memory");
+  };
 
   const uint8_t* x_rows[NT];  // this lane's token of each block of 8; those past the last are not stored
 #pragma unroll
   for (int n = 0; n < NT; ++n) x_rows[n] = xsm + (n * 8 + g < tokens ? n * 8 + g : 0) * row_bytes + t * 16;
-  uint32_t word_at[4];  // of word j of this lane's first row in a slot
+  const uint8_t* word_at[4];  // word j of this lane's first row in a slot
 #pragma unroll
   for (int j = 0; j < 4; ++j) word_at[j] = ring + g * 64 + ((j ^ swizzle) * 16) + t * 4;
-  int slot = 0, turn = 0;
+  int slot = 0, turn = 0, before = -1;
   uint32_t parity = 0;
   bool ok = true;
-  for (int block = (int)(blockIdx.x / split); block < p.blocks; block += step, turn ^= 1) {
+  // in a cluster all groups make the same number of turns, some without rows
+  for (int unit = first; split > 1 ? unit - first < p.units : unit < p.units; unit += step, turn ^= 1) {
     float acc[2][NT][4];
 #pragma unroll
     for (int r = 0; r < 2; ++r)
@@ -353,34 +354,34 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p, const __g
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.f;
-    const int64_t row0 = (int64_t)block * rows;
+    const int64_t row0 = (int64_t)unit * kRows;
     const T* scales = static_cast<const T*>(p.scales) + row0 * groups;
     const uint8_t* zeros = p.zeros + (p.zeros ? row0 * groups : 0);
-    uint32_t more[4];  // groups from the block's first row to this lane's four
+    uint32_t more[4];  // groups from the unit's first row to this lane's four
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      more[i] = (uint32_t)((min(row0 + rw * kRows + g + 8 * i, p.N - 1) - row0) * groups);
+    for (int i = 0; i < 4; ++i) more[i] = (uint32_t)((min(row0 + g + 8 * i, p.N - 1) - row0) * groups);
+    const int seg_end = unit < p.units ? seg_hi : 0;
     GroupWords<T, GPS, MODE> words;
-    if (seg_lo + kw < seg_hi) words.load(scales, zeros, more, (seg_lo + kw) * GPS, (int)groups);
+    if (seg_lo + kw < seg_end) words.load(scales, zeros, more, (seg_lo + kw) * GPS, (int)groups);
 
-    for (int s = seg_lo + kw; s < seg_hi; s += k_warps) {
+    for (int s = seg_lo + kw; s < seg_end; s += k_warps) {
       // (the vote also orders the lanes' reads of the slot before, which fetch() fills)
       if (ok && !__all_sync(0xffffffffu, mbar_wait(bars + 8 * slot, parity))) {
         // gave up: load nothing more, and wait (as long again) for what is in flight
         ok = false;
-        f_block = (int)p.blocks;
+        f_unit = p.units;
         raise_device_error(DEV_MBAR_TIMEOUT);
-        for (int i = 0; i < kStages - 1; ++i) {
-          const int at = (slot + i) % kStages;
-          (void)mbar_wait(bars + 8 * at, slot + i < kStages ? parity : parity ^ 1);
+        for (int i = 0; i < stages - 1; ++i) {
+          const int at = (slot + i) % stages;
+          (void)mbar_wait(bars + 8 * at, slot + i < stages ? parity : parity ^ 1);
         }
       }
       fetch();
       const GroupWords<T, GPS, MODE> cur = words;
       if (s + k_warps < seg_hi) words.load(scales, zeros, more, (s + k_warps) * GPS, (int)groups);
       const int x_at = (s - seg_lo) * (kSeg * 2);
-      const uint32_t slot_at = slot * kItem;
-      if (++slot == kStages) {
+      const int slot_at = slot * kItem;
+      if (++slot == stages) {
         slot = 0;
         parity ^= 1;
       }
@@ -396,7 +397,8 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p, const __g
           uint32_t a[2][2][4];  // [tile][step]
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            uint32_t w0 = lds32(word_at[j] + slot_at + r * 1024), w1 = lds32(word_at[j] + slot_at + r * 1024 + 512);
+            uint32_t w0 = *reinterpret_cast<const uint32_t*>(word_at[j] + slot_at + r * 1024);
+            uint32_t w1 = *reinterpret_cast<const uint32_t*>(word_at[j] + slot_at + r * 1024 + 512);
             const uint32_t z0 = minus[2 * r], z1 = minus[2 * r + 1];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -431,29 +433,39 @@ __global__ void __launch_bounds__(kThreads, 2) w4_kernel(const Args p, const __g
       }
     }
 
-    if (block != (int)(blockIdx.x / split)) {
-      cluster_wait();
-      finish(block - step, turn ^ 1);
-    }
+    auto leave = [&](int turn) {
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+      for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float* to = sums + turn * kTurn + (kw * C + n * 8 + 2 * t) * rows + rw * kRows + r * 16 + g;
-        to[0] = acc[r][n][0];
-        to[rows] = acc[r][n][1];
-        to[8] = acc[r][n][2];
-        to[rows + 8] = acc[r][n][3];
+        for (int n = 0; n < NT; ++n) {
+          float* to = sums + (turn * kWarps + warp) * (kRows * C) + (n * 8 + 2 * t) * kRows + r * 16 + g;
+          to[0] = acc[r][n][0];
+          to[kRows] = acc[r][n][1];
+          to[8] = acc[r][n][2];
+          to[kRows + 8] = acc[r][n][3];
+        }
+    };
+    if (split == 1) {
+      leave(0);
+      group_sync();
+      finish(unit, 0);
+      group_sync();
+    } else {
+      if (before >= 0) {
+        cluster_wait();
+        finish(before, turn ^ 1);
       }
-    cluster_arrive();
-    if (block + step >= p.blocks) {
-      cluster_wait();
-      finish(block, turn);
+      leave(turn);
+      cluster_arrive();
+      before = unit;
     }
   }
-  // the other CTAs read this one's sums
-  cluster_arrive();
-  cluster_wait();
+  if (split > 1) {
+    cluster_wait();
+    finish(before, turn ^ 1);
+    cluster_arrive();  // the other CTAs read this one's sums
+    cluster_wait();
+  }
 }
 
 // Symmetric quantisation: s = max|w| / 7 of a group, rounded to the scales'
@@ -493,44 +505,50 @@ quantize_kernel(const T* __restrict__ w, int64_t total, int group, uint8_t* __re
 template <typename T, int GROUP, int NT, Groups MODE>
 inline int launch_shape(Args a, cudaStream_t st) {
   auto kern = w4_kernel<T, GROUP, NT, MODE>;
-  const int64_t segs = (a.K + kSeg - 1) / kSeg;
-  const int sms = sm_count();
-  auto bytes_for = [&](int split) {
-    return (size_t)Mma<T>::parts * a.tokens * x_row_bytes((segs + split - 1) / split) + kRingBytes + kBarBytes +
-           sums_bytes(NT) + kAlign;
+  const int segs = (int)((a.K + kSeg - 1) / kSeg);
+  auto bytes_for = [&](int split, int stages) {
+    return Mma<T>::parts * a.tokens * x_row_bytes((segs + split - 1) / split) + (size_t)kWarps * stages * kItem +
+           kBarBytes + sums_bytes(NT) * (split > 1 ? 2 : 1) + kAlign;
   };
-  // as little of a cluster as lets two CTAs share an SM, or else fits at all
-  constexpr size_t kTwo = 113 * 1024, kOne = 226 * 1024;
+  constexpr size_t kMost = 227 * 1024;
   int split = 1;
-  while (split < kMaxCluster && bytes_for(split) > kTwo) split *= 2;
-  while (split > 1 && bytes_for(split) > kTwo && bytes_for(split / 2) <= kOne) split /= 2;
-  if (bytes_for(split) > kOne) return fail(KT_ERR_UNSUPPORTED, "w4_linear: K=%lld is too large", (long long)a.K);
-  // more of it while the device is not full and every warp keeps two segments
-  auto blocks_for = [&](int row_warps) { return (a.N + kRows * row_warps - 1) / (kRows * row_warps); };
+  while (split < kMaxCluster && bytes_for(split, kMinStages) > kMost) split *= 2;
+  if (bytes_for(split, kMinStages) > kMost)
+    return fail(KT_ERR_UNSUPPORTED, "w4_linear: K=%lld is too large", (long long)a.K);
+  // How the columns are split: turns x (steps of a warp + what a turn costs
+  // beside them, in steps), least. The last turn is mostly not full, and few
+  // rows fill the device only with their columns split.
   const int64_t m_tiles = (a.M + a.tokens - 1) / a.tokens;
-  while (split < kMaxCluster && blocks_for(1) * split * m_tiles < sms && segs >= 2 * split * 2 * kWarps) split *= 2;
-  const size_t bytes = bytes_for(split);
+  a.units = (int)((a.N + kRows - 1) / kRows);
+  const int sms = sm_count();
+  int64_t least = INT64_MAX;
+  int best_split = split;
+  for (int sp = split; sp <= kMaxCluster; sp *= 2) {
+    const int64_t ctas = sms / sp / m_tiles > 0 ? sms / sp / m_tiles : 1;
+    for (int kw = 1; kw <= kWarps; kw *= 2) {
+      const int64_t at_once = ctas * (kWarps / kw), turns = (a.units + at_once - 1) / at_once;
+      const int64_t steps = ((segs + sp - 1) / sp + kw - 1) / kw;
+      const int64_t cost = turns * (4 * steps + (kw > 1 ? 4 : 2) + (sp > 1 ? 8 : 0));
+      if (cost < least) {
+        least = cost;
+        best_split = sp;
+        a.k_warps = kw;
+      }
+    }
+  }
+  split = best_split;
+  a.stages = kMaxStages;
+  while (a.stages > kMinStages && bytes_for(split, a.stages) > kMost) --a.stages;
+  const size_t bytes = bytes_for(split, a.stages);
   int resident = 0;
   int rc = resident_clusters((const void*)kern, kThreads, bytes, split, &resident, "w4_linear: launch shape");
   if (rc != KT_OK) return rc;
   if (resident < 1) return fail(KT_ERR_UNSUPPORTED, "w4_linear: no cluster fits");
-  const int64_t slots = resident;
-  // rows of a block: many, unless fewer share the blocks out better
-  a.row_warps = 1;
-  double best = 0;
-  for (int r = kWarps; r >= 1; r /= 2) {
-    const int64_t blocks = blocks_for(r) * m_tiles, turns = (blocks + slots - 1) / slots;
-    const double used = (double)blocks / (double)(turns * slots);
-    if (used > best + 0.05) {
-      best = used;
-      a.row_warps = r;
-    }
-  }
-  a.blocks = blocks_for(a.row_warps);
-  const int64_t per_tile = slots / m_tiles > 0 ? slots / m_tiles : 1;
-  const int64_t clusters = a.blocks < per_tile ? a.blocks : per_tile;
+  const int64_t need = (a.units + kWarps / a.k_warps - 1) / (kWarps / a.k_warps);
+  const int64_t room = resident / m_tiles > 0 ? resident / m_tiles : 1;
+  const int64_t clusters = need < room ? need : room;
   if (m_tiles > 65535) return fail(KT_ERR_UNSUPPORTED, "w4_linear: M=%lld is too large", (long long)a.M);
-  if (a.N > INT32_MAX - kRows * kWarps) return fail(KT_ERR_UNSUPPORTED, "w4_linear: N=%lld is too large", (long long)a.N);
+  if (a.N > INT32_MAX / 2) return fail(KT_ERR_UNSUPPORTED, "w4_linear: N=%lld is too large", (long long)a.N);
   CUtensorMap map;
   rc = make_tmap_2d(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.packed, (uint64_t)a.N, (uint64_t)a.K / 2,
                     (uint64_t)a.K / 2, kSeg / 2, kRows, CU_TENSOR_MAP_SWIZZLE_64B);
@@ -563,7 +581,7 @@ inline int launch_typed(Args a, int group, cudaStream_t st) {
   // tokens of a CTA: fewer where a cluster cannot hold the share of more
   a.tokens = (int)(a.M < kMaxTokens ? a.M : kMaxTokens);
   const int64_t segs = (a.K + kSeg - 1) / kSeg;
-  while (a.tokens > 1 && Mma<T>::parts * a.tokens * x_row_bytes((segs + kMaxCluster - 1) / kMaxCluster) > 130 * 1024)
+  while (a.tokens > 1 && Mma<T>::parts * a.tokens * x_row_bytes((segs + kMaxCluster - 1) / kMaxCluster) > 96 * 1024)
     a.tokens /= 2;
   const bool one = a.tokens <= 8;
   if (group == 32) return one ? launch_groups<T, 32, 1>(a, st) : launch_groups<T, 32, 2>(a, st);
