@@ -16,13 +16,14 @@
 // exponential per value takes about 3/4 of the special-function rate that goes
 // with the full read rate.
 //
-// The top k of a row go through a list in shared memory that holds every value
-// above a threshold: the k-th largest of 64 group maxima of what was read so
-// far, a lower bound of the k-th largest value. It is raised after 1, 2, 4, ...
-// tiles, so about k log2(tiles) values are listed. Values are ordered by
-// (value, lower index), which makes every key different; a tile that overflows
-// the list raises the threshold to the k-th best key of the list and is listed
-// again.
+// The top k of a row need no work in that pass: each thread's maximum is one of
+// its values, so the k-th largest of the 256 maxima is a lower bound of the k-th
+// largest value, and only threads whose maximum reaches it (about k of 256) can
+// hold a value of the top k. Their pieces are read once more (from L2), by all
+// threads, and what reaches the bound goes into a list in shared memory. Values
+// are ordered by (value, lower index), which makes every key different; pieces
+// that overflow the list (rows with many equal values) raise the bound to the
+// k-th best key of the list and are listed again.
 //
 // Few rows are split over a cluster of up to 8 CTAs, which join their partial
 // results through distributed shared memory in the order of their ranks.
@@ -38,7 +39,6 @@ constexpr int kBlock = 256;
 constexpr int kPieces = 4;     // 16-byte pieces of a thread per tile
 constexpr int kMaxTop = 32;
 constexpr int kList = 1024;    // entries of the list of candidates
-constexpr int kGroups = 64;    // groups of threads whose maxima bound the k-th value
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -80,6 +80,44 @@ __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+
+// Two fp32 operations by one instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Largest of a 16-byte piece; NaNs are passed over.
+__device__ __forceinline__ float piece_max(const uint4& r, float) {
+  return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+}
+__device__ __forceinline__ float piece_max(const uint4& r, __nv_bfloat16) {
+  const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(&r);
+  const float2 m = __bfloat1622float2(__hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
+  return fmaxf(m.x, m.y);
+}
+__device__ __forceinline__ float piece_max(const uint4& r, __half) {
+  const __half2* v = reinterpret_cast<const __half2*>(&r);
+  const float2 m = __half22float2(__hmax2(__hmax2(v[0], v[1]), __hmax2(v[2], v[3])));
+  return fmaxf(m.x, m.y);
 }
 
 // Order-preserving key of a value and its index: greater values first, NaN
@@ -127,9 +165,11 @@ struct Shared {
   uint64_t list[kList];
   uint64_t best[kMaxTop];  // this CTA's top k, sorted
   uint64_t threshold;      // keys up to this one are not listed
+  uint32_t maxima[kBlock]; // order_bits of the threads' maxima
+  int threads[kBlock];     // those that may hold a value of the top k
+  int thread_count;
   int count;               // listed so far (may exceed kList)
   int best_count;
-  float groups[kGroups];
   Stats warp[kBlock / 32];
   Stats all;
 };
@@ -144,8 +184,83 @@ __device__ __forceinline__ void raise_to_kth(Shared& sh, int n, int k) {
   }
 }
 
+// Lists the values of this CTA's pieces [first, last) that may be in its top k:
+// leaves sh.count of them in sh.list.
+template <typename T>
+__device__ __forceinline__ void list_candidates(Shared& sh, const T* xr, int64_t first, int64_t last, int shift,
+                                                int64_t vocab, int k) {
+  constexpr int V = elem::kVec<T>;
+  const int tid = threadIdx.x, lane = tid & 31;
+  if (tid < 32) {
+    // the largest b, of the top 20 bits, that k maxima reach, by its bits from above
+    uint32_t m[kBlock / 32], bound = 0;
+#pragma unroll
+    for (int i = 0; i < kBlock / 32; ++i) m[i] = sh.maxima[lane + 32 * i];
+    for (uint32_t bit = 0x80000000u; bit >= 0x1000u; bit >>= 1) {
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kBlock / 32; ++i) n += m[i] >= (bound | bit);
+      if (__reduce_add_sync(0xffffffffu, n) >= k) bound |= bit;
+    }
+    if (lane == 0) {
+      sh.threshold = (uint64_t)bound << 32;
+      sh.thread_count = 0;
+      sh.count = 0;
+    }
+  }
+  __syncthreads();
+  if (sh.maxima[tid] >= (uint32_t)(sh.threshold >> 32)) sh.threads[atomicAdd(&sh.thread_count, 1)] = tid;
+  __syncthreads();
+  const int each = (int)((last - first + kBlock - 1) / kBlock);  // pieces of a thread, at most
+  const int64_t total = (int64_t)sh.thread_count * each;
+  for (int64_t at0 = 0; at0 < total; at0 += kBlock) {
+    const int64_t at = at0 + tid;
+    int64_t pc = last;
+    if (at < total) {
+      const int turn = (int)(at / each);
+      pc = first + (at - (int64_t)turn * each) * kBlock + sh.threads[turn];
+    }
+    const int64_t e0 = pc * V - shift;
+    float f[V];
+    elem::unpack_vec<T>(load_logits<T>(xr, e0, 0, pc < last ? vocab : 0), f);
+    int before = sh.count;  // at most kList, as the last turn ended
+    __syncthreads();
+    for (;;) {
+      const uint64_t threshold = sh.threshold;
+      const uint32_t least = (uint32_t)(threshold >> 32);
+      bool over = false;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (pc < last && order_bits(f[j]) >= least && e0 + j >= 0 && e0 + j < vocab) {
+          const uint64_t key = make_key(f[j], (uint32_t)(e0 + j));
+          if (key > threshold) {
+            const int to = atomicAdd(&sh.count, 1);
+            if (to < kList) sh.list[to] = key;
+            else over = true;
+          }
+        }
+      }
+      if (!__syncthreads_or(over)) break;
+      raise_to_kth(sh, kList, k);
+      // keep what earlier turns listed and still passes (at most k keys)
+      uint64_t old[kList / kBlock];
+#pragma unroll
+      for (int i = 0; i < kList / kBlock; ++i) old[i] = tid + i * kBlock < before ? sh.list[tid + i * kBlock] : 0;
+      __syncthreads();
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kList / kBlock; ++i)
+        if (old[i] > sh.threshold) sh.list[atomicAdd(&sh.count, 1)] = old[i];
+      __syncthreads();
+      before = sh.count;
+      __syncthreads();
+    }
+  }
+}
+
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kBlock) fwd_kernel(const FwdArgs p) {
+__global__ void __launch_bounds__(kBlock, 4) fwd_kernel(const FwdArgs p) {
   namespace cg = cooperative_groups;
   constexpr int V = elem::kVec<T>;
   constexpr int64_t kTile = (int64_t)kBlock * kPieces;
@@ -159,125 +274,53 @@ __global__ void __launch_bounds__(kBlock) fwd_kernel(const FwdArgs p) {
   const int64_t pieces = (p.vocab + shift + V - 1) / V;
   const int64_t share = (pieces + split - 1) / split;
   const int64_t first = part * share, last = first + share < pieces ? first + share : pieces;
-  const int64_t lo = 0, hi = p.vocab;
   const float c = p.scale * kLog2e;
   const int k = p.top;
 
-  if (TOP && tid == 0) {
-    sh.count = 0;
-    sh.threshold = 0;
-  }
   Stats st{-INFINITY, 0.f, 0.f};
-  float seen = -INFINITY;  // largest value of this thread so far
+  uint64_t s2 = 0, t2 = 0;  // even and odd values' s and t
   uint4 next[kPieces];
   auto fetch = [&](int64_t tile0) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       const int64_t pc = tile0 + (int64_t)i * kBlock + tid;
-      next[i] = load_logits<T>(xr, pc * V - shift, lo, pc < last ? hi : 0);
+      next[i] = load_logits<T>(xr, pc * V - shift, 0, pc < last ? p.vocab : 0);
     }
   };
   fetch(first);
-  int64_t next_raise = 1, tile = 0;
-  if (TOP) __syncthreads();
   for (int64_t tile0 = first; tile0 < last; tile0 += kTile) {
     uint4 cur[kPieces];
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) cur[i] = next[i];
     if (tile0 + kTile < last) fetch(tile0 + kTile);
-    float top = -INFINITY;
+    float top = piece_max(cur[0], T());
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      float f[V];
-      elem::unpack_vec<T>(cur[i], f);
-#pragma unroll
-      for (int j = 0; j < V; ++j) top = fmaxf(top, f[j]);
+    for (int i = 1; i < kPieces; ++i) top = fmaxf(top, piece_max(cur[i], T()));
+    if (top > st.m) {
+      const Stats even = moved(Stats{st.m, halves(s2).x, halves(t2).x}, top, c);
+      const Stats odd = moved(Stats{st.m, halves(s2).y, halves(t2).y}, top, c);
+      s2 = pair(even.s, odd.s);
+      t2 = pair(even.t, odd.t);
+      st.m = top;
     }
-    seen = fmaxf(seen, top);
-    if (top > st.m) st = moved(st, top, c);
     const float m = st.m == -INFINITY ? 0.f : st.m;
+    const uint64_t minus = pair(-m, -m), by = pair(c, c);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       float f[V];
       elem::unpack_vec<T>(cur[i], f);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float y = (f[j] - m) * c, e = ex2(y);
-        st.s += e;
-        st.t = fmaf(fmaxf(y, -256.f), e, st.t);  // 2^-256 is 0: -inf adds 0, not NaN
-      }
-    }
-    if constexpr (TOP) {
-      ++tile;
-      if (tile == next_raise) {
-        next_raise *= 2;
-        float v = fmaxf(seen, __shfl_xor_sync(0xffffffffu, seen, 1));
-        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
-        if ((lane & 3) == 0) sh.groups[tid >> 2] = v;
-        __syncthreads();
-        if (warp == 0) {
-          const float a = sh.groups[lane], b = sh.groups[lane + 32];
-          int ga = 0, gb = 0, ea = 0, eb = 0;  // groups above, and groups equal
-          for (int j = 0; j < kGroups; ++j) {
-            const float o = sh.groups[j];
-            ga += o > a;
-            gb += o > b;
-            ea += o == a;
-            eb += o == b;
-          }
-          float kth = -INFINITY;
-          if (ga < k && k <= ga + ea) kth = a;
-          if (gb < k && k <= gb + eb) kth = b;
-          kth = warp_max(kth);
-          const uint64_t bound = (uint64_t)order_bits(kth) << 32;
-          if (lane == 0 && bound > sh.threshold) sh.threshold = bound;
-        }
-        __syncthreads();
-      }
-      int before = sh.count;  // at most kList, as the last tile ended
-      __syncthreads();
-      for (;;) {
-        const uint64_t threshold = sh.threshold;
-        const float least = key_value(threshold | 0xFFFFFFFFull);
-        bool over = false;
-        if (!(top < least) || st.s != st.s || threshold == 0) {
-#pragma unroll 1
-          for (int i = 0; i < kPieces; ++i) {
-            float f[V];
-            elem::unpack_vec<T>(i == 0 ? cur[0] : i == 1 ? cur[1] : i == 2 ? cur[2] : cur[3], f);
-            const int64_t pc = tile0 + (int64_t)i * kBlock + tid;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-              const int64_t e = pc * V - shift + j;
-              if (pc < last && e >= lo && e < hi && !(f[j] < least)) {
-                const uint64_t key = make_key(f[j], (uint32_t)e);
-                if (key > threshold) {
-                  const int at = atomicAdd(&sh.count, 1);
-                  if (at < kList) sh.list[at] = key;
-                  else over = true;
-                }
-              }
-            }
-          }
-        }
-        if (!__syncthreads_or(over)) break;
-        raise_to_kth(sh, kList, k);
-        // keep what earlier tiles listed and still passes (at most k keys)
-        uint64_t old[kList / kBlock];
-#pragma unroll
-        for (int i = 0; i < kList / kBlock; ++i) old[i] = tid + i * kBlock < before ? sh.list[tid + i * kBlock] : 0;
-        __syncthreads();
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kList / kBlock; ++i)
-          if (old[i] > sh.threshold) sh.list[atomicAdd(&sh.count, 1)] = old[i];
-        __syncthreads();
-        before = sh.count;
-        __syncthreads();
+      for (int j = 0; j < V; j += 2) {
+        const float2 y = halves(mul2(add2(pair(f[j], f[j + 1]), minus), by));
+        const uint64_t e = pair(ex2(y.x), ex2(y.y));
+        s2 = add2(s2, e);
+        t2 = fma2(pair(fmaxf(y.x, -256.f), fmaxf(y.y, -256.f)), e, t2);  // 2^-256 is 0: -inf adds 0, not NaN
       }
     }
   }
+  st.s = halves(s2).x + halves(s2).y;
+  st.t = halves(t2).x + halves(t2).y;
+  if constexpr (TOP) sh.maxima[tid] = st.s != st.s ? 0xFFFFFFFFu : order_bits(st.m);  // a NaN may be among them
 
   // the CTA's statistics
   {
@@ -296,7 +339,8 @@ __global__ void __launch_bounds__(kBlock) fwd_kernel(const FwdArgs p) {
     }
   }
   if constexpr (TOP) {
-    const int n = sh.count;  // at most kList: every tile ended without an overflow
+    list_candidates<T>(sh, xr, first, last, shift, p.vocab, k);
+    const int n = sh.count;  // at most kList: every turn ended without an overflow
     if (tid == 0) sh.best_count = n < k ? n : k;
     for (int i = tid; i < n; i += kBlock) {
       const uint64_t key = sh.list[i];
