@@ -87,6 +87,15 @@ __device__ __forceinline__ uint4 ld_once16(const void* p) {
   return v;
 }
 
+// A value that the compiler takes for a new one: what is computed from it is
+// not kept in registers across the rows. (Only a row's first and last piece need
+// those computations, and holding them for all pieces costs more registers than
+// the data.)
+__device__ __forceinline__ int opaque(int v) {
+  asm volatile("" : "+r"(v));
+  return v;
+}
+
 // Elements between the 16-byte boundary at or below `p` and `p`.
 template <typename T>
 __host__ __device__ __forceinline__ int misalign(const void* p) {

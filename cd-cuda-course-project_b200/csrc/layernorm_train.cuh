@@ -82,15 +82,6 @@ __device__ __forceinline__ int quant8(float v, float up) {
 }
 
 // ---------------------------------------------------------------- row pieces
-// A value that the compiler takes for a new one: what is computed from it is
-// not kept in registers across the rows. (Only a row's first and last piece need
-// those computations, and holding them for all pieces costs more registers than
-// the data.)
-__device__ __forceinline__ int opaque(int v) {
-  asm volatile("" : "+r"(v));
-  return v;
-}
-
 // `raw` with the columns outside [0, cols) as 0.
 template <typename T>
 __device__ __forceinline__ uint4 masked(const uint4& raw, int e0, int cols) {
@@ -115,7 +106,7 @@ __device__ __forceinline__ uint4 load_piece(const T* x, int64_t row, int64_t row
   constexpr int V = elem::kVec<T>;
   const int64_t at = row * cols + e0;
   if (e0 >= 0 && e0 + V <= cols) return elem::ld_once16(x + at);
-  const int e = opaque(e0);
+  const int e = elem::opaque(e0);
   if (e >= cols) return make_uint4(0, 0, 0, 0);
   if (at >= 0 && at + V <= rows * cols) return masked<T>(elem::ld_once16(x + at), e, cols);
   uint64_t lo = 0, hi = 0;
@@ -139,7 +130,7 @@ __device__ __forceinline__ void store_piece(T* row, int e0, int cols, const floa
     *reinterpret_cast<uint4*>(row + e0) = elem::pack_vec<T>(f);
     return;
   }
-  const int e = opaque(e0);
+  const int e = elem::opaque(e0);
 #pragma unroll
   for (int j = 0; j < V; ++j)
     if (e + j >= 0 && e + j < cols) row[e + j] = elem::from_f<T>(f[j]);
@@ -258,7 +249,7 @@ fwd_rows(const FwdArgs p) {
 #pragma unroll
         for (int j = 0; j < V; ++j) q = fmaf(v[i][j] - mean, v[i][j] - mean, q);
       } else {  // a piece that the row's end cuts, or none of it in the row
-        const int e = opaque(e0);
+        const int e = elem::opaque(e0);
 #pragma unroll
         for (int j = 0; j < V; ++j)
           if (e + j >= 0 && e + j < cols) q = fmaf(v[i][j] - mean, v[i][j] - mean, q);

@@ -16,19 +16,24 @@
 // exponential per value takes about 3/4 of the special-function rate that goes
 // with the full read rate.
 //
-// The top k of a row need no work in that pass: each thread's maximum is one of
-// its values, so the k-th largest of the 256 maxima is a lower bound of the k-th
-// largest value, and only threads whose maximum reaches it (about k of 256) can
-// hold a value of the top k. Their pieces are read once more (from L2), by all
-// threads, and what reaches the bound goes into a list in shared memory. Values
+// The top k of a row need hardly any work in that pass: a thread notes the
+// largest value of each of up to 8 stretches of its pieces. Of the 8 warps, each
+// finds the ceil(k / 8)-th largest of its threads' maxima; the least of the eight
+// is reached by k values at least, so it bounds the k-th largest from below, and
+// only stretches whose maximum reaches it (about 2 k of 2048) can hold a value of
+// the top k. Their pieces are read once more (from L2), one or two by each
+// thread, and what reaches the bound goes into a list in shared memory. Values
 // are ordered by (value, lower index), which makes every key different; pieces
 // that overflow the list (rows with many equal values) raise the bound to the
 // k-th best key of the list and are listed again.
 //
-// Few rows are split over a cluster of up to 8 CTAs, which join their partial
-// results through distributed shared memory in the order of their ranks.
+// A row goes to a CTA, or to a single warp where it has at most 512 pieces of 16
+// bytes. Few long rows are split over a cluster of up to 8 CTAs, which join their
+// partial results through distributed shared memory in the order of their ranks.
 #pragma once
 #include <cooperative_groups.h>
+
+#include <type_traits>
 
 #include "elem.cuh"
 
@@ -37,8 +42,9 @@ namespace logprob {
 
 constexpr int kBlock = 256;
 constexpr int kPieces = 4;     // 16-byte pieces of a thread per tile
+constexpr int kStretches = 8;  // of a thread's pieces in a row
 constexpr int kMaxTop = 32;
-constexpr int kList = 1024;    // entries of the list of candidates
+constexpr int kWarpPieces = 512;  // of rows that a single warp takes, at most
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -150,160 +156,313 @@ __device__ __forceinline__ Stats moved(const Stats& a, float to, float c) {
   return Stats{to, a.s * f, fmaf(a.s, d, a.t) * f};
 }
 
+// `raw` with the columns outside [0, vocab) as -inf.
 template <typename T>
-__device__ __forceinline__ uint4 load_logits(const T* row, int64_t e0, int64_t lo, int64_t hi) {
-  // columns [e0, e0 + V) of the row; those outside [lo, hi) are -inf
-  constexpr int V = elem::kVec<T>;
-  if (e0 >= lo && e0 + V <= hi) return elem::ld_once16(row + e0);
-  float f[V];
+__device__ __forceinline__ uint4 masked(const uint4& raw, int e0, int vocab) {
+  constexpr uint32_t none = std::is_same<T, float>::value ? 0xFF800000u : std::is_same<T, __half>::value ? 0xFC00u
+                                                                                                         : 0xFF80u;
+  uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-  for (int j = 0; j < V; ++j) f[j] = (e0 + j >= lo && e0 + j < hi) ? elem::to_f(row[e0 + j]) : -INFINITY;
-  return elem::pack_vec<T>(f);
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (sizeof(T) == 4) {
+      if (e0 + k < 0 || e0 + k >= vocab) w[k] = none;
+    } else {
+      if (e0 + 2 * k < 0 || e0 + 2 * k >= vocab) w[k] = (w[k] & 0xFFFF0000u) | none;
+      if (e0 + 2 * k + 1 < 0 || e0 + 2 * k + 1 >= vocab) w[k] = (w[k] & 0x0000FFFFu) | none << 16;
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-struct Shared {
+// Columns [e0, e0 + V) of the row, on a 16-byte boundary; those outside
+// [0, vocab) are -inf. A piece that a row's end cuts also holds its neighbour's
+// columns; only at the two ends [begin, end) of the logits may those not be there.
+template <typename T>
+__device__ __forceinline__ uint4 load_logits(const T* row, int e0, int vocab, const T* begin, const T* end) {
+  constexpr int V = elem::kVec<T>;
+  if (e0 >= 0 && e0 + V <= vocab) return elem::ld_once16(row + e0);
+  const int e = elem::opaque(e0);
+  uint4 raw = make_uint4(0, 0, 0, 0);
+  if (e < vocab) {
+    if (row + e >= begin && row + e + V <= end) {
+      raw = elem::ld_once16(row + e);
+    } else {
+      uint64_t lo = 0, hi = 0;
+#pragma unroll 1
+      for (int j = 0; j < V; ++j) {
+        if (e + j < 0 || e + j >= vocab) continue;
+        uint64_t bits;
+        if constexpr (sizeof(T) == 4) bits = reinterpret_cast<const uint32_t*>(row)[e + j];
+        else bits = reinterpret_cast<const uint16_t*>(row)[e + j];
+        bits <<= (j % (V / 2)) * 8 * (int)sizeof(T);
+        if (j < V / 2) lo |= bits;
+        else hi |= bits;
+      }
+      raw = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+    }
+  }
+  return masked<T>(raw, e, vocab);
+}
+
+// What the G threads of a row (or of a CTA's share of it) need to find its top k.
+template <int G>
+struct Top {
+  static constexpr int kList = 512;
   uint64_t list[kList];
-  uint64_t best[kMaxTop];  // this CTA's top k, sorted
+  uint64_t best[kMaxTop];  // sorted
   uint64_t threshold;      // keys up to this one are not listed
-  uint32_t maxima[kBlock]; // order_bits of the threads' maxima
-  int threads[kBlock];     // those that may hold a value of the top k
-  int thread_count;
-  int count;               // listed so far (may exceed kList)
-  int best_count;
-  Stats warp[kBlock / 32];
-  Stats all;
+  uint32_t maxima[kStretches][G];
+  uint32_t bounds[G / 32];
+  uint16_t places[kStretches * G];
+  int place_count, count, best_count;
 };
 
-// The k-th best key of the first n of the list is left in sh.threshold.
-__device__ __forceinline__ void raise_to_kth(Shared& sh, int n, int k) {
-  for (int i = threadIdx.x; i < n; i += kBlock) {
-    const uint64_t key = sh.list[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += sh.list[j] > key;
-    if (rank == k - 1) sh.threshold = key - 1;  // the k-th itself still passes
-  }
+template <int G>
+__device__ __forceinline__ void sync() {
+  if constexpr (G == 32) __syncwarp();
+  else __syncthreads();
+}
+template <int G>
+__device__ __forceinline__ bool any(bool v) {
+  if constexpr (G == 32) return __any_sync(0xffffffffu, v);
+  else return __syncthreads_or(v);
 }
 
-// Lists the values of this CTA's pieces [first, last) that may be in its top k:
-// leaves sh.count of them in sh.list.
-template <typename T>
-__device__ __forceinline__ void list_candidates(Shared& sh, const T* xr, int64_t first, int64_t last, int shift,
-                                                int64_t vocab, int k) {
-  constexpr int V = elem::kVec<T>;
-  const int tid = threadIdx.x, lane = tid & 31;
-  if (tid < 32) {
-    // the largest b, of the top 20 bits, that k maxima reach, by its bits from above
-    uint32_t m[kBlock / 32], bound = 0;
-#pragma unroll
-    for (int i = 0; i < kBlock / 32; ++i) m[i] = sh.maxima[lane + 32 * i];
-    for (uint32_t bit = 0x80000000u; bit >= 0x1000u; bit >>= 1) {
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < kBlock / 32; ++i) n += m[i] >= (bound | bit);
-      if (__reduce_add_sync(0xffffffffu, n) >= k) bound |= bit;
-    }
-    if (lane == 0) {
-      sh.threshold = (uint64_t)bound << 32;
-      sh.thread_count = 0;
-      sh.count = 0;
-    }
+// Sorted top k of the first n listed keys, by the threads t of G.
+template <int G, int H>
+__device__ __forceinline__ void best_of_list(Top<H>& top, int n, int k, int t) {
+#pragma unroll 1
+  for (int i = t; i < n; i += G) {
+    const uint64_t key = top.list[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) rank += top.list[j] > key;
+    if (key != 0 && rank < k) top.best[rank] = key;
   }
-  __syncthreads();
-  if (sh.maxima[tid] >= (uint32_t)(sh.threshold >> 32)) sh.threads[atomicAdd(&sh.thread_count, 1)] = tid;
-  __syncthreads();
-  const int each = (int)((last - first + kBlock - 1) / kBlock);  // pieces of a thread, at most
-  const int64_t total = (int64_t)sh.thread_count * each;
-  for (int64_t at0 = 0; at0 < total; at0 += kBlock) {
-    const int64_t at = at0 + tid;
-    int64_t pc = last;
-    if (at < total) {
-      const int turn = (int)(at / each);
-      pc = first + (at - (int64_t)turn * each) * kBlock + sh.threads[turn];
+  if (t == 0) top.best_count = n < k ? n : k;
+  sync<G>();
+}
+
+// One row's geometry for this CTA (or warp): pieces [first, last) of 16 bytes,
+// thread t of G holding first + t, first + t + G, ...
+template <typename T>
+struct Row {
+  const T* x;
+  int shift, first, last;
+  // a stretch: so many pieces of a thread, as whole tiles
+  template <int G>
+  __device__ __forceinline__ int stretch() const {
+    const int tiles = (last - first + G * kPieces - 1) / (G * kPieces);
+    return (tiles + kStretches - 1) / kStretches * kPieces;
+  }
+  __device__ __forceinline__ Row(const FwdArgs& p, int64_t row, int split, int part) {
+    x = static_cast<const T*>(p.x) + row * p.ld;
+    shift = elem::misalign<T>(x);
+    const int pieces = ((int)p.vocab + shift + elem::kVec<T> - 1) / elem::kVec<T>;
+    const int share = (pieces + split - 1) / split;
+    first = part * share;
+    last = first + share < pieces ? first + share : pieces;
+  }
+};
+template <typename T>
+__device__ __forceinline__ uint4 load_logits(const FwdArgs& p, const Row<T>& r, int pc) {
+  const T* begin = static_cast<const T*>(p.x);
+  const int vocab = (int)p.vocab;
+  return load_logits<T>(r.x, pc < r.last ? pc * elem::kVec<T> - r.shift : vocab, vocab, begin,
+                        begin + (p.rows - 1) * p.ld + vocab);
+}
+
+// The top k of the pieces of a row that G threads (number t) have streamed:
+// top.maxima[stretch][t] holds their maximum_bits. Left in top.best.
+template <typename T, int G>
+__device__ __forceinline__ void find_top(Top<G>& top, const FwdArgs& p, const Row<T>& r, int t) {
+  constexpr int V = elem::kVec<T>;
+  constexpr int W = G / 32;
+  constexpr int B = G == 32 ? 4 : 2;  // pieces of a thread at a time
+  constexpr int kList = Top<G>::kList;
+  const int lane = t & 31, k = p.top;
+  const int stretch = r.template stretch<G>();
+  const int per_thread = (r.last - r.first + G - 1) / G;  // pieces, at most
+  const int stretches = (per_thread + stretch - 1) / stretch;
+  // the ceil(k / W)-th largest of this warp's maxima; its low 12 bits are dropped,
+  // which only lowers it (and drops bit 0 of maximum_bits)
+  {
+    uint32_t mine = 0, bound = 0;
+    for (int s = 0; s < stretches; ++s) mine = max(mine, top.maxima[s][t] & 0xFFFFF000u);
+    for (int left = (k + W - 1) / W; left > 0;) {
+      bound = __reduce_max_sync(0xffffffffu, mine);
+      left -= __popc(__ballot_sync(0xffffffffu, mine == bound));
+      if (mine == bound) mine = 0;
     }
-    const int64_t e0 = pc * V - shift;
-    float f[V];
-    elem::unpack_vec<T>(load_logits<T>(xr, e0, 0, pc < last ? vocab : 0), f);
-    int before = sh.count;  // at most kList, as the last turn ended
-    __syncthreads();
-    for (;;) {
-      const uint64_t threshold = sh.threshold;
-      const uint32_t least = (uint32_t)(threshold >> 32);
-      bool over = false;
+    if (lane == 0) top.bounds[t / 32] = bound;
+    if (t == 0) top.place_count = top.count = 0;
+  }
+  sync<G>();
+  uint32_t bound = top.bounds[0];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (pc < last && order_bits(f[j]) >= least && e0 + j >= 0 && e0 + j < vocab) {
-          const uint64_t key = make_key(f[j], (uint32_t)(e0 + j));
-          if (key > threshold) {
-            const int to = atomicAdd(&sh.count, 1);
-            if (to < kList) sh.list[to] = key;
+  for (int i = 1; i < W; ++i) bound = min(bound, top.bounds[i]);
+  for (int s = 0; s < stretches; ++s) {
+    const uint32_t v = top.maxima[s][t];
+    if (v >= bound || (v & 1u)) top.places[atomicAdd(&top.place_count, 1)] = (uint16_t)(s * G + t);
+  }
+  if (t == 0) top.threshold = (uint64_t)bound << 32;
+  sync<G>();
+
+  const int total = top.place_count * stretch;
+#pragma unroll 1
+  for (int at0 = 0; at0 < total; at0 += G * B) {
+    uint4 raw[B];
+    int e0[B];  // first column; past the last where there is no piece
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      const int at = at0 + i * G + t;
+      int pc = r.last;
+      if (at < total) {
+        const int which = at / stretch, place = top.places[which];
+        pc = r.first + (place / G * stretch + at - which * stretch) * G + place % G;
+      }
+      e0[i] = pc < r.last ? pc * V - r.shift : (int)p.vocab;
+      raw[i] = load_logits<T>(p, r, pc);
+    }
+#pragma unroll 1
+    for (int i = 0; i < B; ++i) {
+      const uint4 now = B == 2 ? (i == 0 ? raw[0] : raw[1])
+                               : (i == 0 ? raw[0] : i == 1 ? raw[1] : i == 2 ? raw[B - 2] : raw[B - 1]);
+      const int from = B == 2 ? (i == 0 ? e0[0] : e0[1])
+                              : (i == 0 ? e0[0] : i == 1 ? e0[1] : i == 2 ? e0[B - 2] : e0[B - 1]);
+      int before = top.count;  // at most kList, as the last step ended
+      sync<G>();
+      for (;;) {
+        const uint64_t threshold = top.threshold;
+        bool over = false;
+        float f[V];
+        elem::unpack_vec<T>(now, f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if (order_bits(f[j]) < (uint32_t)(threshold >> 32)) continue;
+          const uint64_t key = make_key(f[j], (uint32_t)(from + j));
+          if (from + j >= 0 && from + j < (int)p.vocab && key > threshold) {
+            const int to = atomicAdd(&top.count, 1);
+            if (to < kList) top.list[to] = key;
             else over = true;
           }
         }
+        if (!any<G>(over)) break;
+        // too many: raise the threshold to the k-th best of the list (it and better
+        // ones pass), keep what was listed before this step and still passes (at
+        // most k keys), and list the step again; each time drops kList - 2 k keys
+        for (int q = t; q < kList; q += G) {
+          const uint64_t key = top.list[q];
+          int rank = 0;
+          for (int j = 0; j < kList; ++j) rank += top.list[j] > key;
+          if (rank == k - 1) top.threshold = key - 1;
+        }
+        uint64_t old[kList / G];
+#pragma unroll
+        for (int q = 0; q < kList / G; ++q) old[q] = t + q * G < before ? top.list[t + q * G] : 0;
+        sync<G>();
+        if (t == 0) top.count = 0;
+        sync<G>();
+#pragma unroll
+        for (int q = 0; q < kList / G; ++q)
+          if (old[q] > top.threshold) top.list[atomicAdd(&top.count, 1)] = old[q];
+        sync<G>();
+        before = top.count;
+        sync<G>();
       }
-      if (!__syncthreads_or(over)) break;
-      raise_to_kth(sh, kList, k);
-      // keep what earlier turns listed and still passes (at most k keys)
-      uint64_t old[kList / kBlock];
-#pragma unroll
-      for (int i = 0; i < kList / kBlock; ++i) old[i] = tid + i * kBlock < before ? sh.list[tid + i * kBlock] : 0;
-      __syncthreads();
-      if (tid == 0) sh.count = 0;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kList / kBlock; ++i)
-        if (old[i] > sh.threshold) sh.list[atomicAdd(&sh.count, 1)] = old[i];
-      __syncthreads();
-      before = sh.count;
-      __syncthreads();
     }
+  }
+  sync<G>();
+  best_of_list<G>(top, top.count, k, t);
+}
+
+// The outputs of a row, by one warp, from its statistics and sorted top k.
+// A row's target and its logit, loaded before the row is streamed.
+struct Target {
+  int64_t at;
+  float x;
+  bool is_column;
+};
+template <typename T>
+__device__ __forceinline__ Target load_target(const FwdArgs& p, int64_t row) {
+  Target t{p.ignore, 0.f, false};
+  if (p.targets) t.at = p.targets[row];
+  t.is_column = t.at != p.ignore && t.at >= 0 && t.at < p.vocab;
+  if (t.is_column) t.x = elem::to_f(static_cast<const T*>(p.x)[row * p.ld + t.at]);
+  return t;
+}
+
+template <bool TOP>
+__device__ __forceinline__ void write_row(const FwdArgs& p, int64_t row, const Stats& a, const Target& target,
+                                          const uint64_t* best) {
+  const int lane = threadIdx.x & 31, k = p.top;
+  const float log2s = log2f(a.s);
+  const bool none = a.m == -INFINITY && a.s == 0.f;
+  auto log_p = [&](float x) { return none ? -INFINITY : fmaf(-log2s, kLn2, (x - a.m) * p.scale); };
+  if (lane == 0) {
+    p.lse[row] = none ? -INFINITY : fmaf(log2s, kLn2, a.m * p.scale);
+    if (p.entropy) p.entropy[row] = none ? 0.f : (log2s - a.t / a.s) * kLn2;
+    if (p.targets) {
+      float v = target.is_column ? log_p(target.x) : 0.f;
+      if (!target.is_column && target.at != p.ignore) {
+        v = __uint_as_float(0x7FC00000u);
+        raise_device_error(DEV_BAD_SHAPE);
+      }
+      p.logprob[row] = v;
+    }
+  }
+  if (TOP && lane < k) {
+    const uint64_t key = best[lane];
+    p.top_logprob[row * k + lane] = log_p(key_value(key));
+    p.top_index[row * k + lane] = (int64_t)key_index(key);
   }
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kBlock, 4) fwd_kernel(const FwdArgs p) {
-  namespace cg = cooperative_groups;
-  constexpr int V = elem::kVec<T>;
-  constexpr int64_t kTile = (int64_t)kBlock * kPieces;
-  __shared__ Shared sh;
-  const cg::cluster_group cluster = cg::this_cluster();
-  const int split = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
-  const int64_t row = blockIdx.x / split;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const T* xr = static_cast<const T*>(p.x) + row * p.ld;
-  const int shift = elem::misalign<T>(xr);
-  const int64_t pieces = (p.vocab + shift + V - 1) / V;
-  const int64_t share = (pieces + split - 1) / split;
-  const int64_t first = part * share, last = first + share < pieces ? first + share : pieces;
-  const float c = p.scale * kLog2e;
-  const int k = p.top;
+// What find_top takes of a stretch: its largest value but for NaNs, a lower bound
+// of its largest, and in bit 0 whether a NaN (or an infinity) is among its values.
+__device__ __forceinline__ uint32_t maximum_bits(float largest, float s) {
+  return (order_bits(largest) & ~1u) | (s != s ? 1u : 0u);
+}
 
-  Stats st{-INFINITY, 0.f, 0.f};
-  uint64_t s2 = 0, t2 = 0;  // even and odd values' s and t
+// Statistics of the values that one of G threads (number t) streams, and, with
+// TOP, its stretches' maximum_bits in maxima[stretch][t].
+template <typename T, int G, bool TOP>
+__device__ __forceinline__ Stats stream(const FwdArgs& p, const Row<T>& r, int t, float c, uint32_t (*maxima)[G]) {
+  constexpr int V = elem::kVec<T>;
+  constexpr int kTile = G * kPieces;
+  float largest = -INFINITY, recent = -INFINITY;  // of all, and of this stretch
+  uint64_t s2 = 0, t2 = 0;                        // even and odd values' s and t
+  const int stretch = TOP ? r.template stretch<G>() / kPieces : 0;
+  int left = stretch, at = 0;
   uint4 next[kPieces];
-  auto fetch = [&](int64_t tile0) {
+  const int whole = ((int)p.vocab + r.shift) / V;  // pieces before this one end inside the row
+  auto fetch = [&](int tile0) {
+    if (tile0 * V >= r.shift && tile0 + kTile <= min(r.last, whole)) {  // no row's end in this tile
+      const uint4* at = reinterpret_cast<const uint4*>(r.x - r.shift) + tile0 + t;
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int64_t pc = tile0 + (int64_t)i * kBlock + tid;
-      next[i] = load_logits<T>(xr, pc * V - shift, 0, pc < last ? p.vocab : 0);
+      for (int i = 0; i < kPieces; ++i) next[i] = elem::ld_once16(at + i * G);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) next[i] = load_logits<T>(p, r, tile0 + i * G + t);
     }
   };
-  fetch(first);
-  for (int64_t tile0 = first; tile0 < last; tile0 += kTile) {
+  fetch(r.first);
+  for (int tile0 = r.first; tile0 < r.last; tile0 += kTile) {
     uint4 cur[kPieces];
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) cur[i] = next[i];
-    if (tile0 + kTile < last) fetch(tile0 + kTile);
+    if (tile0 + kTile < r.last) fetch(tile0 + kTile);
     float top = piece_max(cur[0], T());
 #pragma unroll
     for (int i = 1; i < kPieces; ++i) top = fmaxf(top, piece_max(cur[i], T()));
-    if (top > st.m) {
-      const Stats even = moved(Stats{st.m, halves(s2).x, halves(t2).x}, top, c);
-      const Stats odd = moved(Stats{st.m, halves(s2).y, halves(t2).y}, top, c);
+    if (top > largest) {
+      const Stats even = moved(Stats{largest, halves(s2).x, halves(t2).x}, top, c);
+      const Stats odd = moved(Stats{largest, halves(s2).y, halves(t2).y}, top, c);
       s2 = pair(even.s, odd.s);
       t2 = pair(even.t, odd.t);
-      st.m = top;
+      largest = top;
     }
-    const float m = st.m == -INFINITY ? 0.f : st.m;
+    const float m = largest == -INFINITY ? 0.f : largest;
     const uint64_t minus = pair(-m, -m), by = pair(c, c);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
@@ -317,99 +476,94 @@ __global__ void __launch_bounds__(kBlock, 4) fwd_kernel(const FwdArgs p) {
         t2 = fma2(pair(fmaxf(y.x, -256.f), fmaxf(y.y, -256.f)), e, t2);  // 2^-256 is 0: -inf adds 0, not NaN
       }
     }
+    if constexpr (TOP) {
+      recent = fmaxf(recent, top);
+      if (--left == 0 || tile0 + kTile >= r.last) {
+        maxima[at++][t] = maximum_bits(recent, halves(s2).x + halves(s2).y);
+        left = stretch;
+        recent = -INFINITY;
+      }
+    }
   }
-  st.s = halves(s2).x + halves(s2).y;
-  st.t = halves(t2).x + halves(t2).y;
-  if constexpr (TOP) sh.maxima[tid] = st.s != st.s ? 0xFFFFFFFFu : order_bits(st.m);  // a NaN may be among them
+  return Stats{largest, halves(s2).x + halves(s2).y, halves(t2).x + halves(t2).y};
+}
 
-  // the CTA's statistics
-  {
-    const float m = warp_max(st.m);
-    st = moved(st, m, c);
-    st.s = warp_sum(st.s);
-    st.t = warp_sum(st.t);
-    if (lane == 0) sh.warp[warp] = st;
-    __syncthreads();
-    if (warp == 0) {
-      Stats w = lane < kBlock / 32 ? sh.warp[lane] : Stats{-INFINITY, 0.f, 0.f};
-      w = moved(w, warp_max(w.m), c);
-      w.s = warp_sum(w.s);
-      w.t = warp_sum(w.t);
-      if (lane == 0) sh.all = w;
-    }
-  }
-  if constexpr (TOP) {
-    list_candidates<T>(sh, xr, first, last, shift, p.vocab, k);
-    const int n = sh.count;  // at most kList: every turn ended without an overflow
-    if (tid == 0) sh.best_count = n < k ? n : k;
-    for (int i = tid; i < n; i += kBlock) {
-      const uint64_t key = sh.list[i];
-      int rank = 0;
-      for (int j = 0; j < n; ++j) rank += sh.list[j] > key;
-      if (rank < k) sh.best[rank] = key;
-    }
-  }
+// The statistics of the lanes' values together.
+__device__ __forceinline__ Stats warp_stats(const Stats& a, float c) {
+  Stats w = moved(a, warp_max(a.m), c);
+  w.s = warp_sum(w.s);
+  w.t = warp_sum(w.t);
+  return w;
+}
+
+template <bool TOP>
+struct Shared {
+  Top<TOP ? kBlock : 32> top;
+  Stats warp[kBlock / 32];
+  Stats all;
+};
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kBlock, 4) fwd_kernel(const FwdArgs p) {
+  namespace cg = cooperative_groups;
+  __shared__ Shared<TOP> sh;
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int split = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float c = p.scale * kLog2e;
+  const int64_t row = blockIdx.x / split;
+  const Row<T> r(p, row, split, part);
+  Target target{};
+  if (part == 0 && threadIdx.x == 0) target = load_target<T>(p, row);
+  uint32_t(*maxima)[kBlock] = nullptr;
+  if constexpr (TOP) maxima = sh.top.maxima;
+  Stats a = warp_stats(stream<T, kBlock, TOP>(p, r, threadIdx.x, c, maxima), c);
+  if (lane == 0) sh.warp[warp] = a;
   __syncthreads();
-
-  // the row's, joined by the first CTA of the cluster
-  if (split > 1) {
+  if (warp == 0) {
+    a = warp_stats(lane < kBlock / 32 ? sh.warp[lane] : Stats{-INFINITY, 0.f, 0.f}, c);
+    if (lane == 0) sh.all = a;
+  }
+  if constexpr (TOP) find_top<T, kBlock>(sh.top, p, r, threadIdx.x);
+  if (split > 1) {  // the first CTA joins the others' results
     cluster.sync();
-    if (part == 0) {
-      Stats w{-INFINITY, 0.f, 0.f};
-      if (warp == 0) {
-        if (lane < split) w = cluster.map_shared_rank(&sh, lane)->all;
-        w = moved(w, warp_max(w.m), c);
-        w.s = warp_sum(w.s);
-        w.t = warp_sum(w.t);
-        __syncwarp();
-        if (lane == 0) sh.all = w;
-      }
+    if (part == 0 && warp == 0) {
+      a = Stats{-INFINITY, 0.f, 0.f};
+      if (lane < split) a = cluster.map_shared_rank(&sh, lane)->all;
+      a = warp_stats(a, c);
       if constexpr (TOP) {
-        const int from = tid / kMaxTop, at = tid % kMaxTop;  // 8 lists of up to 32
-        uint64_t key = 0;
-        if (from < split) {
-          const Shared* o = cluster.map_shared_rank(&sh, from);
-          if (at < o->best_count) key = o->best[at];
+        const int n = split * p.top;  // up to 8 x 32
+        for (int i = lane; i < n; i += 32) {
+          const auto& o = cluster.map_shared_rank(&sh, i / p.top)->top;
+          sh.top.list[i] = i % p.top < o.best_count ? o.best[i % p.top] : 0;  // 0 is below every key
         }
-        sh.list[tid] = key;  // 0 is below every key
-        __syncthreads();
-        int rank = 0;
-        for (int j = 0; j < kBlock; ++j) rank += sh.list[j] > key;
-        if (key != 0 && rank < k) sh.best[rank] = key;
-      }
-      __syncthreads();
-    }
-  }
-  if (part == 0) {
-    const Stats a = sh.all;
-    const float log2s = log2f(a.s);
-    const bool none = a.m == -INFINITY && a.s == 0.f;
-    const float lse = none ? -INFINITY : fmaf(log2s, kLn2, a.m * p.scale);
-    auto log_p = [&](float x) { return none ? -INFINITY : fmaf(-log2s, kLn2, (x - a.m) * p.scale); };
-    if (tid == 0) {
-      p.lse[row] = lse;
-      if (p.entropy) p.entropy[row] = none ? 0.f : (log2s - a.t / a.s) * kLn2;
-      if (p.targets) {
-        const int64_t target = p.targets[row];
-        float v = 0.f;
-        if (target != p.ignore) {
-          if (target >= 0 && target < p.vocab) {
-            v = log_p(elem::to_f(xr[target]));
-          } else {
-            v = __uint_as_float(0x7FC00000u);
-            raise_device_error(DEV_BAD_SHAPE);
-          }
-        }
-        p.logprob[row] = v;
+        __syncwarp();
+        best_of_list<32>(sh.top, n, p.top, lane);
       }
     }
-    if (TOP && tid >= 32 && tid < 32 + k) {
-      const uint64_t key = sh.best[tid - 32];
-      p.top_logprob[row * k + tid - 32] = log_p(key_value(key));
-      p.top_index[row * k + tid - 32] = (int64_t)key_index(key);
-    }
   }
+  if (part == 0 && warp == 0) write_row<TOP>(p, row, a, target, sh.top.best);
   if (split > 1) cluster.sync();  // the other CTAs' shared memory is read above
+}
+
+// Short rows by single warps.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(TOP ? 128 : kBlock) fwd_warp_kernel(const FwdArgs p) {
+  __shared__ Top<32> tops[TOP ? 4 : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float c = p.scale * kLog2e;
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / 32) + warp;
+  if (row >= p.rows) return;
+  const Row<T> r(p, row, 1, 0);
+  Target target{};
+  if (lane == 0) target = load_target<T>(p, row);
+  Top<32>& top = tops[TOP ? warp : 0];
+  const Stats a = warp_stats(stream<T, 32, TOP>(p, r, lane, c, top.maxima), c);
+  if constexpr (TOP) {
+    __syncwarp();
+    find_top<T, 32>(top, p, r, lane);
+  }
+  write_row<TOP>(p, row, a, target, top.best);
 }
 
 template <typename T, bool VECTOR>
@@ -467,17 +621,24 @@ inline int check_common(const char* what, int64_t rows, int64_t vocab, int64_t l
   if (elem::size_of(dtype) == 0) return fail(KT_ERR_ARG, "%s: unknown dtype %d", what, dtype);
   if (!(scale > 0.f) || isinf(scale)) return fail(KT_ERR_ARG, "%s: scale must be positive and finite", what);
   if (rows > 0 && vocab == 0) return fail(KT_ERR_ARG, "%s: rows without columns", what);
-  if (vocab > (int64_t)INT32_MAX - 64) return fail(KT_ERR_UNSUPPORTED, "%s: vocab > 2^31 - 65", what);
+  if (vocab > (int64_t)1 << 30) return fail(KT_ERR_UNSUPPORTED, "%s: vocab > 2^30", what);
   return KT_OK;
 }
 
 template <typename T, bool TOP>
 inline int fwd_typed(const FwdArgs& a, cudaStream_t st) {
   constexpr int64_t kTile = (int64_t)kBlock * kPieces * elem::kVec<T>;
-  // a cluster per row while the CTAs fit on the device once, and each has a tile
+  if (a.vocab <= (int64_t)kWarpPieces * elem::kVec<T>) {
+    const int block = TOP ? 128 : kBlock;
+    const int64_t grid = (a.rows + block / 32 - 1) / (block / 32);
+    if (grid > INT32_MAX) return fail(KT_ERR_UNSUPPORTED, "token_logprobs: too many rows");
+    fwd_warp_kernel<T, TOP><<<(unsigned)grid, block, 0, st>>>(a);
+    return check_launch("token_logprobs warps");
+  }
+  // a cluster per row while all CTAs fit on the device at once and each has a tile
   int split = 1;
   while (split < kMaxCluster && a.rows * split * 2 <= 2 * sm_count() && a.vocab > kTile * split) split *= 2;
-  if (a.rows * split > (int64_t)INT32_MAX) return fail(KT_ERR_UNSUPPORTED, "token_logprobs: too many rows");
+  if (a.rows * split > INT32_MAX) return fail(KT_ERR_UNSUPPORTED, "token_logprobs: too many rows");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * split));
   cfg.blockDim = dim3(kBlock);

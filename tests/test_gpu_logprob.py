@@ -209,6 +209,23 @@ def test_nan_and_infinity(dev, lib, t):
     assert torch.equal(r.top_index, index)
 
 
+@pytest.mark.parametrize("t", TYPES)
+def test_top_k_among_many_infinities_and_nans(dev, lib, t):
+    for V in (900, 30000):
+        x, targets = logits(dev, 5, V, t)
+        x[0, ::7] = INF
+        x[1, ::7] = float("nan")
+        x[2, ::7] = INF
+        x[2, 5::700] = float("nan")
+        x[3, ::3] = INF
+        x[3, 1::3] = -INF
+        x[4, :-1] = -INF
+        r = kt_ops.token_logprobs(x, targets, top_k=16, lib=lib)
+        index = torch.sort(x.float(), dim=1, descending=True, stable=True).indices[:, :16]
+        assert torch.equal(r.top_index, index)
+        assert r.lse[:4].isnan().all() and r.lse[4] == x[4, -1].float()
+
+
 def test_ignored_and_impossible_targets(dev, lib):
     x, targets = logits(dev, 8, 600, torch.bfloat16)
     want = kt_ops.token_logprobs(x, targets, lib=lib)
