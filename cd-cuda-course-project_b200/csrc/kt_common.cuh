@@ -102,7 +102,7 @@ inline FactsTable& facts() {
 }
 // Caller holds facts().mu.
 inline int ensure_smem_locked(FactsTable& t, const void* fn, int dev, size_t bytes, const char* what) {
-  if (bytes <= 48 * 1024) return KT_OK;
+  if (bytes <= 32 * 1024) return KT_OK;  // the default limit of 48 KB also holds the kernel's static arrays
   for (int i = 0; i < t.n_smem; ++i)
     if (t.smem[i].fn == fn && t.smem[i].dev == dev) {
       if (t.smem[i].bytes >= bytes) return KT_OK;

@@ -17,12 +17,15 @@
 // for NaN. mu and r come from the unrounded x.
 //
 // Bound by memory: forward reads x and writes y, backward reads dy and x (or 8
-// bits of it) and writes dx. TPR threads hold one row in registers as 16-byte
-// pieces. The rows of a CTA are grid.x apart, which makes them equally aligned,
-// so a thread always holds the same columns: gamma and beta stay in its
-// registers, and dgamma and dbeta are summed there over all rows of the CTA and
-// written once, as one partial row per CTA. A second kernel adds the partial
-// rows in their order, so results do not change from run to run.
+// bits of it) and writes dx. TPR threads take one row as 16-byte pieces. Each
+// thread copies its own pieces of the next rows into shared memory with cp.async
+// (no thread waits for another's), so the reads in flight, which at one row
+// ahead in registers held 16-bit rows to 2/3 of the bandwidth, cost no registers.
+// The rows of a CTA are grid.x apart, which makes them equally aligned, so a
+// thread always holds the same columns: gamma and beta stay in its registers, and
+// dgamma and dbeta are summed there over all rows of the CTA and written once, as
+// one partial row per CTA. A second kernel adds the partial rows in their order,
+// so results do not change from run to run.
 #pragma once
 #include <type_traits>
 
@@ -98,29 +101,48 @@ __device__ __forceinline__ uint4 masked(const uint4& raw, int e0, int cols) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Columns [e0, e0+V) of row `row` as raw 16 bytes; columns outside [0, cols) are
-// 0. They lie on a 16-byte boundary. A piece that a row's end cuts also holds
-// its neighbour's columns; only at the tensor's two ends may those not be there.
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+               : "memory");
+}
+template <int BYTES>  // 4 or 8
+__device__ __forceinline__ void copy_async_small(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from),
+               "n"(BYTES)
+               : "memory");
+}
+
+// Starts the copy of columns [e0, e0+V) of row `row`, on a 16-byte boundary, to
+// this thread's place `to`. A piece that a row's end cuts also holds its
+// neighbour's columns (read_piece drops them); only at the tensor's two ends may
+// those not be there, and only the columns of the row are read then.
 template <typename T>
-__device__ __forceinline__ uint4 load_piece(const T* x, int64_t row, int64_t rows, int e0, int cols) {
+__device__ __forceinline__ void copy_piece(uint4* to, const T* x, int64_t row, int64_t rows, int e0, int cols) {
   constexpr int V = elem::kVec<T>;
   const int64_t at = row * cols + e0;
-  if (e0 >= 0 && e0 + V <= cols) return elem::ld_once16(x + at);
+  if (e0 >= 0 && e0 + V <= cols) {
+    copy_async(to, x + at);
+    return;
+  }
+  const int e = elem::opaque(e0);
+  if (e >= cols) return;
+  if (at >= 0 && at + V <= rows * cols) {
+    copy_async(to, x + at);
+    return;
+  }
+#pragma unroll 1
+  for (int j = 0; j < V; ++j)
+    if (e + j >= 0 && e + j < cols) reinterpret_cast<T*>(to)[j] = x[at + j];
+}
+
+// The piece at columns [e0, e0+V); columns outside [0, cols) are 0.
+template <typename T>
+__device__ __forceinline__ uint4 read_piece(const uint4* from, int e0, int cols) {
+  constexpr int V = elem::kVec<T>;
+  if (e0 >= 0 && e0 + V <= cols) return *from;
   const int e = elem::opaque(e0);
   if (e >= cols) return make_uint4(0, 0, 0, 0);
-  if (at >= 0 && at + V <= rows * cols) return masked<T>(elem::ld_once16(x + at), e, cols);
-  uint64_t lo = 0, hi = 0;
-#pragma unroll 1
-  for (int j = 0; j < V; ++j) {
-    if (e + j < 0 || e + j >= cols) continue;
-    uint64_t bits;
-    if constexpr (sizeof(T) == 4) bits = reinterpret_cast<const uint32_t*>(x)[at + j];
-    else bits = reinterpret_cast<const uint16_t*>(x)[at + j];
-    bits <<= (j % (V / 2)) * 8 * (int)sizeof(T);
-    if (j < V / 2) lo |= bits;
-    else hi |= bits;
-  }
-  return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+  return masked<T>(*from, e, cols);
 }
 
 template <typename T>
@@ -142,7 +164,25 @@ constexpr int kRows = TPR < 128 ? 128 / TPR : 1;
 template <int TPR>
 constexpr int kThreads = TPR * kRows<TPR>;
 
+// Threads per SM that the registers are shared among: 16 columns of a thread take
+// 80 (forward) and 128 (backward) with their weights and sums. A thread of wider
+// rows has 32 columns and reads gamma and beta again in every row.
 constexpr int kFwdThreads = 768, kBwdThreads = 512;
+template <typename T, int VPT>
+constexpr bool kHold = VPT * elem::kVec<T> <= 16;
+template <int TPR, int PER_SM>
+constexpr int kCtas = PER_SM / kThreads<TPR>;
+// Rows in shared memory: as many as 200 KB per SM hold, up to 4.
+template <int TPR, int PIECES, int PER_SM>
+constexpr int kDepth = 200 * 1024 / (PIECES * 16 * kThreads<TPR> * kCtas<TPR, PER_SM>) >= 4
+                           ? 4
+                           : 200 * 1024 / (PIECES * 16 * kThreads<TPR> * kCtas<TPR, PER_SM>);
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
 // Waits for the TPR threads of this row.
 template <int TPR>
 __device__ __forceinline__ void row_sync() {
@@ -186,29 +226,40 @@ template <typename T>
 __device__ __forceinline__ void load_weights(const void* w, int wdtype, int e0, int cols, float other,
                                              float (&f)[elem::kVec<T>]) {
   constexpr int V = elem::kVec<T>;
-  const char* at = static_cast<const char*>(w) + (int64_t)e0 * (wdtype == KT_F32 ? 4 : 2);
-  if (w != nullptr && e0 >= 0 && e0 + V <= cols && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
-    if (wdtype == KT_F32) {
+  const int e = elem::opaque(e0);
+  if (w == nullptr) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = other;
+  } else if (wdtype == KT_F32) {
+    const float* at = static_cast<const float*>(w) + e;
+    if (e >= 0 && e + V <= cols && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
 #pragma unroll
       for (int k = 0; k < V / 4; ++k) {
         const float4 v = reinterpret_cast<const float4*>(at)[k];
         f[4 * k] = v.x; f[4 * k + 1] = v.y; f[4 * k + 2] = v.z; f[4 * k + 3] = v.w;
       }
-    } else if constexpr (sizeof(T) == 2) {
-      elem::unpack_vec<T>(*reinterpret_cast<const uint4*>(at), f);
-    }
-    return;
-  }
+    } else {
 #pragma unroll
-  for (int j = 0; j < V; ++j)
-    f[j] = w != nullptr && e0 + j >= 0 && e0 + j < cols ? elem::ld_weight(w, wdtype, e0 + j) : other;
+      for (int j = 0; j < V; ++j) f[j] = e + j >= 0 && e + j < cols ? at[j] : other;
+    }
+  } else if constexpr (sizeof(T) == 2) {  // of the input's type
+    const T* at = static_cast<const T*>(w) + e;
+    if (e >= 0 && e + V <= cols && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {
+      elem::unpack_vec<T>(*reinterpret_cast<const uint4*>(at), f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = e + j >= 0 && e + j < cols ? elem::to_f(at[j]) : other;
+    }
+  }
 }
 
 // ---------------------------------------------------------------- forward
 template <typename T, int TPR, int VPT, bool CKPT>
-__global__ void __launch_bounds__(kThreads<TPR>, kFwdThreads / kThreads<TPR>)
+__global__ void __launch_bounds__(kThreads<TPR>, kCtas<TPR, kFwdThreads>)
 fwd_rows(const FwdArgs p) {
   constexpr int V = elem::kVec<T>;
+  constexpr int D = kDepth<TPR, VPT, kFwdThreads>;
+  extern __shared__ uint4 ring[];  // [D][VPT][threads]
   __shared__ float red[2][32];
   const int t = threadIdx.x % TPR;
   const int cols = (int)p.cols;
@@ -217,29 +268,39 @@ fwd_rows(const FwdArgs p) {
   const int64_t stride = (int64_t)gridDim.x * kRows<TPR>;
   const int shift = elem::misalign<T>(static_cast<const T*>(p.x) + first * cols);
   const int e_first = t * V - shift;  // this thread's pieces start at e_first + i TPR V
-  uint4 raw[VPT];
-  auto fetch = [&](int64_t row) {
+  auto place = [&](int slot, int i) { return ring + (slot * VPT + i) * kThreads<TPR> + threadIdx.x; };
+  auto fetch = [&](int slot, int64_t row) {
+    if (row < p.rows) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      raw[i] = load_piece<T>(static_cast<const T*>(p.x), row, p.rows, e_first + i * TPR * V, cols);
+      for (int i = 0; i < VPT; ++i)
+        copy_piece<T>(place(slot, i), static_cast<const T*>(p.x), row, p.rows, e_first + i * TPR * V, cols);
+    }
+    commit_copies();
   };
-  if (first < p.rows) fetch(first);
+#pragma unroll 1
+  for (int d = 0; d < D; ++d) fetch(d, first + d * stride);
   float g[VPT][V], b[VPT][V];
-#pragma unroll
-  for (int i = 0; i < VPT; ++i) {
+  auto weights = [&](int i) {
     load_weights<T>(p.gamma, p.wdtype, e_first + i * TPR * V, cols, 1.f, g[i]);
     load_weights<T>(p.beta, p.wdtype, e_first + i * TPR * V, cols, 0.f, b[i]);
+  };
+  if constexpr (kHold<T, VPT>) {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) weights(i);
   }
+  int slot = 0;
   for (int64_t row = first; row < p.rows; row += stride) {
+    wait_copies<D - 1>();
     float v[VPT][V];
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      elem::unpack_vec<T>(raw[i], v[i]);
+      elem::unpack_vec<T>(read_piece<T>(place(slot, i), e_first + i * TPR * V, cols), v[i]);
 #pragma unroll
       for (int j = 0; j < V; ++j) s += v[i][j];
     }
-    if (row + stride < p.rows) fetch(row + stride);
+    fetch(slot, row + D * stride);
+    slot = slot + 1 == D ? 0 : slot + 1;
     const float mean = row_sum<TPR>(s, red[0]) / fcols;
     float q = 0.f;
 #pragma unroll
@@ -288,6 +349,7 @@ fwd_rows(const FwdArgs p) {
         }
       }
       if (e0 < cols) {
+        if constexpr (!kHold<T, VPT>) weights(i);
         float o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = fmaf((v[i][j] - mean) * rstd, g[i][j], b[i][j]);
@@ -358,11 +420,12 @@ __device__ __forceinline__ void x_hats(const uint4& raw, float mean, float rstd,
 
 // Columns outside the row have dy = 0, so they add nothing to any sum.
 template <typename T, int TPR, int VPT, bool CKPT>
-__global__ void __launch_bounds__(kThreads<TPR>, kBwdThreads / kThreads<TPR>)
+__global__ void __launch_bounds__(kThreads<TPR>, kCtas<TPR, kBwdThreads>)
 bwd_rows(const BwdArgs p) {
   constexpr int V = elem::kVec<T>;
   constexpr int RB = kRows<TPR>;
-  extern __shared__ float part[];  // RB > 1: 2 x cols sums of the CTA
+  constexpr int D = kDepth<TPR, 2 * VPT, kBwdThreads>;
+  extern __shared__ uint4 ring[];  // [D][dy, x][VPT][threads]; at the end, RB > 1: 2 x cols sums of the CTA
   __shared__ float2 red[2][32];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const int cols = (int)p.cols;
@@ -371,57 +434,79 @@ bwd_rows(const BwdArgs p) {
   const int64_t stride = (int64_t)gridDim.x * RB;
   const int shift = elem::misalign<T>(static_cast<const T*>(p.dy) + first * cols);
   const int e_first = t * V - shift;
-  uint4 ny[VPT], nx[VPT];
+  auto place = [&](int slot, int which, int i) {
+    return ring + ((slot * 2 + which) * VPT + i) * kThreads<TPR> + threadIdx.x;
+  };
+  auto fetch = [&](int slot, int64_t row) {
+    if (row < p.rows) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int e0 = e_first + i * TPR * V;
+        copy_piece<T>(place(slot, 0, i), static_cast<const T*>(p.dy), row, p.rows, e0, cols);
+        if constexpr (CKPT) {
+          if (e0 < cols) copy_async_small<V>(place(slot, 1, i), p.q8 + row * cols + e0);
+        } else {
+          copy_piece<T>(place(slot, 1, i), static_cast<const T*>(p.x), row, p.rows, e0, cols);
+        }
+      }
+    }
+    commit_copies();
+  };
+  // a row's statistics and its blocks' codes, one row ahead
   float nmean = 0.f, nrstd = 0.f;
-  auto fetch = [&](int64_t row) {
+  uint32_t ncode[VPT];
+  auto ahead = [&](int64_t row) {
     nmean = p.mean[row];
     nrstd = p.rstd[row];
+    if constexpr (CKPT) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int e0 = e_first + i * TPR * V;
-      ny[i] = load_piece<T>(static_cast<const T*>(p.dy), row, p.rows, e0, cols);
-      if constexpr (CKPT) {
-        nx[i] = make_uint4(0, 0, 7, 0);
-        if (e0 < cols) {
-          const int8_t* qr = p.q8 + row * cols + e0;
-          if constexpr (V == 8) {
-            const uint2 w = *reinterpret_cast<const uint2*>(qr);
-            nx[i].x = w.x;
-            nx[i].y = w.y;
-          } else {
-            nx[i].x = *reinterpret_cast<const uint32_t*>(qr);
-          }
-          nx[i].z = p.q8_exp[row * ((cols + 31) / 32) + e0 / 32];
-        }
-      } else {
-        nx[i] = load_piece<T>(static_cast<const T*>(p.x), row, p.rows, e0, cols);
+      for (int i = 0; i < VPT; ++i) {
+        const int e0 = e_first + i * TPR * V;
+        ncode[i] = e0 < cols ? p.q8_exp[row * ((cols + 31) / 32) + e0 / 32] : 7u;
       }
     }
   };
-  if (first < p.rows) fetch(first);
+#pragma unroll 1
+  for (int d = 0; d < D; ++d) fetch(d, first + d * stride);
+  if (first < p.rows) ahead(first);
   float g[VPT][V], dg[VPT][V], db[VPT][V];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    load_weights<T>(p.gamma, p.wdtype, e_first + i * TPR * V, cols, 1.f, g[i]);
+    if constexpr (kHold<T, VPT>) load_weights<T>(p.gamma, p.wdtype, e_first + i * TPR * V, cols, 1.f, g[i]);
 #pragma unroll
     for (int j = 0; j < V; ++j) dg[i][j] = db[i][j] = 0.f;
   }
-  int turn = 0;
+  int turn = 0, slot = 0;
   for (int64_t row = first; row < p.rows; row += stride, turn ^= 1) {
-    uint4 ry[VPT], rx[VPT];
     float s1 = 0.f, s2 = 0.f;
     const float mean = nmean, rstd = nrstd;
+    uint32_t code[VPT];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      ry[i] = ny[i];
-      rx[i] = nx[i];
-    }
-    if (row + stride < p.rows) fetch(row + stride);
+    for (int i = 0; i < VPT; ++i) code[i] = ncode[i];
+    if (row + stride < p.rows) ahead(row + stride);
+    // a piece of dy and xh; read for the sums and again for dx, as holding them takes twice the registers
+    auto read = [&](int i, float (&d)[V], float (&xh)[V]) {
+      const int e0 = e_first + i * TPR * V;
+      elem::unpack_vec<T>(read_piece<T>(place(slot, 0, i), e0, cols), d);
+      uint4 x;
+      if constexpr (CKPT) {
+        x = make_uint4(0, 0, code[i], 0);
+        if (e0 < cols) {
+          const uint4* at = place(slot, 1, i);
+          x.x = reinterpret_cast<const uint32_t*>(at)[0];
+          if constexpr (V == 8) x.y = reinterpret_cast<const uint32_t*>(at)[1];
+        }
+      } else {
+        x = read_piece<T>(place(slot, 1, i), e0, cols);
+      }
+      x_hats<T, CKPT>(x, mean, rstd, xh);
+    };
+    wait_copies<D - 1>();
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       float d[V], xh[V];
-      elem::unpack_vec<T>(ry[i], d);
-      x_hats<T, CKPT>(rx[i], mean, rstd, xh);
+      read(i, d, xh);
+      if constexpr (!kHold<T, VPT>) load_weights<T>(p.gamma, p.wdtype, e_first + i * TPR * V, cols, 1.f, g[i]);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         dg[i][j] = fmaf(d[j], xh[j], dg[i][j]);
@@ -438,15 +523,18 @@ bwd_rows(const BwdArgs p) {
     for (int i = 0; i < VPT; ++i) {
       const int e0 = e_first + i * TPR * V;
       if (e0 < cols) {
-        float d[V], xh[V];  // once more from the 16 bytes: holding them would cost twice the registers
-        elem::unpack_vec<T>(ry[i], d);
-        x_hats<T, CKPT>(rx[i], mean, rstd, xh);
+        float d[V], xh[V];
+        read(i, d, xh);
+        if constexpr (!kHold<T, VPT>) load_weights<T>(p.gamma, p.wdtype, e0, cols, 1.f, g[i]);
 #pragma unroll
         for (int j = 0; j < V; ++j) d[j] = rstd * (fmaf(d[j], g[i][j], -c2) - xh[j] * c1);
         store_piece<T>(dxr, e0, cols, d);
       }
     }
+    fetch(slot, row + D * stride);
+    slot = slot + 1 == D ? 0 : slot + 1;
   }
+  wait_copies<0>();
   if (p.partial == nullptr) return;
   float* out = p.partial + (int64_t)blockIdx.x * 2 * cols;
   if constexpr (RB == 1) {
@@ -461,6 +549,8 @@ bwd_rows(const BwdArgs p) {
         }
     }
   } else {
+    float* part = reinterpret_cast<float*>(ring);
+    __syncthreads();
     for (int w = 0; w < RB; ++w) {  // in the order of the rows
       if (sub == w) {
 #pragma unroll
@@ -582,8 +672,8 @@ inline int row_grid(K kern, int block, int rb, size_t smem, int64_t rows, int* g
 }
 
 // Calls f with the threads per row and pieces per thread for a row of `pieces`
-// 16-byte pieces: 16 columns per thread, which leaves two to three CTAs of
-// 256 threads per SM their registers. False when a row is too wide.
+// 16-byte pieces: 16 columns per thread (32 in the widest rows). False when a row
+// is too wide.
 template <typename T, class F>
 inline bool with_shape(int64_t pieces, F f) {
   constexpr int VPT = 16 / elem::kVec<T>;
@@ -595,6 +685,7 @@ inline bool with_shape(int64_t pieces, F f) {
   if (pieces <= 128 * VPT) return f(std::integral_constant<int, 128>{}, All{}), true;
   if (pieces <= 256 * VPT) return f(std::integral_constant<int, 256>{}, All{}), true;
   if (pieces <= 512 * VPT) return f(std::integral_constant<int, 512>{}, All{}), true;
+  if (pieces <= 1024 * VPT) return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 2 * VPT>{}), true;
   return false;
 }
 
@@ -620,10 +711,11 @@ inline int fwd_typed(const FwdArgs& a, cudaStream_t st) {
         constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
         constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
         auto kern = fwd_rows<T, TPR, VPT, CKPT>;
+        constexpr size_t smem = (size_t)kDepth<TPR, VPT, kFwdThreads> * VPT * BLOCK * 16;
         int grid = 0;
-        rc = row_grid(kern, BLOCK, RB, 0, a.rows, &grid);
+        rc = row_grid(kern, BLOCK, RB, smem, a.rows, &grid);
         if (rc != KT_OK) return;
-        kern<<<grid, BLOCK, 0, st>>>(a);
+        kern<<<grid, BLOCK, smem, st>>>(a);
         rc = check_launch("layernorm_train fwd_rows");
       }))
     return rc;
@@ -662,7 +754,8 @@ inline int bwd_typed(const BwdArgs& a, void* dgamma, void* dbeta, cudaStream_t s
           constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
           constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
           auto kern = bwd_rows<T, TPR, VPT, CKPT>;
-          const size_t smem = RB > 1 ? 2 * (size_t)a.cols * sizeof(float) : 0;
+          constexpr size_t smem = (size_t)kDepth<TPR, 2 * VPT, kBwdThreads> * 2 * VPT * BLOCK * 16;
+          static_assert(RB == 1 || smem >= 2 * sizeof(float) * TPR * VPT * V, "the CTA's sums fit the ring");
           rc = row_grid(kern, BLOCK, RB, smem, a.rows, &parts);
           if (rc != KT_OK) return;
           kern<<<parts, BLOCK, smem, st>>>(a);
