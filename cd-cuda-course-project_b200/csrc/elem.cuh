@@ -78,6 +78,49 @@ __device__ __forceinline__ uint4 pack_vec(const float (&f)[kVec<T>]) {
   }
 }
 
+// Two fp32 operations by one instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// A 16-byte piece as pairs of fp32, and back.
+template <typename T>
+__device__ __forceinline__ void unpack_pairs(const uint4& r, uint64_t (&f)[kVec<T> / 2]) {
+  float v[kVec<T>];
+  unpack_vec<T>(r, v);
+#pragma unroll
+  for (int j = 0; j < kVec<T> / 2; ++j) f[j] = pair(v[2 * j], v[2 * j + 1]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack_pairs(const uint64_t (&f)[kVec<T> / 2]) {
+  float v[kVec<T>];
+#pragma unroll
+  for (int j = 0; j < kVec<T> / 2; ++j) {
+    const float2 h = halves(f[j]);
+    v[2 * j] = h.x;
+    v[2 * j + 1] = h.y;
+  }
+  return pack_vec<T>(v);
+}
+
 // Read-only 16-byte load of data used once (not kept in L1).
 __device__ __forceinline__ uint4 ld_once16(const void* p) {
   uint4 v;

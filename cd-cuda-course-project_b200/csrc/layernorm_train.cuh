@@ -84,6 +84,19 @@ __device__ __forceinline__ int quant8(float v, float up) {
   return min(127, max(-127, __float2int_rn(v * up)));
 }
 
+// Four of them to a word.
+__device__ __forceinline__ uint32_t quant8x4(float a, float b, float c, float d, float up, uint32_t code) {
+  // limited to +-127 first, which leaves the same integers as afterwards; the sum
+  // with 1.5 2^23 has the integer, rounded to nearest even, in its low bits
+  constexpr float magic = 12582912.f;
+  const uint32_t q0 = __float_as_uint(fminf(fmaxf(a * up, -127.f), 127.f) + magic);
+  const uint32_t q1 = __float_as_uint(fminf(fmaxf(b * up, -127.f), 127.f) + magic);
+  const uint32_t q2 = __float_as_uint(fminf(fmaxf(c * up, -127.f), 127.f) + magic);
+  const uint32_t q3 = __float_as_uint(fminf(fmaxf(d * up, -127.f), 127.f) + magic);
+  const uint32_t w = __byte_perm(__byte_perm(q0, q1, 0x0040), __byte_perm(q2, q3, 0x0040), 0x5410);
+  return code == 255u ? 0u : w;
+}
+
 // ---------------------------------------------------------------- row pieces
 // `raw` with the columns outside [0, cols) as 0.
 template <typename T>
@@ -112,50 +125,50 @@ __device__ __forceinline__ void copy_async_small(void* to, const void* from) {
                : "memory");
 }
 
-// Starts the copy of columns [e0, e0+V) of row `row`, on a 16-byte boundary, to
-// this thread's place `to`. A piece that a row's end cuts also holds its
-// neighbour's columns (read_piece drops them); only at the tensor's two ends may
-// those not be there, and only the columns of the row are read then.
-template <typename T>
+// Rows whose ends lie on 16-byte boundaries have only whole pieces (EDGE false).
+// Otherwise a piece that a row's end cuts also holds its neighbour's columns.
+
+// Starts the copy of columns [e0, e0+V) of row `row`, on a 16-byte boundary and
+// e0 < cols, to this thread's place `to`. Only at the tensor's two ends may the
+// neighbour's columns not be there, and only the columns of the row are read then.
+template <typename T, bool EDGE>
 __device__ __forceinline__ void copy_piece(uint4* to, const T* x, int64_t row, int64_t rows, int e0, int cols) {
   constexpr int V = elem::kVec<T>;
-  const int64_t at = row * cols + e0;
-  if (e0 >= 0 && e0 + V <= cols) {
-    copy_async(to, x + at);
+  const T* at = x + row * cols + e0;
+  if (!EDGE || (e0 >= 0 && e0 + V <= cols)) {
+    copy_async(to, at);
     return;
   }
   const int e = elem::opaque(e0);
-  if (e >= cols) return;
-  if (at >= 0 && at + V <= rows * cols) {
-    copy_async(to, x + at);
+  if (at >= x && at + V <= x + rows * cols) {
+    copy_async(to, at);
     return;
   }
 #pragma unroll 1
   for (int j = 0; j < V; ++j)
-    if (e + j >= 0 && e + j < cols) reinterpret_cast<T*>(to)[j] = x[at + j];
+    if (e + j >= 0 && e + j < cols) reinterpret_cast<T*>(to)[j] = at[j];
 }
 
-// The piece at columns [e0, e0+V); columns outside [0, cols) are 0.
-template <typename T>
+// The piece at columns [e0, e0+V), e0 < cols; columns outside [0, cols) are 0.
+template <typename T, bool EDGE>
 __device__ __forceinline__ uint4 read_piece(const uint4* from, int e0, int cols) {
-  constexpr int V = elem::kVec<T>;
-  if (e0 >= 0 && e0 + V <= cols) return *from;
-  const int e = elem::opaque(e0);
-  if (e >= cols) return make_uint4(0, 0, 0, 0);
-  return masked<T>(*from, e, cols);
+  if (!EDGE || (e0 >= 0 && e0 + elem::kVec<T> <= cols)) return *from;
+  return masked<T>(*from, elem::opaque(e0), cols);
 }
 
-template <typename T>
-__device__ __forceinline__ void store_piece(T* row, int e0, int cols, const float (&f)[elem::kVec<T>]) {
+template <typename T, bool EDGE>
+__device__ __forceinline__ void store_piece(T* row, int e0, int cols, const uint64_t (&f)[elem::kVec<T> / 2]) {
   constexpr int V = elem::kVec<T>;
-  if (e0 >= 0 && e0 + V <= cols) {
-    *reinterpret_cast<uint4*>(row + e0) = elem::pack_vec<T>(f);
+  if (!EDGE || (e0 >= 0 && e0 + V <= cols)) {
+    *reinterpret_cast<uint4*>(row + e0) = elem::pack_pairs<T>(f);
     return;
   }
   const int e = elem::opaque(e0);
 #pragma unroll
-  for (int j = 0; j < V; ++j)
-    if (e + j >= 0 && e + j < cols) row[e + j] = elem::from_f<T>(f[j]);
+  for (int j = 0; j < V; ++j) {
+    const float2 h = elem::halves(f[j / 2]);
+    if (e + j >= 0 && e + j < cols) row[e + j] = elem::from_f<T>(j % 2 ? h.y : h.x);
+  }
 }
 
 // Rows of a CTA at a time, and its threads: rows of up to 64 threads share a CTA.
@@ -200,7 +213,9 @@ __device__ __forceinline__ float row_sum(float v, float* scratch) {
     const int lane = threadIdx.x & 31, row0 = threadIdx.x / TPR * NW;
     if (lane == 0) scratch[threadIdx.x >> 5] = v;
     row_sync<TPR>();
-    v = warp_sum(lane < NW ? scratch[row0 + lane] : 0.f);
+    v = scratch[row0 + lane % NW];
+#pragma unroll
+    for (int o = NW / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   }
   return v;
 }
@@ -214,9 +229,14 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float2* scratch) {
     const int lane = threadIdx.x & 31, row0 = threadIdx.x / TPR * NW;
     if (lane == 0) scratch[threadIdx.x >> 5] = make_float2(a, b);
     row_sync<TPR>();
-    const float2 s = lane < NW ? scratch[row0 + lane] : make_float2(0.f, 0.f);
-    a = warp_sum(s.x);
-    b = warp_sum(s.y);
+    const float2 s = scratch[row0 + lane % NW];
+    a = s.x;
+    b = s.y;
+#pragma unroll
+    for (int o = NW / 2; o > 0; o >>= 1) {
+      a += __shfl_xor_sync(0xffffffffu, a, o);
+      b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
   }
   return make_float2(a, b);
 }
@@ -224,9 +244,10 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float2* scratch) {
 // Weights of columns [e0, e0 + V); `other` where there are none.
 template <typename T>
 __device__ __forceinline__ void load_weights(const void* w, int wdtype, int e0, int cols, float other,
-                                             float (&f)[elem::kVec<T>]) {
+                                             uint64_t (&pairs)[elem::kVec<T> / 2]) {
   constexpr int V = elem::kVec<T>;
   const int e = elem::opaque(e0);
+  float f[V];
   if (w == nullptr) {
 #pragma unroll
     for (int j = 0; j < V; ++j) f[j] = other;
@@ -251,35 +272,44 @@ __device__ __forceinline__ void load_weights(const void* w, int wdtype, int e0, 
       for (int j = 0; j < V; ++j) f[j] = e + j >= 0 && e + j < cols ? elem::to_f(at[j]) : other;
     }
   }
+#pragma unroll
+  for (int j = 0; j < V / 2; ++j) pairs[j] = elem::pair(f[2 * j], f[2 * j + 1]);
 }
 
 // ---------------------------------------------------------------- forward
-template <typename T, int TPR, int VPT, bool CKPT>
+template <typename T, int TPR, int VPT, bool CKPT, bool EDGE>
 __global__ void __launch_bounds__(kThreads<TPR>, kCtas<TPR, kFwdThreads>)
 fwd_rows(const FwdArgs p) {
+  using elem::add2;
+  using elem::fma2;
+  using elem::halves;
+  using elem::mul2;
+  using elem::pair;
   constexpr int V = elem::kVec<T>;
   constexpr int D = kDepth<TPR, VPT, kFwdThreads>;
   extern __shared__ uint4 ring[];  // [D][VPT][threads]
   __shared__ float red[2][32];
   const int t = threadIdx.x % TPR;
   const int cols = (int)p.cols;
-  const float fcols = (float)cols;
+  const float per_col = 1.f / (float)cols;
   const int64_t first = (int64_t)blockIdx.x * kRows<TPR> + threadIdx.x / TPR;
   const int64_t stride = (int64_t)gridDim.x * kRows<TPR>;
-  const int shift = elem::misalign<T>(static_cast<const T*>(p.x) + first * cols);
+  const int shift = EDGE ? elem::misalign<T>(static_cast<const T*>(p.x) + first * cols) : 0;
   const int e_first = t * V - shift;  // this thread's pieces start at e_first + i TPR V
   auto place = [&](int slot, int i) { return ring + (slot * VPT + i) * kThreads<TPR> + threadIdx.x; };
   auto fetch = [&](int slot, int64_t row) {
     if (row < p.rows) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i)
-        copy_piece<T>(place(slot, i), static_cast<const T*>(p.x), row, p.rows, e_first + i * TPR * V, cols);
+      for (int i = 0; i < VPT; ++i) {
+        const int e0 = e_first + i * TPR * V;
+        if (e0 < cols) copy_piece<T, EDGE>(place(slot, i), static_cast<const T*>(p.x), row, p.rows, e0, cols);
+      }
     }
     commit_copies();
   };
 #pragma unroll 1
   for (int d = 0; d < D; ++d) fetch(d, first + d * stride);
-  float g[VPT][V], b[VPT][V];
+  uint64_t g[VPT][V / 2], b[VPT][V / 2];
   auto weights = [&](int i) {
     load_weights<T>(p.gamma, p.wdtype, e_first + i * TPR * V, cols, 1.f, g[i]);
     load_weights<T>(p.beta, p.wdtype, e_first + i * TPR * V, cols, 0.f, b[i]);
@@ -291,70 +321,83 @@ fwd_rows(const FwdArgs p) {
   int slot = 0;
   for (int64_t row = first; row < p.rows; row += stride) {
     wait_copies<D - 1>();
-    float v[VPT][V];
-    float s = 0.f;
+    uint64_t v[VPT][V / 2];
+    uint64_t s2 = 0;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      elem::unpack_vec<T>(read_piece<T>(place(slot, i), e_first + i * TPR * V, cols), v[i]);
+      const int e0 = e_first + i * TPR * V;
+      uint4 raw = make_uint4(0, 0, 0, 0);
+      if (e0 < cols) raw = read_piece<T, EDGE>(place(slot, i), e0, cols);
+      elem::unpack_pairs<T>(raw, v[i]);
 #pragma unroll
-      for (int j = 0; j < V; ++j) s += v[i][j];
+      for (int j = 0; j < V / 2; ++j) s2 = add2(s2, v[i][j]);
     }
     fetch(slot, row + D * stride);
     slot = slot + 1 == D ? 0 : slot + 1;
-    const float mean = row_sum<TPR>(s, red[0]) / fcols;
-    float q = 0.f;
+    const float mean = row_sum<TPR>(halves(s2).x + halves(s2).y, red[0]) * per_col;
+    const uint64_t minus = pair(-mean, -mean);
+    if constexpr (CKPT) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int e0 = e_first + i * TPR * V;
-      if (e0 >= 0 && e0 + V <= cols) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) q = fmaf(v[i][j] - mean, v[i][j] - mean, q);
-      } else {  // a piece that the row's end cuts, or none of it in the row
-        const int e = elem::opaque(e0);
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (e + j >= 0 && e + j < cols) q = fmaf(v[i][j] - mean, v[i][j] - mean, q);
-      }
-    }
-    const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red[1]) / fcols + p.eps);
-    if (t == 0) {
-      p.mean[row] = mean;
-      p.rstd[row] = rstd;
-    }
-    T* yr = static_cast<T*>(p.y) + row * cols;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int e0 = e_first + i * TPR * V;
-      if constexpr (CKPT) {
+      for (int i = 0; i < VPT; ++i) {
         constexpr int LPB = 32 / V;  // lanes that share a block of 32 columns
+        const int e0 = e_first + i * TPR * V;
         uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) top = max(top, abs_bits(v[i][j]));
+        for (int j = 0; j < V / 2; ++j) top = max(top, max(abs_bits(halves(v[i][j]).x), abs_bits(halves(v[i][j]).y)));
 #pragma unroll
         for (int o = 1; o < LPB; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const uint32_t code = block_code(top);
         if (e0 < cols) {
+          const uint32_t code = block_code(top);
           const float up = code_up(code);
           uint32_t w[V / 4];
 #pragma unroll
-          for (int k = 0; k < V / 4; ++k) {
-            w[k] = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[k] |= ((uint32_t)quant8(v[i][4 * k + j], up) & 255u) << (8 * j);
-          }
+          for (int k = 0; k < V / 4; ++k)
+            w[k] = quant8x4(halves(v[i][2 * k]).x, halves(v[i][2 * k]).y, halves(v[i][2 * k + 1]).x,
+                            halves(v[i][2 * k + 1]).y, up, code);
           int8_t* qr = p.q8 + row * cols + e0;
           if constexpr (V == 8) *reinterpret_cast<uint2*>(qr) = make_uint2(w[0], w[1]);
           else *reinterpret_cast<uint32_t*>(qr) = w[0];
           if (t % LPB == 0) p.q8_exp[row * ((cols + 31) / 32) + e0 / 32] = (uint8_t)code;
         }
       }
-      if (e0 < cols) {
-        if constexpr (!kHold<T, VPT>) weights(i);
-        float o[V];
+    }
+    uint64_t q2 = 0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = fmaf((v[i][j] - mean) * rstd, g[i][j], b[i][j]);
-        store_piece<T>(yr, e0, cols, o);
+    for (int i = 0; i < VPT; ++i) {
+      const int e0 = e_first + i * TPR * V;
+      if (e0 >= cols) continue;
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) v[i][j] = add2(v[i][j], minus);
+      if (!EDGE || (e0 >= 0 && e0 + V <= cols)) {
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) q2 = fma2(v[i][j], v[i][j], q2);
+      } else {  // a piece that the row's end cuts
+        const int e = elem::opaque(e0);
+        float q = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float2 h = halves(v[i][j / 2]);
+          const float d = j % 2 ? h.y : h.x;
+          if (e + j >= 0 && e + j < cols) q = fmaf(d, d, q);
+        }
+        q2 = add2(q2, pair(q, 0.f));
       }
+    }
+    const float rstd = rsqrtf(fmaf(row_sum<TPR>(halves(q2).x + halves(q2).y, red[1]), per_col, p.eps));
+    if (t == 0) {
+      p.mean[row] = mean;
+      p.rstd[row] = rstd;
+    }
+    T* yr = static_cast<T*>(p.y) + row * cols;
+    const uint64_t by = pair(rstd, rstd);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int e0 = e_first + i * TPR * V;
+      if (e0 >= cols) continue;
+      if constexpr (!kHold<T, VPT>) weights(i);
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) v[i][j] = fma2(mul2(v[i][j], by), g[i][j], b[i][j]);
+      store_piece<T, EDGE>(yr, e0, cols, v[i]);
     }
   }
 }
@@ -402,26 +445,35 @@ __global__ void __launch_bounds__(256) fwd_any(const FwdArgs p) {
 // A piece of xh from x, or from its 8-bit checkpoint (.x, .y: eight values, .z:
 // the block's code).
 template <typename T, bool CKPT>
-__device__ __forceinline__ void x_hats(const uint4& raw, float mean, float rstd, float (&xh)[elem::kVec<T>]) {
+__device__ __forceinline__ void x_hats(const uint4& raw, float mean, float rstd, uint64_t (&xh)[elem::kVec<T> / 2]) {
+  using elem::pair;
   constexpr int V = elem::kVec<T>;
+  const uint64_t minus = pair(-mean, -mean), by = pair(rstd, rstd);
   if constexpr (CKPT) {
     const float down = code_down(raw.z);
+    const uint64_t scale = pair(down, down);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const uint32_t word = j < 4 ? raw.x : raw.y;
-      xh[j] = (fmaf((float)(int8_t)(word >> (8 * (j & 3))), down, -mean)) * rstd;  // the product is exact
+    for (int j = 0; j < V / 2; ++j) {
+      const uint32_t word = j < 2 ? raw.x : raw.y;
+      const uint64_t q = pair((float)(int8_t)(word >> (16 * (j & 1))), (float)(int8_t)(word >> (16 * (j & 1) + 8)));
+      xh[j] = elem::mul2(elem::fma2(q, scale, minus), by);  // (the product is exact)
     }
   } else {
-    elem::unpack_vec<T>(raw, xh);
+    elem::unpack_pairs<T>(raw, xh);
 #pragma unroll
-    for (int j = 0; j < V; ++j) xh[j] = (xh[j] - mean) * rstd;
+    for (int j = 0; j < V / 2; ++j) xh[j] = elem::mul2(elem::add2(xh[j], minus), by);
   }
 }
 
 // Columns outside the row have dy = 0, so they add nothing to any sum.
-template <typename T, int TPR, int VPT, bool CKPT>
+template <typename T, int TPR, int VPT, bool CKPT, bool EDGE>
 __global__ void __launch_bounds__(kThreads<TPR>, kCtas<TPR, kBwdThreads>)
 bwd_rows(const BwdArgs p) {
+  using elem::add2;
+  using elem::fma2;
+  using elem::halves;
+  using elem::mul2;
+  using elem::pair;
   constexpr int V = elem::kVec<T>;
   constexpr int RB = kRows<TPR>;
   constexpr int D = kDepth<TPR, 2 * VPT, kBwdThreads>;
@@ -429,10 +481,10 @@ bwd_rows(const BwdArgs p) {
   __shared__ float2 red[2][32];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const int cols = (int)p.cols;
-  const float fcols = (float)cols;
+  const float per_col = 1.f / (float)cols;
   const int64_t first = (int64_t)blockIdx.x * RB + sub;
   const int64_t stride = (int64_t)gridDim.x * RB;
-  const int shift = elem::misalign<T>(static_cast<const T*>(p.dy) + first * cols);
+  const int shift = EDGE ? elem::misalign<T>(static_cast<const T*>(p.dy) + first * cols) : 0;
   const int e_first = t * V - shift;
   auto place = [&](int slot, int which, int i) {
     return ring + ((slot * 2 + which) * VPT + i) * kThreads<TPR> + threadIdx.x;
@@ -442,12 +494,10 @@ bwd_rows(const BwdArgs p) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int e0 = e_first + i * TPR * V;
-        copy_piece<T>(place(slot, 0, i), static_cast<const T*>(p.dy), row, p.rows, e0, cols);
-        if constexpr (CKPT) {
-          if (e0 < cols) copy_async_small<V>(place(slot, 1, i), p.q8 + row * cols + e0);
-        } else {
-          copy_piece<T>(place(slot, 1, i), static_cast<const T*>(p.x), row, p.rows, e0, cols);
-        }
+        if (e0 >= cols) continue;
+        copy_piece<T, EDGE>(place(slot, 0, i), static_cast<const T*>(p.dy), row, p.rows, e0, cols);
+        if constexpr (CKPT) copy_async_small<V>(place(slot, 1, i), p.q8 + row * cols + e0);
+        else copy_piece<T, EDGE>(place(slot, 1, i), static_cast<const T*>(p.x), row, p.rows, e0, cols);
       }
     }
     commit_copies();
@@ -469,67 +519,64 @@ bwd_rows(const BwdArgs p) {
 #pragma unroll 1
   for (int d = 0; d < D; ++d) fetch(d, first + d * stride);
   if (first < p.rows) ahead(first);
-  float g[VPT][V], dg[VPT][V], db[VPT][V];
+  uint64_t g[VPT][V / 2], dg[VPT][V / 2], db[VPT][V / 2];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     if constexpr (kHold<T, VPT>) load_weights<T>(p.gamma, p.wdtype, e_first + i * TPR * V, cols, 1.f, g[i]);
 #pragma unroll
-    for (int j = 0; j < V; ++j) dg[i][j] = db[i][j] = 0.f;
+    for (int j = 0; j < V / 2; ++j) dg[i][j] = db[i][j] = 0;
   }
   int turn = 0, slot = 0;
   for (int64_t row = first; row < p.rows; row += stride, turn ^= 1) {
-    float s1 = 0.f, s2 = 0.f;
     const float mean = nmean, rstd = nrstd;
     uint32_t code[VPT];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) code[i] = ncode[i];
+    for (int i = 0; i < VPT; ++i) code[i] = CKPT ? ncode[i] : 0;
     if (row + stride < p.rows) ahead(row + stride);
     // a piece of dy and xh; read for the sums and again for dx, as holding them takes twice the registers
-    auto read = [&](int i, float (&d)[V], float (&xh)[V]) {
-      const int e0 = e_first + i * TPR * V;
-      elem::unpack_vec<T>(read_piece<T>(place(slot, 0, i), e0, cols), d);
+    auto read = [&](int i, int e0, uint64_t (&d)[V / 2], uint64_t (&xh)[V / 2]) {
+      elem::unpack_pairs<T>(read_piece<T, EDGE>(place(slot, 0, i), e0, cols), d);
       uint4 x;
       if constexpr (CKPT) {
-        x = make_uint4(0, 0, code[i], 0);
-        if (e0 < cols) {
-          const uint4* at = place(slot, 1, i);
-          x.x = reinterpret_cast<const uint32_t*>(at)[0];
-          if constexpr (V == 8) x.y = reinterpret_cast<const uint32_t*>(at)[1];
-        }
+        const uint32_t* at = reinterpret_cast<const uint32_t*>(place(slot, 1, i));
+        x = make_uint4(at[0], V == 8 ? at[1] : 0, code[i], 0);
       } else {
-        x = read_piece<T>(place(slot, 1, i), e0, cols);
+        x = read_piece<T, EDGE>(place(slot, 1, i), e0, cols);
       }
       x_hats<T, CKPT>(x, mean, rstd, xh);
     };
     wait_copies<D - 1>();
+    uint64_t s1 = 0, s2 = 0;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      float d[V], xh[V];
-      read(i, d, xh);
-      if constexpr (!kHold<T, VPT>) load_weights<T>(p.gamma, p.wdtype, e_first + i * TPR * V, cols, 1.f, g[i]);
+      const int e0 = e_first + i * TPR * V;
+      if (e0 >= cols) continue;
+      uint64_t d[V / 2], xh[V / 2];
+      read(i, e0, d, xh);
+      if constexpr (!kHold<T, VPT>) load_weights<T>(p.gamma, p.wdtype, e0, cols, 1.f, g[i]);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        dg[i][j] = fmaf(d[j], xh[j], dg[i][j]);
-        db[i][j] += d[j];
-        const float w = d[j] * g[i][j];
-        s1 = fmaf(w, xh[j], s1);
-        s2 += w;
+      for (int j = 0; j < V / 2; ++j) {
+        dg[i][j] = fma2(d[j], xh[j], dg[i][j]);
+        db[i][j] = add2(db[i][j], d[j]);
+        const uint64_t w = mul2(d[j], g[i][j]);
+        s1 = fma2(w, xh[j], s1);
+        s2 = add2(s2, w);
       }
     }
-    const float2 s = row_sum2<TPR>(s1, s2, red[turn]);
-    const float c1 = s.x / fcols, c2 = s.y / fcols;
+    const float2 s = row_sum2<TPR>(halves(s1).x + halves(s1).y, halves(s2).x + halves(s2).y, red[turn]);
+    const float c1 = -s.x * per_col, c2 = -s.y * per_col;
+    const uint64_t m1 = pair(c1, c1), m2 = pair(c2, c2), by = pair(rstd, rstd);
     T* dxr = static_cast<T*>(p.dx) + row * cols;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int e0 = e_first + i * TPR * V;
-      if (e0 < cols) {
-        float d[V], xh[V];
-        read(i, d, xh);
-        if constexpr (!kHold<T, VPT>) load_weights<T>(p.gamma, p.wdtype, e0, cols, 1.f, g[i]);
+      if (e0 >= cols) continue;
+      uint64_t d[V / 2], xh[V / 2];
+      read(i, e0, d, xh);
+      if constexpr (!kHold<T, VPT>) load_weights<T>(p.gamma, p.wdtype, e0, cols, 1.f, g[i]);
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[j] = rstd * (fmaf(d[j], g[i][j], -c2) - xh[j] * c1);
-        store_piece<T>(dxr, e0, cols, d);
-      }
+      for (int j = 0; j < V / 2; ++j) d[j] = mul2(by, fma2(xh[j], m1, fma2(d[j], g[i][j], m2)));
+      store_piece<T, EDGE>(dxr, e0, cols, d);
     }
     fetch(slot, row + D * stride);
     slot = slot + 1 == D ? 0 : slot + 1;
@@ -544,8 +591,8 @@ bwd_rows(const BwdArgs p) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (e0 + j >= 0 && e0 + j < cols) {
-          out[e0 + j] = dg[i][j];
-          out[cols + e0 + j] = db[i][j];
+          out[e0 + j] = j % 2 ? halves(dg[i][j / 2]).y : halves(dg[i][j / 2]).x;
+          out[cols + e0 + j] = j % 2 ? halves(db[i][j / 2]).y : halves(db[i][j / 2]).x;
         }
     }
   } else {
@@ -559,8 +606,10 @@ bwd_rows(const BwdArgs p) {
 #pragma unroll
           for (int j = 0; j < V; ++j)
             if (e0 + j >= 0 && e0 + j < cols) {
-              part[e0 + j] = w ? part[e0 + j] + dg[i][j] : dg[i][j];
-              part[cols + e0 + j] = w ? part[cols + e0 + j] + db[i][j] : db[i][j];
+              const float vg = j % 2 ? halves(dg[i][j / 2]).y : halves(dg[i][j / 2]).x;
+              const float vb = j % 2 ? halves(db[i][j / 2]).y : halves(db[i][j / 2]).x;
+              part[e0 + j] = w ? part[e0 + j] + vg : vg;
+              part[cols + e0 + j] = w ? part[cols + e0 + j] + vb : vb;
             }
         }
       }
@@ -705,12 +754,13 @@ inline int fwd_typed(const FwdArgs& a, cudaStream_t st) {
   const int shift = elem::misalign<T>(a.x);
   bool fast = elem::misalign<T>(a.y) == shift;
   if (CKPT) fast = fast && shift == 0 && a.cols % V == 0 && elem::aligned_to(a.q8, V);
-  const int64_t pieces = (a.cols + V - 1) / V + (a.cols % V || shift ? 1 : 0);
+  const bool edge = shift != 0 || a.cols % V != 0;  // (not with checkpoints)
+  const int64_t pieces = (a.cols + V - 1) / V + (edge ? 1 : 0);
   int rc = KT_OK;
   if (fast && with_shape<T>(pieces, [&](auto tpr, auto vpt) {
         constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
         constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
-        auto kern = fwd_rows<T, TPR, VPT, CKPT>;
+        auto kern = edge ? fwd_rows<T, TPR, VPT, CKPT, !CKPT> : fwd_rows<T, TPR, VPT, CKPT, false>;
         constexpr size_t smem = (size_t)kDepth<TPR, VPT, kFwdThreads> * VPT * BLOCK * 16;
         int grid = 0;
         rc = row_grid(kern, BLOCK, RB, smem, a.rows, &grid);
@@ -748,12 +798,13 @@ inline int bwd_typed(const BwdArgs& a, void* dgamma, void* dbeta, cudaStream_t s
   bool fast = elem::misalign<T>(a.dx) == shift;
   if (CKPT) fast = fast && shift == 0 && a.cols % V == 0 && elem::aligned_to(a.q8, V);
   else fast = fast && elem::misalign<T>(a.x) == shift;
-  const int64_t pieces = (a.cols + V - 1) / V + (a.cols % V || shift ? 1 : 0);
+  const bool edge = shift != 0 || a.cols % V != 0;  // (not with checkpoints)
+  const int64_t pieces = (a.cols + V - 1) / V + (edge ? 1 : 0);
   int rc = KT_OK, parts = 0;
   if (!(fast && with_shape<T>(pieces, [&](auto tpr, auto vpt) {
           constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
           constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
-          auto kern = bwd_rows<T, TPR, VPT, CKPT>;
+          auto kern = edge ? bwd_rows<T, TPR, VPT, CKPT, !CKPT> : bwd_rows<T, TPR, VPT, CKPT, false>;
           constexpr size_t smem = (size_t)kDepth<TPR, 2 * VPT, kBwdThreads> * 2 * VPT * BLOCK * 16;
           static_assert(RB == 1 || smem >= 2 * sizeof(float) * TPR * VPT * V, "the CTA's sums fit the ring");
           rc = row_grid(kern, BLOCK, RB, smem, a.rows, &parts);

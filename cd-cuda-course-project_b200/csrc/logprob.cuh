@@ -88,28 +88,11 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// Two fp32 operations by one instruction.
-__device__ __forceinline__ uint64_t pair(float a, float b) {
-  return (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
-}
-__device__ __forceinline__ float2 halves(uint64_t v) {
-  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
+using elem::add2;
+using elem::fma2;
+using elem::halves;
+using elem::mul2;
+using elem::pair;
 
 // Largest of a 16-byte piece; NaNs are passed over.
 __device__ __forceinline__ float piece_max(const uint4& r, float) {
