@@ -181,6 +181,7 @@ constexpr int kThreads = TPR * kRows<TPR>;
 // 80 (forward) and 128 (backward) with their weights and sums. A thread of wider
 // rows has 32 columns and reads gamma and beta again in every row.
 constexpr int kFwdThreads = 768, kBwdThreads = 512;
+constexpr int kScalar = 16;  // columns of a thread, element by element
 template <typename T, int VPT>
 constexpr bool kHold = VPT * elem::kVec<T> <= 16;
 template <int TPR, int PER_SM>
@@ -287,6 +288,7 @@ fwd_rows(const FwdArgs p) {
   using elem::pair;
   constexpr int V = elem::kVec<T>;
   constexpr int D = kDepth<TPR, VPT, kFwdThreads>;
+  static_assert(D >= 1, "a row fits shared memory");
   extern __shared__ uint4 ring[];  // [D][VPT][threads]
   __shared__ float red[2][32];
   const int t = threadIdx.x % TPR;
@@ -402,7 +404,7 @@ fwd_rows(const FwdArgs p) {
   }
 }
 
-// Any width and alignment: a CTA per row, the row read once per step (from L2
+// Wider rows, any alignment: a CTA per row, the row read once per step (from L2
 // after the first). Lanes hold consecutive columns, so a warp's 32 columns are
 // one block of the checkpoint.
 template <typename T, bool CKPT>
@@ -448,20 +450,24 @@ template <typename T, bool CKPT>
 __device__ __forceinline__ void x_hats(const uint4& raw, float mean, float rstd, uint64_t (&xh)[elem::kVec<T> / 2]) {
   using elem::pair;
   constexpr int V = elem::kVec<T>;
-  const uint64_t minus = pair(-mean, -mean), by = pair(rstd, rstd);
+  // x rstd - mean rstd: off by 2^-24 (|xh| + |mean| rstd), as the mean itself is
+  const uint64_t minus = pair(-mean * rstd, -mean * rstd);
   if constexpr (CKPT) {
-    const float down = code_down(raw.z);
-    const uint64_t scale = pair(down, down);
+    const float down = code_down(raw.z) * rstd;
+    const uint64_t scale = pair(down, down), bias = pair(-8388736.f, -8388736.f);  // 2^23 + 128
 #pragma unroll
     for (int j = 0; j < V / 2; ++j) {
-      const uint32_t word = j < 2 ? raw.x : raw.y;
-      const uint64_t q = pair((float)(int8_t)(word >> (16 * (j & 1))), (float)(int8_t)(word >> (16 * (j & 1) + 8)));
-      xh[j] = elem::mul2(elem::fma2(q, scale, minus), by);  // (the product is exact)
+      // q + 128 in the low bits of 2^23
+      const uint32_t word = (j < 2 ? raw.x : raw.y) ^ 0x80808080u;
+      const uint64_t q = (uint64_t)__byte_perm(word, 0x4B000000u, 0x7440 + (2 * (j & 1) + 1)) << 32 |
+                         __byte_perm(word, 0x4B000000u, 0x7440 + 2 * (j & 1));
+      xh[j] = elem::fma2(elem::add2(q, bias), scale, minus);
     }
   } else {
+    const uint64_t by = pair(rstd, rstd);
     elem::unpack_pairs<T>(raw, xh);
 #pragma unroll
-    for (int j = 0; j < V / 2; ++j) xh[j] = elem::mul2(elem::add2(xh[j], minus), by);
+    for (int j = 0; j < V / 2; ++j) xh[j] = elem::fma2(xh[j], by, minus);
   }
 }
 
@@ -477,6 +483,7 @@ bwd_rows(const BwdArgs p) {
   constexpr int V = elem::kVec<T>;
   constexpr int RB = kRows<TPR>;
   constexpr int D = kDepth<TPR, 2 * VPT, kBwdThreads>;
+  static_assert(D >= 1, "a row fits shared memory");
   extern __shared__ uint4 ring[];  // [D][dy, x][VPT][threads]; at the end, RB > 1: 2 x cols sums of the CTA
   __shared__ float2 red[2][32];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
@@ -588,6 +595,14 @@ bwd_rows(const BwdArgs p) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int e0 = e_first + i * TPR * V;
+      if (!EDGE && e0 < cols) {  // cols is a multiple of 4
+#pragma unroll
+        for (int j = 0; j < V / 2; j += 2) {
+          *reinterpret_cast<ulonglong2*>(out + e0 + 2 * j) = make_ulonglong2(dg[i][j], dg[i][j + 1]);
+          *reinterpret_cast<ulonglong2*>(out + cols + e0 + 2 * j) = make_ulonglong2(db[i][j], db[i][j + 1]);
+        }
+        continue;
+      }
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if (e0 + j >= 0 && e0 + j < cols) {
@@ -596,30 +611,138 @@ bwd_rows(const BwdArgs p) {
         }
     }
   } else {
-    float* part = reinterpret_cast<float*>(ring);
+    float* part = reinterpret_cast<float*>(ring);  // [RB][2][cols]
     __syncthreads();
-    for (int w = 0; w < RB; ++w) {  // in the order of the rows
-      if (sub == w) {
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-          const int e0 = e_first + i * TPR * V;
+    for (int i = 0; i < VPT; ++i) {
+      const int e0 = e_first + i * TPR * V;
 #pragma unroll
-          for (int j = 0; j < V; ++j)
-            if (e0 + j >= 0 && e0 + j < cols) {
-              const float vg = j % 2 ? halves(dg[i][j / 2]).y : halves(dg[i][j / 2]).x;
-              const float vb = j % 2 ? halves(db[i][j / 2]).y : halves(db[i][j / 2]).x;
-              part[e0 + j] = w ? part[e0 + j] + vg : vg;
-              part[cols + e0 + j] = w ? part[cols + e0 + j] + vb : vb;
-            }
+      for (int j = 0; j < V; ++j)
+        if (e0 + j >= 0 && e0 + j < cols) {
+          part[sub * 2 * cols + e0 + j] = j % 2 ? halves(dg[i][j / 2]).y : halves(dg[i][j / 2]).x;
+          part[(sub * 2 + 1) * cols + e0 + j] = j % 2 ? halves(db[i][j / 2]).y : halves(db[i][j / 2]).x;
         }
-      }
-      __syncthreads();
     }
-    for (int e = threadIdx.x; e < 2 * cols; e += kThreads<TPR>) out[e] = part[e];
+    __syncthreads();
+    for (int e = threadIdx.x; e < 2 * cols; e += kThreads<TPR>) {  // in the order of the rows
+      float v = part[e];
+#pragma unroll
+      for (int w = 1; w < RB; ++w) v += part[w * 2 * cols + e];
+      out[e] = v;
+    }
   }
 }
 
-// Any width and alignment: dx by a CTA per row, and the partial sums by columns.
+// ---------------------------------------------------------------- element by element
+// Rows of x and dy that are not equally aligned, and checkpoints of rows that are
+// no whole number of pieces: lanes hold consecutive columns (a warp's 32 are one
+// block of the checkpoint), EPT per thread, as above but for the copies ahead.
+template <typename T, int TPR, bool CKPT>
+__global__ void __launch_bounds__(TPR) fwd_scalar(const FwdArgs p) {
+  constexpr int EPT = kScalar;
+  __shared__ float red[2][32];
+  const int t = threadIdx.x, cols = (int)p.cols;
+  const float per_col = 1.f / (float)cols;
+  T next[EPT];
+  auto fetch = [&](int64_t row) {
+    const T* xr = static_cast<const T*>(p.x) + row * cols;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i)
+      if (t + i * TPR < cols) next[i] = xr[t + i * TPR];
+  };
+  fetch(blockIdx.x);
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    float v[EPT];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      v[i] = t + i * TPR < cols ? elem::to_f(next[i]) : 0.f;
+      s += v[i];
+    }
+    if (row + gridDim.x < p.rows) fetch(row + gridDim.x);
+    const float mean = row_sum<TPR>(s, red[0]) * per_col;
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i)
+      if (t + i * TPR < cols) q = fmaf(v[i] - mean, v[i] - mean, q);
+    const float rstd = rsqrtf(fmaf(row_sum<TPR>(q, red[1]), per_col, p.eps));
+    if (t == 0) {
+      p.mean[row] = mean;
+      p.rstd[row] = rstd;
+    }
+    T* yr = static_cast<T*>(p.y) + row * cols;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const int e = t + i * TPR;
+      if constexpr (CKPT) {
+        const uint32_t code = block_code(__reduce_max_sync(0xffffffffu, abs_bits(v[i])));
+        if (e < cols) p.q8[row * cols + e] = (int8_t)quant8(v[i], code_up(code));
+        if (e < cols && (t & 31) == 0) p.q8_exp[row * ((cols + 31) / 32) + e / 32] = (uint8_t)code;
+      }
+      if (e < cols) {
+        const float g = p.gamma ? elem::ld_weight(p.gamma, p.wdtype, e) : 1.f;
+        const float b = p.beta ? elem::ld_weight(p.beta, p.wdtype, e) : 0.f;
+        yr[e] = elem::from_f<T>(fmaf((v[i] - mean) * rstd, g, b));
+      }
+    }
+  }
+}
+
+template <typename T, int TPR, bool CKPT>
+__global__ void __launch_bounds__(TPR) bwd_scalar(const BwdArgs p) {
+  constexpr int EPT = kScalar;
+  __shared__ float2 red[2][32];
+  const int t = threadIdx.x, cols = (int)p.cols;
+  const float per_col = 1.f / (float)cols;
+  float g[EPT], dg[EPT], db[EPT];
+#pragma unroll
+  for (int i = 0; i < EPT; ++i) {
+    g[i] = t + i * TPR < cols && p.gamma ? elem::ld_weight(p.gamma, p.wdtype, t + i * TPR) : 1.f;
+    dg[i] = db[i] = 0.f;
+  }
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    const T* dyr = static_cast<const T*>(p.dy) + row * cols;
+    T* dxr = static_cast<T*>(p.dx) + row * cols;
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    float d[EPT], xh[EPT];
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      const int e = t + i * TPR;
+      d[i] = e < cols ? elem::to_f(dyr[e]) : 0.f;
+      if constexpr (CKPT) {
+        xh[i] = e < cols ? (float)p.q8[row * cols + e] * code_down(p.q8_exp[row * ((cols + 31) / 32) + e / 32]) : 0.f;
+      } else {
+        xh[i] = e < cols ? elem::to_f(static_cast<const T*>(p.x)[row * cols + e]) : 0.f;
+      }
+    }
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {  // columns outside the row have d = 0
+      xh[i] = (xh[i] - mean) * rstd;
+      dg[i] = fmaf(d[i], xh[i], dg[i]);
+      db[i] += d[i];
+      d[i] *= g[i];
+      s1 = fmaf(d[i], xh[i], s1);
+      s2 += d[i];
+    }
+    const float2 s = row_sum2<TPR>(s1, s2, red[turn]);
+    const float c1 = s.x * per_col, c2 = s.y * per_col;
+#pragma unroll
+    for (int i = 0; i < EPT; ++i)
+      if (t + i * TPR < cols) dxr[t + i * TPR] = elem::from_f<T>(rstd * (d[i] - c2 - xh[i] * c1));
+  }
+  if (p.partial == nullptr) return;
+  float* out = p.partial + (int64_t)blockIdx.x * 2 * cols;
+#pragma unroll
+  for (int i = 0; i < EPT; ++i)
+    if (t + i * TPR < cols) {
+      out[t + i * TPR] = dg[i];
+      out[cols + t + i * TPR] = db[i];
+    }
+}
+
+// Wider rows, any alignment: dx by a CTA per row, and the partial sums by columns.
 template <typename T, bool CKPT>
 __device__ __forceinline__ float x_hat(const BwdArgs& p, int64_t row, int64_t e, float mean, float rstd) {
   float v;
@@ -669,25 +792,40 @@ __global__ void __launch_bounds__(256) bwd_any_cols(const BwdArgs p) {
   out[p.cols + e] = db;
 }
 
-// dgamma, dbeta: the partial rows added in their order. 32 columns x 8 slices of
-// the partial rows per CTA, the slices joined in shared memory.
-__global__ void __launch_bounds__(256)
-bwd_join(const float* __restrict__ partial, int parts, int64_t cols, void* dgamma, void* dbeta, int wdtype) {
-  __shared__ float slice[8][32];
+// dgamma, dbeta: the partial rows added in their order. 32 columns per CTA; each
+// of 32 warps adds a slice of the rows, eight loads at a time, and the slices are
+// joined in shared memory. (The loads' latency is what it takes: 8 slices took
+// three times as long.)
+__global__ void __launch_bounds__(1024)
+bwd_join(const float* partial, int parts, int64_t cols, void* dgamma, void* dbeta, int wdtype) {
+  __shared__ float slice[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t e = (int64_t)blockIdx.x * 32 + lane;  // over 2 x cols: dgamma, then dbeta
   float s = 0.f;
-  if (e < 2 * cols)
-    for (int r = parts * w / 8; r < parts * (w + 1) / 8; ++r) s += partial[(int64_t)r * 2 * cols + e];
+  cudaGridDependencySynchronize();
+  if (e < 2 * cols) {
+    const float* from = partial + e;
+    int r = parts * w / 32;
+    const int end = parts * (w + 1) / 32;
+    for (; r + 8 <= end; r += 8) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = from[(int64_t)(r + i) * 2 * cols];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[i];
+    }
+#pragma unroll 4
+    for (; r < end; ++r) s += from[(int64_t)r * 2 * cols];
+  }
   slice[w][lane] = s;
   __syncthreads();
-  if (w == 0 && e < 2 * cols) {
-#pragma unroll
-    for (int k = 1; k < 8; ++k) s += slice[k][lane];
-    if (e < cols) {
-      if (dgamma) elem::st_weight(dgamma, wdtype, e, s);
+  s = warp_sum(slice[lane][w]);  // column w of the CTA's
+  const int64_t out = (int64_t)blockIdx.x * 32 + w;
+  if (lane == 0 && out < 2 * cols) {
+    if (out < cols) {
+      if (dgamma) elem::st_weight(dgamma, wdtype, out, s);
     } else if (dbeta) {
-      elem::st_weight(dbeta, wdtype, e - cols, s);
+      elem::st_weight(dbeta, wdtype, out - cols, s);
     }
   }
 }
@@ -731,10 +869,11 @@ inline bool with_shape(int64_t pieces, F f) {
   if (pieces <= 32) return f(std::integral_constant<int, 32>{}, One{}), true;
   if (pieces <= 32 * VPT) return f(std::integral_constant<int, 32>{}, All{}), true;
   if (pieces <= 64 * VPT) return f(std::integral_constant<int, 64>{}, All{}), true;
+  using Twice = std::integral_constant<int, 2 * VPT>;
   if (pieces <= 128 * VPT) return f(std::integral_constant<int, 128>{}, All{}), true;
   if (pieces <= 256 * VPT) return f(std::integral_constant<int, 256>{}, All{}), true;
   if (pieces <= 512 * VPT) return f(std::integral_constant<int, 512>{}, All{}), true;
-  if (pieces <= 1024 * VPT) return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 2 * VPT>{}), true;
+  if (pieces <= 1024 * VPT) return f(std::integral_constant<int, 512>{}, Twice{}), true;
   return false;
 }
 
@@ -769,6 +908,15 @@ inline int fwd_typed(const FwdArgs& a, cudaStream_t st) {
         rc = check_launch("layernorm_train fwd_rows");
       }))
     return rc;
+  if (a.cols <= 512 * kScalar) {
+    auto kern = a.cols <= 128 * kScalar ? fwd_scalar<T, 128, CKPT> : fwd_scalar<T, 512, CKPT>;
+    const int block = a.cols <= 128 * kScalar ? 128 : 512;
+    int grid = 0;
+    rc = row_grid(kern, block, 1, 0, a.rows, &grid);
+    if (rc != KT_OK) return rc;
+    kern<<<grid, block, 0, st>>>(a);
+    return check_launch("layernorm_train fwd_scalar");
+  }
   const int64_t g = a.rows < 4 * sm_count() ? a.rows : 4 * sm_count();
   fwd_any<T, CKPT><<<(int)g, 256, 0, st>>>(a);
   return check_launch("layernorm_train fwd_any");
@@ -806,24 +954,44 @@ inline int bwd_typed(const BwdArgs& a, void* dgamma, void* dbeta, cudaStream_t s
           constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
           auto kern = edge ? bwd_rows<T, TPR, VPT, CKPT, !CKPT> : bwd_rows<T, TPR, VPT, CKPT, false>;
           constexpr size_t smem = (size_t)kDepth<TPR, 2 * VPT, kBwdThreads> * 2 * VPT * BLOCK * 16;
-          static_assert(RB == 1 || smem >= 2 * sizeof(float) * TPR * VPT * V, "the CTA's sums fit the ring");
+          static_assert(RB == 1 || smem >= RB * 2 * sizeof(float) * TPR * VPT * V, "the CTA's sums fit the ring");
           rc = row_grid(kern, BLOCK, RB, smem, a.rows, &parts);
           if (rc != KT_OK) return;
           kern<<<parts, BLOCK, smem, st>>>(a);
           rc = check_launch("layernorm_train bwd_rows");
         }))) {
-    const int64_t g = a.rows < 4 * sm_count() ? a.rows : 4 * sm_count();
-    bwd_any_dx<T, CKPT><<<(int)g, 256, 0, st>>>(a);
-    rc = check_launch("layernorm_train bwd_any_dx");
-    if (rc == KT_OK && a.partial) {
-      parts = (int)(a.rows < 64 ? a.rows : 64);
-      bwd_any_cols<T, CKPT><<<dim3((unsigned)((a.cols + 255) / 256), (unsigned)parts), 256, 0, st>>>(a);
-      rc = check_launch("layernorm_train bwd_any_cols");
+    if (a.cols <= 512 * kScalar) {
+      auto kern = a.cols <= 128 * kScalar ? bwd_scalar<T, 128, CKPT> : bwd_scalar<T, 512, CKPT>;
+      const int block = a.cols <= 128 * kScalar ? 128 : 512;
+      rc = row_grid(kern, block, 1, 0, a.rows, &parts);
+      if (rc != KT_OK) return rc;
+      kern<<<parts, block, 0, st>>>(a);
+      rc = check_launch("layernorm_train bwd_scalar");
+    } else {
+      const int64_t g = a.rows < 4 * sm_count() ? a.rows : 4 * sm_count();
+      bwd_any_dx<T, CKPT><<<(int)g, 256, 0, st>>>(a);
+      rc = check_launch("layernorm_train bwd_any_dx");
+      if (rc == KT_OK && a.partial) {
+        parts = (int)(a.rows < 64 ? a.rows : 64);
+        bwd_any_cols<T, CKPT><<<dim3((unsigned)((a.cols + 255) / 256), (unsigned)parts), 256, 0, st>>>(a);
+        rc = check_launch("layernorm_train bwd_any_cols");
+      }
     }
   }
   if (rc != KT_OK || a.partial == nullptr) return rc;
-  bwd_join<<<(unsigned)((2 * a.cols + 31) / 32), 256, 0, st>>>(a.partial, parts, a.cols, dgamma, dbeta, a.wdtype);
-  return check_launch("layernorm_train bwd_join");
+  // the join may be launched while the rows finish: it waits for them itself
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((2 * a.cols + 31) / 32));
+  cfg.blockDim = dim3(1024);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const float* partial = a.partial;
+  return cuda_status(cudaLaunchKernelEx(&cfg, bwd_join, partial, parts, a.cols, dgamma, dbeta, a.wdtype),
+                     "layernorm_train bwd_join");
 }
 
 inline int backward(BwdArgs a, int dtype, void* dgamma, void* dbeta, void* workspace, size_t ws_bytes,
