@@ -122,40 +122,38 @@ _DTYPES = {torch.float32: kt_lib.KT_F32, torch.bfloat16: kt_lib.KT_BF16, torch.f
 
 
 def _dtype(t: torch.Tensor, name: str) -> int:
-    try:
-        return _DTYPES[t.dtype]
-    except KeyError:
-        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}") from None
+    dt = _DTYPES.get(t.dtype)
+    if dt is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return dt
 
 
-def _on_device(t: torch.Tensor, like: torch.Tensor, name: str) -> None:
-    if t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, not on {like.device}")
+def _dense(t: torch.Tensor, name: str, dtype: torch.dtype, device: int) -> None:
+    """A contiguous tensor of `dtype` on CUDA device `device`."""
+    if not (t.dtype is dtype and t.get_device() == device and t.is_contiguous()):
+        _check(t, name, dtype)
+        raise ValueError(f"{name} is on {t.device}, not on cuda:{device}")
 
 
-def _rows(t: torch.Tensor, name: str) -> None:
-    """A 2-D CUDA tensor whose rows are dense; the rows may be any distance apart."""
+def _rows(t: torch.Tensor, name: str) -> int:
+    """A 2-D CUDA tensor whose rows are dense and any distance apart; returns that distance in elements."""
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
     if t.dim() != 2:
         raise ValueError(f"{name} must be 2-D")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
         raise ValueError(f"{name}: the elements of a row must be contiguous")
+    return t.stride(0) if rows > 1 else cols
 
 
-def _ld(t: torch.Tensor) -> int:
-    """Distance of a 2-D tensor's rows in elements."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _launch(t: torch.Tensor, fn, *args) -> None:
-    """fn(*args, stream) on t's device and that device's current stream."""
-    d = t.get_device()
-    if d == torch.cuda.current_device():
-        fn(*args, torch.cuda.current_stream(d).cuda_stream)
+def _launch(device: int, fn, *args) -> None:
+    """fn(*args, stream) on that device and its current stream."""
+    if device == torch.cuda.current_device():
+        fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
-        with torch.cuda.device(d):
-            fn(*args, torch.cuda.current_stream(d).cuda_stream)
+        with torch.cuda.device(device):
+            fn(*args, torch._C._cuda_getCurrentRawStream(device))
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -165,14 +163,21 @@ def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
 class LayerNormSaved(NamedTuple):
     """What layernorm_train keeps for layernorm_bwd: the input x, or its 8-bit
     checkpoint (q8, q8_exp; include/kt_abi.h has the format), gamma, the rows'
-    statistics, and beta's type (None without beta)."""
+    statistics (2, rows), and beta's type (None without beta)."""
     x: Optional[torch.Tensor]
     q8: Optional[torch.Tensor]
     q8_exp: Optional[torch.Tensor]
     gamma: Optional[torch.Tensor]
-    mean: torch.Tensor
-    rstd: torch.Tensor
+    stats: torch.Tensor
     beta_dtype: Optional[torch.dtype]
+
+    @property
+    def mean(self) -> torch.Tensor:
+        return self.stats[0]
+
+    @property
+    def rstd(self) -> torch.Tensor:
+        return self.stats[1]
 
 
 def layernorm_train(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Optional[torch.Tensor] = None,
@@ -189,26 +194,35 @@ def layernorm_train(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta:
     if x.dim() != 2:
         raise ValueError("x must be 2-D (rows, cols)")
     rows, cols = x.shape
+    dev = x.get_device()
     wdt = kt_lib.KT_F32
-    for t, n in ((gamma, "gamma"), (beta, "beta")):
-        if t is not None:
-            wdt = _dtype(t, n)
-            _check(t, n, torch.float32 if wdt == kt_lib.KT_F32 else x.dtype)
-            _on_device(t, x, n)
-            if t.numel() != cols:
-                raise ValueError(f"layernorm_train: {n} must have {cols} elements")
-    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
-        raise ValueError("layernorm_train: gamma and beta must be of one type")
-    lib = lib or kt_lib.load()
+    beta_dtype = None
+    if gamma is not None:
+        wdt = _dtype(gamma, "gamma")
+        _dense(gamma, "gamma", torch.float32 if wdt == kt_lib.KT_F32 else x.dtype, dev)
+        if gamma.numel() != cols:
+            raise ValueError(f"layernorm_train: gamma must have {cols} elements")
+    if beta is not None:
+        beta_dtype = beta.dtype
+        wdt_beta = _dtype(beta, "beta")
+        _dense(beta, "beta", torch.float32 if wdt_beta == kt_lib.KT_F32 else x.dtype, dev)
+        if beta.numel() != cols:
+            raise ValueError(f"layernorm_train: beta must have {cols} elements")
+        if gamma is not None and wdt_beta != wdt:
+            raise ValueError("layernorm_train: gamma and beta must be of one type")
+        wdt = wdt_beta
+    if lib is None:
+        lib = kt_lib.load()
     y = torch.empty_like(x)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    mean, rstd = stats[0], stats[1]
-    q8 = torch.empty((rows, cols), dtype=torch.int8, device=x.device) if ckpt8 else None
-    q8_exp = torch.empty((rows, (cols + 31) // 32), dtype=torch.uint8, device=x.device) if ckpt8 else None
-    _launch(x, lib.layernorm_train_fwd, x.data_ptr(), _ptr(gamma), _ptr(beta), y.data_ptr(), mean.data_ptr(),
-            rstd.data_ptr(), _ptr(q8), _ptr(q8_exp), rows, cols, float(eps), dt, wdt)
-    return y, LayerNormSaved(None if ckpt8 else x, q8, q8_exp, gamma, mean, rstd,
-                             beta.dtype if beta is not None else None)
+    stats = x.new_empty((2, rows), dtype=torch.float32)
+    at = stats.data_ptr()
+    q8 = q8_exp = None
+    if ckpt8:
+        q8 = x.new_empty((rows, cols), dtype=torch.int8)
+        q8_exp = x.new_empty((rows, (cols + 31) // 32), dtype=torch.uint8)
+    _launch(dev, lib.layernorm_train_fwd, x.data_ptr(), _ptr(gamma), _ptr(beta), y.data_ptr(), at, at + 4 * rows,
+            _ptr(q8), _ptr(q8_exp), rows, cols, eps, dt, wdt)
+    return y, LayerNormSaved(None if ckpt8 else x, q8, q8_exp, gamma, stats, beta_dtype)
 
 
 def layernorm_bwd(dy: torch.Tensor, saved: LayerNormSaved, weight_grads: bool = True,
@@ -216,30 +230,31 @@ def layernorm_bwd(dy: torch.Tensor, saved: LayerNormSaved, weight_grads: bool = 
                   ) -> tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
     """(dx, dgamma, dbeta) of layernorm_train from dy. dgamma and dbeta are of
     gamma's type and None where gamma or beta was None, or weight_grads is False."""
-    kept = saved.q8 if saved.x is None else saved.x
+    x, q8, q8_exp, gamma, stats, beta_dtype = saved
+    kept = q8 if x is None else x
     dt = _dtype(dy, "dy")
-    _check(dy, "dy", dy.dtype if saved.x is None else saved.x.dtype)
-    _on_device(dy, kept, "dy")
+    dev = kept.get_device()
+    _dense(dy, "dy", dy.dtype if x is None else x.dtype, dev)
     if dy.shape != kept.shape:
         raise ValueError(f"layernorm_bwd: dy is {tuple(dy.shape)}, the input was {tuple(kept.shape)}")
     rows, cols = dy.shape
-    gamma = saved.gamma
-    wt = gamma.dtype if gamma is not None else saved.beta_dtype or torch.float32
-    if wt not in (torch.float32, dy.dtype):
-        raise ValueError(f"dy must be {wt}, got {dy.dtype}")
+    wt = gamma.dtype if gamma is not None else beta_dtype or torch.float32
     wdt = _DTYPES[wt]
-    lib = lib or kt_lib.load()
+    if wdt not in (kt_lib.KT_F32, dt):
+        raise ValueError(f"dy must be {wt}, got {dy.dtype}")
+    if lib is None:
+        lib = kt_lib.load()
     dx = torch.empty_like(dy)
     dgamma = dbeta = ws = None
     ws_bytes = 0
-    if weight_grads and (gamma is not None or saved.beta_dtype is not None):
-        dgamma = torch.empty(cols, dtype=wt, device=dy.device) if gamma is not None else None
-        dbeta = torch.empty(cols, dtype=wt, device=dy.device) if saved.beta_dtype is not None else None
+    if weight_grads and (gamma is not None or beta_dtype is not None):
+        dgamma = torch.empty_like(gamma) if gamma is not None else None
+        dbeta = dy.new_empty(cols, dtype=wt) if beta_dtype is not None else None
         ws_bytes = lib.layernorm_bwd_workspace_bytes(rows, cols)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dy.device)
-    _launch(dy, lib.layernorm_train_bwd, dy.data_ptr(), _ptr(saved.x), _ptr(saved.q8), _ptr(saved.q8_exp),
-            _ptr(gamma), saved.mean.data_ptr(), saved.rstd.data_ptr(), dx.data_ptr(), _ptr(dgamma), _ptr(dbeta),
-            rows, cols, dt, wdt, _ptr(ws), ws_bytes)
+        ws = dy.new_empty(ws_bytes, dtype=torch.uint8)
+    at = stats.data_ptr()
+    _launch(dev, lib.layernorm_train_bwd, dy.data_ptr(), _ptr(x), _ptr(q8), _ptr(q8_exp), _ptr(gamma), at,
+            at + 4 * rows, dx.data_ptr(), _ptr(dgamma), _ptr(dbeta), rows, cols, dt, wdt, _ptr(ws), ws_bytes)
     return dx, dgamma, dbeta
 
 
@@ -253,11 +268,10 @@ class TokenLogprobs(NamedTuple):
     top_index: torch.Tensor
 
 
-def _check_targets(targets: torch.Tensor, logits: torch.Tensor) -> None:
-    _check(targets, "targets", torch.int64)
-    _on_device(targets, logits, "targets")
-    if targets.dim() != 1 or targets.shape[0] != logits.shape[0]:
-        raise ValueError(f"targets must be ({logits.shape[0]},), got {tuple(targets.shape)}")
+def _per_row(t: torch.Tensor, name: str, dtype: torch.dtype, rows: int, device: int) -> None:
+    _dense(t, name, dtype, device)
+    if t.dim() != 1 or t.shape[0] != rows:
+        raise ValueError(f"{name} must be ({rows},), got {tuple(t.shape)}")
 
 
 def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top_k: int = 0, scale: float = 1.0,
@@ -270,22 +284,23 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     other targets that are no column get NaN and set the library's device error.
     """
     dt = _dtype(logits, "logits")
-    _rows(logits, "logits")
+    ld = _rows(logits, "logits")
     rows, vocab = logits.shape
+    dev = logits.get_device()
     if targets is not None:
-        _check_targets(targets, logits)
+        _per_row(targets, "targets", torch.int64, rows, dev)
     if not 0 <= top_k <= 32 or (rows and top_k > vocab):
         raise ValueError(f"top_k must be between 0 and min(32, vocab), got {top_k}")
-    lib = lib or kt_lib.load()
-    dev = logits.device
-    stats = torch.empty((3, rows), dtype=torch.float32, device=dev)
-    logprob, entropy, lse = stats.unbind(0)
-    top_logprob = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
-    top_index = torch.empty((rows, top_k), dtype=torch.int64, device=dev)
-    _launch(logits, lib.token_logprobs, logits.data_ptr(), _ld(logits), _ptr(targets), rows, vocab, float(scale),
-            ignore_index, top_k, logprob.data_ptr(), entropy.data_ptr(), lse.data_ptr(), top_logprob.data_ptr(),
-            top_index.data_ptr(), dt)
-    return TokenLogprobs(logprob if targets is not None else None, entropy, lse, top_logprob, top_index)
+    if lib is None:
+        lib = kt_lib.load()
+    logprob = logits.new_empty(rows, dtype=torch.float32) if targets is not None else None
+    entropy = logits.new_empty(rows, dtype=torch.float32)
+    lse = torch.empty_like(entropy)
+    top_logprob = logits.new_empty((rows, top_k), dtype=torch.float32)
+    top_index = logits.new_empty((rows, top_k), dtype=torch.int64)
+    _launch(dev, lib.token_logprobs, logits.data_ptr(), ld, _ptr(targets), rows, vocab, scale, ignore_index, top_k,
+            _ptr(logprob), entropy.data_ptr(), lse.data_ptr(), top_logprob.data_ptr(), top_index.data_ptr(), dt)
+    return TokenLogprobs(logprob, entropy, lse, top_logprob, top_index)
 
 
 def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], result: TokenLogprobs,
@@ -296,32 +311,33 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], re
     entropies (fp32, (rows,); None: 0); result, scale and ignore_index are those
     of token_logprobs. `out` may be the logits themselves."""
     dt = _dtype(logits, "logits")
-    _rows(logits, "logits")
+    ld = _rows(logits, "logits")
     rows, vocab = logits.shape
-    for t, n in ((grad_logprob, "grad_logprob"), (grad_entropy, "grad_entropy"), (result.lse, "result.lse"),
-                 (result.entropy, "result.entropy")):
-        if t is not None:
-            _check(t, n, torch.float32)
-            _on_device(t, logits, n)
-            if t.dim() != 1 or t.shape[0] != rows:
-                raise ValueError(f"{n} must be ({rows},), got {tuple(t.shape)}")
+    dev = logits.get_device()
+    _per_row(result.lse, "result.lse", torch.float32, rows, dev)
+    _per_row(result.entropy, "result.entropy", torch.float32, rows, dev)
+    if grad_logprob is not None:
+        _per_row(grad_logprob, "grad_logprob", torch.float32, rows, dev)
+        if targets is None:
+            raise ValueError("grad_logprob needs targets")
+    if grad_entropy is not None:
+        _per_row(grad_entropy, "grad_entropy", torch.float32, rows, dev)
     if targets is not None:
-        _check_targets(targets, logits)
-    elif grad_logprob is not None:
-        raise ValueError("grad_logprob needs targets")
+        _per_row(targets, "targets", torch.int64, rows, dev)
     if out is None:
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+        out = logits.new_empty((rows, vocab))
+        ld_out = vocab
     else:
-        _rows(out, "out")
-        _on_device(out, logits, "out")
-        if out.shape != logits.shape or out.dtype != logits.dtype:
-            raise ValueError(f"out must be {tuple(logits.shape)} {logits.dtype}")
-        if rows > 1 and out.stride(0) < vocab:
+        ld_out = _rows(out, "out")
+        if out.shape != logits.shape or out.dtype != logits.dtype or out.get_device() != dev:
+            raise ValueError(f"out must be {tuple(logits.shape)} {logits.dtype} on {logits.device}")
+        if rows > 1 and ld_out < vocab:
             raise ValueError("out: rows overlap")
-    lib = lib or kt_lib.load()
-    _launch(logits, lib.token_logprobs_bwd, logits.data_ptr(), _ld(logits), _ptr(targets), result.lse.data_ptr(),
-            result.entropy.data_ptr(), _ptr(grad_logprob), _ptr(grad_entropy), rows, vocab, float(scale),
-            ignore_index, out.data_ptr(), _ld(out), dt)
+    if lib is None:
+        lib = kt_lib.load()
+    _launch(dev, lib.token_logprobs_bwd, logits.data_ptr(), ld, _ptr(targets), result.lse.data_ptr(),
+            result.entropy.data_ptr(), _ptr(grad_logprob), _ptr(grad_entropy), rows, vocab, scale, ignore_index,
+            out.data_ptr(), ld_out, dt)
     return out
 
 
@@ -348,10 +364,10 @@ def w4_quantize(weight: torch.Tensor, group: int = 128, scale_dtype: Optional[to
     if group not in (32, 64, 128) or K % group:
         raise ValueError(f"group must be 32, 64 or 128 and divide K={K}, got {group}")
     lib = lib or kt_lib.load()
-    packed = torch.empty((N, K // 2), dtype=torch.uint8, device=weight.device)
-    scales = torch.empty((N, K // group), dtype=scale_dtype or weight.dtype, device=weight.device)
-    _launch(weight, lib.w4_quantize, weight.data_ptr(), N, K, group, dt, packed.data_ptr(), scales.data_ptr(),
-            _dtype(scales, "scales"))
+    packed = weight.new_empty((N, K // 2), dtype=torch.uint8)
+    scales = weight.new_empty((N, K // group), dtype=scale_dtype or weight.dtype)
+    _launch(weight.get_device(), lib.w4_quantize, weight.data_ptr(), N, K, group, dt, packed.data_ptr(),
+            scales.data_ptr(), _dtype(scales, "scales"))
     return W4Weight(packed, scales, None, group)
 
 
@@ -360,38 +376,34 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias: Optional[torch.Tensor] = 
     """y = x w^T + bias for a few tokens x (M, K), fp32, bf16 or fp16, with 4-bit weights."""
     packed, scales, zeros, group = weight
     dt = _dtype(x, "x")
-    _rows(x, "x")
+    ldx = _rows(x, "x")
     M, K = x.shape
-    _check(packed, "packed", torch.uint8)
-    _check(scales, "scales", x.dtype)
+    dev = x.get_device()
+    _dense(packed, "packed", torch.uint8, dev)
+    _dense(scales, "scales", x.dtype, dev)
     if packed.dim() != 2 or packed.shape[1] * 2 != K:
         raise ValueError(f"w4_linear: packed must be (N, {K // 2}), got {tuple(packed.shape)}")
     N = packed.shape[0]
     if group not in (32, 64, 128) or K % group:
         raise ValueError(f"group must be 32, 64 or 128 and divide K={K}, got {group}")
-    per = (N, K // group)
-    if scales.shape != per:
-        raise ValueError(f"w4_linear: scales must be {per}, got {tuple(scales.shape)}")
-    _on_device(packed, x, "packed")
-    _on_device(scales, x, "scales")
+    if scales.shape != (N, K // group):
+        raise ValueError(f"w4_linear: scales must be {(N, K // group)}, got {tuple(scales.shape)}")
     if zeros is not None:
-        _check(zeros, "zeros", torch.uint8)
-        _on_device(zeros, x, "zeros")
-        if zeros.shape != per:
-            raise ValueError(f"w4_linear: zeros must be {per}, got {tuple(zeros.shape)}")
+        _dense(zeros, "zeros", torch.uint8, dev)
+        if zeros.shape != scales.shape:
+            raise ValueError(f"w4_linear: zeros must be {(N, K // group)}, got {tuple(zeros.shape)}")
     if bias is not None:
-        _check(bias, "bias", x.dtype)
-        _on_device(bias, x, "bias")
+        _dense(bias, "bias", x.dtype, dev)
         if bias.numel() != N:
             raise ValueError(f"w4_linear: bias must have {N} elements")
     if out is None:
-        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        out = x.new_empty((M, N))
     else:
-        _check(out, "out", x.dtype)
-        _on_device(out, x, "out")
+        _dense(out, "out", x.dtype, dev)
         if out.shape != (M, N):
             raise ValueError(f"out must be {(M, N)}, got {tuple(out.shape)}")
-    lib = lib or kt_lib.load()
-    _launch(x, lib.w4_linear, x.data_ptr(), _ld(x), packed.data_ptr(), scales.data_ptr(), _ptr(zeros), _ptr(bias),
+    if lib is None:
+        lib = kt_lib.load()
+    _launch(dev, lib.w4_linear, x.data_ptr(), ldx, packed.data_ptr(), scales.data_ptr(), _ptr(zeros), _ptr(bias),
             out.data_ptr(), N, M, N, K, group, dt)
     return out
