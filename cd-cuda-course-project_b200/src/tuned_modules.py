@@ -13,15 +13,25 @@ calls it through the C ABI on the current CUDA stream:
                           nn.Linear weight is already the N×K "Bt" layout);
                           TF32 tensor cores by default, exact FFMA on request
                           or when the tuned winner is the FFMA variant
-  TunedLayerNorm          kt_layernorm_f32 over the last dimension
+  TunedLayerNorm          kt_layernorm_f32 over the last dimension; under
+                          autograd, or for bf16 and fp16 inputs, the training
+                          kernels (kt_layernorm_train_fwd / _bwd), which can
+                          keep the input in 8 bits for the backward pass
   TunedMultiheadAttention q/k/v/out projections as TunedLinear, the attention
                           core as kt_fa_fwd_bf16 (bf16 Q/K/V, fp32 softmax and
                           accumulation), optionally causal
 
-They are inference layers (the library has forward kernels only): a call
-with autograd recording raises instead of silently computing something else.
-`apply_tuned_layers` swaps them into a model, copying the weights (the
-reference's version builds fresh layers and drops the trained weights).
+  TunedLinearW4           y = x·W^T (+ b) with 4-bit weights for serving few
+                          tokens (kt_w4_linear), made from an nn.Linear
+  token_log_probs         log probabilities of given tokens, entropies and top
+                          alternatives of logits, with their gradient
+                          (kt_token_logprobs / _bwd)
+
+The linear and attention layers are inference layers (they have forward
+kernels only): a call with autograd recording raises instead of silently
+computing something else. `apply_tuned_layers` swaps layers into a model,
+copying the weights (the reference's version builds fresh layers and drops the
+trained weights).
 `sdpa_comparison` checks and times the attention core against
 torch.nn.functional.scaled_dot_product_attention (the reference's SDPA vs
 manual-attention benchmark, src/pytorch_integration.py:120-192).
@@ -98,22 +108,122 @@ class TunedLinear(nn.Linear):
         return y.view(*lead, self.out_features)
 
 
+class _LayerNormTrain(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, checkpoint8):
+        y, saved = kt_ops.layernorm_train(x, weight, bias, eps, ckpt8=checkpoint8)
+        ctx.save_for_backward(saved.x, saved.q8, saved.q8_exp, saved.gamma, saved.stats)
+        ctx.beta_dtype = saved.beta_dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        saved = kt_ops.LayerNormSaved(*ctx.saved_tensors, ctx.beta_dtype)
+        weights = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dx, dgamma, dbeta = kt_ops.layernorm_bwd(dy.contiguous(), saved, weight_grads=weights)
+        return dx, dgamma, dbeta, None, None
+
+
 class TunedLayerNorm(nn.LayerNorm):
-    """nn.LayerNorm over the last dimension computed by the library's LayerNorm kernel."""
+    """nn.LayerNorm over the last dimension computed by the library's LayerNorm kernels.
+
+    With autograd recording it is differentiable (once); checkpoint8 then keeps
+    the input for the backward pass in 8 bits. Inputs are fp32, bf16 or fp16, the
+    weights fp32 or of the input's type.
+    """
 
     def __init__(self, normalized_shape: int, eps: float = 1e-5, results_dir: Optional[os.PathLike] = None,
-                 device=None, dtype=None) -> None:
+                 device=None, dtype=None, checkpoint8: bool = False) -> None:
         super().__init__(normalized_shape, eps=eps, elementwise_affine=True, device=device, dtype=dtype)
         if len(self.normalized_shape) != 1:
             raise ValueError("TunedLayerNorm normalises the last dimension only")
         self.tuned_params = load_best_params("layernorm", results_dir)
         self._lib = tuned_library("layernorm", results_dir)
+        self.checkpoint8 = checkpoint8
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        _no_autograd("TunedLayerNorm", x, self.weight, self.bias)
         c = self.normalized_shape[0]
-        y = kt_ops.layernorm(x.reshape(-1, c).contiguous(), self.weight, self.bias, self.eps, lib=self._lib)
+        x2 = x.reshape(-1, c).contiguous()
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (x, self.weight, self.bias)):
+            y = _LayerNormTrain.apply(x2, self.weight, self.bias, self.eps, self.checkpoint8)
+        elif x.dtype == torch.float32:
+            y = kt_ops.layernorm(x2, self.weight, self.bias, self.eps, lib=self._lib)
+        else:
+            y, _ = kt_ops.layernorm_train(x2, self.weight, self.bias, self.eps)
         return y.view(x.shape)
+
+
+class TunedLinearW4(nn.Module):
+    """A linear layer with 4-bit weights (kt_ops.W4Weight) for serving few tokens.
+
+    The weights are buffers (packed, scales, zeros); inputs and bias are of the
+    scales' type. Inference only.
+    """
+
+    def __init__(self, weight: kt_ops.W4Weight, bias: Optional[torch.Tensor] = None) -> None:
+        super().__init__()
+        self.group = weight.group
+        self.in_features = 2 * weight.packed.shape[1]
+        self.out_features = weight.packed.shape[0]
+        self.register_buffer("packed", weight.packed)
+        self.register_buffer("scales", weight.scales)
+        self.register_buffer("zeros", weight.zeros)
+        self.register_buffer("bias", bias)
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear, group: int = 128) -> "TunedLinearW4":
+        """Quantise a linear layer's weight (on a CUDA device) symmetrically in groups of `group` columns."""
+        w = kt_ops.w4_quantize(linear.weight.detach().contiguous(), group)
+        return cls(w, linear.bias.detach().clone() if linear.bias is not None else None)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        _no_autograd("TunedLinearW4", x)
+        w = kt_ops.W4Weight(self.packed, self.scales, self.zeros, self.group)
+        y = kt_ops.w4_linear(x.reshape(-1, self.in_features), w, self.bias)
+        return y.view(*x.shape[:-1], self.out_features)
+
+
+class _TokenLogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top_k, scale, ignore_index):
+        r = kt_ops.token_logprobs(logits, targets, top_k, scale, ignore_index)
+        ctx.save_for_backward(logits, targets, r.entropy, r.lse)
+        ctx.scale, ctx.ignore_index = scale, ignore_index
+        ctx.mark_non_differentiable(r.lse, r.top_logprob, r.top_index)
+        ctx.set_materialize_grads(False)
+        return tuple(r)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_logprob, grad_entropy, *_):
+        logits, targets, entropy, lse = ctx.saved_tensors
+        if grad_logprob is None and grad_entropy is None:
+            return None, None, None, None, None
+        grads = [g.contiguous() if g is not None else None for g in (grad_logprob, grad_entropy)]
+        r = kt_ops.TokenLogprobs(None, entropy, lse, None, None)
+        dx = kt_ops.token_logprobs_bwd(logits, targets, r, *grads, scale=ctx.scale, ignore_index=ctx.ignore_index)
+        return dx, None, None, None, None
+
+
+def token_log_probs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top_k: int = 0, scale: float = 1.0,
+                    ignore_index: int = -100) -> kt_ops.TokenLogprobs:
+    """kt_ops.token_logprobs over the last dimension of logits with any leading
+    dimensions (those of targets), differentiable (once) through logprob and entropy."""
+    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    x = logits.reshape(-1, vocab)
+    if x.shape[1] > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    if targets is not None:
+        if targets.shape != lead:
+            raise ValueError(f"targets must be {tuple(lead)}, got {tuple(targets.shape)}")
+        targets = targets.reshape(-1).contiguous()
+    if torch.is_grad_enabled() and logits.requires_grad:
+        r = kt_ops.TokenLogprobs(*_TokenLogProbs.apply(x, targets, top_k, scale, ignore_index))
+    else:
+        r = kt_ops.token_logprobs(x, targets, top_k, scale, ignore_index)
+    return kt_ops.TokenLogprobs(r.logprob.view(lead) if r.logprob is not None else None, r.entropy.view(lead),
+                                r.lse.view(lead), r.top_logprob.view(*lead, top_k), r.top_index.view(*lead, top_k))
 
 
 class TunedMultiheadAttention(nn.Module):
@@ -164,13 +274,20 @@ class TunedMultiheadAttention(nn.Module):
 
 def apply_tuned_layers(model: nn.Module, kernel: str = "matmul", results_dir: Optional[os.PathLike] = None) -> nn.Module:
     """Replace nn.Linear (kernel "matmul" or "all") and nn.LayerNorm ("layernorm" or "all")
-    in `model` by their tuned versions, in place, keeping the weights."""
+    in `model` by their tuned versions, in place, keeping the weights; "w4" replaces
+    nn.Linear by layers with 4-bit weights in groups of 128 (or else 64, 32) columns
+    where one divides the input features."""
     for name, module in list(model.named_modules()):
         if not name:
             continue
         parent_name, _, child = name.rpartition(".")
         parent = model.get_submodule(parent_name) if parent_name else model
         new = None
+        if kernel == "w4" and type(module) is nn.Linear:
+            group = next((g for g in (128, 64, 32) if module.in_features % g == 0), None)
+            if group is not None:
+                setattr(parent, child, TunedLinearW4.from_linear(module, group))
+            continue
         if kernel in ("matmul", "all") and type(module) is nn.Linear:
             new = TunedLinear(module.in_features, module.out_features, module.bias is not None,
                               results_dir=results_dir, device=module.weight.device, dtype=module.weight.dtype)
