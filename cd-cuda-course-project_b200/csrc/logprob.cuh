@@ -487,7 +487,7 @@ struct Shared {
 };
 
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kBlock, 4) fwd_kernel(const FwdArgs p) {
+__global__ void __launch_bounds__(kBlock, TOP ? 5 : 4) fwd_kernel(const FwdArgs p) {
   namespace cg = cooperative_groups;
   __shared__ Shared<TOP> sh;
   const cg::cluster_group cluster = cg::this_cluster();
