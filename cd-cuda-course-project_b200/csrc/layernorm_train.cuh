@@ -860,15 +860,18 @@ inline int row_grid(K kern, int block, int rb, size_t smem, int64_t rows, int* g
 
 // Calls f with the threads per row and pieces per thread for a row of `pieces`
 // 16-byte pieces: 16 columns per thread (32 in the widest rows). False when a row
-// is too wide.
+// is too wide. Rows of up to 64 threads share a CTA where there are more than four
+// per SM (16384x512 bf16 forward: 7.5 us, and 15 by 128 threads a row); fewer rows
+// are spread over the SMs (64x512 backward: 4.1 us, and 4.8 by 32 threads a row).
 template <typename T, class F>
-inline bool with_shape(int64_t pieces, F f) {
+inline bool with_shape(int64_t pieces, int64_t rows, F f) {
   constexpr int VPT = 16 / elem::kVec<T>;
+  const bool many = rows > 4 * sm_count();
   using One = std::integral_constant<int, 1>;
   using All = std::integral_constant<int, VPT>;
-  if (pieces <= 32) return f(std::integral_constant<int, 32>{}, One{}), true;
-  if (pieces <= 32 * VPT) return f(std::integral_constant<int, 32>{}, All{}), true;
-  if (pieces <= 64 * VPT) return f(std::integral_constant<int, 64>{}, All{}), true;
+  if (pieces <= 32 && many) return f(std::integral_constant<int, 32>{}, One{}), true;
+  if (pieces <= 32 * VPT && many) return f(std::integral_constant<int, 32>{}, All{}), true;
+  if (pieces <= 64 * VPT && many) return f(std::integral_constant<int, 64>{}, All{}), true;
   using Twice = std::integral_constant<int, 2 * VPT>;
   if (pieces <= 128 * VPT) return f(std::integral_constant<int, 128>{}, All{}), true;
   if (pieces <= 256 * VPT) return f(std::integral_constant<int, 256>{}, All{}), true;
@@ -896,7 +899,7 @@ inline int fwd_typed(const FwdArgs& a, cudaStream_t st) {
   const bool edge = shift != 0 || a.cols % V != 0;  // (not with checkpoints)
   const int64_t pieces = (a.cols + V - 1) / V + (edge ? 1 : 0);
   int rc = KT_OK;
-  if (fast && with_shape<T>(pieces, [&](auto tpr, auto vpt) {
+  if (fast && with_shape<T>(pieces, a.rows, [&](auto tpr, auto vpt) {
         constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
         constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
         auto kern = edge ? fwd_rows<T, TPR, VPT, CKPT, !CKPT> : fwd_rows<T, TPR, VPT, CKPT, false>;
@@ -949,7 +952,7 @@ inline int bwd_typed(const BwdArgs& a, void* dgamma, void* dbeta, cudaStream_t s
   const bool edge = shift != 0 || a.cols % V != 0;  // (not with checkpoints)
   const int64_t pieces = (a.cols + V - 1) / V + (edge ? 1 : 0);
   int rc = KT_OK, parts = 0;
-  if (!(fast && with_shape<T>(pieces, [&](auto tpr, auto vpt) {
+  if (!(fast && with_shape<T>(pieces, a.rows, [&](auto tpr, auto vpt) {
           constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
           constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
           auto kern = edge ? bwd_rows<T, TPR, VPT, CKPT, !CKPT> : bwd_rows<T, TPR, VPT, CKPT, false>;
