@@ -309,7 +309,7 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], re
                        lib: Optional[kt_lib.KtLibrary] = None) -> torch.Tensor:
     """Gradient of the logits from those of the log probabilities and the
     entropies (fp32, (rows,); None: 0); result, scale and ignore_index are those
-    of token_logprobs. `out` may be the logits themselves."""
+    of token_logprobs. `out` may be the logits themselves, not a part of their memory."""
     dt = _dtype(logits, "logits")
     ld = _rows(logits, "logits")
     rows, vocab = logits.shape
@@ -333,6 +333,10 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], re
             raise ValueError(f"out must be {tuple(logits.shape)} {logits.dtype} on {logits.device}")
         if rows > 1 and ld_out < vocab:
             raise ValueError("out: rows overlap")
+        at, to, size = logits.data_ptr(), out.data_ptr(), logits.element_size()
+        if rows and (at, ld) != (to, ld_out) and at < to + ((rows - 1) * ld_out + vocab) * size \
+                and to < at + ((rows - 1) * ld + vocab) * size:
+            raise ValueError("out overlaps the logits without being the same")
     if lib is None:
         lib = kt_lib.load()
     _launch(dev, lib.token_logprobs_bwd, logits.data_ptr(), ld, _ptr(targets), result.lse.data_ptr(),

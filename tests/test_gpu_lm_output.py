@@ -129,6 +129,12 @@ def test_token_log_probs_autograd(dev, lib):
     x.grad = None
     tm.token_log_probs(x, t).logprob.mean().backward()  # a gradient that is expanded
     assert x.grad.isfinite().all()
+    x.grad = None
+    tm.token_log_probs(x).entropy.sum().backward()  # no targets
+    xd.grad = None
+    logp = torch.log_softmax(xd, -1)
+    (-(logp.exp() * logp).sum()).backward()
+    assert normwise(x.grad, xd.grad) <= 1e-5
     with pytest.raises(ValueError):
         tm.token_log_probs(x, t[:2])
 

@@ -290,6 +290,8 @@ def test_empty_and_refusals(dev, lib):
            lambda: kt_ops.token_logprobs_bwd(x, targets, r, r.lse[:2], lib=lib),
            lambda: kt_ops.token_logprobs_bwd(x, targets, r, r.lse, out=x[:, :50], lib=lib),
            lambda: kt_ops.token_logprobs_bwd(x, targets, r, r.lse, out=x[:1].expand(4, 100), lib=lib)]
+    both = torch.zeros(5, 100, dtype=x.dtype, device=dev)
+    bad.append(lambda: kt_ops.token_logprobs_bwd(both[:4], targets, r, r.lse, out=both[1:], lib=lib))
     for f in bad:
         with pytest.raises(ValueError):
             f()

@@ -127,6 +127,22 @@ def test_large_and_deterministic(dev, lib, m, n, k, t, group):
     assert torch.equal(y, kt_ops.w4_linear(x, w, bias, lib=lib))
 
 
+@pytest.mark.parametrize("m,k,group", [(1, 4096, 128), (8, 8192, 64), (16, 8192, 32), (13, 16384, 128)])
+def test_many_calls_agree(dev, lib, m, k, group):
+    """Bits of many calls, behind one another and on two streams at once."""
+    x, w, bias = make(dev, m, 5000, k, group, torch.bfloat16)
+    want = check(x, w, bias, lib)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(30):
+        got.append(kt_ops.w4_linear(x, w, bias, lib=lib))
+        with torch.cuda.stream(side):
+            got.append(kt_ops.w4_linear(x, w, bias, lib=lib))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
 def test_offsets_past_32_bits(dev, lib):
     """9 billion weights: byte offsets need 33 bits, those of columns 34."""
     n, k = 1_100_000, 8192
