@@ -12,9 +12,9 @@
 // s = sum 2^y and t = sum y 2^y with y = (x - m) scale log2 e, and rescales them
 // when its maximum grows, so H = ln 2 (log2 s - t / s) needs no second pass.
 // (One fused multiply-add per y would be off by the rounding of m scale log2 e:
-// a certain token would not get log probability 0.) Bound by memory for 32-bit logits; for 16-bit ones the one
-// exponential per value takes about 3/4 of the special-function rate that goes
-// with the full read rate.
+// a certain token would not get log probability 0.) Bound by memory for 32-bit
+// logits; for 16-bit ones the one exponential per value takes about 3/4 of the
+// special-function rate that goes with the full read rate.
 //
 // The top k of a row need hardly any work in that pass: a thread notes the
 // largest value of each of up to 8 stretches of its pieces. Of the 8 warps, each
@@ -28,8 +28,13 @@
 // k-th best key of the list and are listed again.
 //
 // A row goes to a CTA, or to a single warp where it has at most 512 pieces of 16
-// bytes. Few long rows are split over a cluster of up to 8 CTAs, which join their
+// bytes and rows are many. Few long rows are split over a cluster of up to 8 CTAs, which join their
 // partial results through distributed shared memory in the order of their ranks.
+//
+// Measured on a B200: 2048x131072 bf16 87 us (6.2 TB/s, 95 % of measured copy
+// bandwidth), with 20 alternatives 107 us, its gradient 187 us (5.7 TB/s);
+// 512x131072 fp32 41 us, with 8 alternatives 47 us; one row of 32768 fp32 3.1 us,
+// with 5 alternatives 6.7 us; 2048x1000 bf16 3.8 us.
 #pragma once
 #include <cooperative_groups.h>
 

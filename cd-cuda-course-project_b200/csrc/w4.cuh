@@ -4,8 +4,8 @@
 // columns, z = 8 where no zeros are given.
 //
 // Bound by memory: the weights are read once, N K / 2 bytes. At 6.5 TB/s that
-// is 13 weights per clock and lane slot at most 2.6 instructions each, which
-// fp32 multiply-adds per token would exceed from the second token on. So the
+// is 13 10^12 weights a second, which leaves 2.6 lane instructions for each;
+// fp32 multiply-adds per token would exceed that from the second token on. So the
 // sums run on the tensor cores (mma.sync m16n8k16: 16 weight rows by 8 tokens,
 // fp32 accumulation; a tcgen05 tile of 128 rows would need the weights
 // unpacked through shared memory): q - z is exact in 16 bits, and so are its
@@ -21,7 +21,7 @@
 // that factor comes back when the sums are done.
 //
 // A warp takes 32 rows and segments of 128 columns, 2 KB of weights, which one
-// TMA load brings into a ring of its own, kStages deep: no warp waits for
+// TMA load brings into a ring of its own, 2 to 4 deep: no warp waits for
 // another, and the loads in flight cost neither registers nor address
 // arithmetic. A step of m16n8k16 may take any 16 columns if x has the same
 // order, so a lane reads the words of one group (TMA's 64-byte swizzle: no bank
@@ -36,6 +36,12 @@
 // row by row together, and add their sums through distributed shared memory one
 // turn late (a warp that has left its sums arrives at the cluster's barrier, goes
 // on with the next rows, and waits there before it adds the sums before).
+//
+// Measured on a B200, 131072x8192: one token in bf16, groups of 128, 106 us
+// (5.2 TB/s, 80 % of measured copy bandwidth); 8 tokens in fp16, groups of 64 with
+// zeros, 138 us (4.3 TB/s; issue slots 66 % busy, the ALU pipe 52 %); 16 tokens in
+// bf16 180 us. 4096x4096, one token: 5.4 us. 16 fp32 tokens, 32768x8192: 109 us,
+// bound by the three tensor products per weight.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -537,7 +543,10 @@ inline int launch_shape(Args a, cudaStream_t st) {
     return fail(KT_ERR_UNSUPPORTED, "w4_linear: K=%lld is too large", (long long)a.K);
   // How the columns are split: turns x (steps of a warp + what a turn costs
   // beside them, in steps), least. The last turn is mostly not full, and few
-  // rows fill the device only with their columns split.
+  // rows fill the device only with their columns split: one token by 8192x8192
+  // takes 13 us with 8 warps to 32 rows and 25 with one, by 1024x16384 6.7 us with
+  // the columns split over a cluster and 11.6 without; 16 tokens by 16384x16384
+  // take 82 us with the one warp that this finds, and 242 with 16.
   const int64_t m_tiles = (a.M + a.tokens - 1) / a.tokens;
   a.units = (int)((a.N + kRows - 1) / kRows);
   const int sms = sm_count();
