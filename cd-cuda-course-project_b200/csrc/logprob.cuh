@@ -45,7 +45,9 @@
 namespace kt {
 namespace logprob {
 
-constexpr int kBlock = 256;
+constexpr int kBlock = 256;     // threads of a row; kSmall where rows are many and not the longest
+constexpr int kSmall = 128;
+constexpr int kBwdBlock = 128;
 constexpr int kPieces = 4;     // 16-byte pieces of a thread per tile
 constexpr int kStretches = 8;  // of a thread's pieces in a row
 constexpr int kMaxTop = 32;
@@ -494,17 +496,17 @@ __device__ __forceinline__ Stats warp_stats(const Stats& a, float c) {
   return w;
 }
 
-template <bool TOP>
+template <int G, bool TOP>
 struct Shared {
-  Top<TOP ? kBlock : 32> top;
-  Stats warp[kBlock / 32];
+  Top<TOP ? G : 32> top;
+  Stats warp[G / 32];
   Stats all;
 };
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kBlock, TOP ? 5 : 4) fwd_kernel(const FwdArgs p) {
+template <typename T, bool TOP, int G>
+__global__ void __launch_bounds__(G, (TOP ? 5 : 4) * kBlock / G) fwd_kernel(const FwdArgs p) {
   namespace cg = cooperative_groups;
-  __shared__ Shared<TOP> sh;
+  __shared__ Shared<G, TOP> sh;
   const cg::cluster_group cluster = cg::this_cluster();
   const int split = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -513,17 +515,18 @@ __global__ void __launch_bounds__(kBlock, TOP ? 5 : 4) fwd_kernel(const FwdArgs 
   const Row<T> r(p, row, split, part);
   Target target{};
   if (part == 0 && threadIdx.x == 0) target = load_target<T>(p, row);
-  uint32_t(*maxima)[kBlock] = nullptr;
+  uint32_t(*maxima)[G] = nullptr;
   if constexpr (TOP) maxima = sh.top.maxima;
-  Stats a = warp_stats(stream<T, kBlock, TOP>(p, r, threadIdx.x, c, maxima), c);
+  Stats a = warp_stats(stream<T, G, TOP>(p, r, threadIdx.x, c, maxima), c);
   if (lane == 0) sh.warp[warp] = a;
   __syncthreads();
   if (warp == 0) {
-    a = warp_stats(lane < kBlock / 32 ? sh.warp[lane] : Stats{-INFINITY, 0.f, 0.f}, c);
+    a = warp_stats(lane < G / 32 ? sh.warp[lane] : Stats{-INFINITY, 0.f, 0.f}, c);
     if (lane == 0) sh.all = a;
   }
-  if constexpr (TOP) find_top<T, kBlock>(sh.top, p, r, threadIdx.x);
-  if (split > 1) {  // the first CTA joins the others' results
+  if constexpr (TOP) find_top<T, G>(sh.top, p, r, threadIdx.x);
+  static_assert(!TOP || kBlock >= kMaxCluster * kMaxTop, "a thread per key of the joined lists");
+  if (G == kBlock && split > 1) {  // the first CTA joins the others' results
     cluster.sync();
     if (part == 0) {
       if (warp == 0) {
@@ -538,12 +541,12 @@ __global__ void __launch_bounds__(kBlock, TOP ? 5 : 4) fwd_kernel(const FwdArgs 
           sh.top.list[i] = i % p.top < o.best_count ? o.best[i % p.top] : 0;  // 0 is below every key
         }
         __syncthreads();
-        best_of_list<kBlock>(sh.top, n, p.top, i);
+        best_of_list<G>(sh.top, n, p.top, i);
       }
     }
   }
   if (part == 0 && warp == 0) write_row<TOP>(p, row, a, target, sh.top.best);
-  if (split > 1) cluster.sync();  // the other CTAs' shared memory is read above
+  if (G == kBlock && split > 1) cluster.sync();  // the other CTAs' shared memory is read above
 }
 
 // Short rows by single warps.
@@ -567,7 +570,7 @@ __global__ void __launch_bounds__(TOP ? 128 : kBlock) fwd_warp_kernel(const FwdA
 }
 
 template <typename T, bool VECTOR>
-__global__ void __launch_bounds__(kBlock) bwd_kernel(const BwdArgs p) {
+__global__ void __launch_bounds__(kBwdBlock) bwd_kernel(const BwdArgs p) {
   constexpr int V = VECTOR ? elem::kVec<T> : 1;
   const int64_t row = blockIdx.x / p.chunks;
   const int64_t at = blockIdx.x - row * p.chunks;
@@ -590,7 +593,7 @@ __global__ void __launch_bounds__(kBlock) bwd_kernel(const BwdArgs p) {
   };
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
-    const int64_t e0 = ((at * kPieces + i) * kBlock + threadIdx.x) * V - shift;
+    const int64_t e0 = ((at * kPieces + i) * kBwdBlock + threadIdx.x) * V - shift;
     if (e0 >= p.vocab) continue;
     if (V > 1 && e0 >= 0 && e0 + V <= p.vocab) {
       float f[elem::kVec<T>];
@@ -635,6 +638,15 @@ inline int fwd_typed(const FwdArgs& a, cudaStream_t st) {
     fwd_warp_kernel<T, TOP><<<(unsigned)grid, block, 0, st>>>(a);
     return check_launch("token_logprobs warps");
   }
+  // CTAs of 128 threads where more rows than four per SM have at most 8192 pieces:
+  // more of them end and begin at a time, and the last wave is shorter. 2048 rows of
+  // 50001 bf16 columns take 42 us by 128 threads each and 48 by 256 (8 alternatives:
+  // 55 and 63); of 131072 columns 89 and 88 (20: 114 and 106).
+  if (a.rows > 4 * sm_count() && a.vocab <= (int64_t)8192 * elem::kVec<T>) {
+    if (a.rows > INT32_MAX) return fail(KT_ERR_UNSUPPORTED, "token_logprobs: too many rows");
+    fwd_kernel<T, TOP, kSmall><<<(unsigned)a.rows, kSmall, 0, st>>>(a);
+    return check_launch("token_logprobs small CTAs");
+  }
   // a cluster per row while all CTAs fit on the device at once and each has a tile:
   // one row of 131072 bf16 columns takes 4 us by 8 CTAs and 10 by one
   int split = 1;
@@ -650,7 +662,7 @@ inline int fwd_typed(const FwdArgs& a, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, fwd_kernel<T, TOP>, a), "token_logprobs launch");
+  return cuda_status(cudaLaunchKernelEx(&cfg, fwd_kernel<T, TOP, kBlock>, a), "token_logprobs launch");
 }
 
 inline int forward(const FwdArgs& a, int dtype, cudaStream_t st) {
@@ -675,12 +687,12 @@ inline int bwd_typed(BwdArgs a, cudaStream_t st) {
   constexpr int V = elem::kVec<T>;
   // pieces are aligned in both tensors, for every row
   const bool vec = elem::misalign<T>(a.x) == elem::misalign<T>(a.dx) && (a.rows == 1 || (a.ld - a.ld_dx) % V == 0);
-  const int64_t per = (int64_t)kBlock * kPieces * (vec ? V : 1);
+  const int64_t per = (int64_t)kBwdBlock * kPieces * (vec ? V : 1);
   a.chunks = (a.vocab + (vec ? V - 1 : 0) + per - 1) / per;
   if (a.rows * a.chunks > (int64_t)INT32_MAX) return fail(KT_ERR_UNSUPPORTED, "token_logprobs_bwd: too many values");
   const unsigned grid = (unsigned)(a.rows * a.chunks);
-  if (vec) bwd_kernel<T, true><<<grid, kBlock, 0, st>>>(a);
-  else bwd_kernel<T, false><<<grid, kBlock, 0, st>>>(a);
+  if (vec) bwd_kernel<T, true><<<grid, kBwdBlock, 0, st>>>(a);
+  else bwd_kernel<T, false><<<grid, kBwdBlock, 0, st>>>(a);
   return check_launch("token_logprobs_bwd");
 }
 

@@ -100,7 +100,7 @@ def logits(dev, rows, V, t, seed=0, spread=2.5):
 
 SHAPES = [(1, 1), (3, 2), (5, 7), (4, 32), (9, 33), (2, 255), (7, 1000), (1, 1024), (33, 2049), (3, 4096), (2, 4097),
           (300, 5003), (1, 8191), (1, 16384), (2, 32768), (5, 50001), (1, 131072), (4, 131071), (700, 1500),
-          (1, 300000)]
+          (1, 300000), (700, 9001), (1500, 5000)]
 
 
 @pytest.mark.parametrize("t", TYPES)
@@ -144,8 +144,8 @@ def test_ties_and_orders_that_fill_the_list(dev, lib, t):
     for rows in (slice(0, 8), slice(1, 2), slice(3, 4), slice(7, 8)):
         for k in (1, 8, 32):
             check(x[rows], targets[rows], k=k, lib=lib)
-    many = x.repeat(40, 1)
-    check(many, targets.repeat(40), k=32, grads=False, lib=lib)
+    for copies in (40, 90):  # 256 and 128 threads a row
+        check(x.repeat(copies, 1), targets.repeat(copies), k=32, grads=False, lib=lib)
 
 
 @pytest.mark.parametrize("t", TYPES)
