@@ -30,7 +30,8 @@
 // Measured on a B200, 16384x4096, the join included: bf16 forward 46 us (5.8 TB/s,
 // 88 % of measured copy bandwidth) and backward 72 us (5.6 TB/s); with checkpoints
 // 58 us (5.8 TB/s) and 76 us (4.4 TB/s, issue slots 62 % busy); fp32 98 and 141 us
-// (5.5 and 5.7 TB/s). 8x512 fp32: 2.6 and 4.4 us.
+// (5.5 and 5.7 TB/s). 8x512 fp32: 2.4 and 3.9 us. 4096x16384 bf16: 55 and 79 us
+// (79 and 136 us with gamma and beta read again from L2 in every row).
 #pragma once
 #include <type_traits>
 
@@ -184,18 +185,23 @@ constexpr int kThreads = TPR * kRows<TPR>;
 
 // Threads per SM that the registers are shared among: 16 columns of a thread take
 // 80 (forward) and 128 (backward) with their weights and sums. A thread of wider
-// rows has 32 columns and reads gamma and beta again in every row.
+// rows has 32 columns and keeps gamma and beta in shared memory.
 constexpr int kFwdThreads = 768, kBwdThreads = 512;
 constexpr int kScalar = 16;  // columns of a thread, element by element
 template <typename T, int VPT>
 constexpr bool kHold = VPT * elem::kVec<T> <= 16;
 template <int TPR, int PER_SM>
 constexpr int kCtas = PER_SM / kThreads<TPR>;
-// Rows in shared memory: as many as 200 KB per SM hold, up to 4.
-template <int TPR, int PIECES, int PER_SM>
-constexpr int kDepth = 200 * 1024 / (PIECES * 16 * kThreads<TPR> * kCtas<TPR, PER_SM>) >= 4
-                           ? 4
-                           : 200 * 1024 / (PIECES * 16 * kThreads<TPR> * kCtas<TPR, PER_SM>);
+// Bytes of `tensors` weight vectors in shared memory.
+template <typename T, int TPR, int VPT>
+constexpr int kWeightBytes = kHold<T, VPT> ? 0 : VPT * elem::kVec<T> * 4 * kThreads<TPR>;
+// Rows in shared memory: as many as 200 KB per SM hold (224 KB less the weights), up to 4.
+template <typename T, int TPR, int VPT, int TENSORS, int PER_SM>
+constexpr int kFit = ((kHold<T, VPT> ? 200 : 224) * 1024 / kCtas<TPR, PER_SM> -
+                      (PER_SM == kFwdThreads ? 2 : 1) * kWeightBytes<T, TPR, VPT>) /
+                     (TENSORS * VPT * 16 * kThreads<TPR>);
+template <typename T, int TPR, int VPT, int TENSORS, int PER_SM>
+constexpr int kDepth = kFit<T, TPR, VPT, TENSORS, PER_SM> >= 4 ? 4 : kFit<T, TPR, VPT, TENSORS, PER_SM>;
 template <int N>
 __device__ __forceinline__ void wait_copies() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -282,6 +288,23 @@ __device__ __forceinline__ void load_weights(const void* w, int wdtype, int e0, 
   for (int j = 0; j < V / 2; ++j) pairs[j] = elem::pair(f[2 * j], f[2 * j + 1]);
 }
 
+// A piece's weights in this thread's places of shared memory.
+template <typename T, int THREADS>
+__device__ __forceinline__ void keep_weights(uint4* at, const uint64_t (&w)[elem::kVec<T> / 2]) {
+#pragma unroll
+  for (int j = 0; j < elem::kVec<T> / 4; ++j)
+    *reinterpret_cast<ulonglong2*>(at + j * THREADS) = make_ulonglong2(w[2 * j], w[2 * j + 1]);
+}
+template <typename T, int THREADS>
+__device__ __forceinline__ void kept_weights(const uint4* at, uint64_t (&w)[elem::kVec<T> / 2]) {
+#pragma unroll
+  for (int j = 0; j < elem::kVec<T> / 4; ++j) {
+    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(at + j * THREADS);
+    w[2 * j] = v.x;
+    w[2 * j + 1] = v.y;
+  }
+}
+
 // ---------------------------------------------------------------- forward
 template <typename T, int TPR, int VPT, bool CKPT, bool EDGE>
 __global__ void __launch_bounds__(kThreads<TPR>, kCtas<TPR, kFwdThreads>)
@@ -292,9 +315,9 @@ fwd_rows(const FwdArgs p) {
   using elem::mul2;
   using elem::pair;
   constexpr int V = elem::kVec<T>;
-  constexpr int D = kDepth<TPR, VPT, kFwdThreads>;
+  constexpr int D = kDepth<T, TPR, VPT, 1, kFwdThreads>;
   static_assert(D >= 1, "a row fits shared memory");
-  extern __shared__ uint4 ring[];  // [D][VPT][threads]
+  extern __shared__ uint4 ring[];  // [D][VPT][threads], then gamma and beta unless they are held
   __shared__ float red[2][32];
   const int t = threadIdx.x % TPR;
   const int cols = (int)p.cols;
@@ -316,14 +339,20 @@ fwd_rows(const FwdArgs p) {
   };
 #pragma unroll 1
   for (int d = 0; d < D; ++d) fetch(d, first + d * stride);
-  uint64_t g[VPT][V / 2], b[VPT][V / 2];
-  auto weights = [&](int i) {
-    load_weights<T>(p.gamma, p.wdtype, e_first + i * TPR * V, cols, 1.f, g[i]);
-    load_weights<T>(p.beta, p.wdtype, e_first + i * TPR * V, cols, 0.f, b[i]);
+  constexpr bool HOLD = kHold<T, VPT>;
+  uint64_t g[HOLD ? VPT : 1][V / 2], b[HOLD ? VPT : 1][V / 2];
+  auto kept = [&](int which, int i) {
+    return ring + D * VPT * kThreads<TPR> + (which * VPT + i) * (V / 4) * kThreads<TPR> + threadIdx.x;
   };
-  if constexpr (kHold<T, VPT>) {
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) weights(i);
+  for (int i = 0; i < VPT; ++i) {
+    const int h = HOLD ? i : 0;
+    load_weights<T>(p.gamma, p.wdtype, e_first + i * TPR * V, cols, 1.f, g[h]);
+    load_weights<T>(p.beta, p.wdtype, e_first + i * TPR * V, cols, 0.f, b[h]);
+    if constexpr (!HOLD) {
+      keep_weights<T, kThreads<TPR>>(kept(0, i), g[h]);
+      keep_weights<T, kThreads<TPR>>(kept(1, i), b[h]);
+    }
   }
   int slot = 0;
   for (int64_t row = first; row < p.rows; row += stride) {
@@ -401,9 +430,13 @@ fwd_rows(const FwdArgs p) {
     for (int i = 0; i < VPT; ++i) {
       const int e0 = e_first + i * TPR * V;
       if (e0 >= cols) continue;
-      if constexpr (!kHold<T, VPT>) weights(i);
+      const int h = HOLD ? i : 0;
+      if constexpr (!HOLD) {
+        kept_weights<T, kThreads<TPR>>(kept(0, i), g[h]);
+        kept_weights<T, kThreads<TPR>>(kept(1, i), b[h]);
+      }
 #pragma unroll
-      for (int j = 0; j < V / 2; ++j) v[i][j] = fma2(mul2(v[i][j], by), g[i][j], b[i][j]);
+      for (int j = 0; j < V / 2; ++j) v[i][j] = fma2(mul2(v[i][j], by), g[h][j], b[h][j]);
       store_piece<T, EDGE>(yr, e0, cols, v[i]);
     }
   }
@@ -487,9 +520,10 @@ bwd_rows(const BwdArgs p) {
   using elem::pair;
   constexpr int V = elem::kVec<T>;
   constexpr int RB = kRows<TPR>;
-  constexpr int D = kDepth<TPR, 2 * VPT, kBwdThreads>;
+  constexpr int D = kDepth<T, TPR, VPT, 2, kBwdThreads>;
   static_assert(D >= 1, "a row fits shared memory");
-  extern __shared__ uint4 ring[];  // [D][dy, x][VPT][threads]; at the end, RB > 1: 2 x cols sums of the CTA
+  // [D][dy, x][VPT][threads], then gamma unless it is held; at the end, RB > 1: the rows' sums
+  extern __shared__ uint4 ring[];
   __shared__ float2 red[2][32];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const int cols = (int)p.cols;
@@ -531,10 +565,15 @@ bwd_rows(const BwdArgs p) {
 #pragma unroll 1
   for (int d = 0; d < D; ++d) fetch(d, first + d * stride);
   if (first < p.rows) ahead(first);
-  uint64_t g[VPT][V / 2], dg[VPT][V / 2], db[VPT][V / 2];
+  constexpr bool HOLD = kHold<T, VPT>;
+  uint64_t g[HOLD ? VPT : 1][V / 2], dg[VPT][V / 2], db[VPT][V / 2];
+  auto kept = [&](int i) {
+    return ring + D * 2 * VPT * kThreads<TPR> + i * (V / 4) * kThreads<TPR> + threadIdx.x;
+  };
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
-    if constexpr (kHold<T, VPT>) load_weights<T>(p.gamma, p.wdtype, e_first + i * TPR * V, cols, 1.f, g[i]);
+    load_weights<T>(p.gamma, p.wdtype, e_first + i * TPR * V, cols, 1.f, g[HOLD ? i : 0]);
+    if constexpr (!HOLD) keep_weights<T, kThreads<TPR>>(kept(i), g[0]);
 #pragma unroll
     for (int j = 0; j < V / 2; ++j) dg[i][j] = db[i][j] = 0;
   }
@@ -565,12 +604,13 @@ bwd_rows(const BwdArgs p) {
       if (e0 >= cols) continue;
       uint64_t d[V / 2], xh[V / 2];
       read(i, e0, d, xh);
-      if constexpr (!kHold<T, VPT>) load_weights<T>(p.gamma, p.wdtype, e0, cols, 1.f, g[i]);
+      const int h = HOLD ? i : 0;
+      if constexpr (!HOLD) kept_weights<T, kThreads<TPR>>(kept(i), g[h]);
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) {
         dg[i][j] = fma2(d[j], xh[j], dg[i][j]);
         db[i][j] = add2(db[i][j], d[j]);
-        const uint64_t w = mul2(d[j], g[i][j]);
+        const uint64_t w = mul2(d[j], g[h][j]);
         s1 = fma2(w, xh[j], s1);
         s2 = add2(s2, w);
       }
@@ -585,9 +625,10 @@ bwd_rows(const BwdArgs p) {
       if (e0 >= cols) continue;
       uint64_t d[V / 2], xh[V / 2];
       read(i, e0, d, xh);
-      if constexpr (!kHold<T, VPT>) load_weights<T>(p.gamma, p.wdtype, e0, cols, 1.f, g[i]);
+      const int h = HOLD ? i : 0;
+      if constexpr (!HOLD) kept_weights<T, kThreads<TPR>>(kept(i), g[h]);
 #pragma unroll
-      for (int j = 0; j < V / 2; ++j) d[j] = mul2(by, fma2(xh[j], m1, fma2(d[j], g[i][j], m2)));
+      for (int j = 0; j < V / 2; ++j) d[j] = mul2(by, fma2(xh[j], m1, fma2(d[j], g[h][j], m2)));
       store_piece<T, EDGE>(dxr, e0, cols, d);
     }
     fetch(slot, row + D * stride);
@@ -908,7 +949,8 @@ inline int fwd_typed(const FwdArgs& a, cudaStream_t st) {
         constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
         constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
         auto kern = edge ? fwd_rows<T, TPR, VPT, CKPT, !CKPT> : fwd_rows<T, TPR, VPT, CKPT, false>;
-        constexpr size_t smem = (size_t)kDepth<TPR, VPT, kFwdThreads> * VPT * BLOCK * 16;
+        constexpr size_t smem = (size_t)kDepth<T, TPR, VPT, 1, kFwdThreads> * VPT * BLOCK * 16 +
+                                2 * kWeightBytes<T, TPR, VPT>;
         int grid = 0;
         rc = row_grid(kern, BLOCK, RB, smem, a.rows, &grid);
         if (rc != KT_OK) return;
@@ -961,7 +1003,8 @@ inline int bwd_typed(const BwdArgs& a, void* dgamma, void* dbeta, cudaStream_t s
           constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
           constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
           auto kern = edge ? bwd_rows<T, TPR, VPT, CKPT, !CKPT> : bwd_rows<T, TPR, VPT, CKPT, false>;
-          constexpr size_t smem = (size_t)kDepth<TPR, 2 * VPT, kBwdThreads> * 2 * VPT * BLOCK * 16;
+          constexpr size_t smem = (size_t)kDepth<T, TPR, VPT, 2, kBwdThreads> * 2 * VPT * BLOCK * 16 +
+                                  kWeightBytes<T, TPR, VPT>;
           static_assert(RB == 1 || smem >= RB * 2 * sizeof(float) * TPR * VPT * V, "the CTA's sums fit the ring");
           rc = row_grid(kern, BLOCK, RB, smem, a.rows, &parts);
           if (rc != KT_OK) return;
