@@ -217,8 +217,12 @@ __device__ __forceinline__ void sync() {
 }
 template <int G>
 __device__ __forceinline__ bool any(bool v) {
-  if constexpr (G == 32) return __any_sync(0xffffffffu, v);
-  else return __syncthreads_or(v);
+  if constexpr (G == 32) {
+    __syncwarp();  // a vote orders no memory
+    return __any_sync(0xffffffffu, v);
+  } else {
+    return __syncthreads_or(v);
+  }
 }
 
 // Sorted top k of the first n listed keys, by the threads t of G.
@@ -622,7 +626,8 @@ inline int check_common(const char* what, int64_t rows, int64_t vocab, int64_t l
     return fail(KT_ERR_ARG, "%s: negative shape rows=%lld vocab=%lld ld=%lld", what, (long long)rows,
                 (long long)vocab, (long long)ld);
   if (elem::size_of(dtype) == 0) return fail(KT_ERR_ARG, "%s: unknown dtype %d", what, dtype);
-  if (!(scale > 0.f) || isinf(scale)) return fail(KT_ERR_ARG, "%s: scale must be positive and finite", what);
+  if (!(scale > 0.f) || isinf(scale * kLog2e))  // (the kernels use scale log2 e)
+    return fail(KT_ERR_ARG, "%s: scale must be positive and at most 2^127", what);
   if (rows > 0 && vocab == 0) return fail(KT_ERR_ARG, "%s: rows without columns", what);
   if (vocab > (int64_t)1 << 30) return fail(KT_ERR_UNSUPPORTED, "%s: vocab > 2^30", what);
   return KT_OK;
