@@ -642,6 +642,10 @@ inline int linear(const Args& a, int group, int dtype, cudaStream_t st) {
   if (!elem::aligned_to(a.x, sz) || !elem::aligned_to(a.y, sz) || !elem::aligned_to(a.bias, sz) ||
       !elem::aligned_to(a.scales, sz))
     return fail(KT_ERR_ARG, "w4_linear: a pointer is not aligned to its elements");
+  // CTAs read x while others store their rows of y
+  const uintptr_t x0 = (uintptr_t)a.x, y0 = (uintptr_t)a.y;
+  if (x0 < y0 + (uintptr_t)((a.M - 1) * a.ldy + a.N) * sz && y0 < x0 + (uintptr_t)((a.M - 1) * a.ldx + a.K) * sz)
+    return fail(KT_ERR_ARG, "w4_linear: y overlaps x");
   if (dtype == KT_F32) return launch_typed<float>(a, group, st);
   if (dtype == KT_BF16) return launch_typed<__nv_bfloat16>(a, group, st);
   return launch_typed<__half>(a, group, st);

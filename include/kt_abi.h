@@ -260,7 +260,8 @@ KT_API int kt_w4_quantize(const void* w, int64_t N, int64_t K, int group, int dt
  * zeros (N x K/group, values of 0..15) may be NULL: 8; bias (N, of `dtype`) may
  * be NULL; K up to 131072. Made for few tokens:
  * the weights are read once for every 16. A group's sum of x*(q-z) is fp32 and
- * scaled afterwards, so it must not overflow. `packed` is 16-byte aligned. */
+ * scaled afterwards, so it must not overflow. `packed` is 16-byte aligned; y
+ * and x must not overlap. */
 KT_API int kt_w4_linear(const void* x, int64_t ldx, const uint8_t* packed, const void* scales, const uint8_t* zeros,
                         const void* bias, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int group, int dtype,
                         kt_stream_t stream);

@@ -65,7 +65,8 @@ def logprobs(lib, logits=P, ld=100, targets=P, rows=4, vocab=100, scale=1.0, top
 
 @pytest.mark.parametrize("bad", [dict(logits=0), dict(lse=0), dict(logprob=None), dict(rows=-1), dict(vocab=-1),
                                  dict(vocab=0), dict(ld=-1), dict(scale=0.0), dict(scale=-2.0),
-                                 dict(scale=float("inf")), dict(scale=float("nan")), dict(top_k=-1), dict(top_k=33),
+                                 dict(scale=float("inf")), dict(scale=float("nan")), dict(scale=3e38),
+                                 dict(top_k=-1), dict(top_k=33),
                                  dict(vocab=3, top_k=4), dict(top_k=2, top_logprob=None),
                                  dict(top_k=2, top_index=None), dict(dtype=5), dict(logits=P + 2),
                                  dict(targets=P + 4)])
@@ -85,15 +86,15 @@ def test_token_logprobs_bwd(lib, bad):
     refused(lambda: logprobs_bwd(lib, **bad))
 
 
-def w4(lib, x=P, ldx=256, packed=P, scales=P, zeros=None, bias=None, y=P, ldy=64, M=2, N=64, K=256, group=128,
-       dtype=0):
+def w4(lib, x=P, ldx=256, packed=P, scales=P, zeros=None, bias=None, y=P + (1 << 16), ldy=64, M=2, N=64, K=256,
+       group=128, dtype=0):
     lib.w4_linear(x, ldx, packed, scales, zeros, bias, y, ldy, M, N, K, group, dtype)
 
 
 @pytest.mark.parametrize("bad", [dict(x=0), dict(packed=0), dict(scales=0), dict(y=0), dict(M=-1), dict(N=-1),
                                  dict(K=-128), dict(K=0), dict(K=192), dict(group=48), dict(group=0), dict(dtype=3),
                                  dict(ldx=-1), dict(ldy=63), dict(packed=P + 8), dict(x=P + 2), dict(scales=P + 1),
-                                 dict(K=1 << 18)])
+                                 dict(K=1 << 18), dict(y=P), dict(y=P + 2 * 256 * 4 - 4), dict(y=P - 128 * 4 + 4)])
 def test_w4_linear(lib, bad):
     refused(lambda: w4(lib, **bad), kt_lib.KT_ERR_ARG, kt_lib.KT_ERR_UNSUPPORTED)
 
