@@ -180,7 +180,10 @@ class TunedLinearW4(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         _no_autograd("TunedLinearW4", x)
         w = kt_ops.W4Weight(self.packed, self.scales, self.zeros, self.group)
-        y = kt_ops.w4_linear(x.reshape(-1, self.in_features), w, self.bias)
+        x2 = x.reshape(-1, self.in_features)
+        if x2.stride(1) != 1:
+            x2 = x2.contiguous()
+        y = kt_ops.w4_linear(x2, w, self.bias)
         return y.view(*x.shape[:-1], self.out_features)
 
 

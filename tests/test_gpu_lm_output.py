@@ -152,6 +152,8 @@ def test_linear_w4_layer(dev, lib):
         step = layer.scales.double().repeat_interleave(128, 1)
         assert bool(((w - lin.weight.double()).abs() <= step * (0.5 + 8 * 2.0 ** -8)).all())
         assert normwise(y, x.double() @ w.T + lin.bias.double()) <= 2.0 ** -8
+        turned = x[0].t().contiguous().t()  # (3, 384), columns first
+        assert torch.equal(layer(turned), y[0]) and torch.equal(layer(turned[:1]), y[0, :1])
     with pytest.raises(RuntimeError):
         layer(x.requires_grad_())
     model = torch.nn.Sequential(torch.nn.Linear(384, 96), torch.nn.Linear(96, 40), torch.nn.Linear(40, 8)).to(dev)
