@@ -225,24 +225,25 @@ size_t kt_layernorm_bwd_workspace_bytes(int64_t rows, int64_t cols) {
 }
 
 int kt_layernorm_train_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean, float* rstd,
-                           int8_t* q8, uint8_t* q8_exp, int64_t rows, int64_t cols, float eps, int dtype,
-                           int wdtype, kt_stream_t stream) {
+                           int8_t* q8, uint8_t* q8_exp, int64_t ld_q8, int64_t rows, int64_t cols, float eps,
+                           int dtype, int wdtype, kt_stream_t stream) {
   kt::clear_error();
 #if KT_WITH_LM
-  return kt::ln_train::forward({x, gamma, beta, y, mean, rstd, q8, q8_exp, rows, cols, eps, wdtype}, dtype, stream);
+  return kt::ln_train::forward({x, gamma, beta, y, mean, rstd, q8, q8_exp, ld_q8, rows, cols, eps, wdtype}, dtype,
+                               stream);
 #else
   return kt::unsupported("layernorm training");
 #endif
 }
 
-int kt_layernorm_train_bwd(const void* dy, const void* x, const int8_t* q8, const uint8_t* q8_exp, const void* gamma,
-                           const float* mean, const float* rstd, void* dx, void* dgamma, void* dbeta, int64_t rows,
-                           int64_t cols, int dtype, int wdtype, void* workspace, size_t ws_bytes,
-                           kt_stream_t stream) {
+int kt_layernorm_train_bwd(const void* dy, const void* x, const int8_t* q8, const uint8_t* q8_exp, int64_t ld_q8,
+                           const void* gamma, const float* mean, const float* rstd, void* dx, void* dgamma,
+                           void* dbeta, int64_t rows, int64_t cols, int dtype, int wdtype, void* workspace,
+                           size_t ws_bytes, kt_stream_t stream) {
   kt::clear_error();
 #if KT_WITH_LM
-  return kt::ln_train::backward({dy, x, q8, q8_exp, gamma, mean, rstd, dx, nullptr, rows, cols, wdtype}, dtype, dgamma,
-                                dbeta, workspace, ws_bytes, stream);
+  return kt::ln_train::backward({dy, x, q8, q8_exp, ld_q8, gamma, mean, rstd, dx, nullptr, rows, cols, wdtype}, dtype,
+                                dgamma, dbeta, workspace, ws_bytes, stream);
 #else
   return kt::unsupported("layernorm training");
 #endif

@@ -32,6 +32,7 @@
 // 58 us (5.8 TB/s) and 76 us (4.4 TB/s, issue slots 62 % busy); fp32 98 and 141 us
 // (5.5 and 5.7 TB/s). 8x512 fp32: 2.4 and 3.9 us. 4096x16384 bf16: 55 and 79 us
 // (79 and 136 us with gamma and beta read again from L2 in every row).
+// Odd widths: 16384x2049 bf16 62 and 122 us, with checkpoints 105 and 135 us.
 #pragma once
 #include <type_traits>
 
@@ -49,6 +50,7 @@ struct FwdArgs {
   float* rstd;
   int8_t* q8;        // with 8-bit checkpoints
   uint8_t* q8_exp;   // rows x ceil(cols / 32)
+  int64_t ld_q8;
   int64_t rows;
   int64_t cols;
   float eps;
@@ -60,6 +62,7 @@ struct BwdArgs {
   const void* x;  // null with 8-bit checkpoints
   const int8_t* q8;
   const uint8_t* q8_exp;
+  int64_t ld_q8;
   const void* gamma;
   const float* mean;
   const float* rstd;
@@ -174,6 +177,36 @@ __device__ __forceinline__ void store_piece(T* row, int e0, int cols, const uint
   for (int j = 0; j < V; ++j) {
     const float2 h = elem::halves(f[j / 2]);
     if (e + j >= 0 && e + j < cols) row[e + j] = elem::from_f<T>(j % 2 ? h.y : h.x);
+  }
+}
+
+// The 16 bytes at byte `at` (0 to 15, a whole number of elements) of a and b.
+template <typename T>
+__device__ __forceinline__ uint4 bytes_at(const uint4& a, const uint4& b, int at) {
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  const bool two = at & 8, one = at & 4;
+#pragma unroll
+  for (int k = 0; k < 6; ++k) w[k] = two ? w[k + 2] : w[k];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) w[k] = one ? w[k + 1] : w[k];
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t half = at & 2 ? 0x5432u : 0x3210u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = __byte_perm(w[k], w[k + 1], half);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// V bytes at byte `at` (1 to V) of the 2 V in raw.
+template <int V>
+__device__ __forceinline__ uint2 bytes8_at(const uint4& raw, int at) {
+  const uint32_t by = 0x3210u + 0x1111u * (at & 3);
+  if constexpr (V == 8) {
+    const bool one = at >= 4, two = at >= 8;
+    const uint32_t a = two ? raw.z : one ? raw.y : raw.x, b = two ? raw.w : one ? raw.z : raw.y;
+    return make_uint2(__byte_perm(a, b, by), __byte_perm(b, one ? raw.w : raw.z, by));
+  } else {
+    return make_uint2(__byte_perm(at >= 4 ? raw.y : raw.x, raw.y, by), 0);
   }
 }
 
@@ -306,6 +339,10 @@ __device__ __forceinline__ void kept_weights(const uint4* at, uint64_t (&w)[elem
 }
 
 // ---------------------------------------------------------------- forward
+// With EDGE a thread's pieces do not begin where blocks of the checkpoint do. Its
+// eight (four) columns of a block are then part of its own piece and of the next
+// thread's, which it reads too; q8 has whole words in a row and so needs no such
+// care.
 template <typename T, int TPR, int VPT, bool CKPT, bool EDGE>
 __global__ void __launch_bounds__(kThreads<TPR>, kCtas<TPR, kFwdThreads>)
 fwd_rows(const FwdArgs p) {
@@ -357,6 +394,29 @@ fwd_rows(const FwdArgs p) {
   int slot = 0;
   for (int64_t row = first; row < p.rows; row += stride) {
     wait_copies<D - 1>();
+    if constexpr (CKPT && EDGE) row_sync<TPR>();  // the other threads' copies
+    // writes columns [k0, k0 + V) of the checkpoint; the lanes of a block together
+    auto keep8 = [&](const uint64_t (&f)[V / 2], int k0) {
+      constexpr int LPB = 32 / V;  // lanes that share a block of 32 columns
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) top = max(top, max(abs_bits(halves(f[j]).x), abs_bits(halves(f[j]).y)));
+#pragma unroll
+      for (int o = 1; o < LPB; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (k0 < cols) {
+        const uint32_t code = block_code(top);
+        const float up = code_up(code);
+        uint32_t w[V / 4];
+#pragma unroll
+        for (int k = 0; k < V / 4; ++k)
+          w[k] = quant8x4(halves(f[2 * k]).x, halves(f[2 * k]).y, halves(f[2 * k + 1]).x, halves(f[2 * k + 1]).y, up,
+                          code);
+        int8_t* qr = p.q8 + row * p.ld_q8 + k0;
+        if constexpr (V == 8) *reinterpret_cast<uint2*>(qr) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(qr) = w[0];
+        if (t % LPB == 0) p.q8_exp[row * ((cols + 31) / 32) + k0 / 32] = (uint8_t)code;
+      }
+    };
     uint64_t v[VPT][V / 2];
     uint64_t s2 = 0;
 #pragma unroll
@@ -368,34 +428,32 @@ fwd_rows(const FwdArgs p) {
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) s2 = add2(s2, v[i][j]);
     }
-    fetch(slot, row + D * stride);
-    slot = slot + 1 == D ? 0 : slot + 1;
-    const float mean = row_sum<TPR>(halves(s2).x + halves(s2).y, red[0]) * per_col;
-    const uint64_t minus = pair(-mean, -mean);
-    if constexpr (CKPT) {
+    if constexpr (CKPT && EDGE) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
-        constexpr int LPB = 32 / V;  // lanes that share a block of 32 columns
-        const int e0 = e_first + i * TPR * V;
-        uint32_t top = 0;
-#pragma unroll
-        for (int j = 0; j < V / 2; ++j) top = max(top, max(abs_bits(halves(v[i][j]).x), abs_bits(halves(v[i][j]).y)));
-#pragma unroll
-        for (int o = 1; o < LPB; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (e0 < cols) {
-          const uint32_t code = block_code(top);
-          const float up = code_up(code);
-          uint32_t w[V / 4];
-#pragma unroll
-          for (int k = 0; k < V / 4; ++k)
-            w[k] = quant8x4(halves(v[i][2 * k]).x, halves(v[i][2 * k]).y, halves(v[i][2 * k + 1]).x,
-                            halves(v[i][2 * k + 1]).y, up, code);
-          int8_t* qr = p.q8 + row * cols + e0;
-          if constexpr (V == 8) *reinterpret_cast<uint2*>(qr) = make_uint2(w[0], w[1]);
-          else *reinterpret_cast<uint32_t*>(qr) = w[0];
-          if (t % LPB == 0) p.q8_exp[row * ((cols + 31) / 32) + e0 / 32] = (uint8_t)code;
-        }
+        const int e0 = e_first + i * TPR * V, k0 = e0 + shift;
+        uint4 own = make_uint4(0, 0, 0, 0), next = own;
+        if (e0 < cols) own = *place(slot, i);
+        if (e0 + V < cols) next = t + 1 < TPR ? place(slot, i)[1] : *(place(slot, i + 1) - (TPR - 1));
+        uint4 raw = bytes_at<T>(own, next, shift * (int)sizeof(T));
+        if (k0 + V > cols) raw = masked<T>(raw, k0, cols);
+        uint64_t f[V / 2];
+        elem::unpack_pairs<T>(raw, f);
+        keep8(f, k0);
       }
+    } else {
+      fetch(slot, row + D * stride);
+    }
+    const float mean = row_sum<TPR>(halves(s2).x + halves(s2).y, red[0]) * per_col;
+    if constexpr (CKPT && EDGE) {  // every thread has read its neighbour's piece
+      if (TPR == 32) __syncwarp();
+      fetch(slot, row + D * stride);
+    }
+    slot = slot + 1 == D ? 0 : slot + 1;
+    const uint64_t minus = pair(-mean, -mean);
+    if constexpr (CKPT && !EDGE) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) keep8(v[i], e_first + i * TPR * V);
     }
     uint64_t q2 = 0;
 #pragma unroll
@@ -469,7 +527,7 @@ __global__ void __launch_bounds__(256) fwd_any(const FwdArgs p) {
       const float v = e < p.cols ? elem::to_f(xr[e]) : 0.f;
       if constexpr (CKPT) {
         const uint32_t code = block_code(__reduce_max_sync(0xffffffffu, abs_bits(v)));
-        if (e < p.cols) p.q8[row * p.cols + e] = (int8_t)quant8(v, code_up(code));
+        if (e < p.cols) p.q8[row * p.ld_q8 + e] = (int8_t)quant8(v, code_up(code));
         if ((threadIdx.x & 31) == 0) p.q8_exp[row * ((p.cols + 31) / 32) + e0 / 32] = (uint8_t)code;
       }
       if (e < p.cols) {
@@ -483,22 +541,26 @@ __global__ void __launch_bounds__(256) fwd_any(const FwdArgs p) {
 
 // ---------------------------------------------------------------- backward
 // A piece of xh from x, or from its 8-bit checkpoint (.x, .y: eight values, .z:
-// the block's code).
-template <typename T, bool CKPT>
-__device__ __forceinline__ void x_hats(const uint4& raw, float mean, float rstd, uint64_t (&xh)[elem::kVec<T> / 2]) {
+// the code of the block, and 256 times that of the block before, to which the
+// first `shift` columns of a piece may belong).
+template <typename T, bool CKPT, bool EDGE>
+__device__ __forceinline__ void x_hats(const uint4& raw, int shift, float mean, float rstd,
+                                       uint64_t (&xh)[elem::kVec<T> / 2]) {
   using elem::pair;
   constexpr int V = elem::kVec<T>;
   // x rstd - mean rstd: off by 2^-24 (|xh| + |mean| rstd), as the mean itself is
   const uint64_t minus = pair(-mean * rstd, -mean * rstd);
   if constexpr (CKPT) {
-    const float down = code_down(raw.z) * rstd;
-    const uint64_t scale = pair(down, down), bias = pair(-8388736.f, -8388736.f);  // 2^23 + 128
+    const float down = code_down(raw.z & 255u) * rstd, first = code_down(raw.z >> 8) * rstd;
+    const uint64_t bias = pair(-8388736.f, -8388736.f);  // 2^23 + 128
 #pragma unroll
     for (int j = 0; j < V / 2; ++j) {
       // q + 128 in the low bits of 2^23
       const uint32_t word = (j < 2 ? raw.x : raw.y) ^ 0x80808080u;
       const uint64_t q = (uint64_t)__byte_perm(word, 0x4B000000u, 0x7440 + (2 * (j & 1) + 1)) << 32 |
                          __byte_perm(word, 0x4B000000u, 0x7440 + 2 * (j & 1));
+      const uint64_t scale = EDGE ? pair(2 * j < shift ? first : down, 2 * j + 1 < shift ? first : down)
+                                  : pair(down, down);
       xh[j] = elem::fma2(elem::add2(q, bias), scale, minus);
     }
   } else {
@@ -542,8 +604,13 @@ bwd_rows(const BwdArgs p) {
         const int e0 = e_first + i * TPR * V;
         if (e0 >= cols) continue;
         copy_piece<T, EDGE>(place(slot, 0, i), static_cast<const T*>(p.dy), row, p.rows, e0, cols);
-        if constexpr (CKPT) copy_async_small<V>(place(slot, 1, i), p.q8 + row * cols + e0);
-        else copy_piece<T, EDGE>(place(slot, 1, i), static_cast<const T*>(p.x), row, p.rows, e0, cols);
+        if constexpr (CKPT) {  // with EDGE the word before as well
+          const int8_t* from = p.q8 + row * p.ld_q8 + (e0 + shift);
+          uint8_t* to = reinterpret_cast<uint8_t*>(place(slot, 1, i));
+          if (!EDGE || e0 + shift < cols) copy_async_small<V>(to + (EDGE ? V : 0), from);
+          if (EDGE && e0 + shift > 0) copy_async_small<V>(to, from - V);
+        }
+        if constexpr (!CKPT) copy_piece<T, EDGE>(place(slot, 1, i), static_cast<const T*>(p.x), row, p.rows, e0, cols);
       }
     }
     commit_copies();
@@ -558,7 +625,10 @@ bwd_rows(const BwdArgs p) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int e0 = e_first + i * TPR * V;
-        ncode[i] = e0 < cols ? p.q8_exp[row * ((cols + 31) / 32) + e0 / 32] : 7u;
+        const int k0 = e0 + shift;
+        const uint8_t* codes = p.q8_exp + row * ((cols + 31) / 32);
+        ncode[i] = k0 < cols ? codes[k0 / 32] : 7u;
+        if constexpr (EDGE) ncode[i] |= (k0 > 0 && e0 < cols ? codes[(k0 - 1) / 32] : 7u) << 8;
       }
     }
   };
@@ -589,12 +659,17 @@ bwd_rows(const BwdArgs p) {
       elem::unpack_pairs<T>(read_piece<T, EDGE>(place(slot, 0, i), e0, cols), d);
       uint4 x;
       if constexpr (CKPT) {
-        const uint32_t* at = reinterpret_cast<const uint32_t*>(place(slot, 1, i));
-        x = make_uint4(at[0], V == 8 ? at[1] : 0, code[i], 0);
+        if constexpr (EDGE) {
+          const uint2 q = bytes8_at<V>(*place(slot, 1, i), V - shift);
+          x = make_uint4(q.x, q.y, code[i], 0);
+        } else {
+          const uint32_t* at = reinterpret_cast<const uint32_t*>(place(slot, 1, i));
+          x = make_uint4(at[0], V == 8 ? at[1] : 0, code[i], 0);
+        }
       } else {
         x = read_piece<T, EDGE>(place(slot, 1, i), e0, cols);
       }
-      x_hats<T, CKPT>(x, mean, rstd, xh);
+      x_hats<T, CKPT, EDGE>(x, shift, mean, rstd, xh);
     };
     wait_copies<D - 1>();
     uint64_t s1 = 0, s2 = 0;
@@ -680,8 +755,8 @@ bwd_rows(const BwdArgs p) {
 }
 
 // ---------------------------------------------------------------- element by element
-// Rows of x and dy that are not equally aligned, and checkpoints of rows that are
-// no whole number of pieces: lanes hold consecutive columns (a warp's 32 are one
+// Rows of x and dy that are not equally aligned, and checkpoints whose rows are
+// no whole words: lanes hold consecutive columns (a warp's 32 are one
 // block of the checkpoint), EPT per thread, as above but for the copies ahead.
 template <typename T, int TPR, bool CKPT>
 __global__ void __launch_bounds__(TPR) fwd_scalar(const FwdArgs p) {
@@ -722,7 +797,7 @@ __global__ void __launch_bounds__(TPR) fwd_scalar(const FwdArgs p) {
       const int e = t + i * TPR;
       if constexpr (CKPT) {
         const uint32_t code = block_code(__reduce_max_sync(0xffffffffu, abs_bits(v[i])));
-        if (e < cols) p.q8[row * cols + e] = (int8_t)quant8(v[i], code_up(code));
+        if (e < cols) p.q8[row * p.ld_q8 + e] = (int8_t)quant8(v[i], code_up(code));
         if (e < cols && (t & 31) == 0) p.q8_exp[row * ((cols + 31) / 32) + e / 32] = (uint8_t)code;
       }
       if (e < cols) {
@@ -757,7 +832,7 @@ __global__ void __launch_bounds__(TPR) bwd_scalar(const BwdArgs p) {
       const int e = t + i * TPR;
       d[i] = e < cols ? elem::to_f(dyr[e]) : 0.f;
       if constexpr (CKPT) {
-        xh[i] = e < cols ? (float)p.q8[row * cols + e] * code_down(p.q8_exp[row * ((cols + 31) / 32) + e / 32]) : 0.f;
+        xh[i] = e < cols ? (float)p.q8[row * p.ld_q8 + e] * code_down(p.q8_exp[row * ((cols + 31) / 32) + e / 32]) : 0.f;
       } else {
         xh[i] = e < cols ? elem::to_f(static_cast<const T*>(p.x)[row * cols + e]) : 0.f;
       }
@@ -793,7 +868,7 @@ template <typename T, bool CKPT>
 __device__ __forceinline__ float x_hat(const BwdArgs& p, int64_t row, int64_t e, float mean, float rstd) {
   float v;
   if constexpr (CKPT)
-    v = (float)p.q8[row * p.cols + e] * code_down(p.q8_exp[row * ((p.cols + 31) / 32) + e / 32]);
+    v = (float)p.q8[row * p.ld_q8 + e] * code_down(p.q8_exp[row * ((p.cols + 31) / 32) + e / 32]);
   else
     v = elem::to_f(static_cast<const T*>(p.x)[row * p.cols + e]);
   return (v - mean) * rstd;
@@ -941,14 +1016,14 @@ inline int fwd_typed(const FwdArgs& a, cudaStream_t st) {
   constexpr int V = elem::kVec<T>;
   const int shift = elem::misalign<T>(a.x);
   bool fast = elem::misalign<T>(a.y) == shift;
-  if (CKPT) fast = fast && shift == 0 && a.cols % V == 0 && elem::aligned_to(a.q8, V);
-  const bool edge = shift != 0 || a.cols % V != 0;  // (not with checkpoints)
+  if (CKPT) fast = fast && a.ld_q8 % V == 0 && elem::aligned_to(a.q8, V);
+  const bool edge = shift != 0 || a.cols % V != 0;
   const int64_t pieces = (a.cols + V - 1) / V + (edge ? 1 : 0);
   int rc = KT_OK;
   if (fast && with_shape<T>(pieces, a.rows, [&](auto tpr, auto vpt) {
         constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
         constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
-        auto kern = edge ? fwd_rows<T, TPR, VPT, CKPT, !CKPT> : fwd_rows<T, TPR, VPT, CKPT, false>;
+        auto kern = edge ? fwd_rows<T, TPR, VPT, CKPT, true> : fwd_rows<T, TPR, VPT, CKPT, false>;
         constexpr size_t smem = (size_t)kDepth<T, TPR, VPT, 1, kFwdThreads> * VPT * BLOCK * 16 +
                                 2 * kWeightBytes<T, TPR, VPT>;
         int grid = 0;
@@ -978,6 +1053,7 @@ inline int forward(const FwdArgs& a, int dtype, cudaStream_t st) {
   if (!(a.eps >= 0.f)) return fail(KT_ERR_ARG, "layernorm_train: eps must be >= 0");
   if ((a.q8 == nullptr) != (a.q8_exp == nullptr))
     return fail(KT_ERR_ARG, "layernorm_train: q8 and q8_exp are given together");
+  if (a.q8 && a.ld_q8 < a.cols) return fail(KT_ERR_ARG, "layernorm_train: rows of q8 overlap");
   if (a.rows == 0 || a.cols == 0) return KT_OK;
   if (!a.x || !a.y || !a.mean || !a.rstd) return fail(KT_ERR_ARG, "layernorm_train: null pointer");
   const int sz = elem::size_of(dtype), wsz = elem::size_of(a.wdtype);
@@ -994,15 +1070,15 @@ inline int bwd_typed(const BwdArgs& a, void* dgamma, void* dbeta, cudaStream_t s
   constexpr int V = elem::kVec<T>;
   const int shift = elem::misalign<T>(a.dy);
   bool fast = elem::misalign<T>(a.dx) == shift;
-  if (CKPT) fast = fast && shift == 0 && a.cols % V == 0 && elem::aligned_to(a.q8, V);
+  if (CKPT) fast = fast && a.ld_q8 % V == 0 && elem::aligned_to(a.q8, V);
   else fast = fast && elem::misalign<T>(a.x) == shift;
-  const bool edge = shift != 0 || a.cols % V != 0;  // (not with checkpoints)
+  const bool edge = shift != 0 || a.cols % V != 0;
   const int64_t pieces = (a.cols + V - 1) / V + (edge ? 1 : 0);
   int rc = KT_OK, parts = 0;
   if (!(fast && with_shape<T>(pieces, a.rows, [&](auto tpr, auto vpt) {
           constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
           constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
-          auto kern = edge ? bwd_rows<T, TPR, VPT, CKPT, !CKPT> : bwd_rows<T, TPR, VPT, CKPT, false>;
+          auto kern = edge ? bwd_rows<T, TPR, VPT, CKPT, true> : bwd_rows<T, TPR, VPT, CKPT, false>;
           constexpr size_t smem = (size_t)kDepth<T, TPR, VPT, 2, kBwdThreads> * 2 * VPT * BLOCK * 16 +
                                   kWeightBytes<T, TPR, VPT>;
           static_assert(RB == 1 || smem >= RB * 2 * sizeof(float) * TPR * VPT * V, "the CTA's sums fit the ring");
@@ -1051,6 +1127,7 @@ inline int backward(BwdArgs a, int dtype, void* dgamma, void* dbeta, void* works
   if (rc != KT_OK) return rc;
   if ((a.q8 == nullptr) != (a.q8_exp == nullptr))
     return fail(KT_ERR_ARG, "layernorm_train bwd: q8 and q8_exp are given together");
+  if (a.q8 && a.ld_q8 < a.cols) return fail(KT_ERR_ARG, "layernorm_train bwd: rows of q8 overlap");
   if (a.cols == 0) return KT_OK;
   const int sz = elem::size_of(dtype), wsz = elem::size_of(a.wdtype);
   if (!elem::aligned_to(dgamma, wsz) || !elem::aligned_to(dbeta, wsz))

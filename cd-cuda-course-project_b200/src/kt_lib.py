@@ -122,9 +122,9 @@ _SIGNATURES = {
                                        ctypes.c_uint64, _vp]),
     "kt_gemm_f32": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _vp]),
     "kt_fa_fwd_bf16": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _f32, _int, _vp]),
-    "kt_layernorm_train_fwd": (_int, [_vp] * 8 + [_i64, _i64, _f32, _int, _int, _vp]),
+    "kt_layernorm_train_fwd": (_int, [_vp] * 8 + [_i64] * 3 + [_f32, _int, _int, _vp]),
     "kt_layernorm_bwd_workspace_bytes": (_size, [_i64, _i64]),
-    "kt_layernorm_train_bwd": (_int, [_vp] * 10 + [_i64, _i64, _int, _int, _vp, _size, _vp]),
+    "kt_layernorm_train_bwd": (_int, [_vp] * 4 + [_i64] + [_vp] * 6 + [_i64, _i64, _int, _int, _vp, _size, _vp]),
     "kt_token_logprobs": (_int, [_vp, _i64, _vp, _i64, _i64, _f32, _i64, _int, _vp, _vp, _vp, _vp, _vp, _int, _vp]),
     "kt_token_logprobs_bwd": (_int, [_vp, _i64] + [_vp] * 5 + [_i64, _i64, _f32, _i64, _vp, _i64, _int, _vp]),
     "kt_w4_quantize": (_int, [_vp, _i64, _i64, _int, _int, _vp, _vp, _int, _vp]),
@@ -216,20 +216,20 @@ class KtLibrary:
                     "kt_fa_fwd_bf16")
 
     def layernorm_train_fwd(self, x: int, gamma: Optional[int], beta: Optional[int], y: int, mean: int, rstd: int,
-                            q8: Optional[int], q8_exp: Optional[int], rows: int, cols: int, eps: float, dtype: int,
-                            wdtype: int, stream: Optional[int] = None) -> None:
-        self._check(self._lib.kt_layernorm_train_fwd(x, gamma, beta, y, mean, rstd, q8, q8_exp, rows, cols, eps,
-                                                     dtype, wdtype, stream), "kt_layernorm_train_fwd")
+                            q8: Optional[int], q8_exp: Optional[int], ld_q8: int, rows: int, cols: int, eps: float,
+                            dtype: int, wdtype: int, stream: Optional[int] = None) -> None:
+        self._check(self._lib.kt_layernorm_train_fwd(x, gamma, beta, y, mean, rstd, q8, q8_exp, ld_q8, rows, cols,
+                                                     eps, dtype, wdtype, stream), "kt_layernorm_train_fwd")
 
     def layernorm_bwd_workspace_bytes(self, rows: int, cols: int) -> int:
         return int(self._lib.kt_layernorm_bwd_workspace_bytes(rows, cols))
 
     def layernorm_train_bwd(self, dy: int, x: Optional[int], q8: Optional[int], q8_exp: Optional[int],
-                            gamma: Optional[int], mean: int, rstd: int, dx: int, dgamma: Optional[int],
+                            ld_q8: int, gamma: Optional[int], mean: int, rstd: int, dx: int, dgamma: Optional[int],
                             dbeta: Optional[int], rows: int, cols: int, dtype: int, wdtype: int,
                             workspace: Optional[int], ws_bytes: int, stream: Optional[int] = None) -> None:
-        self._check(self._lib.kt_layernorm_train_bwd(dy, x, q8, q8_exp, gamma, mean, rstd, dx, dgamma, dbeta, rows,
-                                                     cols, dtype, wdtype, workspace, ws_bytes, stream),
+        self._check(self._lib.kt_layernorm_train_bwd(dy, x, q8, q8_exp, ld_q8, gamma, mean, rstd, dx, dgamma, dbeta,
+                                                     rows, cols, dtype, wdtype, workspace, ws_bytes, stream),
                     "kt_layernorm_train_bwd")
 
     def token_logprobs(self, logits: int, ld: int, targets: Optional[int], rows: int, vocab: int, scale: float,

@@ -217,11 +217,15 @@ def layernorm_train(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta:
     stats = x.new_empty((2, rows), dtype=torch.float32)
     at = stats.data_ptr()
     q8 = q8_exp = None
+    ld_q8 = 0
     if ckpt8:
-        q8 = x.new_empty((rows, cols), dtype=torch.int8)
+        ld_q8 = (cols + 7) // 8 * 8  # rows of whole 8-byte words
+        q8 = x.new_empty((rows, ld_q8), dtype=torch.int8)
+        if ld_q8 != cols:
+            q8 = q8[:, :cols]
         q8_exp = x.new_empty((rows, (cols + 31) // 32), dtype=torch.uint8)
     _launch(dev, lib.layernorm_train_fwd, x.data_ptr(), _ptr(gamma), _ptr(beta), y.data_ptr(), at, at + 4 * rows,
-            _ptr(q8), _ptr(q8_exp), rows, cols, eps, dt, wdt)
+            _ptr(q8), _ptr(q8_exp), ld_q8, rows, cols, eps, dt, wdt)
     return y, LayerNormSaved(None if ckpt8 else x, q8, q8_exp, gamma, stats, beta_dtype)
 
 
@@ -238,6 +242,11 @@ def layernorm_bwd(dy: torch.Tensor, saved: LayerNormSaved, weight_grads: bool = 
     if dy.shape != kept.shape:
         raise ValueError(f"layernorm_bwd: dy is {tuple(dy.shape)}, the input was {tuple(kept.shape)}")
     rows, cols = dy.shape
+    ld_q8 = 0
+    if q8 is not None:
+        ld_q8 = q8.stride(0) if rows > 1 else max(q8.stride(0), cols)
+        if cols > 1 and q8.stride(1) != 1:
+            raise ValueError("q8: the elements of a row must be contiguous")
     wt = gamma.dtype if gamma is not None else beta_dtype or torch.float32
     wdt = _DTYPES[wt]
     if wdt not in (kt_lib.KT_F32, dt):
@@ -253,7 +262,7 @@ def layernorm_bwd(dy: torch.Tensor, saved: LayerNormSaved, weight_grads: bool = 
         ws_bytes = lib.layernorm_bwd_workspace_bytes(rows, cols)
         ws = dy.new_empty(ws_bytes, dtype=torch.uint8)
     at = stats.data_ptr()
-    _launch(dev, lib.layernorm_train_bwd, dy.data_ptr(), _ptr(x), _ptr(q8), _ptr(q8_exp), _ptr(gamma), at,
+    _launch(dev, lib.layernorm_train_bwd, dy.data_ptr(), _ptr(x), _ptr(q8), _ptr(q8_exp), ld_q8, _ptr(gamma), at,
             at + 4 * rows, dx.data_ptr(), _ptr(dgamma), _ptr(dbeta), rows, cols, dt, wdt, _ptr(ws), ws_bytes)
     return dx, dgamma, dbeta
 

@@ -204,14 +204,16 @@ KT_API int kt_fa_fwd_bf16(const uint16_t* Q, const uint16_t* K, const uint16_t* 
  * saved for the backward pass. gamma and beta (may be NULL: 1 and 0) are of
  * `wdtype`, fp32 or the input's type.
  * With q8 and q8_exp (both or neither), an 8-bit checkpoint of x is written
- * too: q8 is rows x cols, q8_exp rows x ceil(cols/32). Each block of 32 columns
+ * too: q8 is rows x cols, ld_q8 bytes apart, q8_exp rows x ceil(cols/32). (Rows
+ * whose ld_q8 is a multiple of 8 may be written up to their next whole 8 bytes,
+ * and take a fraction of the time of others.) Each block of 32 columns
  * has E = the exponent field of its largest magnitude as fp32, at least 7 (255:
  * the block holds an infinity or NaN and stands for NaN), and
  * q = x * 2^(133-E) rounded to nearest even, limited to +-127, standing for
  * q * 2^(E-133). */
 KT_API int kt_layernorm_train_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean,
-                                  float* rstd, int8_t* q8, uint8_t* q8_exp, int64_t rows, int64_t cols, float eps,
-                                  int dtype, int wdtype, kt_stream_t stream);
+                                  float* rstd, int8_t* q8, uint8_t* q8_exp, int64_t ld_q8, int64_t rows,
+                                  int64_t cols, float eps, int dtype, int wdtype, kt_stream_t stream);
 
 /* Bytes of device scratch kt_layernorm_train_bwd needs for dgamma and dbeta. */
 KT_API size_t kt_layernorm_bwd_workspace_bytes(int64_t rows, int64_t cols);
@@ -222,9 +224,9 @@ KT_API size_t kt_layernorm_bwd_workspace_bytes(int64_t rows, int64_t cols);
  * any content) is caller-owned scratch, not needed without dgamma and dbeta;
  * calls that may overlap need one each. */
 KT_API int kt_layernorm_train_bwd(const void* dy, const void* x, const int8_t* q8, const uint8_t* q8_exp,
-                                  const void* gamma, const float* mean, const float* rstd, void* dx, void* dgamma,
-                                  void* dbeta, int64_t rows, int64_t cols, int dtype, int wdtype, void* workspace,
-                                  size_t ws_bytes, kt_stream_t stream);
+                                  int64_t ld_q8, const void* gamma, const float* mean, const float* rstd, void* dx,
+                                  void* dgamma, void* dbeta, int64_t rows, int64_t cols, int dtype, int wdtype,
+                                  void* workspace, size_t ws_bytes, kt_stream_t stream);
 
 /* Per row of logits (`vocab` columns, rows `ld` elements apart), with
  * z = scale*logits, scale > 0: lse = log(sum(exp(z))); logprob = z[target]-lse

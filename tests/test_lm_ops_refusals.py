@@ -24,26 +24,27 @@ def refused(fn, *statuses):
 
 
 def ln_fwd(lib, x=P, gamma=P, beta=P, y=P, mean=P, rstd=P, q8=None, q8_exp=None, rows=4, cols=64, eps=1e-5, dtype=0,
-           wdtype=0):
-    lib.layernorm_train_fwd(x, gamma, beta, y, mean, rstd, q8, q8_exp, rows, cols, eps, dtype, wdtype)
+           wdtype=0, ld_q8=64):
+    lib.layernorm_train_fwd(x, gamma, beta, y, mean, rstd, q8, q8_exp, ld_q8, rows, cols, eps, dtype, wdtype)
 
 
 def ln_bwd(lib, dy=P, x=P, q8=None, q8_exp=None, gamma=P, mean=P, rstd=P, dx=P, dgamma=P, dbeta=P, rows=4, cols=64,
-           dtype=0, wdtype=0, ws=P, ws_bytes=1 << 20):
-    lib.layernorm_train_bwd(dy, x, q8, q8_exp, gamma, mean, rstd, dx, dgamma, dbeta, rows, cols, dtype, wdtype, ws,
-                            ws_bytes)
+           dtype=0, wdtype=0, ws=P, ws_bytes=1 << 20, ld_q8=64):
+    lib.layernorm_train_bwd(dy, x, q8, q8_exp, ld_q8, gamma, mean, rstd, dx, dgamma, dbeta, rows, cols, dtype, wdtype,
+                            ws, ws_bytes)
 
 
 @pytest.mark.parametrize("bad", [dict(x=0), dict(y=0), dict(mean=0), dict(rstd=0), dict(rows=-1), dict(cols=-1),
                                  dict(eps=-1.0), dict(eps=float("nan")), dict(dtype=3), dict(dtype=-1),
                                  dict(dtype=1, wdtype=2), dict(dtype=0, wdtype=1), dict(q8=P), dict(q8_exp=P),
-                                 dict(x=P + 2), dict(gamma=P + 1), dict(dtype=1, x=P + 1)])
+                                 dict(q8=P, q8_exp=P, ld_q8=63), dict(x=P + 2), dict(gamma=P + 1), dict(dtype=1, x=P + 1)])
 def test_layernorm_train_fwd(lib, bad):
     refused(lambda: ln_fwd(lib, **bad))
 
 
 @pytest.mark.parametrize("bad", [dict(dy=0), dict(dx=0), dict(mean=0), dict(rstd=0), dict(x=None),
                                  dict(q8=P, q8_exp=P), dict(q8=P), dict(rows=-1), dict(dtype=9),
+                                 dict(x=None, q8=P, q8_exp=P, ld_q8=63),
                                  dict(dtype=2, wdtype=1), dict(ws=0), dict(ws_bytes=16), dict(ws=P + 8),
                                  dict(dgamma=P + 2), dict(dy=P + 3)])
 def test_layernorm_train_bwd(lib, bad):
