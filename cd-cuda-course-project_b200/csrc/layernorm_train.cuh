@@ -32,7 +32,7 @@
 // 58 us (5.8 TB/s) and 76 us (4.4 TB/s, issue slots 62 % busy); fp32 98 and 141 us
 // (5.5 and 5.7 TB/s). 8x512 fp32: 2.4 and 3.9 us. 4096x16384 bf16: 55 and 79 us
 // (79 and 136 us with gamma and beta read again from L2 in every row).
-// Odd widths: 16384x2049 bf16 62 and 122 us, with checkpoints 105 and 135 us.
+// Odd widths: 16384x2049 bf16 54 and 81 us, with checkpoints 89 and 110 us.
 #pragma once
 #include <type_traits>
 
@@ -127,6 +127,12 @@ __device__ __forceinline__ void copy_async(void* to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
                : "memory");
 }
+// the first `bytes` of the 16; the others become 0
+__device__ __forceinline__ void copy_async_part(void* to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)),
+               "l"(from), "r"(bytes)
+               : "memory");
+}
 template <int BYTES>  // 4 or 8
 __device__ __forceinline__ void copy_async_small(void* to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from),
@@ -135,37 +141,62 @@ __device__ __forceinline__ void copy_async_small(void* to, const void* from) {
 }
 
 // Rows whose ends lie on 16-byte boundaries have only whole pieces (EDGE false).
-// Otherwise a piece that a row's end cuts also holds its neighbour's columns.
+// Otherwise a piece that a row's end cuts also has its neighbour's columns, which
+// have to count as 0: those behind the row are not copied, those before it are
+// cleared by their thread when the copy has landed (testing every piece as it is
+// read took up to 1.5 times as long).
 
 // Starts the copy of columns [e0, e0+V) of row `row`, on a 16-byte boundary and
-// e0 < cols, to this thread's place `to`. Only at the tensor's two ends may the
-// neighbour's columns not be there, and only the columns of the row are read then.
+// e0 < cols, to this thread's place `to`. Only before the tensor's first row may
+// the neighbour's columns not be there, and only the row's are read then.
 template <typename T, bool EDGE>
-__device__ __forceinline__ void copy_piece(uint4* to, const T* x, int64_t row, int64_t rows, int e0, int cols) {
+__device__ __forceinline__ void copy_piece(uint4* to, const T* x, int64_t row, int e0, int cols) {
   constexpr int V = elem::kVec<T>;
   const T* at = x + row * cols + e0;
-  if (!EDGE || (e0 >= 0 && e0 + V <= cols)) {
+  if constexpr (!EDGE) {
     copy_async(to, at);
-    return;
-  }
-  const int e = elem::opaque(e0);
-  if (at >= x && at + V <= x + rows * cols) {
-    copy_async(to, at);
-    return;
-  }
+  } else if (e0 >= 0 || at >= x) {
+    copy_async_part(to, at, min(V, cols - e0) * (int)sizeof(T));
+  } else {
+    const int e = elem::opaque(e0);
 #pragma unroll 1
-  for (int j = 0; j < V; ++j)
-    if (e + j >= 0 && e + j < cols) reinterpret_cast<T*>(to)[j] = at[j];
+    for (int j = 0; j < V; ++j) reinterpret_cast<T*>(to)[j] = e + j >= 0 && e + j < cols ? at[j] : T(0.f);
+  }
 }
 
-// The piece at columns [e0, e0+V), e0 < cols; columns outside [0, cols) are 0.
-template <typename T, bool EDGE>
-__device__ __forceinline__ uint4 read_piece(const uint4* from, int e0, int cols) {
-  if (!EDGE || (e0 >= 0 && e0 + elem::kVec<T> <= cols)) return *from;
-  return masked<T>(*from, elem::opaque(e0), cols);
+// Stores the elements [lo, hi) of a piece of 16-bit values: the largest aligned
+// parts in turn.
+template <typename T>
+__device__ __forceinline__ void store_part(T* at, const uint4& raw, int lo, int hi) {
+  static_assert(sizeof(T) == 2, "");
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  auto one = [&](int e) {
+    const uint32_t word = e < 2 ? w[0] : e < 4 ? w[1] : e < 6 ? w[2] : w[3];
+    reinterpret_cast<uint16_t*>(at)[e] = (uint16_t)(e & 1 ? word >> 16 : word);
+  };
+  uint32_t* words = reinterpret_cast<uint32_t*>(at);
+  uint2* halves = reinterpret_cast<uint2*>(at);
+  if (lo > 0 && hi < 8) {
+#pragma unroll 1
+    for (int e = lo; e < hi; ++e) one(e);
+  } else if (lo > 0) {
+    if (lo & 1) one(lo++);
+    if (lo & 2) {
+      words[lo / 2] = lo == 2 ? w[1] : w[3];
+      lo += 2;
+    }
+    if (lo == 4) halves[1] = make_uint2(w[2], w[3]);
+  } else {
+    if (hi & 4) halves[0] = make_uint2(w[0], w[1]);
+    if (hi & 2) words[hi / 4 * 2] = hi & 4 ? w[2] : w[0];
+    if (hi & 1) one(hi - 1);
+  }
 }
 
-template <typename T, bool EDGE>
+// PARTS: a cut piece by its parts, else by its elements, which takes fewer
+// registers (16384x2049 bf16 by parts 54 and 77 us, by elements 59 and 89; where a
+// thread of the backward pass has 32 columns, 4000x12345 bf16, 104 and 90 us).
+template <typename T, bool EDGE, bool PARTS>
 __device__ __forceinline__ void store_piece(T* row, int e0, int cols, const uint64_t (&f)[elem::kVec<T> / 2]) {
   constexpr int V = elem::kVec<T>;
   if (!EDGE || (e0 >= 0 && e0 + V <= cols)) {
@@ -173,10 +204,14 @@ __device__ __forceinline__ void store_piece(T* row, int e0, int cols, const uint
     return;
   }
   const int e = elem::opaque(e0);
+  if constexpr (PARTS) {
+    store_part<T>(row + e, elem::pack_pairs<T>(f), max(-e, 0), min(cols - e, V));
+  } else {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const float2 h = elem::halves(f[j / 2]);
-    if (e + j >= 0 && e + j < cols) row[e + j] = elem::from_f<T>(j % 2 ? h.y : h.x);
+    for (int j = 0; j < V; ++j) {
+      const float2 h = elem::halves(f[j / 2]);
+      if (e + j >= 0 && e + j < cols) row[e + j] = elem::from_f<T>(j % 2 ? h.y : h.x);
+    }
   }
 }
 
@@ -225,13 +260,15 @@ template <typename T, int VPT>
 constexpr bool kHold = VPT * elem::kVec<T> <= 16;
 template <int TPR, int PER_SM>
 constexpr int kCtas = PER_SM / kThreads<TPR>;
+template <typename T, int TPR, int VPT>
+constexpr int kFwdPerSm = kHold<T, VPT> || TPR != 256 ? kFwdThreads : 512;
 // Bytes of `tensors` weight vectors in shared memory.
 template <typename T, int TPR, int VPT>
 constexpr int kWeightBytes = kHold<T, VPT> ? 0 : VPT * elem::kVec<T> * 4 * kThreads<TPR>;
 // Rows in shared memory: as many as 200 KB per SM hold (224 KB less the weights), up to 4.
 template <typename T, int TPR, int VPT, int TENSORS, int PER_SM>
 constexpr int kFit = ((kHold<T, VPT> ? 200 : 224) * 1024 / kCtas<TPR, PER_SM> -
-                      (PER_SM == kFwdThreads ? 2 : 1) * kWeightBytes<T, TPR, VPT>) /
+                      (TENSORS == 1 ? 2 : 1) * kWeightBytes<T, TPR, VPT>) /
                      (TENSORS * VPT * 16 * kThreads<TPR>);
 template <typename T, int TPR, int VPT, int TENSORS, int PER_SM>
 constexpr int kDepth = kFit<T, TPR, VPT, TENSORS, PER_SM> >= 4 ? 4 : kFit<T, TPR, VPT, TENSORS, PER_SM>;
@@ -344,7 +381,7 @@ __device__ __forceinline__ void kept_weights(const uint4* at, uint64_t (&w)[elem
 // thread's, which it reads too; q8 has whole words in a row and so needs no such
 // care.
 template <typename T, int TPR, int VPT, bool CKPT, bool EDGE>
-__global__ void __launch_bounds__(kThreads<TPR>, kCtas<TPR, kFwdThreads>)
+__global__ void __launch_bounds__(kThreads<TPR>, kCtas<TPR, kFwdPerSm<T, TPR, VPT>>)
 fwd_rows(const FwdArgs p) {
   using elem::add2;
   using elem::fma2;
@@ -352,7 +389,7 @@ fwd_rows(const FwdArgs p) {
   using elem::mul2;
   using elem::pair;
   constexpr int V = elem::kVec<T>;
-  constexpr int D = kDepth<T, TPR, VPT, 1, kFwdThreads>;
+  constexpr int D = kDepth<T, TPR, VPT, 1, kFwdPerSm<T, TPR, VPT>>;
   static_assert(D >= 1, "a row fits shared memory");
   extern __shared__ uint4 ring[];  // [D][VPT][threads], then gamma and beta unless they are held
   __shared__ float red[2][32];
@@ -369,7 +406,7 @@ fwd_rows(const FwdArgs p) {
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int e0 = e_first + i * TPR * V;
-        if (e0 < cols) copy_piece<T, EDGE>(place(slot, i), static_cast<const T*>(p.x), row, p.rows, e0, cols);
+        if (e0 < cols) copy_piece<T, EDGE>(place(slot, i), static_cast<const T*>(p.x), row, e0, cols);
       }
     }
     commit_copies();
@@ -394,6 +431,7 @@ fwd_rows(const FwdArgs p) {
   int slot = 0;
   for (int64_t row = first; row < p.rows; row += stride) {
     wait_copies<D - 1>();
+    if (EDGE && e_first < 0) *place(slot, 0) = masked<T>(*place(slot, 0), e_first, cols);
     if constexpr (CKPT && EDGE) row_sync<TPR>();  // the other threads' copies
     // writes columns [k0, k0 + V) of the checkpoint; the lanes of a block together
     auto keep8 = [&](const uint64_t (&f)[V / 2], int k0) {
@@ -423,7 +461,7 @@ fwd_rows(const FwdArgs p) {
     for (int i = 0; i < VPT; ++i) {
       const int e0 = e_first + i * TPR * V;
       uint4 raw = make_uint4(0, 0, 0, 0);
-      if (e0 < cols) raw = read_piece<T, EDGE>(place(slot, i), e0, cols);
+      if (e0 < cols) raw = *place(slot, i);
       elem::unpack_pairs<T>(raw, v[i]);
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) s2 = add2(s2, v[i][j]);
@@ -436,7 +474,6 @@ fwd_rows(const FwdArgs p) {
         if (e0 < cols) own = *place(slot, i);
         if (e0 + V < cols) next = t + 1 < TPR ? place(slot, i)[1] : *(place(slot, i + 1) - (TPR - 1));
         uint4 raw = bytes_at<T>(own, next, shift * (int)sizeof(T));
-        if (k0 + V > cols) raw = masked<T>(raw, k0, cols);
         uint64_t f[V / 2];
         elem::unpack_pairs<T>(raw, f);
         keep8(f, k0);
@@ -462,20 +499,17 @@ fwd_rows(const FwdArgs p) {
       if (e0 >= cols) continue;
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) v[i][j] = add2(v[i][j], minus);
-      if (!EDGE || (e0 >= 0 && e0 + V <= cols)) {
-#pragma unroll
-        for (int j = 0; j < V / 2; ++j) q2 = fma2(v[i][j], v[i][j], q2);
-      } else {  // a piece that the row's end cuts
+      if (EDGE && (e0 < 0 || e0 + V > cols)) {  // a piece that the row's end cuts
         const int e = elem::opaque(e0);
-        float q = 0.f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float2 h = halves(v[i][j / 2]);
-          const float d = j % 2 ? h.y : h.x;
-          if (e + j >= 0 && e + j < cols) q = fmaf(d, d, q);
+        for (int j = 0; j < V / 2; ++j) {
+          const float2 h = halves(v[i][j]);
+          v[i][j] = pair(e + 2 * j >= 0 && e + 2 * j < cols ? h.x : 0.f,
+                         e + 2 * j + 1 >= 0 && e + 2 * j + 1 < cols ? h.y : 0.f);
         }
-        q2 = add2(q2, pair(q, 0.f));
       }
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) q2 = fma2(v[i][j], v[i][j], q2);
     }
     const float rstd = rsqrtf(fmaf(row_sum<TPR>(halves(q2).x + halves(q2).y, red[1]), per_col, p.eps));
     if (t == 0) {
@@ -495,7 +529,7 @@ fwd_rows(const FwdArgs p) {
       }
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) v[i][j] = fma2(mul2(v[i][j], by), g[h][j], b[h][j]);
-      store_piece<T, EDGE>(yr, e0, cols, v[i]);
+      store_piece<T, EDGE, sizeof(T) == 2>(yr, e0, cols, v[i]);
     }
   }
 }
@@ -603,14 +637,14 @@ bwd_rows(const BwdArgs p) {
       for (int i = 0; i < VPT; ++i) {
         const int e0 = e_first + i * TPR * V;
         if (e0 >= cols) continue;
-        copy_piece<T, EDGE>(place(slot, 0, i), static_cast<const T*>(p.dy), row, p.rows, e0, cols);
+        copy_piece<T, EDGE>(place(slot, 0, i), static_cast<const T*>(p.dy), row, e0, cols);
         if constexpr (CKPT) {  // with EDGE the word before as well
           const int8_t* from = p.q8 + row * p.ld_q8 + (e0 + shift);
           uint8_t* to = reinterpret_cast<uint8_t*>(place(slot, 1, i));
           if (!EDGE || e0 + shift < cols) copy_async_small<V>(to + (EDGE ? V : 0), from);
           if (EDGE && e0 + shift > 0) copy_async_small<V>(to, from - V);
         }
-        if constexpr (!CKPT) copy_piece<T, EDGE>(place(slot, 1, i), static_cast<const T*>(p.x), row, p.rows, e0, cols);
+        if constexpr (!CKPT) copy_piece<T, EDGE>(place(slot, 1, i), static_cast<const T*>(p.x), row, e0, cols);
       }
     }
     commit_copies();
@@ -655,8 +689,8 @@ bwd_rows(const BwdArgs p) {
     for (int i = 0; i < VPT; ++i) code[i] = CKPT ? ncode[i] : 0;
     if (row + stride < p.rows) ahead(row + stride);
     // a piece of dy and xh; read for the sums and again for dx, as holding them takes twice the registers
-    auto read = [&](int i, int e0, uint64_t (&d)[V / 2], uint64_t (&xh)[V / 2]) {
-      elem::unpack_pairs<T>(read_piece<T, EDGE>(place(slot, 0, i), e0, cols), d);
+    auto read = [&](int i, uint64_t (&d)[V / 2], uint64_t (&xh)[V / 2]) {
+      elem::unpack_pairs<T>(*place(slot, 0, i), d);
       uint4 x;
       if constexpr (CKPT) {
         if constexpr (EDGE) {
@@ -667,18 +701,22 @@ bwd_rows(const BwdArgs p) {
           x = make_uint4(at[0], V == 8 ? at[1] : 0, code[i], 0);
         }
       } else {
-        x = read_piece<T, EDGE>(place(slot, 1, i), e0, cols);
+        x = *place(slot, 1, i);
       }
       x_hats<T, CKPT, EDGE>(x, shift, mean, rstd, xh);
     };
     wait_copies<D - 1>();
+    if (EDGE && e_first < 0) {
+      *place(slot, 0, 0) = masked<T>(*place(slot, 0, 0), e_first, cols);
+      if constexpr (!CKPT) *place(slot, 1, 0) = masked<T>(*place(slot, 1, 0), e_first, cols);
+    }
     uint64_t s1 = 0, s2 = 0;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int e0 = e_first + i * TPR * V;
       if (e0 >= cols) continue;
       uint64_t d[V / 2], xh[V / 2];
-      read(i, e0, d, xh);
+      read(i, d, xh);
       const int h = HOLD ? i : 0;
       if constexpr (!HOLD) kept_weights<T, kThreads<TPR>>(kept(i), g[h]);
 #pragma unroll
@@ -699,12 +737,12 @@ bwd_rows(const BwdArgs p) {
       const int e0 = e_first + i * TPR * V;
       if (e0 >= cols) continue;
       uint64_t d[V / 2], xh[V / 2];
-      read(i, e0, d, xh);
+      read(i, d, xh);
       const int h = HOLD ? i : 0;
       if constexpr (!HOLD) kept_weights<T, kThreads<TPR>>(kept(i), g[h]);
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) d[j] = mul2(by, fma2(xh[j], m1, fma2(d[j], g[h][j], m2)));
-      store_piece<T, EDGE>(dxr, e0, cols, d);
+      store_piece<T, EDGE, sizeof(T) == 2 && HOLD>(dxr, e0, cols, d);
     }
     fetch(slot, row + D * stride);
     slot = slot + 1 == D ? 0 : slot + 1;
@@ -984,8 +1022,11 @@ inline int row_grid(K kern, int block, int rb, size_t smem, int64_t rows, int* g
 // is too wide. Rows of up to 64 threads share a CTA where there are more than four
 // per SM (16384x512 bf16 forward: 7.5 us, and 15 by 128 threads a row); fewer rows
 // are spread over the SMs (64x512 backward: 4.1 us, and 4.8 by 32 threads a row).
+// Where `twice` says so, rows of 4097 to 8192 columns go to 256 threads of 32
+// columns: two CTAs share an SM, and one works while the other waits for a row's
+// sum (8000x8000 fp16 forward 46.5 us, and 53.1 by 512 threads; 1021x8192 11 and 10).
 template <typename T, class F>
-inline bool with_shape(int64_t pieces, int64_t rows, F f) {
+inline bool with_shape(int64_t pieces, int64_t rows, bool twice, F f) {
   constexpr int VPT = 16 / elem::kVec<T>;
   const bool many = rows > 4 * sm_count();
   using One = std::integral_constant<int, 1>;
@@ -996,6 +1037,7 @@ inline bool with_shape(int64_t pieces, int64_t rows, F f) {
   using Twice = std::integral_constant<int, 2 * VPT>;
   if (pieces <= 128 * VPT) return f(std::integral_constant<int, 128>{}, All{}), true;
   if (pieces <= 256 * VPT) return f(std::integral_constant<int, 256>{}, All{}), true;
+  if (pieces <= 512 * VPT && twice) return f(std::integral_constant<int, 256>{}, Twice{}), true;
   if (pieces <= 512 * VPT) return f(std::integral_constant<int, 512>{}, All{}), true;
   if (pieces <= 1024 * VPT) return f(std::integral_constant<int, 512>{}, Twice{}), true;
   return false;
@@ -1020,11 +1062,11 @@ inline int fwd_typed(const FwdArgs& a, cudaStream_t st) {
   const bool edge = shift != 0 || a.cols % V != 0;
   const int64_t pieces = (a.cols + V - 1) / V + (edge ? 1 : 0);
   int rc = KT_OK;
-  if (fast && with_shape<T>(pieces, a.rows, [&](auto tpr, auto vpt) {
+  if (fast && with_shape<T>(pieces, a.rows, a.rows > 16 * sm_count(), [&](auto tpr, auto vpt) {
         constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
         constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
         auto kern = edge ? fwd_rows<T, TPR, VPT, CKPT, true> : fwd_rows<T, TPR, VPT, CKPT, false>;
-        constexpr size_t smem = (size_t)kDepth<T, TPR, VPT, 1, kFwdThreads> * VPT * BLOCK * 16 +
+        constexpr size_t smem = (size_t)kDepth<T, TPR, VPT, 1, kFwdPerSm<T, TPR, VPT>> * VPT * BLOCK * 16 +
                                 2 * kWeightBytes<T, TPR, VPT>;
         int grid = 0;
         rc = row_grid(kern, BLOCK, RB, smem, a.rows, &grid);
@@ -1075,7 +1117,11 @@ inline int bwd_typed(const BwdArgs& a, void* dgamma, void* dbeta, cudaStream_t s
   const bool edge = shift != 0 || a.cols % V != 0;
   const int64_t pieces = (a.cols + V - 1) / V + (edge ? 1 : 0);
   int rc = KT_OK, parts = 0;
-  if (!(fast && with_shape<T>(pieces, a.rows, [&](auto tpr, auto vpt) {
+  // (8000x8000 fp16 72 us, and 77 by 512 threads; odd widths with checkpoints 140
+  // and 162; whole pieces with checkpoints 88 and 81, 4096x8192 fp32 87 and 71,
+  // 2400x8192 bf16 33 and 31)
+  const bool twice = sizeof(T) == 2 && (!CKPT || edge) && a.rows > 32 * sm_count();
+  if (!(fast && with_shape<T>(pieces, a.rows, twice, [&](auto tpr, auto vpt) {
           constexpr int TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
           constexpr int RB = kRows<TPR>, BLOCK = kThreads<TPR>;
           auto kern = edge ? bwd_rows<T, TPR, VPT, CKPT, true> : bwd_rows<T, TPR, VPT, CKPT, false>;
