@@ -34,7 +34,6 @@ BASE_FLAGS = [
     "-lineinfo",
     "-std=c++17",
     "-Xptxas", "-v",
-    "--split-compile", "4",  # a library's kernels are optimised in parallel; a fixed number, as the code depends on it
     "--shared",
     "-Xcompiler", "-fPIC",
     # hidden by default: only the KT_API entry points are exported, so the

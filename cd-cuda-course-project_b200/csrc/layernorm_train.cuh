@@ -27,12 +27,12 @@
 // one partial row per CTA. A second kernel adds the partial rows in their order,
 // so results do not change from run to run.
 //
-// Measured on a B200, 16384x4096, the join included: bf16 forward 46 us (5.8 TB/s,
-// 88 % of measured copy bandwidth) and backward 72 us (5.6 TB/s); with checkpoints
-// 58 us (5.8 TB/s) and 76 us (4.4 TB/s, issue slots 62 % busy); fp32 98 and 141 us
+// Measured on a B200, 16384x4096, the join included: bf16 forward 48 us (5.6 TB/s,
+// 85 % of measured copy bandwidth) and backward 73 us (5.5 TB/s); with checkpoints
+// 62 us (5.5 TB/s) and 74 us (4.5 TB/s, issue slots 62 % busy); fp32 98 and 141 us
 // (5.5 and 5.7 TB/s). 8x512 fp32: 2.4 and 3.9 us. 4096x16384 bf16: 55 and 79 us
 // (79 and 136 us with gamma and beta read again from L2 in every row).
-// Odd widths: 16384x2049 bf16 54 and 81 us, with checkpoints 89 and 110 us.
+// Odd widths: 16384x2049 bf16 54 and 80 us, with checkpoints 86 and 110 us.
 #pragma once
 #include <type_traits>
 
@@ -93,17 +93,37 @@ __device__ __forceinline__ int quant8(float v, float up) {
   return min(127, max(-127, __float2int_rn(v * up)));
 }
 
-// Four of them to a word.
-__device__ __forceinline__ uint32_t quant8x4(float a, float b, float c, float d, float up, uint32_t code) {
-  // limited to +-127 first, which leaves the same integers as afterwards; the sum
-  // with 1.5 2^23 has the integer, rounded to nearest even, in its low bits
-  constexpr float magic = 12582912.f;
-  const uint32_t q0 = __float_as_uint(fminf(fmaxf(a * up, -127.f), 127.f) + magic);
-  const uint32_t q1 = __float_as_uint(fminf(fmaxf(b * up, -127.f), 127.f) + magic);
-  const uint32_t q2 = __float_as_uint(fminf(fmaxf(c * up, -127.f), 127.f) + magic);
-  const uint32_t q3 = __float_as_uint(fminf(fmaxf(d * up, -127.f), 127.f) + magic);
-  const uint32_t w = __byte_perm(__byte_perm(q0, q1, 0x0040), __byte_perm(q2, q3, 0x0040), 0x5410);
+// Four of them to a word, from two pairs. A block's values times `up` are below
+// 128, so their sums with 1.5 2^23 have the integers, rounded to nearest even, in
+// their low 16 bits, where +-128 becomes +-127.
+__device__ __forceinline__ uint32_t quant8x4(uint64_t ab, uint64_t cd, float up, uint32_t code) {
+  const uint64_t by = elem::pair(up, up), magic = elem::pair(12582912.f, 12582912.f);
+  const float2 s = elem::halves(elem::fma2(ab, by, magic)), t = elem::halves(elem::fma2(cd, by, magic));
+  uint32_t p = __byte_perm(__float_as_uint(s.x), __float_as_uint(s.y), 0x5410);
+  uint32_t q = __byte_perm(__float_as_uint(t.x), __float_as_uint(t.y), 0x5410);
+  p = __vmaxs2(__vmins2(p, 0x007F007Fu), 0xFF81FF81u);
+  q = __vmaxs2(__vmins2(q, 0x007F007Fu), 0xFF81FF81u);
+  const uint32_t w = __byte_perm(p, q, 0x6420);
   return code == 255u ? 0u : w;
+}
+
+// The largest magnitude of a 16-byte piece as a bit pattern of T, and as one of fp32.
+template <typename T>
+__device__ __forceinline__ uint32_t top_bits(const uint4& r) {
+  if constexpr (sizeof(T) == 4) {
+    constexpr uint32_t m = 0x7FFFFFFFu;
+    return max(max(r.x & m, r.y & m), max(r.z & m, r.w & m));
+  } else {
+    constexpr uint32_t m = 0x7FFF7FFFu;
+    const uint32_t t = __vmaxu2(__vmaxu2(r.x & m, r.y & m), __vmaxu2(r.z & m, r.w & m));
+    return max(t & 0xFFFFu, t >> 16);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t as_fp32(uint32_t bits) {
+  if constexpr (std::is_same<T, float>::value) return bits;
+  else if constexpr (std::is_same<T, __nv_bfloat16>::value) return bits << 16;
+  else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)bits)));
 }
 
 // ---------------------------------------------------------------- row pieces
@@ -194,7 +214,7 @@ __device__ __forceinline__ void store_part(T* at, const uint4& raw, int lo, int 
 }
 
 // PARTS: a cut piece by its parts, else by its elements, which takes fewer
-// registers (16384x2049 bf16 by parts 54 and 77 us, by elements 59 and 89; where a
+// registers (16384x2049 bf16 by parts 54 and 80 us, by elements 59 and 89; where a
 // thread of the backward pass has 32 columns, 4000x12345 bf16, 104 and 90 us).
 template <typename T, bool EDGE, bool PARTS>
 __device__ __forceinline__ void store_piece(T* row, int e0, int cols, const uint64_t (&f)[elem::kVec<T> / 2]) {
@@ -434,21 +454,16 @@ fwd_rows(const FwdArgs p) {
     if (EDGE && e_first < 0) *place(slot, 0) = masked<T>(*place(slot, 0), e_first, cols);
     if constexpr (CKPT && EDGE) row_sync<TPR>();  // the other threads' copies
     // writes columns [k0, k0 + V) of the checkpoint; the lanes of a block together
-    auto keep8 = [&](const uint64_t (&f)[V / 2], int k0) {
+    auto keep8 = [&](const uint64_t (&f)[V / 2], uint32_t top, int k0) {
       constexpr int LPB = 32 / V;  // lanes that share a block of 32 columns
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < V / 2; ++j) top = max(top, max(abs_bits(halves(f[j]).x), abs_bits(halves(f[j]).y)));
 #pragma unroll
       for (int o = 1; o < LPB; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       if (k0 < cols) {
-        const uint32_t code = block_code(top);
+        const uint32_t code = block_code(as_fp32<T>(top));
         const float up = code_up(code);
         uint32_t w[V / 4];
 #pragma unroll
-        for (int k = 0; k < V / 4; ++k)
-          w[k] = quant8x4(halves(f[2 * k]).x, halves(f[2 * k]).y, halves(f[2 * k + 1]).x, halves(f[2 * k + 1]).y, up,
-                          code);
+        for (int k = 0; k < V / 4; ++k) w[k] = quant8x4(f[2 * k], f[2 * k + 1], up, code);
         int8_t* qr = p.q8 + row * p.ld_q8 + k0;
         if constexpr (V == 8) *reinterpret_cast<uint2*>(qr) = make_uint2(w[0], w[1]);
         else *reinterpret_cast<uint32_t*>(qr) = w[0];
@@ -456,6 +471,7 @@ fwd_rows(const FwdArgs p) {
       }
     };
     uint64_t v[VPT][V / 2];
+    uint32_t tops[VPT];
     uint64_t s2 = 0;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -463,6 +479,7 @@ fwd_rows(const FwdArgs p) {
       uint4 raw = make_uint4(0, 0, 0, 0);
       if (e0 < cols) raw = *place(slot, i);
       elem::unpack_pairs<T>(raw, v[i]);
+      if constexpr (CKPT && !EDGE) tops[i] = top_bits<T>(raw);
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) s2 = add2(s2, v[i][j]);
     }
@@ -476,7 +493,7 @@ fwd_rows(const FwdArgs p) {
         uint4 raw = bytes_at<T>(own, next, shift * (int)sizeof(T));
         uint64_t f[V / 2];
         elem::unpack_pairs<T>(raw, f);
-        keep8(f, k0);
+        keep8(f, top_bits<T>(raw), k0);
       }
     } else {
       fetch(slot, row + D * stride);
@@ -490,7 +507,7 @@ fwd_rows(const FwdArgs p) {
     const uint64_t minus = pair(-mean, -mean);
     if constexpr (CKPT && !EDGE) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) keep8(v[i], e_first + i * TPR * V);
+      for (int i = 0; i < VPT; ++i) keep8(v[i], tops[i], e_first + i * TPR * V);
     }
     uint64_t q2 = 0;
 #pragma unroll

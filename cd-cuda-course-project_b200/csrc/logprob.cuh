@@ -31,8 +31,8 @@
 // bytes and rows are many. Few long rows are split over a cluster of up to 8 CTAs, which join their
 // partial results through distributed shared memory in the order of their ranks.
 //
-// Measured on a B200: 2048x131072 bf16 87 us (6.2 TB/s, 95 % of measured copy
-// bandwidth), with 20 alternatives 107 us, its gradient 187 us (5.7 TB/s);
+// Measured on a B200: 2048x131072 bf16 86 us (6.2 TB/s, 95 % of measured copy
+// bandwidth), with 20 alternatives 108 us, its gradient 183 us (5.9 TB/s);
 // 512x131072 fp32 41 us, with 8 alternatives 47 us; one row of 32768 fp32 3.1 us,
 // with 5 alternatives 6.7 us; 2048x1000 bf16 3.8 us.
 #pragma once

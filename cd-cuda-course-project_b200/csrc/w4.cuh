@@ -37,10 +37,10 @@
 // turn late (a warp that has left its sums arrives at the cluster's barrier, goes
 // on with the next rows, and waits there before it adds the sums before).
 //
-// Measured on a B200, 131072x8192: one token in bf16, groups of 128, 106 us
-// (5.2 TB/s, 80 % of measured copy bandwidth); 8 tokens in fp16, groups of 64 with
-// zeros, 138 us (4.3 TB/s; issue slots 66 % busy, the ALU pipe 52 %); 16 tokens in
-// bf16 180 us. 4096x4096, one token: 5.4 us. 16 fp32 tokens, 32768x8192: 109 us,
+// Measured on a B200, 131072x8192: one token in bf16, groups of 128, 109 us
+// (5.1 TB/s, 78 % of measured copy bandwidth); 8 tokens in fp16, groups of 64 with
+// zeros, 142 us (4.2 TB/s; issue slots 66 % busy, the ALU pipe 52 %); 16 tokens in
+// bf16 184 us. 4096x4096, one token: 5.5 us. 16 fp32 tokens, 32768x8192: 104 us,
 // bound by the three tensor products per weight.
 #pragma once
 #include <cooperative_groups.h>
