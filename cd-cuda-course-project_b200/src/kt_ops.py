@@ -235,22 +235,35 @@ def layernorm_bwd(dy: torch.Tensor, saved: LayerNormSaved, weight_grads: bool = 
     """(dx, dgamma, dbeta) of layernorm_train from dy. dgamma and dbeta are of
     gamma's type and None where gamma or beta was None, or weight_grads is False."""
     x, q8, q8_exp, gamma, stats, beta_dtype = saved
-    kept = q8 if x is None else x
     dt = _dtype(dy, "dy")
-    dev = kept.get_device()
-    _dense(dy, "dy", dy.dtype if x is None else x.dtype, dev)
-    if dy.shape != kept.shape:
-        raise ValueError(f"layernorm_bwd: dy is {tuple(dy.shape)}, the input was {tuple(kept.shape)}")
+    _check(dy, "dy", dy.dtype if x is None else x.dtype)
+    dev = dy.get_device()
+    kept = q8 if x is None else x
+    if kept is None or dy.shape != kept.shape or dy.dim() != 2:
+        raise ValueError(f"layernorm_bwd: dy is {tuple(dy.shape)}, the input was "
+                         f"{tuple(kept.shape) if kept is not None else 'not saved'}")
     rows, cols = dy.shape
     ld_q8 = 0
-    if q8 is not None:
+    if x is None:
         ld_q8 = q8.stride(0) if rows > 1 else max(q8.stride(0), cols)
-        if cols > 1 and q8.stride(1) != 1:
-            raise ValueError("q8: the elements of a row must be contiguous")
+        if q8.dtype is not torch.int8 or q8.get_device() != dev or (cols > 1 and q8.stride(1) != 1) or ld_q8 < cols:
+            raise ValueError("q8 must be int8 on dy's device, the elements of a row contiguous")
+        if q8_exp is None or q8_exp.shape != (rows, (cols + 31) // 32):
+            raise ValueError(f"q8_exp must be {(rows, (cols + 31) // 32)}")
+        _dense(q8_exp, "q8_exp", torch.uint8, dev)
+    else:
+        _dense(x, "x", dy.dtype, dev)
+    _dense(stats, "stats", torch.float32, dev)
+    if stats.shape != (2, rows):
+        raise ValueError(f"stats must be {(2, rows)}, got {tuple(stats.shape)}")
     wt = gamma.dtype if gamma is not None else beta_dtype or torch.float32
-    wdt = _DTYPES[wt]
-    if wdt not in (kt_lib.KT_F32, dt):
-        raise ValueError(f"dy must be {wt}, got {dy.dtype}")
+    wdt = _DTYPES.get(wt)
+    if wdt not in (kt_lib.KT_F32, dt) or (gamma is not None and beta_dtype not in (None, wt)):
+        raise ValueError(f"dy and the weights must be of one type or the weights fp32, got {dy.dtype} and {wt}")
+    if gamma is not None:
+        _dense(gamma, "gamma", wt, dev)
+        if gamma.numel() != cols:
+            raise ValueError(f"layernorm_bwd: gamma must have {cols} elements")
     if lib is None:
         lib = kt_lib.load()
     dx = torch.empty_like(dy)

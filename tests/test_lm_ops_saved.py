@@ -1,0 +1,54 @@
+"""
+The backward pass of LayerNorm takes what it reads from the tensors that the
+forward pass left, so it refuses those that are not on dy's device, or whose type
+or size is not what the forward pass leaves.
+"""
+
+from __future__ import annotations
+
+import pytest
+
+import kt_ops
+
+torch = pytest.importorskip("torch")
+
+
+def saved_like(rows, cols, ckpt8, device):
+    q8 = torch.zeros(rows, (cols + 7) // 8 * 8, dtype=torch.int8, device=device)[:, :cols]
+    exp = torch.zeros(rows, (cols + 31) // 32, dtype=torch.uint8, device=device)
+    return kt_ops.LayerNormSaved(None if ckpt8 else torch.zeros(rows, cols, device=device),
+                                 q8 if ckpt8 else None, exp if ckpt8 else None, torch.ones(cols, device=device),
+                                 torch.ones(2, rows, device=device), torch.float32)
+
+
+@pytest.mark.parametrize("ckpt8", [False, True])
+def test_tensors_on_the_host_are_refused(ckpt8):
+    with pytest.raises(ValueError, match="CUDA"):
+        kt_ops.layernorm_bwd(torch.zeros(4, 64), saved_like(4, 64, ckpt8, "cpu"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ckpt8", [False, True])
+def test_saved_tensors_that_do_not_fit_are_refused(dev, lib, ckpt8):
+    rows, cols = 6, 100
+    dy = torch.ones(rows, cols, device=dev)
+    good = saved_like(rows, cols, ckpt8, dev)
+    kt_ops.layernorm_bwd(dy, good, lib=lib)
+    bad = [dict(stats=good.stats.cpu()), dict(stats=good.stats[:, :5].contiguous()), dict(stats=good.stats[0]),
+           dict(stats=good.stats.double()), dict(stats=torch.ones(4, rows, device=dev)[::2]),
+           dict(gamma=good.gamma.cpu()), dict(gamma=good.gamma[:99]), dict(gamma=good.gamma.double()),
+           dict(gamma=torch.ones(200, device=dev)[::2]), dict(beta_dtype=torch.float64)]
+    if ckpt8:
+        bad += [dict(q8=good.q8.cpu()), dict(q8=good.q8.float()), dict(q8=good.q8[:5]), dict(q8=good.q8[:, :99]),
+                dict(q8=good.q8.contiguous().view(-1)), dict(q8=None), dict(q8=good.q8[:1].expand(rows, cols)),
+                dict(q8_exp=good.q8_exp.cpu()), dict(q8_exp=good.q8_exp[:, :3].contiguous()), dict(q8_exp=None),
+                dict(q8_exp=good.q8_exp.float()), dict(q8_exp=torch.zeros(rows, 8, dtype=torch.uint8, device=dev)[:, ::2]),
+                dict(q8_exp=good.q8_exp[:5])]
+    else:
+        bad += [dict(x=good.x.cpu()), dict(x=good.x.half()), dict(x=good.x[:5]), dict(x=good.x.t().contiguous().t()),
+                dict(x=good.x.view(-1)), dict(x=None)]
+    for change in bad:
+        with pytest.raises(ValueError):
+            kt_ops.layernorm_bwd(dy, good._replace(**change), lib=lib)
+    with pytest.raises(ValueError):
+        kt_ops.layernorm_bwd(dy.cpu(), good, lib=lib)
