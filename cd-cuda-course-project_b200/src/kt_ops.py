@@ -248,6 +248,11 @@ def layernorm_bwd(dy: torch.Tensor, saved: LayerNormSaved, weight_grads: bool = 
         ld_q8 = q8.stride(0) if rows > 1 else max(q8.stride(0), cols)
         if q8.dtype is not torch.int8 or q8.get_device() != dev or (cols > 1 and q8.stride(1) != 1) or ld_q8 < cols:
             raise ValueError("q8 must be int8 on dy's device, the elements of a row contiguous")
+        # the kernels read whole 8 bytes of rows that are a multiple of 8 apart; a copy's last row may end before
+        if cols % 8 and ld_q8 % 8 == 0 and q8.untyped_storage().nbytes() < \
+                q8.storage_offset() + (rows - 1) * ld_q8 + (cols + 7) // 8 * 8:
+            q8 = q8.contiguous()
+            ld_q8 = cols
         if q8_exp is None or q8_exp.shape != (rows, (cols + 31) // 32):
             raise ValueError(f"q8_exp must be {(rows, (cols + 31) // 32)}")
         _dense(q8_exp, "q8_exp", torch.uint8, dev)

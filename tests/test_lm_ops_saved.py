@@ -52,3 +52,31 @@ def test_saved_tensors_that_do_not_fit_are_refused(dev, lib, ckpt8):
             kt_ops.layernorm_bwd(dy, good._replace(**change), lib=lib)
     with pytest.raises(ValueError):
         kt_ops.layernorm_bwd(dy.cpu(), good, lib=lib)
+
+
+class Recorder:
+    """Takes the library's place and launches nothing."""
+
+    def layernorm_bwd_workspace_bytes(self, rows, cols):
+        return 16
+
+    def layernorm_train_bwd(self, dy, x, q8, q8_exp, ld_q8, *rest):
+        self.q8, self.ld_q8 = q8, ld_q8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(1, 13), (1, 16), (7, 13), (7, 16)])
+def test_checkpoint_rows_are_read_within_their_memory(dev, rows, cols):
+    """The kernels read rows whose distance is a multiple of 8 up to their next
+    whole 8 bytes. A copy of a row has the distance and not the bytes."""
+    dy, saved, lib = torch.ones(rows, cols, device=dev), saved_like(rows, cols, True, dev), Recorder()
+    tight = torch.zeros((rows - 1) * 16 + cols, dtype=torch.int8, device=dev)
+    copies = [saved.q8, saved.q8.clone(), saved.q8.contiguous(), torch.as_strided(tight, (rows, cols), (16, 1))]
+    for q8 in copies:
+        kt_ops.layernorm_bwd(dy, saved._replace(q8=q8), lib=lib)
+        assert lib.ld_q8 >= cols
+        if lib.q8 == q8.data_ptr():
+            last = cols if lib.ld_q8 % 8 else (cols + 7) // 8 * 8
+            assert q8.storage_offset() + (rows - 1) * lib.ld_q8 + last <= q8.untyped_storage().nbytes()
+    kt_ops.layernorm_bwd(dy, saved, lib=lib)
+    assert lib.ld_q8 == 16  # with its bytes behind the row, as the forward pass leaves it
