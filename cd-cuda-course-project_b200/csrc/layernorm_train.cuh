@@ -1070,12 +1070,19 @@ inline int check_common(const char* what, int64_t rows, int64_t cols, int dtype,
   return KT_OK;
 }
 
+// Whether a checkpoint's rows are written and read by V bytes at a time: the last
+// of them reach behind a row only where its distance is a multiple of 8.
+template <int V>
+inline bool whole_words(const int8_t* q8, int64_t ld, int64_t cols) {
+  return elem::aligned_to(q8, V) && (ld % 8 == 0 || (ld % V == 0 && cols % V == 0));
+}
+
 template <typename T, bool CKPT>
 inline int fwd_typed(const FwdArgs& a, cudaStream_t st) {
   constexpr int V = elem::kVec<T>;
   const int shift = elem::misalign<T>(a.x);
   bool fast = elem::misalign<T>(a.y) == shift;
-  if (CKPT) fast = fast && a.ld_q8 % V == 0 && elem::aligned_to(a.q8, V);
+  if (CKPT) fast = fast && whole_words<V>(a.q8, a.ld_q8, a.cols);
   const bool edge = shift != 0 || a.cols % V != 0;
   const int64_t pieces = (a.cols + V - 1) / V + (edge ? 1 : 0);
   int rc = KT_OK;
@@ -1129,7 +1136,7 @@ inline int bwd_typed(const BwdArgs& a, void* dgamma, void* dbeta, cudaStream_t s
   constexpr int V = elem::kVec<T>;
   const int shift = elem::misalign<T>(a.dy);
   bool fast = elem::misalign<T>(a.dx) == shift;
-  if (CKPT) fast = fast && a.ld_q8 % V == 0 && elem::aligned_to(a.q8, V);
+  if (CKPT) fast = fast && whole_words<V>(a.q8, a.ld_q8, a.cols);
   else fast = fast && elem::misalign<T>(a.x) == shift;
   const bool edge = shift != 0 || a.cols % V != 0;
   const int64_t pieces = (a.cols + V - 1) / V + (edge ? 1 : 0);

@@ -205,10 +205,11 @@ KT_API int kt_fa_fwd_bf16(const uint16_t* Q, const uint16_t* K, const uint16_t* 
  * `wdtype`, fp32 or the input's type.
  * With q8 and q8_exp (both or neither), an 8-bit checkpoint of x is written
  * too: q8 is rows x cols, ld_q8 bytes apart, q8_exp rows x ceil(cols/32). (Rows
- * whose ld_q8 is a multiple of 8 may be written up to their next whole 8 bytes,
- * and take a fraction of the time of others.) Each block of 32 columns
- * has E = the exponent field of its largest magnitude as fp32, at least 7 (255:
- * the block holds an infinity or NaN and stands for NaN), and
+ * whose ld_q8 is a multiple of 8, the last one too, may be written up to their
+ * next whole 8 bytes, and the backward pass may read those; they take a fraction
+ * of the time of others, of which nothing but the columns is touched.) Each block
+ * of 32 columns has E = the exponent field of its largest magnitude as fp32, at
+ * least 7 (255: the block holds an infinity or NaN and stands for NaN), and
  * q = x * 2^(133-E) rounded to nearest even, limited to +-127, standing for
  * q * 2^(E-133). */
 KT_API int kt_layernorm_train_fwd(const void* x, const void* gamma, const void* beta, void* y, float* mean,
