@@ -1077,6 +1077,13 @@ inline bool whole_words(const int8_t* q8, int64_t ld, int64_t cols) {
   return elem::aligned_to(q8, V) && (ld % 8 == 0 || (ld % V == 0 && cols % V == 0));
 }
 
+// Whether two tensors of one size share memory without being one: CTAs would read
+// what others have stored.
+inline bool partly_one(const void* a, const void* b, size_t bytes) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return a && b && x != y && x < y + bytes && y < x + bytes;
+}
+
 template <typename T, bool CKPT>
 inline int fwd_typed(const FwdArgs& a, cudaStream_t st) {
   constexpr int V = elem::kVec<T>;
@@ -1126,6 +1133,8 @@ inline int forward(const FwdArgs& a, int dtype, cudaStream_t st) {
   if (!elem::aligned_to(a.x, sz) || !elem::aligned_to(a.y, sz) || !elem::aligned_to(a.gamma, wsz) ||
       !elem::aligned_to(a.beta, wsz) || !elem::aligned_to(a.mean, 4) || !elem::aligned_to(a.rstd, 4))
     return fail(KT_ERR_ARG, "layernorm_train: a pointer is not aligned to its elements");
+  if (partly_one(a.x, a.y, (size_t)(a.rows * a.cols) * sz))
+    return fail(KT_ERR_ARG, "layernorm_train: y overlaps x without being it");
   if (dtype == KT_F32) return a.q8 ? fwd_typed<float, true>(a, st) : fwd_typed<float, false>(a, st);
   if (dtype == KT_BF16) return a.q8 ? fwd_typed<__nv_bfloat16, true>(a, st) : fwd_typed<__nv_bfloat16, false>(a, st);
   return a.q8 ? fwd_typed<__half, true>(a, st) : fwd_typed<__half, false>(a, st);
@@ -1165,14 +1174,15 @@ inline int bwd_typed(const BwdArgs& a, void* dgamma, void* dbeta, cudaStream_t s
       kern<<<parts, block, 0, st>>>(a);
       rc = check_launch("layernorm_train bwd_scalar");
     } else {
-      const int64_t g = a.rows < 4 * sm_count() ? a.rows : 4 * sm_count();
-      bwd_any_dx<T, CKPT><<<(int)g, 256, 0, st>>>(a);
-      rc = check_launch("layernorm_train bwd_any_dx");
-      if (rc == KT_OK && a.partial) {
+      if (a.partial) {  // before dx, which may take dy's or x's place
         parts = (int)(a.rows < 64 ? a.rows : 64);
         bwd_any_cols<T, CKPT><<<dim3((unsigned)((a.cols + 255) / 256), (unsigned)parts), 256, 0, st>>>(a);
         rc = check_launch("layernorm_train bwd_any_cols");
+        if (rc != KT_OK) return rc;
       }
+      const int64_t g = a.rows < 4 * sm_count() ? a.rows : 4 * sm_count();
+      bwd_any_dx<T, CKPT><<<(int)g, 256, 0, st>>>(a);
+      rc = check_launch("layernorm_train bwd_any_dx");
     }
   }
   if (rc != KT_OK || a.partial == nullptr) return rc;
@@ -1214,6 +1224,8 @@ inline int backward(BwdArgs a, int dtype, void* dgamma, void* dbeta, void* works
   if (!elem::aligned_to(a.dy, sz) || !elem::aligned_to(a.x, sz) || !elem::aligned_to(a.dx, sz) ||
       !elem::aligned_to(a.gamma, wsz) || !elem::aligned_to(a.mean, 4) || !elem::aligned_to(a.rstd, 4))
     return fail(KT_ERR_ARG, "layernorm_train bwd: a pointer is not aligned to its elements");
+  if (partly_one(a.dx, a.dy, (size_t)(a.rows * a.cols) * sz) || partly_one(a.dx, a.x, (size_t)(a.rows * a.cols) * sz))
+    return fail(KT_ERR_ARG, "layernorm_train bwd: dx overlaps dy or x without being it");
   a.partial = nullptr;
   if (dgamma || dbeta) {
     if (workspace == nullptr || ws_bytes < workspace_bytes(a.rows, a.cols) || !aligned16(workspace))

@@ -202,7 +202,8 @@ KT_API int kt_fa_fwd_bf16(const uint16_t* Q, const uint16_t* K, const uint16_t* 
 /* LayerNorm over the last dim for training: y = gamma*(x-mean)*rstd + beta with
  * rstd = 1/sqrt(var+eps), biased variance, and mean, rstd (fp32, `rows` each)
  * saved for the backward pass. gamma and beta (may be NULL: 1 and 0) are of
- * `wdtype`, fp32 or the input's type.
+ * `wdtype`, fp32 or the input's type. y may be x itself, no other part of its
+ * memory.
  * With q8 and q8_exp (both or neither), an 8-bit checkpoint of x is written
  * too: q8 is rows x cols, ld_q8 bytes apart, q8_exp rows x ceil(cols/32). (Rows
  * whose ld_q8 is a multiple of 8, the last one too, may be written up to their
@@ -221,7 +222,8 @@ KT_API size_t kt_layernorm_bwd_workspace_bytes(int64_t rows, int64_t cols);
 
 /* Its backward pass: dx, and dgamma, dbeta (of `wdtype`, either may be NULL)
  * summed over the rows in a fixed order. Takes x or its 8-bit checkpoint (then
- * x is NULL). `workspace` (kt_layernorm_bwd_workspace_bytes, 16-byte aligned,
+ * x is NULL). dx may be dy or x itself, no other part of their memory.
+ * `workspace` (kt_layernorm_bwd_workspace_bytes, 16-byte aligned,
  * any content) is caller-owned scratch, not needed without dgamma and dbeta;
  * calls that may overlap need one each. */
 KT_API int kt_layernorm_train_bwd(const void* dy, const void* x, const int8_t* q8, const uint8_t* q8_exp,

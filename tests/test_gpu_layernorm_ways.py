@@ -16,6 +16,56 @@ import kt_ops  # noqa: E402
 from test_gpu_layernorm_train import E, TYPES, check, half_step, inputs  # noqa: E402
 
 
+@pytest.mark.parametrize("ckpt8", [False, True])
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,cols", [(3, 16387), (700, 16387), (70, 20000), (300, 1000), (50, 1023), (9, 8192)])
+def test_gradient_of_the_input_in_place(dev, lib, rows, cols, t, ckpt8):
+    """dx over dy's memory, and over x's: the weights' gradients stay those of the inputs."""
+    x, dy, gamma, beta = inputs(dev, rows, cols, t)
+    _, saved = kt_ops.layernorm_train(x, gamma, beta, ckpt8=ckpt8, lib=lib)
+    want = kt_ops.layernorm_bwd(dy, saved, lib=lib)
+    for over in ("dy",) if ckpt8 else ("dy", "x"):
+        dx, x2 = dy.clone(), x.clone()
+        dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(beta)
+        if over == "x":
+            dx, src = x2, dy
+        else:
+            src = dx
+        size = lib.layernorm_bwd_workspace_bytes(rows, cols)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        at = saved.stats.data_ptr()
+        q = (None, saved.q8.data_ptr(), saved.q8_exp.data_ptr(), saved.q8.stride(0)) if ckpt8 else \
+            (x2.data_ptr(), None, None, 0)
+        lib.layernorm_train_bwd(src.data_ptr(), *q, gamma.data_ptr(), at, at + 4 * rows, dx.data_ptr(),
+                                dgamma.data_ptr(), dbeta.data_ptr(), rows, cols, kt_ops._DTYPES[t], kt_lib.KT_F32,
+                                ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        for got, w in zip((dx, dgamma, dbeta), want):
+            assert torch.equal(got, w), over
+
+
+@pytest.mark.parametrize("ckpt8", [False, True])
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,cols", [(700, 16387), (3000, 1000), (2000, 1023), (9, 8192), (2000, 77)])
+def test_output_in_place(dev, lib, rows, cols, t, ckpt8):
+    """y over x's memory."""
+    x, _, gamma, beta = inputs(dev, rows, cols, t)
+    y, saved = kt_ops.layernorm_train(x, gamma, beta, ckpt8=ckpt8, lib=lib)
+    stats = torch.empty_like(saved.stats)
+    q8, exp, ld = None, None, 0
+    if ckpt8:
+        ld = saved.q8.stride(0)
+        q8, exp = torch.empty(rows, ld, dtype=torch.int8, device=dev), torch.empty_like(saved.q8_exp)
+    at = stats.data_ptr()
+    lib.layernorm_train_fwd(x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), x.data_ptr(), at, at + 4 * rows,
+                            q8.data_ptr() if ckpt8 else None, exp.data_ptr() if ckpt8 else None, ld, rows, cols, 1e-5,
+                            kt_ops._DTYPES[t], kt_lib.KT_F32, torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(x, y) and torch.equal(stats, saved.stats)
+    if ckpt8:
+        assert torch.equal(q8[:, :cols], saved.q8) and torch.equal(exp, saved.q8_exp)
+
+
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("cols,ld", [(9, 12), (30, 36), (61, 68), (1001, 1004), (8191, 8196), (9, 9), (9, 10), (12, 12),
                                      (64, 68), (16, 24)])

@@ -1,14 +1,17 @@
 """
 The backward pass of LayerNorm takes what it reads from the tensors that the
 forward pass left, so it refuses those that are not on dy's device, or whose type
-or size is not what the forward pass leaves.
+or size is not what the forward pass leaves. Both refuse an output that shares a
+part of an input's memory.
 """
 
 from __future__ import annotations
 
 import pytest
 
+import kt_lib
 import kt_ops
+from test_lm_ops_refusals import P, ln_bwd, ln_fwd, refused
 
 torch = pytest.importorskip("torch")
 
@@ -52,6 +55,16 @@ def test_saved_tensors_that_do_not_fit_are_refused(dev, lib, ckpt8):
             kt_ops.layernorm_bwd(dy, good._replace(**change), lib=lib)
     with pytest.raises(ValueError):
         kt_ops.layernorm_bwd(dy.cpu(), good, lib=lib)
+
+
+def test_outputs_that_overlap_a_part_of_an_input_are_refused(lib):
+    size = 4 * 64 * 4  # of the tensors
+    for shift in (4, -4, size - 4, 4 - size):
+        refused(lambda: ln_fwd(lib, y=P + shift))
+        refused(lambda: ln_bwd(lib, dx=P + shift))
+        refused(lambda: ln_bwd(lib, dx=P + 2 * size, x=P + 2 * size + shift))
+        refused(lambda: ln_bwd(lib, x=None, q8=P, q8_exp=P, dx=P + shift))
+        refused(lambda: ln_fwd(lib, y=P + shift // 2, dtype=kt_lib.KT_BF16, wdtype=kt_lib.KT_BF16))
 
 
 class Recorder:
