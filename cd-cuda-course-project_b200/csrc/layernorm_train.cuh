@@ -591,18 +591,18 @@ __global__ void __launch_bounds__(256) fwd_any(const FwdArgs p) {
 }
 
 // ---------------------------------------------------------------- backward
-// A piece of xh from x, or from its 8-bit checkpoint (.x, .y: eight values, .z:
-// the code of the block, and 256 times that of the block before, to which the
-// first `shift` columns of a piece may belong).
+// A piece of x - mean from x, or from its 8-bit checkpoint (.x, .y: eight values,
+// .z: the code of the block, and 256 times that of the block before, to which the
+// first `shift` columns of a piece may belong). The mean goes off before r is
+// multiplied: x r - mean r would be off by the rounding of mean r where x is near
+// the mean (a row of one value has xh = 0), and not finite where mean r is not.
 template <typename T, bool CKPT, bool EDGE>
-__device__ __forceinline__ void x_hats(const uint4& raw, int shift, float mean, float rstd,
-                                       uint64_t (&xh)[elem::kVec<T> / 2]) {
+__device__ __forceinline__ void centred(const uint4& raw, int shift, float mean, uint64_t (&xm)[elem::kVec<T> / 2]) {
   using elem::pair;
   constexpr int V = elem::kVec<T>;
-  // x rstd - mean rstd: off by 2^-24 (|xh| + |mean| rstd), as the mean itself is
-  const uint64_t minus = pair(-mean * rstd, -mean * rstd);
+  const uint64_t minus = pair(-mean, -mean);
   if constexpr (CKPT) {
-    const float down = code_down(raw.z & 255u) * rstd, first = code_down(raw.z >> 8) * rstd;
+    const float down = code_down(raw.z & 255u), first = code_down(raw.z >> 8);
     const uint64_t bias = pair(-8388736.f, -8388736.f);  // 2^23 + 128
 #pragma unroll
     for (int j = 0; j < V / 2; ++j) {
@@ -612,13 +612,12 @@ __device__ __forceinline__ void x_hats(const uint4& raw, int shift, float mean, 
                          __byte_perm(word, 0x4B000000u, 0x7440 + 2 * (j & 1));
       const uint64_t scale = EDGE ? pair(2 * j < shift ? first : down, 2 * j + 1 < shift ? first : down)
                                   : pair(down, down);
-      xh[j] = elem::fma2(elem::add2(q, bias), scale, minus);
+      xm[j] = elem::fma2(elem::add2(q, bias), scale, minus);
     }
   } else {
-    const uint64_t by = pair(rstd, rstd);
-    elem::unpack_pairs<T>(raw, xh);
+    elem::unpack_pairs<T>(raw, xm);
 #pragma unroll
-    for (int j = 0; j < V / 2; ++j) xh[j] = elem::fma2(xh[j], by, minus);
+    for (int j = 0; j < V / 2; ++j) xm[j] = elem::add2(xm[j], minus);
   }
 }
 
@@ -705,8 +704,8 @@ bwd_rows(const BwdArgs p) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) code[i] = CKPT ? ncode[i] : 0;
     if (row + stride < p.rows) ahead(row + stride);
-    // a piece of dy and xh; read for the sums and again for dx, as holding them takes twice the registers
-    auto read = [&](int i, uint64_t (&d)[V / 2], uint64_t (&xh)[V / 2]) {
+    // a piece of dy and x - mean; read for the sums and again for dx, as holding them takes twice the registers
+    auto read = [&](int i, uint64_t (&d)[V / 2], uint64_t (&xm)[V / 2]) {
       elem::unpack_pairs<T>(*place(slot, 0, i), d);
       uint4 x;
       if constexpr (CKPT) {
@@ -720,45 +719,47 @@ bwd_rows(const BwdArgs p) {
       } else {
         x = *place(slot, 1, i);
       }
-      x_hats<T, CKPT, EDGE>(x, shift, mean, rstd, xh);
+      centred<T, CKPT, EDGE>(x, shift, mean, xm);
     };
     wait_copies<D - 1>();
     if (EDGE && e_first < 0) {
       *place(slot, 0, 0) = masked<T>(*place(slot, 0, 0), e_first, cols);
       if constexpr (!CKPT) *place(slot, 1, 0) = masked<T>(*place(slot, 1, 0), e_first, cols);
     }
+    const uint64_t by = pair(rstd, rstd);
     uint64_t s1 = 0, s2 = 0;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int e0 = e_first + i * TPR * V;
       if (e0 >= cols) continue;
-      uint64_t d[V / 2], xh[V / 2];
-      read(i, d, xh);
+      uint64_t d[V / 2], xm[V / 2];
+      read(i, d, xm);
       const int h = HOLD ? i : 0;
       if constexpr (!HOLD) kept_weights<T, kThreads<TPR>>(kept(i), g[h]);
 #pragma unroll
       for (int j = 0; j < V / 2; ++j) {
-        dg[i][j] = fma2(d[j], xh[j], dg[i][j]);
+        const uint64_t xh = mul2(xm[j], by);
+        dg[i][j] = fma2(d[j], xh, dg[i][j]);
         db[i][j] = add2(db[i][j], d[j]);
         const uint64_t w = mul2(d[j], g[h][j]);
-        s1 = fma2(w, xh[j], s1);
+        s1 = fma2(w, xh, s1);
         s2 = add2(s2, w);
       }
     }
     const float2 s = row_sum2<TPR>(halves(s1).x + halves(s1).y, halves(s2).x + halves(s2).y, red[turn]);
-    const float c1 = -s.x * per_col, c2 = -s.y * per_col;
-    const uint64_t m1 = pair(c1, c1), m2 = pair(c2, c2), by = pair(rstd, rstd);
+    const float c1 = -s.x * per_col * rstd, c2 = -s.y * per_col;
+    const uint64_t m1 = pair(c1, c1), m2 = pair(c2, c2);
     T* dxr = static_cast<T*>(p.dx) + row * cols;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int e0 = e_first + i * TPR * V;
       if (e0 >= cols) continue;
-      uint64_t d[V / 2], xh[V / 2];
-      read(i, d, xh);
+      uint64_t d[V / 2], xm[V / 2];
+      read(i, d, xm);
       const int h = HOLD ? i : 0;
       if constexpr (!HOLD) kept_weights<T, kThreads<TPR>>(kept(i), g[h]);
 #pragma unroll
-      for (int j = 0; j < V / 2; ++j) d[j] = mul2(by, fma2(xh[j], m1, fma2(d[j], g[h][j], m2)));
+      for (int j = 0; j < V / 2; ++j) d[j] = mul2(by, fma2(xm[j], m1, fma2(d[j], g[h][j], m2)));
       store_piece<T, EDGE, sizeof(T) == 2 && HOLD>(dxr, e0, cols, d);
     }
     fetch(slot, row + D * stride);

@@ -17,6 +17,30 @@ from test_gpu_layernorm_train import E, TYPES, check, half_step, inputs  # noqa:
 
 
 @pytest.mark.parametrize("ckpt8", [False, True])
+@pytest.mark.parametrize("rows,cols", [(40, 64), (9, 1024), (3, 8192), (700, 256), (2, 32768)])
+@pytest.mark.parametrize("value", [1000.0, 2.0 ** 80, -2.0 ** 120])
+def test_rows_of_one_value(dev, lib, rows, cols, value, ckpt8):
+    """A constant row (of a value that 8 bits hold) whose mean is exact has xh = 0:
+    y is beta, dgamma 0 and dx = r (w - mean w). The mean of w is off by K 2^-24 of
+    the mean |w|, w and the difference by a step each, r by 2^-22 (rsqrtf) and the
+    rounding of eps."""
+    if abs(value) * cols > 2.0 ** 127:
+        cols = 64
+    x = torch.full((rows, cols), value, device=dev)
+    _, dy, gamma, beta = inputs(dev, rows, cols, torch.float32)
+    y, saved = kt_ops.layernorm_train(x, gamma, beta, ckpt8=ckpt8, lib=lib)
+    assert torch.equal(saved.mean, x[:, 0]) and torch.equal(y, beta.expand(rows, cols))
+    dx, dgamma, dbeta = kt_ops.layernorm_bwd(dy, saved, lib=lib)
+    assert dgamma.eq(0).all()
+    w = dy.double() * gamma.double()
+    r = 1e-5 ** -0.5
+    want = r * (w - w.mean(1, keepdim=True))
+    K = 64 + cols / 128
+    tol = E * r * (2 * w.abs() + K * w.abs().mean(1, keepdim=True)) + 8 * E * want.abs()
+    assert bool(((dx.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("ckpt8", [False, True])
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("rows,cols", [(3, 16387), (700, 16387), (70, 20000), (300, 1000), (50, 1023), (9, 8192)])
 def test_gradient_of_the_input_in_place(dev, lib, rows, cols, t, ckpt8):
