@@ -10,6 +10,7 @@ There is no CPU or torch fallback: a missing library raises.
 
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple, Optional
 
@@ -229,6 +230,12 @@ def layernorm_train(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta:
     return y, LayerNormSaved(None if ckpt8 else x, q8, q8_exp, gamma, stats, beta_dtype)
 
 
+@functools.lru_cache(maxsize=1024)
+def _ln_workspace(lib: kt_lib.KtLibrary, rows: int, cols: int) -> int:
+    """The workspace's size, a pure function of the shape; a call into the library takes 1 us."""
+    return lib.layernorm_bwd_workspace_bytes(rows, cols)
+
+
 def layernorm_bwd(dy: torch.Tensor, saved: LayerNormSaved, weight_grads: bool = True,
                   lib: Optional[kt_lib.KtLibrary] = None
                   ) -> tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
@@ -246,29 +253,27 @@ def layernorm_bwd(dy: torch.Tensor, saved: LayerNormSaved, weight_grads: bool = 
     ld_q8 = 0
     if x is None:
         ld_q8 = q8.stride(0) if rows > 1 else max(q8.stride(0), cols)
-        if q8.dtype is not torch.int8 or q8.get_device() != dev or (cols > 1 and q8.stride(1) != 1) or ld_q8 < cols:
+        if not (q8.dtype is torch.int8 and q8.get_device() == dev and (q8.stride(1) == 1 or cols == 1) and ld_q8 >= cols):
             raise ValueError("q8 must be int8 on dy's device, the elements of a row contiguous")
         # the kernels read whole 8 bytes of rows that are a multiple of 8 apart; a copy's last row may end before
         if cols % 8 and ld_q8 % 8 == 0 and q8.untyped_storage().nbytes() < \
                 q8.storage_offset() + (rows - 1) * ld_q8 + (cols + 7) // 8 * 8:
             q8 = q8.contiguous()
             ld_q8 = cols
-        if q8_exp is None or q8_exp.shape != (rows, (cols + 31) // 32):
-            raise ValueError(f"q8_exp must be {(rows, (cols + 31) // 32)}")
-        _dense(q8_exp, "q8_exp", torch.uint8, dev)
+        if q8_exp is None or not (q8_exp.dtype is torch.uint8 and q8_exp.get_device() == dev
+                                  and q8_exp.is_contiguous() and q8_exp.numel() == rows * ((cols + 31) // 32)):
+            raise ValueError(f"q8_exp must be uint8 on dy's device, contiguous and {(rows, (cols + 31) // 32)}")
     else:
         _dense(x, "x", dy.dtype, dev)
-    _dense(stats, "stats", torch.float32, dev)
-    if stats.shape != (2, rows):
-        raise ValueError(f"stats must be {(2, rows)}, got {tuple(stats.shape)}")
+    if not (stats.dtype is torch.float32 and stats.get_device() == dev and stats.is_contiguous()
+            and stats.numel() == 2 * rows):
+        raise ValueError(f"stats must be float32 on dy's device, contiguous and {(2, rows)}")
     wt = gamma.dtype if gamma is not None else beta_dtype or torch.float32
     wdt = _DTYPES.get(wt)
     if wdt not in (kt_lib.KT_F32, dt) or (gamma is not None and beta_dtype not in (None, wt)):
         raise ValueError(f"dy and the weights must be of one type or the weights fp32, got {dy.dtype} and {wt}")
-    if gamma is not None:
-        _dense(gamma, "gamma", wt, dev)
-        if gamma.numel() != cols:
-            raise ValueError(f"layernorm_bwd: gamma must have {cols} elements")
+    if gamma is not None and not (gamma.get_device() == dev and gamma.is_contiguous() and gamma.numel() == cols):
+        raise ValueError(f"gamma must be on dy's device, contiguous and have {cols} elements")
     if lib is None:
         lib = kt_lib.load()
     dx = torch.empty_like(dy)
@@ -276,9 +281,10 @@ def layernorm_bwd(dy: torch.Tensor, saved: LayerNormSaved, weight_grads: bool = 
     ws_bytes = 0
     if weight_grads and (gamma is not None or beta_dtype is not None):
         dgamma = torch.empty_like(gamma) if gamma is not None else None
-        dbeta = dy.new_empty(cols, dtype=wt) if beta_dtype is not None else None
-        ws_bytes = lib.layernorm_bwd_workspace_bytes(rows, cols)
-        ws = dy.new_empty(ws_bytes, dtype=torch.uint8)
+        if beta_dtype is not None:
+            dbeta = torch.empty_like(gamma) if gamma is not None and gamma.dim() == 1 else dy.new_empty(cols, dtype=wt)
+        ws_bytes = _ln_workspace(lib, rows, cols)
+        ws = stats.new_empty(ws_bytes // 4)
     at = stats.data_ptr()
     _launch(dev, lib.layernorm_train_bwd, dy.data_ptr(), _ptr(x), _ptr(q8), _ptr(q8_exp), ld_q8, _ptr(gamma), at,
             at + 4 * rows, dx.data_ptr(), _ptr(dgamma), _ptr(dbeta), rows, cols, dt, wdt, _ptr(ws), ws_bytes)
