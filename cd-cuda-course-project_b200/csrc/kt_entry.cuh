@@ -255,7 +255,20 @@ int kt_token_logprobs(const void* logits, int64_t ld, const int64_t* targets, in
   kt::clear_error();
 #if KT_WITH_LM
   return kt::logprob::forward({logits, ld, targets, rows, vocab, ignore_index, scale, top_k, logprob, entropy, lse,
-                               top_logprob, top_index}, dtype, stream);
+                               nullptr, top_logprob, top_index}, dtype, stream);
+#else
+  return kt::unsupported("token log probabilities");
+#endif
+}
+
+int kt_token_logprobs_train(const void* logits, int64_t ld, const int64_t* targets, int64_t rows, int64_t vocab,
+                            float scale, int64_t ignore_index, int top_k, float* logprob, float* entropy, float* lse,
+                            float* norm, float* top_logprob, int64_t* top_index, int dtype, kt_stream_t stream) {
+  kt::clear_error();
+#if KT_WITH_LM
+  if (norm == nullptr && rows > 0) return kt::fail(KT_ERR_ARG, "token_logprobs_train: null pointer");
+  return kt::logprob::forward({logits, ld, targets, rows, vocab, ignore_index, scale, top_k, logprob, entropy, lse,
+                               reinterpret_cast<float2*>(norm), top_logprob, top_index}, dtype, stream);
 #else
   return kt::unsupported("token log probabilities");
 #endif
@@ -267,8 +280,23 @@ int kt_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* targets
                           int dtype, kt_stream_t stream) {
   kt::clear_error();
 #if KT_WITH_LM
-  return kt::logprob::backward({logits, ld, targets, lse, entropy, grad_logprob, grad_entropy, rows, vocab,
+  return kt::logprob::backward({logits, ld, targets, nullptr, lse, entropy, grad_logprob, grad_entropy, rows, vocab,
                                 ignore_index, scale, dlogits, ld_dlogits, 0}, dtype, stream);
+#else
+  return kt::unsupported("token log probabilities");
+#endif
+}
+
+int kt_token_logprobs_train_bwd(const void* logits, int64_t ld, const int64_t* targets, const float* norm,
+                                const float* entropy, const float* grad_logprob, const float* grad_entropy,
+                                int64_t rows, int64_t vocab, float scale, int64_t ignore_index, void* dlogits,
+                                int64_t ld_dlogits, int dtype, kt_stream_t stream) {
+  kt::clear_error();
+#if KT_WITH_LM
+  if (norm == nullptr && rows > 0) return kt::fail(KT_ERR_ARG, "token_logprobs_train_bwd: null pointer");
+  return kt::logprob::backward({logits, ld, targets, reinterpret_cast<const float2*>(norm), nullptr, entropy,
+                                grad_logprob, grad_entropy, rows, vocab, ignore_index, scale, dlogits, ld_dlogits, 0},
+                               dtype, stream);
 #else
   return kt::unsupported("token log probabilities");
 #endif

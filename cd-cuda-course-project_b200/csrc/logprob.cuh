@@ -8,6 +8,11 @@
 // A row of only -inf has no distribution: lse and every log probability are
 // -inf, its entropy and its gradient 0. A NaN or +inf makes the row NaN.
 //
+// The gradient takes z - lse from the row's norm, its maximum m and log2 of s
+// (below), as (x - m) scale log2 e - log2 s: off by 2^-24 of |z - m| and of log s.
+// From lse, one rounded number, it would be off by 2^-24 |lse|, which is 4e-3 at a
+// common offset of 1e5, and everything for a row of the type's lowest value.
+//
 // Forward reads the logits once: every thread keeps a running maximum m of x,
 // s = sum 2^y and t = sum y 2^y with y = (x - m) scale log2 e, and rescales them
 // when its maximum grows, so H = ln 2 (log2 s - t / s) needs no second pass.
@@ -71,6 +76,7 @@ struct FwdArgs {
   float* logprob;
   float* entropy;
   float* lse;
+  float2* norm;  // may be null
   float* top_logprob;
   int64_t* top_index;
 };
@@ -79,6 +85,7 @@ struct BwdArgs {
   const void* x;
   int64_t ld;
   const int64_t* targets;
+  const float2* norm;  // or, where null,
   const float* lse;
   const float* entropy;
   const float* g;  // may be null: 0
@@ -405,6 +412,7 @@ __device__ __forceinline__ void write_row(const FwdArgs& p, int64_t row, const S
   auto log_p = [&](float x) { return none ? -INFINITY : fmaf(-log2s, kLn2, (x - a.m) * p.scale); };
   if (lane == 0) {
     p.lse[row] = none ? -INFINITY : fmaf(log2s, kLn2, a.m * p.scale);
+    if (p.norm) p.norm[row] = make_float2(a.m, log2s);
     if (p.entropy) p.entropy[row] = none ? 0.f : (log2s - a.t / a.s) * kLn2;
     if (p.targets) {
       float v = target.is_column ? log_p(target.x) : 0.f;
@@ -582,18 +590,32 @@ __global__ void __launch_bounds__(kBwdBlock) bwd_kernel(const BwdArgs p) {
   T* dr = static_cast<T*>(p.dx) + row * p.ld_dx;
   const int shift = VECTOR ? elem::misalign<T>(xr) : 0;
   const int64_t target = p.targets ? p.targets[row] : p.ignore;
-  const float lse = p.lse[row];
+  // log2 of a probability is fma(fma(x, a, b), c, d); its natural logarithm, from
+  // lse, is the inner one
+  float a = 1.f, b, c = p.scale * kLog2e, d;
+  bool none;  // the row has no distribution
+  if (p.norm) {
+    const float2 n = p.norm[row];
+    b = -n.x;
+    d = -n.y;
+    none = n.x == -INFINITY;
+  } else {
+    a = p.scale;
+    b = -p.lse[row];
+    c = kLog2e;
+    d = 0.f;
+    none = b == INFINITY;
+  }
   const bool scored = target != p.ignore && target >= 0 && target < p.vocab;
   const float g = scored && p.g ? p.g[row] * p.scale : 0.f;
   const float h = p.h ? p.h[row] * p.scale : 0.f;
-  const float entropy = p.h ? p.entropy[row] : 0.f;
   // nothing comes from above, or the row has no distribution: the gradient is 0
-  const bool zero = (g == 0.f && h == 0.f) || lse == -INFINITY;
+  const bool zero = (g == 0.f && h == 0.f) || none;
+  const float each = p.h ? fmaf(h, p.entropy[row], g) : g, by = h * kLn2;
   auto grad = [&](float x, int64_t e) {
-    const float logp = fmaf(x, p.scale, -lse);
-    const float prob = ex2(logp * kLog2e);
-    const float d = -prob * fmaf(h, fmaxf(logp, -1e4f) + entropy, g);  // p = 0: 0, not NaN
-    return e == target ? d + g : d;
+    const float y = fmaf(fmaf(x, a, b), c, d);
+    const float v = -ex2(y) * fmaf(by, fmaxf(y, -1e4f), each);  // p = 0: 0, not NaN
+    return e == target ? v + g : v;
   };
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
@@ -679,7 +701,7 @@ inline int forward(const FwdArgs& a, int dtype, cudaStream_t st) {
   if (!a.x || !a.lse || (a.targets && !a.logprob) || (a.top > 0 && (!a.top_logprob || !a.top_index)))
     return fail(KT_ERR_ARG, "token_logprobs: null pointer");
   if (!elem::aligned_to(a.x, elem::size_of(dtype)) || !elem::aligned_to(a.targets, 8) ||
-      !elem::aligned_to(a.top_index, 8))
+      !elem::aligned_to(a.top_index, 8) || !elem::aligned_to(a.norm, 8))
     return fail(KT_ERR_ARG, "token_logprobs: a pointer is not aligned to its elements");
   const bool top = a.top > 0;
   if (dtype == KT_F32) return top ? fwd_typed<float, true>(a, st) : fwd_typed<float, false>(a, st);
@@ -706,10 +728,11 @@ inline int backward(const BwdArgs& a, int dtype, cudaStream_t st) {
   if (rc != KT_OK) return rc;
   if (a.rows == 0) return KT_OK;
   if (a.ld_dx < a.vocab) return fail(KT_ERR_ARG, "token_logprobs_bwd: rows of the gradient overlap");
-  if (!a.x || !a.lse || !a.dx || (a.g && !a.targets) || (a.h && !a.entropy))
+  if (!a.x || (!a.norm && !a.lse) || !a.dx || (a.g && !a.targets) || (a.h && !a.entropy))
     return fail(KT_ERR_ARG, "token_logprobs_bwd: null pointer");
   const int sz = elem::size_of(dtype);
-  if (!elem::aligned_to(a.x, sz) || !elem::aligned_to(a.dx, sz) || !elem::aligned_to(a.targets, 8))
+  if (!elem::aligned_to(a.x, sz) || !elem::aligned_to(a.dx, sz) || !elem::aligned_to(a.targets, 8) ||
+      !elem::aligned_to(a.norm, 8))
     return fail(KT_ERR_ARG, "token_logprobs_bwd: a pointer is not aligned to its elements");
   if (dtype == KT_F32) return bwd_typed<float>(a, st);
   if (dtype == KT_BF16) return bwd_typed<__nv_bfloat16>(a, st);

@@ -65,7 +65,8 @@ EXPORTED_SYMBOLS = (
     "kt_reduce_sum_f32_xrank",
     "kt_gemm_f32", "kt_fa_fwd_bf16",
     "kt_layernorm_train_fwd", "kt_layernorm_bwd_workspace_bytes", "kt_layernorm_train_bwd",
-    "kt_token_logprobs", "kt_token_logprobs_bwd", "kt_w4_quantize", "kt_w4_linear",
+    "kt_token_logprobs", "kt_token_logprobs_train", "kt_token_logprobs_train_bwd", "kt_token_logprobs_bwd",
+    "kt_w4_quantize", "kt_w4_linear",
     "kt_naive_softmax_f32", "kt_naive_layernorm_f32", "kt_naive_reduce_sum_f32",
     "kt_naive_gemm_f32", "kt_naive_attention_bf16",
     "kt_run", "kt_time", "kt_device_error",
@@ -126,6 +127,8 @@ _SIGNATURES = {
     "kt_layernorm_bwd_workspace_bytes": (_size, [_i64, _i64]),
     "kt_layernorm_train_bwd": (_int, [_vp] * 4 + [_i64] + [_vp] * 6 + [_i64, _i64, _int, _int, _vp, _size, _vp]),
     "kt_token_logprobs": (_int, [_vp, _i64, _vp, _i64, _i64, _f32, _i64, _int, _vp, _vp, _vp, _vp, _vp, _int, _vp]),
+    "kt_token_logprobs_train": (_int, [_vp, _i64, _vp, _i64, _i64, _f32, _i64, _int] + [_vp] * 6 + [_int, _vp]),
+    "kt_token_logprobs_train_bwd": (_int, [_vp, _i64] + [_vp] * 5 + [_i64, _i64, _f32, _i64, _vp, _i64, _int, _vp]),
     "kt_token_logprobs_bwd": (_int, [_vp, _i64] + [_vp] * 5 + [_i64, _i64, _f32, _i64, _vp, _i64, _int, _vp]),
     "kt_w4_quantize": (_int, [_vp, _i64, _i64, _int, _int, _vp, _vp, _int, _vp]),
     "kt_w4_linear": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _vp]),
@@ -239,6 +242,22 @@ class KtLibrary:
         self._check(self._lib.kt_token_logprobs(logits, ld, targets, rows, vocab, scale, ignore_index, top_k, logprob,
                                                 entropy, lse, top_logprob, top_index, dtype, stream),
                     "kt_token_logprobs")
+
+    def token_logprobs_train(self, logits: int, ld: int, targets: Optional[int], rows: int, vocab: int, scale: float,
+                             ignore_index: int, top_k: int, logprob: Optional[int], entropy: Optional[int], lse: int,
+                             norm: int, top_logprob: Optional[int], top_index: Optional[int], dtype: int,
+                             stream: Optional[int] = None) -> None:
+        self._check(self._lib.kt_token_logprobs_train(logits, ld, targets, rows, vocab, scale, ignore_index, top_k,
+                                                      logprob, entropy, lse, norm, top_logprob, top_index, dtype,
+                                                      stream), "kt_token_logprobs_train")
+
+    def token_logprobs_train_bwd(self, logits: int, ld: int, targets: Optional[int], norm: int,
+                                 entropy: Optional[int], grad_logprob: Optional[int], grad_entropy: Optional[int],
+                                 rows: int, vocab: int, scale: float, ignore_index: int, dlogits: int, ld_dlogits: int,
+                                 dtype: int, stream: Optional[int] = None) -> None:
+        self._check(self._lib.kt_token_logprobs_train_bwd(logits, ld, targets, norm, entropy, grad_logprob,
+                                                          grad_entropy, rows, vocab, scale, ignore_index, dlogits,
+                                                          ld_dlogits, dtype, stream), "kt_token_logprobs_train_bwd")
 
     def token_logprobs_bwd(self, logits: int, ld: int, targets: Optional[int], lse: int, entropy: Optional[int],
                            grad_logprob: Optional[int], grad_entropy: Optional[int], rows: int, vocab: int,

@@ -150,7 +150,7 @@ def _rows(t: torch.Tensor, name: str) -> int:
 
 def _launch(device: int, fn, *args) -> None:
     """fn(*args, stream) on that device and its current stream."""
-    if device == torch.cuda.current_device():
+    if device == torch._C._cuda_getDevice():  # (torch.cuda.current_device takes twice as long)
         fn(*args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
@@ -291,9 +291,7 @@ def layernorm_bwd(dy: torch.Tensor, saved: LayerNormSaved, weight_grads: bool = 
     return dx, dgamma, dbeta
 
 
-class TokenLogprobs(NamedTuple):
-    """Per row of logits: the target's log probability (None without targets),
-    the entropy (nats), log sum exp, and the top k log probabilities with their columns (int64)."""
+class _TokenLogprobs(NamedTuple):
     logprob: Optional[torch.Tensor]
     entropy: torch.Tensor
     lse: torch.Tensor
@@ -301,9 +299,19 @@ class TokenLogprobs(NamedTuple):
     top_index: torch.Tensor
 
 
+class TokenLogprobs(_TokenLogprobs):
+    """Per row of logits: the target's log probability (None without targets),
+    the entropy (nats), log sum exp, and the top k log probabilities with their columns (int64).
+
+    Beside these five, token_logprobs' result has `norm`, (rows, 2) fp32: what
+    the gradient takes in lse's place, which is rounded (include/kt_abi.h)."""
+    norm: Optional[torch.Tensor] = None
+
+
 def _per_row(t: torch.Tensor, name: str, dtype: torch.dtype, rows: int, device: int) -> None:
-    _dense(t, name, dtype, device)
-    if t.dim() != 1 or t.shape[0] != rows:
+    if not (t.dtype is dtype and t.get_device() == device and t.dim() == 1 and t.numel() == rows
+            and t.is_contiguous()):
+        _dense(t, name, dtype, device)
         raise ValueError(f"{name} must be ({rows},), got {tuple(t.shape)}")
 
 
@@ -326,14 +334,22 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
         raise ValueError(f"top_k must be between 0 and min(32, vocab), got {top_k}")
     if lib is None:
         lib = kt_lib.load()
-    logprob = logits.new_empty(rows, dtype=torch.float32) if targets is not None else None
     entropy = logits.new_empty(rows, dtype=torch.float32)
+    logprob = torch.empty_like(entropy) if targets is not None else None
     lse = torch.empty_like(entropy)
-    top_logprob = logits.new_empty((rows, top_k), dtype=torch.float32)
-    top_index = logits.new_empty((rows, top_k), dtype=torch.int64)
-    _launch(dev, lib.token_logprobs, logits.data_ptr(), ld, _ptr(targets), rows, vocab, scale, ignore_index, top_k,
-            _ptr(logprob), entropy.data_ptr(), lse.data_ptr(), top_logprob.data_ptr(), top_index.data_ptr(), dt)
-    return TokenLogprobs(logprob, entropy, lse, top_logprob, top_index)
+    # (sizes one by one, and a tensor of the right type to start from, take a third less time)
+    norm = entropy.new_empty(rows, 2)
+    top_logprob = entropy.new_empty(rows, top_k)
+    if targets is not None:
+        top_index = targets.new_empty(rows, top_k)
+    else:
+        top_index = logits.new_empty(rows, top_k, dtype=torch.int64)
+    _launch(dev, lib.token_logprobs_train, logits.data_ptr(), ld, _ptr(targets), rows, vocab, scale, ignore_index,
+            top_k, _ptr(logprob), entropy.data_ptr(), lse.data_ptr(), norm.data_ptr(), top_logprob.data_ptr(),
+            top_index.data_ptr(), dt)
+    result = tuple.__new__(TokenLogprobs, (logprob, entropy, lse, top_logprob, top_index))
+    result.norm = norm
+    return result
 
 
 def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], result: TokenLogprobs,
@@ -342,12 +358,12 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], re
                        lib: Optional[kt_lib.KtLibrary] = None) -> torch.Tensor:
     """Gradient of the logits from those of the log probabilities and the
     entropies (fp32, (rows,); None: 0); result, scale and ignore_index are those
-    of token_logprobs. `out` may be the logits themselves, not a part of their memory."""
+    of token_logprobs. `out` may be the logits themselves, not a part of their memory.
+    A result without its norm (put together anew) has it computed again from the logits."""
     dt = _dtype(logits, "logits")
     ld = _rows(logits, "logits")
     rows, vocab = logits.shape
     dev = logits.get_device()
-    _per_row(result.lse, "result.lse", torch.float32, rows, dev)
     _per_row(result.entropy, "result.entropy", torch.float32, rows, dev)
     if grad_logprob is not None:
         _per_row(grad_logprob, "grad_logprob", torch.float32, rows, dev)
@@ -372,7 +388,13 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], re
             raise ValueError("out overlaps the logits without being the same")
     if lib is None:
         lib = kt_lib.load()
-    _launch(dev, lib.token_logprobs_bwd, logits.data_ptr(), ld, _ptr(targets), result.lse.data_ptr(),
+    norm = result.norm
+    if norm is None:
+        norm = token_logprobs(logits, scale=scale, lib=lib).norm
+    _dense(norm, "result.norm", torch.float32, dev)
+    if norm.numel() != 2 * rows:
+        raise ValueError(f"result.norm must be {(rows, 2)}, got {tuple(norm.shape)}")
+    _launch(dev, lib.token_logprobs_train_bwd, logits.data_ptr(), ld, _ptr(targets), norm.data_ptr(),
             result.entropy.data_ptr(), _ptr(grad_logprob), _ptr(grad_entropy), rows, vocab, scale, ignore_index,
             out.data_ptr(), ld_out, dt)
     return out

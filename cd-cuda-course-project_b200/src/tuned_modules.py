@@ -25,7 +25,7 @@ calls it through the C ABI on the current CUDA stream:
                           tokens (kt_w4_linear), made from an nn.Linear
   token_log_probs         log probabilities of given tokens, entropies and top
                           alternatives of logits, with their gradient
-                          (kt_token_logprobs / _bwd)
+                          (kt_token_logprobs_train / _train_bwd)
 
 The linear and attention layers are inference layers (they have forward
 kernels only): a call with autograd recording raises instead of silently
@@ -191,7 +191,7 @@ class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, top_k, scale, ignore_index):
         r = kt_ops.token_logprobs(logits, targets, top_k, scale, ignore_index)
-        ctx.save_for_backward(logits, targets, r.entropy, r.lse)
+        ctx.save_for_backward(logits, targets, r.entropy, r.norm)
         ctx.scale, ctx.ignore_index = scale, ignore_index
         ctx.mark_non_differentiable(r.lse, r.top_logprob, r.top_index)
         ctx.set_materialize_grads(False)
@@ -200,11 +200,12 @@ class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_logprob, grad_entropy, *_):
-        logits, targets, entropy, lse = ctx.saved_tensors
+        logits, targets, entropy, norm = ctx.saved_tensors
         if grad_logprob is None and grad_entropy is None:
             return None, None, None, None, None
         grads = [g.contiguous() if g is not None else None for g in (grad_logprob, grad_entropy)]
-        r = kt_ops.TokenLogprobs(None, entropy, lse, None, None)
+        r = kt_ops.TokenLogprobs(None, entropy, None, None, None)
+        r.norm = norm
         dx = kt_ops.token_logprobs_bwd(logits, targets, r, *grads, scale=ctx.scale, ignore_index=ctx.ignore_index)
         return dx, None, None, None, None
 

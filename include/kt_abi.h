@@ -243,10 +243,25 @@ KT_API int kt_token_logprobs(const void* logits, int64_t ld, const int64_t* targ
                              float scale, int64_t ignore_index, int top_k, float* logprob, float* entropy, float* lse,
                              float* top_logprob, int64_t* top_index, int dtype, kt_stream_t stream);
 
+/* The same for training: leaves the rows' norms too (rows x 2 fp32, 8-byte
+ * aligned: the largest logit, and log2 of the sum of exponentials from there). */
+KT_API int kt_token_logprobs_train(const void* logits, int64_t ld, const int64_t* targets, int64_t rows, int64_t vocab,
+                                   float scale, int64_t ignore_index, int top_k, float* logprob, float* entropy,
+                                   float* lse, float* norm, float* top_logprob, int64_t* top_index, int dtype,
+                                   kt_stream_t stream);
+
 /* Gradient of the logits from those of logprob and entropy (either may be
- * NULL: 0); lse and entropy are kt_token_logprobs'. Rows whose two gradients
- * are 0, and rows of only -inf, get 0. dlogits (rows `ld_dlogits` apart) may be
- * the logits themselves. */
+ * NULL: 0); norm and entropy are kt_token_logprobs_train's. Rows whose two
+ * gradients are 0, and rows of only -inf, get 0. dlogits (rows `ld_dlogits`
+ * apart) may be the logits themselves. */
+KT_API int kt_token_logprobs_train_bwd(const void* logits, int64_t ld, const int64_t* targets, const float* norm,
+                                       const float* entropy, const float* grad_logprob, const float* grad_entropy,
+                                       int64_t rows, int64_t vocab, float scale, int64_t ignore_index, void* dlogits,
+                                       int64_t ld_dlogits, int dtype, kt_stream_t stream);
+
+/* The same from lse, kt_token_logprobs', in norm's place. lse is one rounded
+ * number: each probability is off by 2^-24 |lse| of itself, and where lse is not
+ * finite, but for rows of only -inf, there is no gradient. For logits near 0 only. */
 KT_API int kt_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* targets, const float* lse,
                                  const float* entropy, const float* grad_logprob, const float* grad_entropy,
                                  int64_t rows, int64_t vocab, float scale, int64_t ignore_index, void* dlogits,

@@ -2,7 +2,7 @@
 The backward pass of LayerNorm takes what it reads from the tensors that the
 forward pass left, so it refuses those that are not on dy's device, or whose type
 or size is not what the forward pass leaves. Both refuse an output that shares a
-part of an input's memory.
+part of an input's memory. The same for what token log probabilities leave.
 """
 
 from __future__ import annotations
@@ -65,6 +65,25 @@ def test_outputs_that_overlap_a_part_of_an_input_are_refused(lib):
         refused(lambda: ln_bwd(lib, dx=P + 2 * size, x=P + 2 * size + shift))
         refused(lambda: ln_bwd(lib, x=None, q8=P, q8_exp=P, dx=P + shift))
         refused(lambda: ln_fwd(lib, y=P + shift // 2, dtype=kt_lib.KT_BF16, wdtype=kt_lib.KT_BF16))
+
+
+def train(lib, norm=P, logits=P, lse=P, rows=4, vocab=100, scale=1.0, top_k=0, targets=P, logprob=P):
+    lib.token_logprobs_train(logits, vocab, targets, rows, vocab, scale, -100, top_k, logprob, P, lse, norm, None, None, 0)
+
+
+def train_bwd(lib, norm=P, logits=P, dx=P, rows=4, vocab=100, scale=1.0, targets=P, entropy=P, ld_dx=100):
+    lib.token_logprobs_train_bwd(logits, vocab, targets, norm, entropy, P, P, rows, vocab, scale, -100, dx, ld_dx, 0)
+
+
+def test_token_logprobs_for_training_refuse(lib):
+    for bad in (dict(norm=None), dict(norm=P + 4), dict(logits=0), dict(lse=0), dict(rows=-1), dict(scale=0.0),
+                dict(top_k=2), dict(logprob=None)):
+        refused(lambda: train(lib, **bad))
+    for bad in (dict(norm=None), dict(norm=P + 4), dict(logits=0), dict(dx=0), dict(rows=-1), dict(scale=0.0),
+                dict(targets=None), dict(entropy=None), dict(ld_dx=99)):
+        refused(lambda: train_bwd(lib, **bad))
+    train(lib, norm=None, logits=0, rows=0)
+    train_bwd(lib, norm=None, logits=0, rows=0)
 
 
 class Recorder:
