@@ -607,7 +607,8 @@ __global__ void __launch_bounds__(kBwdBlock) bwd_kernel(const BwdArgs p) {
     none = b == INFINITY;
   }
   const bool scored = target != p.ignore && target >= 0 && target < p.vocab;
-  const float g = scored && p.g ? p.g[row] * p.scale : 0.f;
+  float g = p.g && target != p.ignore ? p.g[row] * p.scale : 0.f;
+  if (!scored && g != 0.f) g = __uint_as_float(0x7FC00000u);  // of a target that is no column: NaN, as its value
   const float h = p.h ? p.h[row] * p.scale : 0.f;
   // nothing comes from above, or the row has no distribution: the gradient is 0
   const bool zero = (g == 0.f && h == 0.f) || none;

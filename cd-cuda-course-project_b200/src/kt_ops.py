@@ -322,7 +322,8 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
 
     logits: (rows, vocab) fp32, bf16 or fp16, rows any distance apart; targets:
     (rows,) int64. Rows whose target is ignore_index get log probability 0;
-    other targets that are no column get NaN and set the library's device error.
+    other targets that are no column get NaN, in the gradient too, and set the
+    library's device error.
     """
     dt = _dtype(logits, "logits")
     ld = _rows(logits, "logits")

@@ -252,7 +252,8 @@ KT_API int kt_token_logprobs_train(const void* logits, int64_t ld, const int64_t
 
 /* Gradient of the logits from those of logprob and entropy (either may be
  * NULL: 0); norm and entropy are kt_token_logprobs_train's. Rows whose two
- * gradients are 0, and rows of only -inf, get 0. dlogits (rows `ld_dlogits`
+ * gradients are 0, and rows of only -inf, get 0; rows whose target is no column
+ * get NaN where logprob has a gradient other than 0. dlogits (rows `ld_dlogits`
  * apart) may be the logits themselves. */
 KT_API int kt_token_logprobs_train_bwd(const void* logits, int64_t ld, const int64_t* targets, const float* norm,
                                        const float* entropy, const float* grad_logprob, const float* grad_entropy,
