@@ -280,8 +280,8 @@ int kt_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* targets
                           int dtype, kt_stream_t stream) {
   kt::clear_error();
 #if KT_WITH_LM
-  return kt::logprob::backward({logits, ld, targets, nullptr, lse, entropy, grad_logprob, grad_entropy, rows, vocab,
-                                ignore_index, scale, dlogits, ld_dlogits, 0}, dtype, stream);
+  return kt::logprob::backward({logits, ld, targets, nullptr, lse, entropy, grad_logprob, grad_entropy, nullptr, rows,
+                                vocab, ignore_index, scale, dlogits, ld_dlogits, 0}, dtype, stream);
 #else
   return kt::unsupported("token log probabilities");
 #endif
@@ -289,14 +289,14 @@ int kt_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* targets
 
 int kt_token_logprobs_train_bwd(const void* logits, int64_t ld, const int64_t* targets, const float* norm,
                                 const float* entropy, const float* grad_logprob, const float* grad_entropy,
-                                int64_t rows, int64_t vocab, float scale, int64_t ignore_index, void* dlogits,
-                                int64_t ld_dlogits, int dtype, kt_stream_t stream) {
+                                const float* grad_lse, int64_t rows, int64_t vocab, float scale, int64_t ignore_index,
+                                void* dlogits, int64_t ld_dlogits, int dtype, kt_stream_t stream) {
   kt::clear_error();
 #if KT_WITH_LM
   if (norm == nullptr && rows > 0) return kt::fail(KT_ERR_ARG, "token_logprobs_train_bwd: null pointer");
   return kt::logprob::backward({logits, ld, targets, reinterpret_cast<const float2*>(norm), nullptr, entropy,
-                                grad_logprob, grad_entropy, rows, vocab, ignore_index, scale, dlogits, ld_dlogits, 0},
-                               dtype, stream);
+                                grad_logprob, grad_entropy, grad_lse, rows, vocab, ignore_index, scale, dlogits,
+                                ld_dlogits, 0}, dtype, stream);
 #else
   return kt::unsupported("token log probabilities");
 #endif

@@ -3,8 +3,8 @@
 //
 // With z = scale x over the V columns of a row (fp32 throughout):
 //   lse = log sum e^z      logprob = z[target] - lse      H = lse - sum p z
-//   gradient, for upstream g (logprob) and h (entropy):
-//   dx_j = scale (g ([j = target] - p_j) - h p_j (log p_j + H)),  p_j = e^(z_j - lse)
+//   gradient, for upstream g (logprob), h (entropy) and l (lse):
+//   dx_j = scale (g ([j = target] - p_j) - h p_j (log p_j + H) + l p_j),  p_j = e^(z_j - lse)
 // A row of only -inf has no distribution: lse and every log probability are
 // -inf, its entropy and its gradient 0. A NaN or +inf makes the row NaN.
 //
@@ -90,6 +90,7 @@ struct BwdArgs {
   const float* entropy;
   const float* g;  // may be null: 0
   const float* h;  // may be null: 0
+  const float* l;  // may be null: 0
   int64_t rows;
   int64_t vocab;
   int64_t ignore;
@@ -610,9 +611,10 @@ __global__ void __launch_bounds__(kBwdBlock) bwd_kernel(const BwdArgs p) {
   float g = p.g && target != p.ignore ? p.g[row] * p.scale : 0.f;
   if (!scored && g != 0.f) g = __uint_as_float(0x7FC00000u);  // of a target that is no column: NaN, as its value
   const float h = p.h ? p.h[row] * p.scale : 0.f;
+  const float l = p.l ? p.l[row] * p.scale : 0.f;
   // nothing comes from above, or the row has no distribution: the gradient is 0
-  const bool zero = (g == 0.f && h == 0.f) || none;
-  const float each = p.h ? fmaf(h, p.entropy[row], g) : g, by = h * kLn2;
+  const bool zero = (g == 0.f && h == 0.f && l == 0.f) || none;
+  const float each = p.h ? fmaf(h, p.entropy[row], g - l) : g - l, by = h * kLn2;
   auto grad = [&](float x, int64_t e) {
     const float y = fmaf(fmaf(x, a, b), c, d);
     const float v = -ex2(y) * fmaf(by, fmaxf(y, -1e4f), each);  // p = 0: 0, not NaN

@@ -128,7 +128,7 @@ _SIGNATURES = {
     "kt_layernorm_train_bwd": (_int, [_vp] * 4 + [_i64] + [_vp] * 6 + [_i64, _i64, _int, _int, _vp, _size, _vp]),
     "kt_token_logprobs": (_int, [_vp, _i64, _vp, _i64, _i64, _f32, _i64, _int, _vp, _vp, _vp, _vp, _vp, _int, _vp]),
     "kt_token_logprobs_train": (_int, [_vp, _i64, _vp, _i64, _i64, _f32, _i64, _int] + [_vp] * 6 + [_int, _vp]),
-    "kt_token_logprobs_train_bwd": (_int, [_vp, _i64] + [_vp] * 5 + [_i64, _i64, _f32, _i64, _vp, _i64, _int, _vp]),
+    "kt_token_logprobs_train_bwd": (_int, [_vp, _i64] + [_vp] * 6 + [_i64, _i64, _f32, _i64, _vp, _i64, _int, _vp]),
     "kt_token_logprobs_bwd": (_int, [_vp, _i64] + [_vp] * 5 + [_i64, _i64, _f32, _i64, _vp, _i64, _int, _vp]),
     "kt_w4_quantize": (_int, [_vp, _i64, _i64, _int, _int, _vp, _vp, _int, _vp]),
     "kt_w4_linear": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _int, _int, _vp]),
@@ -253,11 +253,12 @@ class KtLibrary:
 
     def token_logprobs_train_bwd(self, logits: int, ld: int, targets: Optional[int], norm: int,
                                  entropy: Optional[int], grad_logprob: Optional[int], grad_entropy: Optional[int],
-                                 rows: int, vocab: int, scale: float, ignore_index: int, dlogits: int, ld_dlogits: int,
-                                 dtype: int, stream: Optional[int] = None) -> None:
+                                 grad_lse: Optional[int], rows: int, vocab: int, scale: float, ignore_index: int,
+                                 dlogits: int, ld_dlogits: int, dtype: int, stream: Optional[int] = None) -> None:
         self._check(self._lib.kt_token_logprobs_train_bwd(logits, ld, targets, norm, entropy, grad_logprob,
-                                                          grad_entropy, rows, vocab, scale, ignore_index, dlogits,
-                                                          ld_dlogits, dtype, stream), "kt_token_logprobs_train_bwd")
+                                                          grad_entropy, grad_lse, rows, vocab, scale, ignore_index,
+                                                          dlogits, ld_dlogits, dtype, stream),
+                    "kt_token_logprobs_train_bwd")
 
     def token_logprobs_bwd(self, logits: int, ld: int, targets: Optional[int], lse: int, entropy: Optional[int],
                            grad_logprob: Optional[int], grad_entropy: Optional[int], rows: int, vocab: int,

@@ -356,9 +356,10 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
 def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], result: TokenLogprobs,
                        grad_logprob: Optional[torch.Tensor] = None, grad_entropy: Optional[torch.Tensor] = None,
                        scale: float = 1.0, ignore_index: int = -100, out: Optional[torch.Tensor] = None,
-                       lib: Optional[kt_lib.KtLibrary] = None) -> torch.Tensor:
-    """Gradient of the logits from those of the log probabilities and the
-    entropies (fp32, (rows,); None: 0); result, scale and ignore_index are those
+                       lib: Optional[kt_lib.KtLibrary] = None,
+                       grad_lse: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of the logits from those of the log probabilities, the entropies
+    and lse (fp32, (rows,); None: 0); result, scale and ignore_index are those
     of token_logprobs. `out` may be the logits themselves, not a part of their memory.
     A result without its norm (put together anew) has it computed again from the logits."""
     dt = _dtype(logits, "logits")
@@ -372,6 +373,8 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], re
             raise ValueError("grad_logprob needs targets")
     if grad_entropy is not None:
         _per_row(grad_entropy, "grad_entropy", torch.float32, rows, dev)
+    if grad_lse is not None:
+        _per_row(grad_lse, "grad_lse", torch.float32, rows, dev)
     if targets is not None:
         _per_row(targets, "targets", torch.int64, rows, dev)
     if out is None:
@@ -396,7 +399,7 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], re
     if norm.numel() != 2 * rows:
         raise ValueError(f"result.norm must be {(rows, 2)}, got {tuple(norm.shape)}")
     _launch(dev, lib.token_logprobs_train_bwd, logits.data_ptr(), ld, _ptr(targets), norm.data_ptr(),
-            result.entropy.data_ptr(), _ptr(grad_logprob), _ptr(grad_entropy), rows, vocab, scale, ignore_index,
+            result.entropy.data_ptr(), _ptr(grad_logprob), _ptr(grad_entropy), _ptr(grad_lse), rows, vocab, scale, ignore_index,
             out.data_ptr(), ld_out, dt)
     return out
 

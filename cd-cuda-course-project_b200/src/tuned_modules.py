@@ -193,27 +193,29 @@ class _TokenLogProbs(torch.autograd.Function):
         r = kt_ops.token_logprobs(logits, targets, top_k, scale, ignore_index)
         ctx.save_for_backward(logits, targets, r.entropy, r.norm)
         ctx.scale, ctx.ignore_index = scale, ignore_index
-        ctx.mark_non_differentiable(r.lse, r.top_logprob, r.top_index)
+        ctx.mark_non_differentiable(r.top_logprob, r.top_index)
         ctx.set_materialize_grads(False)
         return tuple(r)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_logprob, grad_entropy, *_):
+    def backward(ctx, grad_logprob, grad_entropy, grad_lse, *_):
         logits, targets, entropy, norm = ctx.saved_tensors
-        if grad_logprob is None and grad_entropy is None:
+        grads = [g.contiguous() if g is not None else None for g in (grad_logprob, grad_entropy, grad_lse)]
+        if all(g is None for g in grads):
             return None, None, None, None, None
-        grads = [g.contiguous() if g is not None else None for g in (grad_logprob, grad_entropy)]
         r = kt_ops.TokenLogprobs(None, entropy, None, None, None)
         r.norm = norm
-        dx = kt_ops.token_logprobs_bwd(logits, targets, r, *grads, scale=ctx.scale, ignore_index=ctx.ignore_index)
+        dx = kt_ops.token_logprobs_bwd(logits, targets, r, grads[0], grads[1], ctx.scale, ctx.ignore_index,
+                                       grad_lse=grads[2])
         return dx, None, None, None, None
 
 
 def token_log_probs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top_k: int = 0, scale: float = 1.0,
                     ignore_index: int = -100) -> kt_ops.TokenLogprobs:
     """kt_ops.token_logprobs over the last dimension of logits with any leading
-    dimensions (those of targets), differentiable (once) through logprob and entropy."""
+    dimensions (those of targets), differentiable (once) through logprob, entropy
+    and lse; the top alternatives carry no gradient."""
     lead, vocab = logits.shape[:-1], logits.shape[-1]
     x = logits.reshape(-1, vocab)
     if x.shape[1] > 1 and x.stride(1) != 1:

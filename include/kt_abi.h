@@ -250,17 +250,18 @@ KT_API int kt_token_logprobs_train(const void* logits, int64_t ld, const int64_t
                                    float* lse, float* norm, float* top_logprob, int64_t* top_index, int dtype,
                                    kt_stream_t stream);
 
-/* Gradient of the logits from those of logprob and entropy (either may be
- * NULL: 0); norm and entropy are kt_token_logprobs_train's. Rows whose two
+/* Gradient of the logits from those of logprob, entropy and lse (each may be
+ * NULL: 0); norm and entropy are kt_token_logprobs_train's. Rows whose
  * gradients are 0, and rows of only -inf, get 0; rows whose target is no column
  * get NaN where logprob has a gradient other than 0. dlogits (rows `ld_dlogits`
  * apart) may be the logits themselves. */
 KT_API int kt_token_logprobs_train_bwd(const void* logits, int64_t ld, const int64_t* targets, const float* norm,
                                        const float* entropy, const float* grad_logprob, const float* grad_entropy,
-                                       int64_t rows, int64_t vocab, float scale, int64_t ignore_index, void* dlogits,
-                                       int64_t ld_dlogits, int dtype, kt_stream_t stream);
+                                       const float* grad_lse, int64_t rows, int64_t vocab, float scale,
+                                       int64_t ignore_index, void* dlogits, int64_t ld_dlogits, int dtype,
+                                       kt_stream_t stream);
 
-/* The same from lse, kt_token_logprobs', in norm's place. lse is one rounded
+/* The same from lse, kt_token_logprobs', in norm's place, without lse's gradient. lse is one rounded
  * number: each probability is off by 2^-24 |lse| of itself, and where lse is not
  * finite, but for rows of only -inf, there is no gradient. For logits near 0 only. */
 KT_API int kt_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* targets, const float* lse,

@@ -72,7 +72,7 @@ def train(lib, norm=P, logits=P, lse=P, rows=4, vocab=100, scale=1.0, top_k=0, t
 
 
 def train_bwd(lib, norm=P, logits=P, dx=P, rows=4, vocab=100, scale=1.0, targets=P, entropy=P, ld_dx=100):
-    lib.token_logprobs_train_bwd(logits, vocab, targets, norm, entropy, P, P, rows, vocab, scale, -100, dx, ld_dx, 0)
+    lib.token_logprobs_train_bwd(logits, vocab, targets, norm, entropy, P, P, P, rows, vocab, scale, -100, dx, ld_dx, 0)
 
 
 def test_token_logprobs_for_training_refuse(lib):
