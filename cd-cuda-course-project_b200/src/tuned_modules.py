@@ -29,7 +29,8 @@ calls it through the C ABI on the current CUDA stream:
 
 The linear and attention layers are inference layers (they have forward
 kernels only): a call with autograd recording raises instead of silently
-computing something else. `apply_tuned_layers` swaps layers into a model,
+computing something else. None of the layers has forward-mode tangents; inputs
+that carry one are refused. `apply_tuned_layers` swaps layers into a model,
 copying the weights (the reference's version builds fresh layers and drops the
 trained weights).
 `sdpa_comparison` checks and times the attention core against
@@ -48,6 +49,7 @@ from typing import Any, Dict, Optional, Tuple
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd import forward_ad as _forward_ad
 
 import kt_lib
 import kt_ops
@@ -80,10 +82,23 @@ def tuned_library(kernel: str, results_dir: Optional[os.PathLike] = None) -> kt_
     return kt_lib.load()
 
 
-def _no_autograd(name: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _tangents(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether forward-mode differentiation has given one of them a tangent."""
+    if getattr(_forward_ad, "_current_level", 0) < 0:  # (asking a tensor takes 0.7 us)
+        return False
+    return any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _recording(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a result computed from them is to be differentiable. A tangent counts:
+    the autograd functions below have none to give and torch refuses the call."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or _tangents(*tensors)
+
+
+def _no_autograd(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    if _recording(*tensors):
         raise RuntimeError(f"{name} runs forward-only B200 kernels; call it under torch.no_grad() "
-                           "or torch.inference_mode()")
+                           "or torch.inference_mode(), without forward-mode tangents")
 
 
 class TunedLinear(nn.Linear):
@@ -145,7 +160,7 @@ class TunedLayerNorm(nn.LayerNorm):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         c = self.normalized_shape[0]
         x2 = x.reshape(-1, c).contiguous()
-        if torch.is_grad_enabled() and any(t.requires_grad for t in (x, self.weight, self.bias)):
+        if _recording(x, self.weight, self.bias):
             y = _LayerNormTrain.apply(x2, self.weight, self.bias, self.eps, self.checkpoint8)
         elif x.dtype == torch.float32:
             y = kt_ops.layernorm(x2, self.weight, self.bias, self.eps, lib=self._lib)
@@ -224,7 +239,7 @@ def token_log_probs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None
         if targets.shape != lead:
             raise ValueError(f"targets must be {tuple(lead)}, got {tuple(targets.shape)}")
         targets = targets.reshape(-1).contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if _recording(logits):
         r = kt_ops.TokenLogprobs(*_TokenLogProbs.apply(x, targets, top_k, scale, ignore_index))
     else:
         r = kt_ops.token_logprobs(x, targets, top_k, scale, ignore_index)
