@@ -113,3 +113,21 @@ def test_bytes_behind_a_checkpoint_row_stay(dev, lib, cols, ld, t):
     saved = want._replace(q8=buf[:rows, :cols])
     for u, v in zip(kt_ops.layernorm_bwd(dy, saved, lib=lib), kt_ops.layernorm_bwd(dy, want, lib=lib)):
         assert (u.double() - v.double()).norm() <= 4 * (half_step(u.dtype) + 64 * E) * v.double().norm()
+
+
+# The shapes that the dispatch tells apart, with more rows than CTAs, so that each
+# takes several: 32 threads a row of one piece and of 16 columns, 64, 128, 256 and 512 threads of
+# 16 columns, 256 and 512 of 32, and the kernels without a limit of width; whole pieces and cut ones.
+MANY = [(t, *shape) for shape in [(2000, 128), (2000, 300), (2000, 512), (3000, 1000), (2000, 1021), (1500, 2000),
+                                  (1500, 3333), (900, 7000), (900, 6999), (700, 12345), (700, 16384), (700, 16383),
+                                  (1300, 16387)] for t in TYPES]
+MANY += [(t, 5000, cols) for cols in (8000, 4101) for t in TYPES[1:]]
+MANY += [(torch.float32, 2500, cols) for cols in (6000, 4101)]
+
+
+@pytest.mark.parametrize("ckpt8", [False, True])
+@pytest.mark.parametrize("t,rows,cols", MANY)
+def test_several_rows_for_each_cta(dev, lib, t, rows, cols, ckpt8):
+    x, dy, gamma, beta = inputs(dev, rows, cols, t)
+    check(x, dy, gamma, beta, ckpt8=ckpt8, lib=lib)
+    torch.cuda.empty_cache()
