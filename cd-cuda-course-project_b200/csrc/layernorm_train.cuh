@@ -343,6 +343,14 @@ __device__ __forceinline__ float2 row_sum2(float a, float b, float2* scratch) {
   return make_float2(a, b);
 }
 
+// A row's sum over its columns, rounded as by a division (per_col = 1 / cols alone
+// is up to a step off, which x - mean would have in every column of a row of one
+// value); infinities and NaNs as they are.
+__device__ __forceinline__ float mean_of(float sum, int cols, float per_col) {
+  const float m = sum * per_col, left = fmaf(-m, (float)cols, sum);
+  return left == left ? fmaf(left, per_col, m) : m;
+}
+
 // Weights of columns [e0, e0 + V); `other` where there are none.
 template <typename T>
 __device__ __forceinline__ void load_weights(const void* w, int wdtype, int e0, int cols, float other,
@@ -498,7 +506,7 @@ fwd_rows(const FwdArgs p) {
     } else {
       fetch(slot, row + D * stride);
     }
-    const float mean = row_sum<TPR>(halves(s2).x + halves(s2).y, red[0]) * per_col;
+    const float mean = mean_of(row_sum<TPR>(halves(s2).x + halves(s2).y, red[0]), cols, per_col);
     if constexpr (CKPT && EDGE) {  // every thread has read its neighbour's piece
       if (TPR == 32) __syncwarp();
       fetch(slot, row + D * stride);
@@ -747,7 +755,7 @@ bwd_rows(const BwdArgs p) {
       }
     }
     const float2 s = row_sum2<TPR>(halves(s1).x + halves(s1).y, halves(s2).x + halves(s2).y, red[turn]);
-    const float c1 = -s.x * per_col * rstd, c2 = -s.y * per_col;
+    const float c1 = -s.x * per_col * rstd, c2 = -mean_of(s.y, cols, per_col);
     const uint64_t m1 = pair(c1, c1), m2 = pair(c2, c2);
     T* dxr = static_cast<T*>(p.dx) + row * cols;
 #pragma unroll
@@ -837,7 +845,7 @@ __global__ void __launch_bounds__(TPR) fwd_scalar(const FwdArgs p) {
       s += v[i];
     }
     if (row + gridDim.x < p.rows) fetch(row + gridDim.x);
-    const float mean = row_sum<TPR>(s, red[0]) * per_col;
+    const float mean = mean_of(row_sum<TPR>(s, red[0]), cols, per_col);
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < EPT; ++i)
@@ -904,7 +912,7 @@ __global__ void __launch_bounds__(TPR) bwd_scalar(const BwdArgs p) {
       s2 += d[i];
     }
     const float2 s = row_sum2<TPR>(s1, s2, red[turn]);
-    const float c1 = s.x * per_col, c2 = s.y * per_col;
+    const float c1 = s.x * per_col, c2 = mean_of(s.y, cols, per_col);
 #pragma unroll
     for (int i = 0; i < EPT; ++i)
       if (t + i * TPR < cols) dxr[t + i * TPR] = elem::from_f<T>(rstd * (d[i] - c2 - xh[i] * c1));

@@ -42,6 +42,23 @@ def test_rows_of_one_value(dev, lib, rows, cols, value, ckpt8):
 
 @pytest.mark.parametrize("ckpt8", [False, True])
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("cols", [3, 48, 77, 300, 1000, 1021, 3000, 6999, 12344, 12345, 16387])
+def test_means_are_those_of_a_division(dev, lib, cols, t, ckpt8):
+    """1000 in every column: the sum (below 2^24 thousands) is exact and so is its
+    quotient by the columns, though one over the columns is not. Then nothing is
+    left of x - mean, and of dy = 1 less its mean."""
+    for rows, offset in ((5, 0), (700, 0), (5, 1)):
+        base = torch.full((rows * cols + offset,), 1000.0, device=dev).to(t)
+        x = base[offset:].view(rows, cols)
+        beta = torch.linspace(-1, 1, cols, device=dev)
+        y, saved = kt_ops.layernorm_train(x, None, beta, ckpt8=ckpt8, lib=lib)
+        assert saved.mean.eq(1000).all() and torch.equal(y, beta.to(t).expand(rows, cols))
+        dx, _, dbeta = kt_ops.layernorm_bwd(torch.ones_like(x), saved, lib=lib)
+        assert dx.eq(0).all() and dbeta.eq(rows).all()
+
+
+@pytest.mark.parametrize("ckpt8", [False, True])
+@pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("rows,cols", [(3, 16387), (700, 16387), (70, 20000), (300, 1000), (50, 1023), (9, 8192)])
 def test_gradient_of_the_input_in_place(dev, lib, rows, cols, t, ckpt8):
     """dx over dy's memory, and over x's: the weights' gradients stay those of the inputs."""
