@@ -101,6 +101,11 @@ def _no_autograd(name: str, *tensors: Optional[torch.Tensor]) -> None:
                            "or torch.inference_mode(), without forward-mode tangents")
 
 
+def _columns(name: str, x: torch.Tensor, columns: int) -> None:
+    if x.dim() < 1 or x.shape[-1] != columns:
+        raise ValueError(f"{name}: rows of {columns} columns expected, got {tuple(x.shape)}")
+
+
 class TunedLinear(nn.Linear):
     """nn.Linear computed by the library's GEMM (x·W^T with W as the transpose_b operand)."""
 
@@ -159,6 +164,7 @@ class TunedLayerNorm(nn.LayerNorm):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         c = self.normalized_shape[0]
+        _columns("TunedLayerNorm", x, c)
         x2 = x.reshape(-1, c).contiguous()
         if _recording(x, self.weight, self.bias):
             y = _LayerNormTrain.apply(x2, self.weight, self.bias, self.eps, self.checkpoint8)
@@ -193,6 +199,7 @@ class TunedLinearW4(nn.Module):
         return cls(w, linear.bias.detach().clone() if linear.bias is not None else None)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        _columns("TunedLinearW4", x, self.in_features)
         _no_autograd("TunedLinearW4", x)
         w = kt_ops.W4Weight(self.packed, self.scales, self.zeros, self.group)
         x2 = x.reshape(-1, self.in_features)
