@@ -22,11 +22,11 @@
 // special-function rate that goes with the full read rate.
 //
 // The top k of a row need hardly any work in that pass: a thread notes the
-// largest value of each of up to 8 stretches of its pieces. Of the 8 warps, each
-// finds the ceil(k / 8)-th largest of its threads' maxima; the least of the eight
-// is reached by k values at least, so it bounds the k-th largest from below, and
-// only stretches whose maximum reaches it (about 2 k of 2048) can hold a value of
-// the top k. Their pieces are read once more (from L2), one or two by each
+// largest value of each of up to 8 stretches of its pieces. Of the row's w warps (8,
+// 4 or 1), each finds the ceil(k / w)-th largest of its threads' maxima; the least of
+// these is reached by k values at least, so it bounds the k-th largest from below,
+// and only stretches whose maximum reaches it (about 2 k of 2048, by 8 warps) can hold
+// a value of the top k. Their pieces are read once more (from L2), one or two by each
 // thread, and what reaches the bound goes into a list in shared memory. Values
 // are ordered by (value, lower index), which makes every key different; pieces
 // that overflow the list (rows with many equal values) raise the bound to the
@@ -388,7 +388,6 @@ __device__ __forceinline__ void find_top(Top<G>& top, const FwdArgs& p, const Ro
   best_of_list<G>(top, top.count, k, t);
 }
 
-// The outputs of a row, by one warp, from its statistics and sorted top k.
 // A row's target and its logit, loaded before the row is streamed.
 struct Target {
   int64_t at;
@@ -404,6 +403,7 @@ __device__ __forceinline__ Target load_target(const FwdArgs& p, int64_t row) {
   return t;
 }
 
+// The outputs of a row, by one warp, from its statistics and sorted top k.
 template <bool TOP>
 __device__ __forceinline__ void write_row(const FwdArgs& p, int64_t row, const Stats& a, const Target& target,
                                           const uint64_t* best) {

@@ -7,10 +7,12 @@
 // is 13 10^12 weights a second, which leaves 2.6 lane instructions for each;
 // fp32 multiply-adds per token would exceed that from the second token on. So the
 // sums run on the tensor cores (mma.sync m16n8k16: 16 weight rows by 8 tokens,
-// fp32 accumulation; a tcgen05 tile of 128 rows would need the weights
-// unpacked through shared memory): q - z is exact in 16 bits, and so are its
-// products with x; the scale multiplies each group's fp32 sum. fp32 tokens are
-// split exactly into three bf16 parts.
+// fp32 accumulation, the weights unpacked straight into its operand registers; a
+// tcgen05 tile would take them from tensor memory, 128 rows at a time, through a
+// store and a wait for each group, which was not tried): q - z is exact in 16 bits,
+// and so are its products with x; the scale multiplies each group's fp32 sum. fp32
+// tokens are split into three bf16 parts: exactly from 2^-110 on, where the last of
+// their 24 bits is at least bf16's least number 2^-133, and to less than 2^-133 below.
 //
 // Unpacking takes most of the instructions, so it costs 9 for 8 weights: one
 // mask for each pair of nibbles (bits 0-3 and 4-7 of both halves of a word, then
@@ -40,8 +42,9 @@
 // Measured on a B200, 131072x8192: one token in bf16, groups of 128, 109 us
 // (5.1 TB/s, 78 % of measured copy bandwidth); 8 tokens in fp16, groups of 64 with
 // zeros, 142 us (4.2 TB/s; issue slots 66 % busy, the ALU pipe 52 %); 16 tokens in
-// bf16 184 us. 4096x4096, one token: 5.5 us. 16 fp32 tokens, 32768x8192: 104 us,
-// bound by the three tensor products per weight.
+// bf16 184 us. 4096x4096, one token: 5.5 us. 16 fp32 tokens, 32768x8192: 104 us; of
+// its units the tensor pipe is the busiest (53 %, on 128 of 148 SMs; three products
+// per weight), and warps wait for it most.
 #pragma once
 #include <cooperative_groups.h>
 

@@ -272,8 +272,9 @@ KT_API int kt_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* 
 /* 4-bit weights: w (N x K) in groups of `group` (32, 64 or 128, a divisor of K)
  * columns as q in 0..15, two to a byte (`packed`, N x K/2, the even column in
  * the low half), and scales (N x K/group, of scale_dtype),
- * standing for s*(q-8). Quantises symmetrically: s = max|w|/7 of the group,
- * q = 8 + w/s to nearest even; a group that is not finite gets the scale NaN. */
+ * standing for s*(q-8). Quantises symmetrically: s = max|w|/7 of the group in the
+ * scales' type, q = 8 + w/s to nearest even, limited to 0..15 (8 where s is 0); a
+ * group that is not finite gets the scale NaN. */
 KT_API int kt_w4_quantize(const void* w, int64_t N, int64_t K, int group, int dtype, uint8_t* packed, void* scales,
                           int scale_dtype, kt_stream_t stream);
 
@@ -282,7 +283,8 @@ KT_API int kt_w4_quantize(const void* w, int64_t N, int64_t K, int group, int dt
  * zeros (N x K/group, values of 0..15) may be NULL: 8; bias (N, of `dtype`) may
  * be NULL; K up to 131072. Made for few tokens:
  * the weights are read once for every 16. A group's sum of x*(q-z) is fp32 and
- * scaled afterwards, so it must not overflow. `packed` is 16-byte aligned; y
+ * scaled afterwards, so it must not overflow. fp32 tokens below 2^-110 are taken
+ * to within 2^-133. `packed` is 16-byte aligned; y
  * and x must not overlap. */
 KT_API int kt_w4_linear(const void* x, int64_t ldx, const uint8_t* packed, const void* scales, const uint8_t* zeros,
                         const void* bias, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, int group, int dtype,
