@@ -27,12 +27,12 @@
 // one partial row per CTA. A second kernel adds the partial rows in their order,
 // so results do not change from run to run.
 //
-// Measured on a B200, 16384x4096, the join included: bf16 forward 48 us (5.6 TB/s,
-// 85 % of measured copy bandwidth) and backward 73 us (5.5 TB/s); with checkpoints
-// 62 us (5.5 TB/s) and 74 us (4.5 TB/s, issue slots 62 % busy); fp32 98 and 141 us
-// (5.5 and 5.7 TB/s). 8x512 fp32: 2.4 and 3.9 us. 4096x16384 bf16: 55 and 79 us
+// Measured on a B200, 16384x4096, the join included: bf16 forward 46 us (5.8 TB/s,
+// 89 % of measured copy bandwidth) and backward 73 us (5.5 TB/s); with checkpoints
+// 62 us (5.4 TB/s) and 77 us (4.4 TB/s, issue slots 62 % busy); fp32 98 and 140 us
+// (5.5 and 5.7 TB/s). 8x512 fp32: 2.3 and 3.9 us. 4096x16384 bf16: 55 and 80 us
 // (79 and 136 us with gamma and beta read again from L2 in every row).
-// Odd widths: 16384x2049 bf16 54 and 80 us, with checkpoints 86 and 110 us.
+// Odd widths: 16384x2049 bf16 55 and 77 us, with checkpoints 86 and 110 us.
 #pragma once
 #include <type_traits>
 
@@ -819,8 +819,9 @@ bwd_rows(const BwdArgs p) {
 }
 
 // ---------------------------------------------------------------- element by element
-// Rows of x and dy that are not equally aligned, and checkpoints whose rows are
-// no whole words: lanes hold consecutive columns (a warp's 32 are one
+// Rows of x and y, or dy and dx, that are not equally aligned (an input that begins
+// off a 16-byte boundary: 16384x4096 bf16 205 and 249 us), and checkpoints whose rows
+// are no whole words: lanes hold consecutive columns (a warp's 32 are one
 // block of the checkpoint), EPT per thread, as above but for the copies ahead.
 template <typename T, int TPR, bool CKPT>
 __global__ void __launch_bounds__(TPR) fwd_scalar(const FwdArgs p) {
