@@ -282,7 +282,7 @@ template <int TPR, int PER_SM>
 constexpr int kCtas = PER_SM / kThreads<TPR>;
 template <typename T, int TPR, int VPT>
 constexpr int kFwdPerSm = kHold<T, VPT> || TPR != 256 ? kFwdThreads : 512;
-// Bytes that one weight vector of a thread's columns takes in shared memory.
+// Bytes that one weight vector takes in a CTA's shared memory.
 template <typename T, int TPR, int VPT>
 constexpr int kWeightBytes = kHold<T, VPT> ? 0 : VPT * elem::kVec<T> * 4 * kThreads<TPR>;
 // Rows in shared memory: as many as 200 KB per SM hold (224 KB less the weights), up to 4.

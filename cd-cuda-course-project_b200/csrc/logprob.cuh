@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(kBwdBlock) bwd_kernel(const BwdArgs p) {
     const float2 n = p.norm[row];
     b = -n.x;
     d = -n.y;
-    none = n.x == -INFINITY;
+    none = n.x == -INFINITY && n.y == -INFINITY;  // (of NaNs and -inf the maximum is -inf too, the sum NaN)
   } else {
     a = p.scale;
     b = -p.lse[row];

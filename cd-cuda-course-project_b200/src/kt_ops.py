@@ -392,7 +392,7 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: Optional[torch.Tensor], re
             raise ValueError("out overlaps the logits without being the same")
     if lib is None:
         lib = kt_lib.load()
-    norm = result.norm
+    norm = getattr(result, "norm", None)
     if norm is None:
         norm = token_logprobs(logits, scale=scale, lib=lib).norm
     _dense(norm, "result.norm", torch.float32, dev)

@@ -152,3 +152,29 @@ def test_gradient_from_lse(dev, lib):
     H = (p * far).sum(1, keepdim=True)
     more = p * 2 * E * lse * (g.abs()[:, None] + h.abs()[:, None] * (far + H + 1))
     assert bool(((dx.double() - want).abs() <= off + more + E * want.abs() + 2.0 ** -149).all())
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,V", [(8, 700), (400, 700), (8, 30000)])
+def test_rows_that_are_not_finite(dev, lib, rows, V, t):
+    """A NaN or +inf makes a row's gradient NaN, whatever else the row holds; a row
+    of only -inf has none."""
+    x, targets, g, h = case(dev, rows, V)
+    x = x.to(t)
+    whole = kt_ops.token_logprobs(x, targets, lib=lib)
+    x[1] = float("nan")
+    x[2], x[2, V - 1] = -math.inf, float("nan")
+    x[3, 5] = math.inf
+    x[4, 6], x[4, 7] = float("nan"), math.inf
+    x[5] = -math.inf
+    x[6] = math.inf
+    r = kt_ops.token_logprobs(x, targets, lib=lib)
+    l = torch.ones(rows, device=dev)
+    rest = torch.ones(rows, dtype=torch.bool, device=dev)
+    rest[1:7] = False
+    for a, b, c in ((g, None, None), (None, h, None), (None, None, l), (g, h, l)):
+        dx = kt_ops.token_logprobs_bwd(x, targets, r, a, b, lib=lib, grad_lse=c)
+        assert dx[[1, 2, 3, 4, 6]].isnan().all() and dx[5].eq(0).all()
+        assert torch.equal(dx[rest], kt_ops.token_logprobs_bwd(x, targets, whole, a, b, lib=lib, grad_lse=c)[rest])
+    zero = torch.zeros(rows, device=dev)
+    assert kt_ops.token_logprobs_bwd(x, targets, r, zero, zero, lib=lib, grad_lse=zero).eq(0).all()
