@@ -13,7 +13,7 @@ torch = pytest.importorskip("torch")
 
 import kt_lib  # noqa: E402
 import kt_ops  # noqa: E402
-from test_gpu_layernorm_train import E, TYPES, check, half_step, inputs  # noqa: E402
+from test_gpu_layernorm_train import E, TYPES, check, half_step, inputs, rounded8  # noqa: E402
 
 
 @pytest.mark.parametrize("ckpt8", [False, True])
@@ -147,4 +147,34 @@ MANY += [(torch.float32, 2500, cols) for cols in (6000, 4101)]
 def test_several_rows_for_each_cta(dev, lib, t, rows, cols, ckpt8):
     x, dy, gamma, beta = inputs(dev, rows, cols, t)
     check(x, dy, gamma, beta, ckpt8=ckpt8, lib=lib)
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("ckpt8", [False, True])
+@pytest.mark.parametrize("rows,cols", [(600000, 4096), (140000, 16387)])
+def test_offsets_past_32_bits(dev, lib, rows, cols, ckpt8):
+    """The same 40 rows again and again, over more than 2^31 elements: each row's
+    results are those of the first."""
+    few, dfew, gamma, beta = inputs(dev, 40, cols, torch.bfloat16)
+    x, dy = few.repeat(rows // 40, 1), dfew.repeat(rows // 40, 1)
+    assert x.numel() > 1 << 31
+    y, saved = kt_ops.layernorm_train(x, gamma, beta, ckpt8=ckpt8, lib=lib)
+    want, wsaved = kt_ops.layernorm_train(few, gamma, beta, ckpt8=ckpt8, lib=lib)
+    for at in (0, rows // 80 * 40, rows - 40):
+        assert torch.equal(y[at:at + 40], want) and torch.equal(saved.stats[:, at:at + 40], wsaved.stats)
+        if ckpt8:
+            assert torch.equal(saved.q8[at:at + 40], wsaved.q8) and torch.equal(saved.q8_exp[at:at + 40], wsaved.q8_exp)
+    del x, y
+    dx, dgamma, dbeta = kt_ops.layernorm_bwd(dy, saved, lib=lib)
+    dwant, _, _ = kt_ops.layernorm_bwd(dfew, wsaved, lib=lib)
+    for at in (0, rows // 80 * 40, rows - 40):
+        assert torch.equal(dx[at:at + 40], dwant)
+    # rows/64 + 160 additions in a chain, each off by 2^-24 of the magnitudes (a CTA, or a 64th of the rows, adds fewer)
+    d, n = dfew.double(), rows // 40
+    kept = rounded8(few)[2] if ckpt8 else few.double()
+    xh = (kept - wsaved.mean.double()[:, None]) * wsaved.rstd.double()[:, None]
+    tol = (rows / 64 + 160 + 64) * E * n * (d * xh).abs().sum(0) + 64 * E * n * d.abs().sum(0)
+    assert bool(((dgamma.double() - n * (d * xh).sum(0)).abs() <= tol).all())
+    assert bool(((dbeta.double() - n * d.sum(0)).abs() <= (rows / 64 + 160) * E * n * d.abs().sum(0)).all())
+    del dx, dy, saved
     torch.cuda.empty_cache()
