@@ -178,3 +178,24 @@ def test_rows_that_are_not_finite(dev, lib, rows, V, t):
         assert torch.equal(dx[rest], kt_ops.token_logprobs_bwd(x, targets, whole, a, b, lib=lib, grad_lse=c)[rest])
     zero = torch.zeros(rows, device=dev)
     assert kt_ops.token_logprobs_bwd(x, targets, r, zero, zero, lib=lib, grad_lse=zero).eq(0).all()
+
+
+@pytest.mark.parametrize("rows,V", [(24, 1003), (400, 1003), (3, 40000)])
+@pytest.mark.parametrize("offset", [0.0, 1e3, -1e5, 3e30])
+def test_values_at_a_common_offset(dev, lib, rows, V, offset):
+    """Log probabilities and entropies are off by what goes with |z - zmax|, not with |z|."""
+    x, targets, _, _ = case(dev, rows, V, offset)
+    r = kt_ops.token_logprobs(x, targets, top_k=4, lib=lib)
+    z = x.double()
+    logp = torch.log_softmax(z, 1)
+    p = logp.exp()
+    a = z.amax(1, keepdim=True) - z
+    S = torch.where(p > 0, p * a, 0.0).sum(1, keepdim=True)
+    H = -torch.where(p > 0, p * logp, 0.0).sum(1)
+    n = V / 256 + 64
+    L = E * (n + 12 + 4 * S + 4 * a + 4 * logp.abs() + 4 * math.log(V))
+    index = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :4]
+    assert torch.equal(r.top_index, index)
+    for got, at in ((r.logprob[:, None], targets[:, None]), (r.top_logprob, index)):
+        assert bool(((got.double() - logp.gather(1, at)).abs() <= L.gather(1, at)).all())
+    assert bool(((r.entropy.double() - H).abs() <= E * (n + 16) * (2 + 2 * S[:, 0])).all())
